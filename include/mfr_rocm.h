@@ -39,6 +39,8 @@ enum {
 /* Activation applied in a GEMM epilogue or by mfr_bias_act.
  * GELU_TANH is mensurflow::gelu(x, approximate=true), GELU_ERF is gelu(x, false). */
 enum { MFR_ACT_NONE = 0, MFR_ACT_GELU_TANH = 1, MFR_ACT_GELU_ERF = 2 };
+/* x / (1 + exp(-x)) in fp32, for mfr_f8gemm alone (the other entry points refuse it). */
+enum { MFR_ACT_SILU = 3 };
 
 /* Opaque stream: a HIP stream on one device plus the workspace its kernels use
  * (the reference keeps one Stream per device: src/backends/backend.hpp:32-44). */
@@ -385,6 +387,106 @@ typedef struct mfr_attention_desc {
 } mfr_attention_desc;
 
 int mfr_attention(mfr_stream_t stream, const mfr_attention_desc* desc);
+
+/* ---- 8-bit matrices: conversion, norm and GEMM --------------------------------------------
+ *
+ * The serving path of a feed-forward block in 8 bits. The reference has no 8-bit type and no such
+ * op; these entry points stand beside mfr_sgemm and mfr_bias_act, whose layouts and roundings they
+ * follow. Forward only, like the rest of this library. */
+
+#define MFR_F8_BLOCK 128
+
+/* A matrix of e4m3 values (OCP: 4 exponent bits, 3 of mantissa, no infinities, largest 448) with
+ * fp32 scales: element (r, c) stands for value(r, c) * scale(r / block_rows, c / 128), scale (i, j)
+ * at scales[i * scales_rs + j * scales_cs]. Rows are contiguous and rs bytes apart; the base and rs
+ * are multiples of 16 bytes, rs at least the row's length. A row is read in whole 16-byte pieces,
+ * so the bytes between its end and the next multiple of 16 are read (not used, never written).
+ * block_rows is 1 (activations: a scale per row and 128 columns) or 128 (weights: one per 128 x 128
+ * block). Columns of scales that lie together (scales_rs = 1) suit mfr_f8gemm's loads best. */
+typedef struct mfr_f8_matrix {
+    uint8_t* values;
+    int64_t rs;
+    float* scales;
+    int64_t scales_rs, scales_cs;
+    int32_t block_rows;
+    int32_t reserved;
+} mfr_f8_matrix;
+
+/* out = x in 8 bits, x [rows, cols] fp32 with unit column stride and row stride x_rs. For each
+ * block (out->block_rows x 128), in fp32:
+ *   scale = max(fl(largest magnitude / 448), 2^-126),  value = e4m3(fl(x * fl(1 / scale))),
+ * rounded to nearest, ties to even. A block that holds a NaN or an infinity stands for NaN as a
+ * whole. A block of zeros has the scale 2^-126. */
+int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float* x, int64_t x_rs,
+                    const mfr_f8_matrix* out);
+
+/* Root-mean-square norm of rows, with the residual's addition in front of it and a result in fp32,
+ * 8 bits or both:
+ *
+ *   t = x + residual,   y(r, c) = t(r, c) / sqrt(mean_c(t(r, c)^2) + eps) * weight(c)
+ *
+ * sum = t is written where sum is not NULL (the residual stream for the next block), out = y where
+ * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize) where out_f8.values is
+ * not NULL; at least one of out and out_f8. residual and weight may be NULL (0 and 1). t is
+ * rounded to fp32, the squares are summed in double in an order that depends on cols alone, and y
+ * is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
+ * least cols. sum or out may be x or residual itself (the same base and row stride), not one
+ * another; other overlaps of outputs with anything are undefined. A NaN in a row makes the row NaN;
+ * an infinity becomes NaN and the row's other elements 0, the formula's values. A row of zeros gives
+ * zeros where eps > 0, NaN where eps is 0. */
+typedef struct mfr_rms_norm_desc {
+    int64_t rows, cols;
+    const float* x;
+    int64_t x_rs;
+    const float* residual;      /* may be NULL */
+    int64_t residual_rs;
+    const float* weight;        /* [cols] or NULL */
+    float* sum;                 /* may be NULL */
+    int64_t sum_rs;
+    float* out;                 /* may be NULL */
+    int64_t out_rs;
+    mfr_f8_matrix out_f8;       /* values may be NULL */
+    float eps;
+    int32_t reserved;
+} mfr_rms_norm_desc;
+
+int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
+
+/* A product of 8-bit matrices with a fused epilogue. A is [m, k] with a scale per row and 128
+ * depths (block_rows 1), B [n, k] (a weight as it is stored, one row per output) with a scale per
+ * 128 x 128 block (block_rows 128):
+ *
+ *   P(i, j) = sum_b fl(A.scale(i, b) * B.scale(j / 128, b)) * sum_{p in block b} A.v(i, p) B.v(j, p)
+ *   c(i, j) = act( fl( fl(P(i, j) + fl(beta * c0(i, j))) + bias[j] ) )
+ *
+ * or, with a second weight `up` of B's shape (up.values not NULL), the gated pair of projections in
+ * one kernel; c0 and bias are NULL then:
+ *
+ *   c(i, j) = fl( act(P_B(i, j)) * P_up(i, j) ).
+ *
+ * The inner sums are of exact products on the 8-bit matrix cores in fp32, the outer ones in fp32 in
+ * the order of b (ranges of b where the depth is split, added in order): the same inputs give the
+ * same bits on every call. c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8
+ * is given, out_f8.values may be NULL where c is: c in 8 bits, as mfr_f8_quantize gives it
+ * (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
+ * outputs with operands are undefined. k == 0 gives the epilogue of zero products. The product of
+ * two scales has to be in fp32's range. act is any MFR_ACT_*. */
+typedef struct mfr_f8gemm_desc {
+    int64_t m, n, k;
+    mfr_f8_matrix a;
+    mfr_f8_matrix b;
+    mfr_f8_matrix up;           /* values may be NULL: not gated */
+    float* c;                   /* may be NULL */
+    int64_t c_rs;
+    const float* c0;            /* may be NULL; may equal c */
+    int64_t c0_rs;
+    const float* bias;          /* [n] or NULL */
+    mfr_f8_matrix out_f8;       /* values may be NULL */
+    float beta;
+    int32_t act;                /* MFR_ACT_* */
+} mfr_f8gemm_desc;
+
+int mfr_f8gemm(mfr_stream_t stream, const mfr_f8gemm_desc* desc);
 
 /* ---- layout ------------------------------------------------------------------------------- */
 

@@ -21,13 +21,16 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import abi
-from .abi import ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, GemmDesc  # noqa: F401
+from .abi import (ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, ACT_SILU, F8GemmDesc,  # noqa: F401
+                  GemmDesc, RmsNormDesc)
 
 __all__ = [
     "ACT_NONE", "ACT_GELU_TANH", "ACT_GELU_ERF", "GemmDesc", "device_count", "device_info",
     "Stream", "DeviceArray", "Event", "sgemm", "gemm", "gemm_batched", "sgemv", "matvec", "dot",
     "bias_act", "where", "where_nd", "elementwise", "softmax", "argmax", "strided_copy", "fill", "attention",
     "attention_fused", "attention_composed", "gemm_plan",
+    "ACT_SILU", "F8Matrix", "F8GemmDesc", "RmsNormDesc", "quantize_f8", "rms_norm_desc",
+    "rms_norm_run", "rms_norm", "rms_norm_f8", "f8gemm_desc", "f8gemm", "gemm_f8", "gemm_f8_gated",
 ]
 
 
@@ -74,10 +77,13 @@ class Stream:
     _LARGE_STEP = 2 << 20
 
     def __init__(self, device: int = 0):
+        handle = ctypes.c_void_p()
+        abi.check(abi.load().mfr_stream_create(device, ctypes.byref(handle)), "mfr_stream_create")
+        self._adopt(handle, device)
+
+    def _adopt(self, handle, device: int) -> None:
         lib = abi.load()
         self.device = device
-        handle = ctypes.c_void_p()
-        abi.check(lib.mfr_stream_create(device, ctypes.byref(handle)), "mfr_stream_create")
         self.handle = handle
         self._scratch: dict = {}
         self._idle: dict = {}
@@ -86,6 +92,20 @@ class Stream:
         mem = ctypes.c_size_t(0)
         lib.mfr_get_device_info(device, None, 0, ctypes.byref(mem), None, None)
         self._idle_limit = max(mem.value // 8, 1 << 30)
+
+    @classmethod
+    def wrap(cls, hip_stream: int, device: int = 0) -> "Stream":
+        """A Stream over a HIP stream that another library owns (its handle as an integer, 0 for
+        the default stream): kernels order with that library's work (mfr_stream_wrap). The HIP
+        stream stays its owner's."""
+        lib = abi.load()
+        out = cls.__new__(cls)
+        out.handle = None
+        handle = ctypes.c_void_p()
+        abi.check(lib.mfr_stream_wrap(device, ctypes.c_void_p(hip_stream or None),
+                                      ctypes.byref(handle)), "mfr_stream_wrap")
+        out._adopt(handle, device)
+        return out
 
     @classmethod
     def size_class(cls, nbytes: int) -> int:
@@ -252,6 +272,15 @@ class DeviceArray:
     @classmethod
     def empty(cls, shape, stream: Stream, dtype=np.float32) -> "DeviceArray":
         return cls(shape, dtype, stream)
+
+    @classmethod
+    def wrap(cls, ptr: int, shape, stream: Stream, dtype=np.float32, strides=None) -> "DeviceArray":
+        """A view of memory that another library owns on the stream's device, `ptr` the address of
+        its first element, `strides` in elements (contiguous if None). Nothing frees it here; it
+        has to outlive the work queued on it."""
+        owner = cls.__new__(cls)
+        owner._base, owner._ptr, owner._device = None, 0, stream.device
+        return cls(shape, dtype, stream, _base=owner, _strides=strides, _ptr=int(ptr))
 
     # -- data movement ---------------------------------------------------------------------------
     @property
@@ -594,6 +623,192 @@ def fill(x: DeviceArray, value) -> None:
         {1: np.uint8, 2: np.uint16, 4: np.uint32, 8: np.uint64}[x.dtype.itemsize])[0]
     abi.check(abi.load().mfr_fill(x.stream.handle, x.ptr, x.dtype.itemsize, x.size, int(bits)),
               "mfr_fill")
+
+
+# ---- 8-bit matrices -------------------------------------------------------------------------------
+
+
+@dataclass
+class F8Matrix:
+    """An e4m3 matrix with block scales (mfr_f8_matrix): `values` a uint8 array [rows, cols] whose
+    rows are contiguous and 16 bytes aligned, `scales` a float32 array [rows or row blocks,
+    column blocks of 128] of any strides, `block_rows` 1 (activations) or 128 (weights)."""
+    values: DeviceArray
+    scales: DeviceArray
+    block_rows: int = 1
+
+    @classmethod
+    def empty(cls, rows: int, cols: int, stream: Stream, block_rows: int = 1) -> "F8Matrix":
+        """Room for [rows, cols]: rows padded to 16 bytes; scales of rows stored [blocks, rows],
+        as mfr_f8gemm reads them best."""
+        blocks = -(-cols // abi.F8_BLOCK)
+        values = DeviceArray.empty((rows, -(-cols // 16) * 16), stream, np.uint8)
+        if block_rows == 1:
+            scales = DeviceArray.empty((blocks, rows), stream).T
+        else:
+            scales = DeviceArray.empty((-(-rows // block_rows), blocks), stream)
+        return cls(values.slice(1, 0, cols), scales, block_rows)
+
+    @property
+    def shape(self):
+        return self.values.shape
+
+    @property
+    def stream(self) -> Stream:
+        return self.values.stream
+
+
+def _f8_desc(m: F8Matrix | None, what: str) -> abi.F8Desc:
+    d = abi.F8Desc()
+    d.block_rows = 1
+    if m is None:
+        return d
+    rows, cols = m.values.shape
+    blocks = (-(-rows // m.block_rows) if m.block_rows > 0 else rows, -(-cols // abi.F8_BLOCK))
+    if m.values.dtype.itemsize != 1 or m.scales.dtype != np.float32:
+        raise ValueError(f"{what}: values of one byte and float32 scales are needed")
+    if m.scales.shape != blocks:
+        raise ValueError(f"{what}: scales {m.scales.shape}, {blocks} are needed")
+    if cols > 1 and m.values.strides[1] != 1:
+        raise ValueError(f"{what}: rows need unit stride")
+    d.values, d.rs = m.values.ptr, m.values.strides[0]
+    d.scales, (d.scales_rs, d.scales_cs) = m.scales.ptr, m.scales.strides
+    d.block_rows = m.block_rows
+    return d
+
+
+def _rows_of(t: DeviceArray | None, shape, what: str) -> tuple:
+    """(address, row stride) of a float32 matrix of unit column stride; (None, 0) for None."""
+    if t is None:
+        return None, 0
+    if t.dtype != np.float32 or t.shape != tuple(shape):
+        raise ValueError(f"{what}: {t.dtype} {t.shape}, float32 {tuple(shape)} is needed")
+    if shape[1] > 1 and t.strides[1] != 1:
+        raise ValueError(f"{what}: rows need unit stride")
+    return t.ptr, t.strides[0]
+
+
+def _vector_of(t: DeviceArray | None, length: int, what: str):
+    if t is None:
+        return None
+    if t.dtype != np.float32 or t.shape != (length,) or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous float32 vector of {length} is needed")
+    return t.ptr
+
+
+def quantize_f8(x: DeviceArray, block_rows: int = 1, out: F8Matrix | None = None) -> F8Matrix:
+    """x [rows, cols] as e4m3 with a scale per block of block_rows x 128 (mfr_f8_quantize): 1 for
+    activations, 128 for weights."""
+    rows, cols = x.shape
+    ptr, rs = _rows_of(x, (rows, cols), "quantize_f8: x")
+    if out is None:
+        out = F8Matrix.empty(rows, cols, x.stream, block_rows)
+    if out.shape != x.shape or out.block_rows != block_rows:
+        raise ValueError(f"quantize_f8: out is {out.shape} with block_rows {out.block_rows}")
+    d = _f8_desc(out, "quantize_f8: out")
+    abi.check(abi.load().mfr_f8_quantize(x.stream.handle, rows, cols, ptr, rs, ctypes.byref(d)),
+              "mfr_f8_quantize")
+    return out
+
+
+def rms_norm_desc(x: DeviceArray, weight: DeviceArray | None = None, *,
+                  residual: DeviceArray | None = None, eps: float = 1e-6,
+                  summed: DeviceArray | None = None, out: DeviceArray | None = None,
+                  out_f8: F8Matrix | None = None) -> RmsNormDesc:
+    """The descriptor of one rms_norm over the rows of x [rows, cols], to be filled once and run
+    many times (rms_norm_run): t = x + residual to `summed`, t / rms(t) * weight to `out` (fp32)
+    and `out_f8` (8 bits), whichever are given."""
+    rows, cols = x.shape
+    d = RmsNormDesc()
+    d.rows, d.cols, d.eps = rows, cols, eps
+    d.x, d.x_rs = _rows_of(x, x.shape, "rms_norm: x")
+    d.residual, d.residual_rs = _rows_of(residual, x.shape, "rms_norm: residual")
+    d.sum, d.sum_rs = _rows_of(summed, x.shape, "rms_norm: summed")
+    d.out, d.out_rs = _rows_of(out, x.shape, "rms_norm: out")
+    d.weight = _vector_of(weight, cols, "rms_norm: weight")
+    if out_f8 is not None and out_f8.shape != x.shape:
+        raise ValueError(f"rms_norm: out_f8 is {out_f8.shape}, x {x.shape}")
+    d.out_f8 = _f8_desc(out_f8, "rms_norm: out_f8")
+    return d
+
+
+def rms_norm_run(stream: Stream, desc: RmsNormDesc) -> None:
+    """mfr_rms_norm on a filled descriptor."""
+    abi.check(abi.load().mfr_rms_norm(stream.handle, ctypes.byref(desc)), "mfr_rms_norm")
+
+
+def rms_norm(x: DeviceArray, weight: DeviceArray | None = None, *,
+             residual: DeviceArray | None = None, eps: float = 1e-6,
+             summed: DeviceArray | None = None, out: DeviceArray | None = None) -> DeviceArray:
+    """(x + residual) / rms * weight over the last dimension of a matrix, in fp32; x + residual is
+    written to `summed` where that is given (it may be x or residual)."""
+    if out is None:
+        out = DeviceArray.empty(x.shape, x.stream)
+    rms_norm_run(x.stream, rms_norm_desc(x, weight, residual=residual, eps=eps, summed=summed,
+                                         out=out))
+    return out
+
+
+def rms_norm_f8(x: DeviceArray, weight: DeviceArray | None = None, *,
+                residual: DeviceArray | None = None, eps: float = 1e-6,
+                summed: DeviceArray | None = None, out: F8Matrix | None = None) -> F8Matrix:
+    """rms_norm with its result in 8 bits, a scale per row and 128 columns: what gemm_f8 reads."""
+    if out is None:
+        out = F8Matrix.empty(*x.shape, x.stream)
+    rms_norm_run(x.stream, rms_norm_desc(x, weight, residual=residual, eps=eps, summed=summed,
+                                         out_f8=out))
+    return out
+
+
+def f8gemm_desc(a: F8Matrix, b: F8Matrix, *, up: F8Matrix | None = None, act=ACT_NONE,
+                c0: DeviceArray | None = None, beta=0.0, bias: DeviceArray | None = None,
+                out: DeviceArray | None = None, out_f8: F8Matrix | None = None) -> F8GemmDesc:
+    """The descriptor of one product of 8-bit matrices (mfr_f8gemm_desc), to be filled once and run
+    many times (f8gemm): a [m, k] with a scale per row, b and up [n, k] with 128 x 128 blocks; the
+    result goes to `out` (fp32), `out_f8` (8 bits) or both."""
+    (m, k), n = a.shape, b.shape[0]
+    for w in (b, up):
+        if w is not None and w.shape != (n, k):
+            raise ValueError(f"f8gemm: a is {a.shape}, a weight {w.shape}")
+    if out_f8 is not None and out_f8.shape != (m, n):
+        raise ValueError(f"f8gemm: out_f8 is {out_f8.shape}, {(m, n)} is needed")
+    d = F8GemmDesc()
+    d.m, d.n, d.k = m, n, k
+    d.a, d.b, d.up = _f8_desc(a, "f8gemm: a"), _f8_desc(b, "f8gemm: b"), _f8_desc(up, "f8gemm: up")
+    d.c, d.c_rs = _rows_of(out, (m, n), "f8gemm: out")
+    d.c0, d.c0_rs = _rows_of(c0, (m, n), "f8gemm: c0")
+    d.bias = _vector_of(bias, n, "f8gemm: bias")
+    d.out_f8 = _f8_desc(out_f8, "f8gemm: out_f8")
+    d.beta, d.act = beta, act
+    return d
+
+
+def f8gemm(stream: Stream, desc: F8GemmDesc) -> None:
+    """mfr_f8gemm on a filled descriptor."""
+    abi.check(abi.load().mfr_f8gemm(stream.handle, ctypes.byref(desc)), "mfr_f8gemm")
+
+
+def gemm_f8(a: F8Matrix, b: F8Matrix, *, c0: DeviceArray | None = None, beta=0.0,
+            bias: DeviceArray | None = None, act=ACT_NONE, out: DeviceArray | None = None,
+            out_f8: F8Matrix | None = None):
+    """act(a b^T + beta c0 + bias) of 8-bit matrices, b [n, k] as weights are stored: a new fp32
+    array, or `out` and / or `out_f8` where they are given. Returns out_f8 where only that is."""
+    if out is None and out_f8 is None:
+        out = DeviceArray.empty((a.shape[0], b.shape[0]), a.stream)
+    f8gemm(a.stream, f8gemm_desc(a, b, act=act, c0=c0, beta=beta, bias=bias, out=out,
+                                 out_f8=out_f8))
+    return out if out is not None else out_f8
+
+
+def gemm_f8_gated(a: F8Matrix, gate: F8Matrix, up: F8Matrix, *, act=ACT_SILU,
+                  out: DeviceArray | None = None, out_f8: F8Matrix | None = None):
+    """act(a gate^T) * (a up^T), both projections in one kernel: in 8 bits for the next product (a
+    new F8Matrix), or to `out` (fp32) and / or `out_f8` where they are given. Returns out_f8 where
+    that is given or made, else out."""
+    if out is None and out_f8 is None:
+        out_f8 = F8Matrix.empty(a.shape[0], gate.shape[0], a.stream)
+    f8gemm(a.stream, f8gemm_desc(a, gate, up=up, act=act, out=out, out_f8=out_f8))
+    return out_f8 if out_f8 is not None else out
 
 
 def attention_fused(q: DeviceArray, k: DeviceArray, v: DeviceArray,

@@ -22,6 +22,7 @@ MFR_E_NO_DEVICE = 4
 ACT_NONE = 0
 ACT_GELU_TANH = 1
 ACT_GELU_ERF = 2
+ACT_SILU = 3  # f8gemm alone
 
 EW_ADD = 0
 EW_MUL = 1
@@ -43,6 +44,7 @@ STAGE_NEVER = 1
 STAGE_ALWAYS = 2
 MAX_SPLITS = 64
 
+F8_BLOCK = 128  # MFR_F8_BLOCK: columns (and, of weights, rows) that share a scale
 MAX_BATCH_DIMS = 4
 MAX_COPY_DIMS = 8
 SGEMM_SCRATCH_BYTES = 64 << 20  # MFR_SGEMM_SCRATCH_BYTES: mfr_sgemm_noalloc's fixed scratch
@@ -84,6 +86,35 @@ class AttentionDesc(ctypes.Structure):
         ("out", _vp), ("out_rs", _i64), ("out_bs", _i64 * MAX_BATCH_DIMS),
         ("mask", _vp), ("mask_rs", _i64), ("mask_cs", _i64), ("mask_bs", _i64 * MAX_BATCH_DIMS),
         ("scale", _f32), ("reserved", _i32),
+    ]
+
+
+class F8Desc(ctypes.Structure):
+    """mfr_f8_matrix (include/mfr_rocm.h)."""
+
+    _fields_ = [("values", _vp), ("rs", _i64), ("scales", _vp), ("scales_rs", _i64),
+                ("scales_cs", _i64), ("block_rows", _i32), ("reserved", _i32)]
+
+
+class RmsNormDesc(ctypes.Structure):
+    """mfr_rms_norm_desc (include/mfr_rocm.h)."""
+
+    _fields_ = [
+        ("rows", _i64), ("cols", _i64),
+        ("x", _vp), ("x_rs", _i64), ("residual", _vp), ("residual_rs", _i64),
+        ("weight", _vp), ("sum", _vp), ("sum_rs", _i64), ("out", _vp), ("out_rs", _i64),
+        ("out_f8", F8Desc), ("eps", _f32), ("reserved", _i32),
+    ]
+
+
+class F8GemmDesc(ctypes.Structure):
+    """mfr_f8gemm_desc (include/mfr_rocm.h)."""
+
+    _fields_ = [
+        ("m", _i64), ("n", _i64), ("k", _i64),
+        ("a", F8Desc), ("b", F8Desc), ("up", F8Desc),
+        ("c", _vp), ("c_rs", _i64), ("c0", _vp), ("c0_rs", _i64), ("bias", _vp),
+        ("out_f8", F8Desc), ("beta", _f32), ("act", _i32),
     ]
 
 
@@ -129,6 +160,9 @@ SIGNATURES = {
     "mfr_argmax": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i64]),
     "mfr_elementwise": (ctypes.c_int, [_vp, ctypes.c_int, _vp, _vp, _f32, _vp, _i64]),
     "mfr_attention": (ctypes.c_int, [_vp, ctypes.POINTER(AttentionDesc)]),
+    "mfr_f8_quantize": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, ctypes.POINTER(F8Desc)]),
+    "mfr_rms_norm": (ctypes.c_int, [_vp, ctypes.POINTER(RmsNormDesc)]),
+    "mfr_f8gemm": (ctypes.c_int, [_vp, ctypes.POINTER(F8GemmDesc)]),
     "mfr_strided_copy": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, ctypes.POINTER(_i64),
                                         ctypes.POINTER(_i64)]),
     "mfr_fill": (ctypes.c_int, [_vp, _vp, _i32, _i64, ctypes.c_uint64]),

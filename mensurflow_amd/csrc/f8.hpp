@@ -1,0 +1,132 @@
+// 8-bit matrices (mfr_f8_matrix): what the kernels that write and read them share.
+//
+// A block of values x is held as e4m3 numbers v and one fp32 scale s, x ~ v s. With the largest
+// magnitude of the block put on e4m3's largest number, 448, a value is off by at most half a step:
+// 2^-4 of itself, or 2^-10 s below the least normal number 2^-6. The scale is at least 2^-126, so
+// that its reciprocal is a normal number; blocks below 448 2^-126 lose bits there.
+#pragma once
+
+#include "common.hpp"
+
+#include <string>
+
+namespace mfr::f8 {
+
+constexpr int kBlock = MFR_F8_BLOCK;
+constexpr float kTop = 448.0f;
+constexpr float kLeastScale = 0x1p-126f;
+
+constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
+
+// One matrix as a kernel's argument.
+struct Matrix {
+    uint8_t* values;
+    int64_t rs;
+    float* scales;
+    int64_t srs, scs;
+};
+
+// Checks `d` as a [rows, cols] matrix with `block_rows`, and takes it over. An empty matrix may
+// have null pointers.
+inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int block_rows,
+                      bool output, const char* what, const char* name) {
+    const std::string at = std::string(what) + ": " + name;
+    require(d.block_rows == 1 || d.block_rows == 128, at + " needs block_rows 1 or 128");
+    if (d.block_rows != block_rows) {
+        throw Error(MFR_E_UNSUPPORTED,
+                    at + " is taken with block_rows " + std::to_string(block_rows) + " only");
+    }
+    const Matrix m{d.values, d.rs, d.scales, d.scales_rs, d.scales_cs};
+    if (rows == 0 || cols == 0) {
+        return m;
+    }
+    require(d.values != nullptr && d.scales != nullptr, at + " has a null pointer");
+    require(d.rs >= cols, at + " has rows that overlap");
+    require(d.scales_rs >= 0 && d.scales_cs >= 0, at + " has negative scale strides");
+    if (!aligned16(d.values) || d.rs % 16 != 0) {
+        throw Error(MFR_E_UNSUPPORTED, at + " needs 16-byte aligned rows");
+    }
+    if (output) {
+        // No two scales in one place.
+        const int64_t r = (rows + block_rows - 1) / block_rows;
+        const int64_t c = blocks_of(cols);
+        const auto apart = [](int64_t inner, int64_t count, int64_t outer, int64_t others) {
+            return (count == 1 || inner >= 1) && (others == 1 || outer > inner * (count - 1));
+        };
+        require(apart(d.scales_rs, r, d.scales_cs, c) || apart(d.scales_cs, c, d.scales_rs, r),
+                at + " has scales that overlap");
+    }
+    return m;
+}
+
+} // namespace mfr::f8
+
+namespace mfr::f8::dev {
+
+// A magnitude as its bits, which order like the magnitude with infinity and then NaN on top: an
+// unsigned maximum over a block finds its NaN where fmaxf would pass it by.
+__device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+__device__ inline uint32_t magnitude(float4 v) {
+    return max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)));
+}
+
+// The block's scale from its largest magnitude's bits; NaN stays.
+__device__ inline float scale_of(uint32_t top) {
+    const float s = __uint_as_float(top) / kTop;
+    return s < kLeastScale ? kLeastScale : s;
+}
+
+// Four values in e4m3, the first in the low byte (v_cvt_pk_fp8_f32: nearest, ties to even).
+__device__ inline uint32_t pack(float4 v, float inverse) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v.x * inverse, v.y * inverse, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v.z * inverse, v.w * inverse, w, true);
+    return static_cast<uint32_t>(w);
+}
+
+// Stores the first `count` (up to 4) bytes of w at p, which is 4-byte aligned.
+__device__ inline void store_bytes(uint8_t* p, uint32_t w, int64_t count) {
+    if (count >= 4) {
+        *reinterpret_cast<uint32_t*>(p) = w;
+        return;
+    }
+    for (int64_t e = 0; e < count; ++e) {
+        p[e] = static_cast<uint8_t>(w >> (8 * e));
+    }
+}
+
+// Up to four floats of a row from p on, zeros behind `count`. 4-byte alignment.
+__device__ inline float4 load_quad(const float* p, int64_t count) {
+    if (count >= 4) {
+        return mfr::dev::load_loose(p);
+    }
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (count > 0) {
+        v.x = p[0];
+    }
+    if (count > 1) {
+        v.y = p[1];
+    }
+    if (count > 2) {
+        v.z = p[2];
+    }
+    return v;
+}
+
+__device__ inline void store_quad(float* p, float4 v, int64_t count) {
+    if (count >= 4) {
+        mfr::dev::store_loose(p, v);
+        return;
+    }
+    if (count > 0) {
+        p[0] = v.x;
+    }
+    if (count > 1) {
+        p[1] = v.y;
+    }
+    if (count > 2) {
+        p[2] = v.z;
+    }
+}
+
+} // namespace mfr::f8::dev

@@ -1,0 +1,260 @@
+// mfr_f8_quantize and mfr_rms_norm: passes over the rows of an fp32 matrix that end in e4m3 values
+// with a scale per block (f8.hpp), in fp32, or in both.
+#include "f8.hpp"
+
+#include <cmath>
+
+namespace {
+
+using mfr::dev::kWave;
+using mfr::f8::kBlock;
+using mfr::f8::Matrix;
+namespace dev = mfr::f8::dev;
+
+constexpr int kThreads = 256;
+constexpr int kStep = 4 * kThreads; // columns per workgroup step
+
+// The largest of v over the 32 lanes of a half wavefront, in each of them.
+__device__ inline uint32_t half_max(uint32_t v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, kWave)));
+    }
+    return v;
+}
+
+// Four columns from `col` on of row r, in 8 bits. 32 lanes hold a block: columns past the row are
+// zeros and count for nothing.
+__device__ inline void write_f8(const Matrix& q, int64_t r, int64_t col, int64_t cols, float4 v) {
+    const float scale = dev::scale_of(half_max(dev::magnitude(v)));
+    if (col < cols) {
+        dev::store_bytes(q.values + r * q.rs + col, dev::pack(v, 1.0f / scale), cols - col);
+        if (col % kBlock == 0) {
+            q.scales[r * q.srs + col / kBlock * q.scs] = scale;
+        }
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const float* x, int64_t x_rs,
+                                                                 int64_t rows, int64_t cols,
+                                                                 Matrix q) {
+    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+        for (int64_t c0 = 0; c0 < cols; c0 += kStep) {
+            const int64_t col = c0 + 4 * threadIdx.x;
+            write_f8(q, r, col, cols, dev::load_quad(x + r * x_rs + col, cols - col));
+        }
+    }
+}
+
+// A workgroup per 128 x 128 block.
+__global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(const float* x, int64_t x_rs,
+                                                                   int64_t rows, int64_t cols,
+                                                                   Matrix q, int64_t col_blocks) {
+    __shared__ uint32_t tops[kThreads / 32];
+    const int64_t rb = blockIdx.x / col_blocks;
+    const int64_t cb = blockIdx.x % col_blocks;
+    const int64_t col = cb * kBlock + 4 * (threadIdx.x % 32);
+    const int64_t row = rb * kBlock + threadIdx.x / 32;
+    float4 v[16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t r = row + 8 * i;
+        v[i] = dev::load_quad(x + r * x_rs + col, r < rows ? cols - col : 0);
+        top = max(top, dev::magnitude(v[i]));
+    }
+    tops[threadIdx.x / 32] = half_max(top); // the 32 lanes store one value
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) {
+        top = max(top, tops[i]);
+    }
+    const float scale = dev::scale_of(top);
+    const float inverse = 1.0f / scale;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int64_t r = row + 8 * i;
+        if (r < rows && col < cols) {
+            dev::store_bytes(q.values + r * q.rs + col, dev::pack(v[i], inverse), cols - col);
+        }
+    }
+    if (threadIdx.x == 0) {
+        q.scales[rb * q.srs + cb * q.scs] = scale;
+    }
+}
+
+struct NormParams {
+    int64_t rows, cols;
+    const float* x;
+    int64_t x_rs;
+    const float* residual;
+    int64_t residual_rs;
+    const float* weight;
+    float* sum;
+    int64_t sum_rs;
+    float* out;
+    int64_t out_rs;
+    Matrix q; // values null: none
+    float eps;
+};
+
+__device__ inline float4 add(float4 a, float4 b) {
+    return make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+}
+
+__device__ inline double squares(float4 v) {
+    const double x = v.x, y = v.y, z = v.z, w = v.w;
+    return fma(x, x, fma(y, y, fma(z, z, w * w)));
+}
+
+// t * scale * weight, rounded once.
+__device__ inline float4 scaled(float4 t, double scale, float4 w) {
+    return make_float4(static_cast<float>(t.x * scale * w.x), static_cast<float>(t.y * scale * w.y),
+                       static_cast<float>(t.z * scale * w.z),
+                       static_cast<float>(t.w * scale * w.w));
+}
+
+// v with zeros behind the first `count` elements.
+__device__ inline float4 inside(float4 v, int64_t count) {
+    return make_float4(count > 0 ? v.x : 0.0f, count > 1 ? v.y : 0.0f, count > 2 ? v.z : 0.0f,
+                       count > 3 ? v.w : 0.0f);
+}
+
+// A workgroup per row, in two passes over it.
+__global__ __launch_bounds__(kThreads) void rms_norm_kernel(NormParams p) {
+    __shared__ double sums[kThreads / kWave];
+    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        const float* x = p.x + r * p.x_rs;
+        const float* residual = p.residual != nullptr ? p.residual + r * p.residual_rs : nullptr;
+        float* sum = p.sum != nullptr ? p.sum + r * p.sum_rs : nullptr;
+        double total = 0.0;
+        for (int64_t col = 4 * threadIdx.x; col < p.cols; col += kStep) {
+            float4 t = dev::load_quad(x + col, p.cols - col);
+            if (residual != nullptr) {
+                t = add(t, dev::load_quad(residual + col, p.cols - col));
+            }
+            if (sum != nullptr) {
+                dev::store_quad(sum + col, t, p.cols - col);
+            }
+            total += squares(t);
+        }
+        total = mfr::dev::wave_sum(total);
+        if (threadIdx.x % kWave == 0) {
+            sums[threadIdx.x / kWave] = total;
+        }
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < kThreads / kWave; ++i) {
+            total += sums[i];
+        }
+        __syncthreads(); // `sums` has been read
+        const double scale = 1.0 / sqrt(total / static_cast<double>(p.cols) + p.eps);
+        for (int64_t c0 = 0; c0 < p.cols; c0 += kStep) {
+            const int64_t col = c0 + 4 * threadIdx.x;
+            float4 t;
+            if (sum != nullptr) {
+                t = dev::load_quad(sum + col, p.cols - col);
+            } else {
+                t = dev::load_quad(x + col, p.cols - col);
+                if (residual != nullptr) {
+                    t = add(t, dev::load_quad(residual + col, p.cols - col));
+                }
+            }
+            float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+            if (p.weight != nullptr) {
+                w = dev::load_quad(p.weight + col, p.cols - col);
+            }
+            float4 y = scaled(t, scale, w);
+            y = inside(y, p.cols - col); // behind the row 0 * scale may be NaN
+            if (p.out != nullptr) {
+                dev::store_quad(p.out + r * p.out_rs + col, y, p.cols - col);
+            }
+            if (p.q.values != nullptr) {
+                write_f8(p.q, r, col, p.cols, y);
+            }
+        }
+    }
+}
+
+// The descriptor's checks (of shapes, layouts and pointers: no device is needed).
+NormParams checked(const mfr_rms_norm_desc* desc) {
+    using mfr::require;
+    require(desc != nullptr, "rms_norm: null descriptor");
+    const mfr_rms_norm_desc& d = *desc;
+    require(d.rows >= 0 && d.cols >= 0, "rms_norm: negative dimension");
+    require(d.eps >= 0.0f && std::isfinite(d.eps), "rms_norm: eps is negative or not finite");
+    NormParams p{d.rows,   d.cols, d.x,      d.x_rs, d.residual, d.residual_rs,
+                 d.weight, d.sum,  d.sum_rs, d.out,  d.out_rs,   Matrix{},
+                 d.eps};
+    if (d.out_f8.values != nullptr) {
+        p.q = mfr::f8::checked(d.out_f8, d.rows, d.cols, 1, true, "rms_norm", "out_f8");
+    }
+    if (d.rows == 0 || d.cols == 0) {
+        return p;
+    }
+    require(d.out != nullptr || d.out_f8.values != nullptr,
+            "rms_norm: neither out nor out_f8 is given");
+    require(d.x != nullptr, "rms_norm: null input");
+    const auto apart = [&](const float* t, int64_t rs) { return t == nullptr || rs >= d.cols; };
+    require(apart(d.x, d.x_rs) && apart(d.residual, d.residual_rs) && apart(d.sum, d.sum_rs) &&
+                apart(d.out, d.out_rs),
+            "rms_norm: a matrix has rows that overlap");
+    require(d.sum == nullptr || d.sum != d.out, "rms_norm: sum and out are one array");
+    const auto in_place = [&](const float* t, int64_t rs) {
+        return t == nullptr ||
+               ((t != d.x || rs == d.x_rs) && (t != d.residual || rs == d.residual_rs));
+    };
+    require(in_place(d.sum, d.sum_rs) && in_place(d.out, d.out_rs),
+            "rms_norm: an output in place of an input needs its row stride");
+    return p;
+}
+
+} // namespace
+
+extern "C" {
+
+int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float* x, int64_t x_rs,
+                    const mfr_f8_matrix* out) {
+    return mfr::guarded([&] {
+        mfr::require(out != nullptr, "f8_quantize: null output");
+        mfr::require(rows >= 0 && cols >= 0, "f8_quantize: negative dimension");
+        mfr::require(out->block_rows == 1 || out->block_rows == 128,
+                     "f8_quantize: out needs block_rows 1 or 128");
+        const Matrix q =
+            mfr::f8::checked(*out, rows, cols, out->block_rows, true, "f8_quantize", "out");
+        const bool empty = rows == 0 || cols == 0;
+        mfr::require(empty || x != nullptr, "f8_quantize: null input");
+        mfr::require(empty || x_rs >= cols, "f8_quantize: x has rows that overlap");
+        auto& s = mfr::stream_of(stream);
+        if (empty) {
+            return;
+        }
+        if (out->block_rows == 1) {
+            quantize_rows_kernel<<<mfr::grid_blocks(rows, 1, int64_t{1} << 20), kThreads, 0,
+                                   s.stream>>>(x, x_rs, rows, cols, q);
+        } else {
+            const int64_t col_blocks = mfr::f8::blocks_of(cols);
+            const int64_t blocks = mfr::f8::blocks_of(rows) * col_blocks;
+            mfr::require(mfr::one_launch(blocks, kThreads), "f8_quantize: matrix too large");
+            quantize_blocks_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s.stream>>>(
+                x, x_rs, rows, cols, q, col_blocks);
+        }
+        mfr::check_launch("f8_quantize kernel");
+    });
+}
+
+int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc) {
+    return mfr::guarded([&] {
+        const NormParams p = checked(desc);
+        auto& s = mfr::stream_of(stream);
+        if (p.rows == 0 || p.cols == 0) {
+            return;
+        }
+        rms_norm_kernel<<<mfr::grid_blocks(p.rows, 1, int64_t{1} << 20), kThreads, 0, s.stream>>>(
+            p);
+        mfr::check_launch("rms_norm_kernel");
+    });
+}
+
+} // extern "C"
