@@ -16,6 +16,10 @@ constexpr int kBlock = MFR_F8_BLOCK;
 constexpr float kTop = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;
 
+// A round of 64 rows, and of 64 rows' scales, is addressed with 32 bits.
+constexpr int64_t kMostRowBytes = int64_t{1} << 25;
+constexpr int64_t kMostScaleStride = int64_t{1} << 23;
+
 constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
 // One matrix as a kernel's argument.
@@ -42,6 +46,9 @@ inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int bl
     }
     require(d.values != nullptr && d.scales != nullptr, at + " has a null pointer");
     require(d.rs >= cols, at + " has rows that overlap");
+    if (d.rs > kMostRowBytes || d.scales_rs > kMostScaleStride) {
+        throw Error(MFR_E_UNSUPPORTED, at + " has rows that lie too far apart");
+    }
     require(d.scales_rs >= 0 && d.scales_cs >= 0, at + " has negative scale strides");
     if (!aligned16(d.values) || d.rs % 16 != 0) {
         throw Error(MFR_E_UNSUPPORTED, at + " needs 16-byte aligned rows");

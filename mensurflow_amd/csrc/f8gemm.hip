@@ -43,6 +43,26 @@ Params checked(const mfr_f8gemm_desc* desc) {
     return p;
 }
 
+int64_t tiles(const Params& p, int64_t bm, int64_t bn) {
+    return ((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn);
+}
+
+void run(const mfr_stream& s, const Params& p) {
+    // The small tile where the large one leaves compute units without a tile.
+    const bool large = tiles(p, 128, 128) >= s.compute_units;
+    if (p.up.values != nullptr) {
+        if (large) {
+            mfr::f8gemm::launch_gated<128, 128, 2, 4>(s, p);
+        } else {
+            mfr::f8gemm::launch_gated<64, 128, 1, 4>(s, p);
+        }
+    } else if (large) {
+        mfr::f8gemm::launch<128, 128, 2, 2>(s, p);
+    } else {
+        mfr::f8gemm::launch<64, 128, 1, 4>(s, p);
+    }
+}
+
 } // namespace
 
 extern "C" {
@@ -54,11 +74,7 @@ int mfr_f8gemm(mfr_stream_t stream, const mfr_f8gemm_desc* desc) {
         if (p.m == 0 || p.n == 0) {
             return;
         }
-        if (p.up.values != nullptr) {
-            mfr::f8gemm::launch_gated<64, 128, 2, 2>(s, p);
-        } else {
-            mfr::f8gemm::launch<64, 128, 2, 2>(s, p);
-        }
+        run(s, p);
     });
 }
 

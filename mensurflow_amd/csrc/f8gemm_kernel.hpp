@@ -33,6 +33,7 @@ struct Params {
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
 
 // Eight e4m3 values as bf16, exactly.
 __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
@@ -51,12 +52,7 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
     return out;
 }
 
-__device__ inline float activate(float v, int act) {
-    if (act == MFR_ACT_SILU) {
-        return v / (1.0f + expf(-v));
-    }
-    return mfr::dev::activate(v, act);
-}
+__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
 // The copies into LDS have landed, and the LDS reads before have been done (a later copy may write there).
 __device__ __forceinline__ void wait_copies() {
@@ -71,46 +67,69 @@ __device__ __forceinline__ void bare_barrier() {
     asm volatile("" ::: "memory");
 }
 
-// 16 bytes from global memory to LDS, lane l's to `to` + 16 l (`to` is the wavefront's).
-__device__ __forceinline__ void copy16(const uint8_t* from, void* to) {
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(from),
-        (__attribute__((address_space(3))) void*)(to), 16, 0, 0);
+typedef int intx4 __attribute__((ext_vector_type(4)));
+
+// A buffer resource over `bytes` bytes from `base` on: loads past them give zeros.
+__device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
+    const uint64_t at = reinterpret_cast<uint64_t>(base);
+    intx4 r;
+    r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(at));
+    r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32) & 0xffff);
+    r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
+    r[3] = 0x00020000; // raw: 32-bit data format
+    return r;
 }
 
-__device__ __forceinline__ void copy4(const float* from, void* to) {
-    __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(from),
-        (__attribute__((address_space(3))) void*)(to), 4, 0, 0);
+// One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at `offset`
+// go to `to` + 16 l (4 l), `to` the wavefront's. In assembly, because the compiler waits for every
+// such copy that it knows of before any read of LDS once there are more than 8 in a kernel;
+// wait_copies() is what waits here. No register is written.
+template <int BYTES>
+__device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t offset, void* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(to)))));
+    if constexpr (BYTES == 16) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
+                     "v"(offset), "s"(from)
+                     : "memory");
+    } else {
+        static_assert(BYTES == 4, "4 or 16 bytes a lane");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at),
+                     "v"(offset), "s"(from)
+                     : "memory");
+    }
 }
 
 // A tile of BM x BN outputs (BN of each projection when GATED) by WM x WN wavefronts. Depth slices
 // of one block (128 bytes of a row) are copied to LDS in 16-byte pieces, piece c of row r at place
-// c ^ (r % 8), so that the 16 rows of a fragment lie in different banks; while one slice is
+// c ^ (r / 2 % 8), so that 16 rows of a fragment lie in different banks (64 of 4 bytes, two rows); while one slice is
 // multiplied the next is on its way.
 //
-// A wavefront keeps its columns' fragments of a slice in registers, as bf16, and takes its rows 16
-// at a time: 4 v_mfma_f32_16x16x32_bf16 give the block's inner sums of 16 x 16 outputs, which the
+// A wavefront keeps its columns' fragments of a slice in registers, as bf16, and takes its rows 32
+// at a time: 8 v_mfma_f32_32x32x16_bf16 give the block's inner sums of 32 x 32 outputs, which the
 // vector units add, times the two scales, to the outer sums. The weight is the instruction's first
-// operand: a lane then holds 4 neighbouring columns of one row of C. The 32 depths that a lane
-// gives to an instruction's 4 rounds are 32 neighbouring ones for both operands: which depth stands
-// where does not matter to a sum as long as it is the same for both.
+// operand: a lane then holds quads of neighbouring columns of one row of C. The 64 depths that a lane
+// gives to the 8 instructions are 64 neighbouring ones for both operands: which depth stands where
+// does not matter to a sum as long as it is the same for both.
 template <int BM, int BN, int WM, int WN, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Params p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     constexpr int kThreads = 64 * WM * WN;
     constexpr int kWeights = GATED ? 2 : 1;
-    constexpr int FM = BM / WM / 16;
-    constexpr int FN = BN / WN / 16; // of each projection
+    constexpr int FM = BM / WM / 32;
+    constexpr int FN = BN / WN / 32; // of each projection
     constexpr int kRowsB = BN * kWeights;
+    constexpr int kBlocksN = BN / kBlock;
     constexpr int kRowStep = kThreads / 8; // rows per round of copies
     constexpr int kCopiesA = BM / kRowStep;
     constexpr int kCopiesB = kRowsB / kRowStep;
-    static_assert(BM % kRowStep == 0 && BN % kRowStep == 0 && BM % 64 == 0, "whole rounds of copies");
+    static_assert(BM % kRowStep == 0 && BN % kRowStep == 0 && BM % 64 == 0 && BM <= kThreads,
+                  "whole rounds of copies");
     static_assert(kBlock % (BN / WN) == 0 && BN % kBlock == 0, "blocks of columns within a tile");
     struct Slice {
         uint4 a[BM * 8];
         uint4 b[kRowsB * 8];
         float scales[BM];
+        float scales_b[kWeights][64]; // of block columns
     };
     // Two objects, so that the compiler sees that the copy into one does not write the other.
     __shared__ __align__(16) Slice slice0;
@@ -120,8 +139,8 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Params p) {
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
     const int wm = wave % WM;
     const int wn = wave / WM;
-    const int r16 = lane % 16;
-    const int g = lane / 16;
+    const int r32 = lane % 32;
+    const int half = lane / 32;
 
     // Workgroup -> tile: consecutive logical indices on one XCD (the hardware sends workgroup i to
     // XCD i % 8), in groups of 8 tile-rows, rows fastest, whose operands that XCD's L2 keeps.
@@ -137,46 +156,63 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Params p) {
     const int64_t n0 = static_cast<int64_t>(in_group / rows_here) * BN;
 
     const int64_t depth_blocks = blocks_of(p.k);
-    const int64_t last_piece = (p.k + 15) / 16 - 1;
 
-    // This thread's rows of a slice; rows past the matrix repeat its last one (their sums are not
-    // stored). A row's pieces past its last one repeat that, and clear() removes them.
-    const int row_in_round = static_cast<int>(threadIdx.x) / 8;
-    const int64_t piece = (threadIdx.x % 8) ^ (row_in_round % 8);
-    const uint8_t* from_a[kCopiesA];
-    const uint8_t* from_b[kCopiesB];
-#pragma unroll
-    for (int i = 0; i < kCopiesA; ++i) {
-        from_a[i] = p.a.values + min(m0 + row_in_round + i * kRowStep, p.m - 1) * p.a.rs;
-    }
-#pragma unroll
-    for (int i = 0; i < kCopiesB; ++i) {
-        const Matrix& w = GATED && i * kRowStep >= BN ? p.up : p.b;
-        from_b[i] =
-            w.values + min(n0 + row_in_round + (i * kRowStep) % BN, p.n - 1) * w.rs;
-    }
-    const float* from_scales =
-        p.a.scales + min(m0 + (wave * 64 + lane) % BM, p.m - 1) * p.a.srs;
-
-    const auto copy = [&](Slice& to, int64_t kb) {
-        const int64_t offset = min(kb * 8 + piece, last_piece) * 16;
-#pragma unroll
-        for (int i = 0; i < kCopiesA; ++i) {
-            copy16(from_a[i] + offset, to.a + i * kThreads + wave * 64);
+    // Copies of a slice: 8 threads take a row's pieces, kRowStep rows a round. Each round has a
+    // resource of its own, made by the scalar unit: it begins at the round's first row and the
+    // slice's first depth and ends with the matrix, so that rows past it come as zeros. (A row's
+    // pieces past its end are the next row's; clear() removes them.)
+    const int64_t row_bytes = (p.k + 15) / 16 * 16;
+    const uint32_t thread_row = threadIdx.x / 8;
+    const uint32_t thread_piece = (threadIdx.x ^ (thread_row / 2)) % 8 * 16;
+    const uint32_t offset_a = thread_row * static_cast<uint32_t>(p.a.rs) + thread_piece;
+    const uint32_t offset_b = thread_row * static_cast<uint32_t>(p.b.rs) + thread_piece;
+    const uint32_t offset_up = thread_row * static_cast<uint32_t>(p.up.rs) + thread_piece;
+    constexpr int kRounds = kCopiesA + kCopiesB;
+    const auto copy = [&](Slice& to, int64_t kb, int x) __attribute__((always_inline)) {
+        const int i = x < kCopiesA ? x : x - kCopiesA;
+        const bool second = GATED && x >= kCopiesA && i * kRowStep >= BN;
+        const Matrix& from = x < kCopiesA ? p.a : second ? p.up : p.b;
+        const int64_t row = x < kCopiesA ? m0 + i * kRowStep : n0 + i * kRowStep % BN;
+        const int64_t rows = (x < kCopiesA ? p.m : p.n) - row;
+        int64_t bytes = (min(rows, static_cast<int64_t>(kRowStep)) - 1) * from.rs + row_bytes -
+                        kb * kBlock;
+        bytes = rows > 0 && kb < depth_blocks ? bytes : 0;
+        copy_to_lds<16>(resource(from.values + row * from.rs + kb * kBlock,
+                                 static_cast<uint32_t>(bytes)),
+                        x < kCopiesA ? offset_a : second ? offset_up : offset_b,
+                        (x < kCopiesA ? to.a : to.b) + i * kThreads + wave * 64);
+    };
+    // The scales: a wavefront each for 64 rows of A and for the block columns of a weight.
+    constexpr int kWaves = WM * WN;
+    static_assert(BM / 64 + kWeights <= kWaves, "a wavefront copies one run of scales at most");
+    const bool of_a = wave < BM / 64;
+    const bool of_b = wave >= kWaves - kWeights;
+    const Matrix& scaled = of_a ? p.a : GATED && wave == kWaves - 2 ? p.up : p.b;
+    const int64_t first_scale = of_a ? m0 + wave * 64 : n0 / kBlock;
+    const int64_t last_scale = (of_a ? p.m : blocks_of(p.n)) - 1 - first_scale;
+    const uint32_t scale_offset =
+        static_cast<uint32_t>(min(static_cast<int64_t>(of_a ? lane : lane % kBlocksN),
+                                  max(last_scale, static_cast<int64_t>(0)))) *
+        static_cast<uint32_t>(scaled.srs) * 4;
+    const auto copy_scales = [&](Slice& to, int64_t kb) __attribute__((always_inline)) {
+        if ((of_a && last_scale >= 0) || of_b) {
+            const float* from = scaled.scales + first_scale * scaled.srs + kb * scaled.scs;
+            copy_to_lds<4>(resource(from, 0xffffffffu), scale_offset,
+                           of_a ? to.scales + wave * 64 : to.scales_b[kWaves - 1 - wave]);
         }
+    };
+    const auto copy_all = [&](Slice& to, int64_t kb) __attribute__((always_inline)) {
+        copy_scales(to, kb);
 #pragma unroll
-        for (int i = 0; i < kCopiesB; ++i) {
-            copy16(from_b[i] + offset, to.b + i * kThreads + wave * 64);
-        }
-        if (wave * 64 < BM) {
-            copy4(from_scales + kb * p.a.scs, to.scales + wave * 64);
+        for (int x = 0; x < kRounds; ++x) {
+            copy(to, kb, x);
         }
     };
     // Zeros for the depths of the last slice that lie behind k.
-    const auto clear = [&](Slice& s) {
+    const auto clear = [&](Slice& s) __attribute__((always_inline)) {
         const int depths = static_cast<int>(p.k - (depth_blocks - 1) * kBlock);
         for (int i = static_cast<int>(threadIdx.x); i < (BM + kRowsB) * 8; i += kThreads) {
-            const int inside = depths - 16 * ((i % 8) ^ (i / 8 % 8));
+            const int inside = depths - 16 * ((i % 8) ^ (i / 16 % 8));
             uint4* const at = i < BM * 8 ? s.a + i : s.b + (i - BM * 8);
             if (inside <= 0) {
                 *at = make_uint4(0, 0, 0, 0);
@@ -190,82 +226,175 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Params p) {
         }
     };
 
-    floatx4 acc[kWeights][FM][FN] = {};
-    // One for the wavefront: its columns lie within a block.
-    const int64_t col_block = min(n0 + wn * (BN / WN), p.n - 1) / kBlock;
-    const float* scale_b[2] = {p.b.scales + col_block * p.b.srs, p.up.scales + col_block * p.up.srs};
+    // The wavefront's blocks of 32 x 32 outputs: FM block rows, and NJ block columns over the weights.
+    constexpr int NJ = kWeights * FN;
+    constexpr int kChains = FM * NJ;
+    static_assert(kChains % 2 == 0 && NJ <= 2 && FM >= 2, "chains alternate between two results");
+    floatx16 acc[kWeights][FM][FN] = {};
+    const int row_a = wm * (BM / WM) + r32;
+    const int row_b = wn * (BN / WN) + r32;
+    // Piece q of four of a row of A's or B's block i or j, of the half of the depths that is this
+    // lane's.
+    const auto piece_a = [&](const Slice& s, int i, int q) __attribute__((always_inline)) {
+        return s.a[(row_a + 32 * i) * 8 + ((4 * half + q) ^ (r32 / 2 % 8))];
+    };
+    const auto piece_b = [&](const Slice& s, int j, int q) __attribute__((always_inline)) {
+        return s.b[(j / FN * BN + row_b + 32 * (j % FN)) * 8 + ((4 * half + q) ^ (r32 / 2 % 8))];
+    };
+    bf16x8 fa[8];
+    bf16x8 fb[NJ][8];
+    uint4 raw_a[4];
+    uint4 raw_b[4];
+    const auto widen_a = [&](int q) __attribute__((always_inline)) {
+        fa[2 * q] = widen(raw_a[q].x, raw_a[q].y);
+        fa[2 * q + 1] = widen(raw_a[q].z, raw_a[q].w);
+        asm volatile("" : "+v"(fa[2 * q]), "+v"(fa[2 * q + 1])); // here, not where it is used
+    };
+    const auto widen_b = [&](int j, int q) __attribute__((always_inline)) {
+        fb[j][2 * q] = widen(raw_b[q].x, raw_b[q].y);
+        fb[j][2 * q + 1] = widen(raw_b[q].z, raw_b[q].w);
+        asm volatile("" : "+v"(fb[j][2 * q]), "+v"(fb[j][2 * q + 1]));
+    };
+    floatx16 part[2] = {};
+    float part_scale = 0.0f; // of the last chain's result
 
-    const auto multiply = [&](const Slice& s, int64_t kb) {
+    // A slice: chains of 8 instructions, one chain per block. Between the instructions of a chain
+    // stands what other chains need, so that the vector units work while the matrix cores do: the
+    // multiply-adds of the chain before, the loads and the widening of fragments that follow, each
+    // into the registers of one that has been used for the last time. Before the last block row,
+    // when everything of this slice is in registers, the workgroup meets: the next slice has
+    // landed, and the one after it may be copied over this one.
+    constexpr int kPace = 8 * NJ / kRounds;
+    static_assert(kPace >= 1, "the copies of a slice stand in the last block row");
+    const auto step = [&](Slice& here, Slice& next, int64_t kb) __attribute__((always_inline)) {
         float sb[kWeights];
-        sb[0] = scale_b[0][kb * p.b.scs];
-        if constexpr (GATED) {
-            sb[1] = scale_b[1][kb * p.up.scs];
-        }
-        const auto piece_at = [&](const uint4* tile, int row, int half) {
-            return tile[row * 8 + ((2 * g + half) ^ (row % 8))];
-        };
-        bf16x8 fb[kWeights][FN][4];
 #pragma unroll
         for (int w = 0; w < kWeights; ++w) {
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint4 v =
-                        piece_at(s.b, w * BN + wn * (BN / WN) + 16 * j + r16, half);
-                    fb[w][j][2 * half] = widen(v.x, v.y);
-                    fb[w][j][2 * half + 1] = widen(v.z, v.w);
-                }
-            }
+            sb[w] = here.scales_b[w][wn * (BN / WN) / kBlock];
         }
+        float sa[FM];
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            const int row = wm * (BM / WM) + 16 * i + r16;
-            floatx4 part[kWeights][FN] = {};
+            sa[i] = here.scales[row_a + 32 * i];
+        }
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint4 v = piece_at(s.a, row, half);
-                const bf16x8 fa[2] = {widen(v.x, v.y), widen(v.z, v.w)};
+        for (int c = 0; c < kChains; ++c) {
+            const int i = c / NJ;
+            const int j = c % NJ;
+            const bool last_row = i == FM - 1;
+            if (last_row && j == 0) {
+                wait_copies();
+                bare_barrier();
+                if (kb + 2 == depth_blocks && p.k % kBlock != 0) {
+                    clear(next);
+                    __syncthreads();
+                }
+                if (kb + 2 < depth_blocks) {
+                    copy_scales(here, kb + 2);
+                }
+            }
+            floatx16& now = part[c % 2];
+            floatx16& before = part[(c + 1) % 2];
+            floatx16& sums =
+                c > 0 ? acc[(c - 1) % NJ / FN][(c - 1) / NJ][(c - 1) % NJ % FN]
+                      : acc[(NJ - 1) / FN][FM - 1][(NJ - 1) % FN];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 8; ++t) {
+                const floatx16 zero = {};
+                now = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[j][t], fa[t], t == 0 ? zero : now,
+                                                              0, 0, 0);
+                // The chain before has ended by the third instruction.
 #pragma unroll
-                    for (int w = 0; w < kWeights; ++w) {
-#pragma unroll
-                        for (int j = 0; j < FN; ++j) {
-                            part[w][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                fb[w][j][2 * half + t], fa[t], part[w][j], 0, 0, 0);
+                for (int e = t == 6 ? 8 : 2 * t - 4; e < (t % 2 != 0 || t == 0 ? 0 : t == 6 ? 16 : 2 * t); ++e) {
+                    sums[e] = fmaf(before[e], part_scale, sums[e]);
+                }
+                if constexpr (NJ == 2) {
+                    // Loads stand five instructions before their use.
+                    if (j == 0 && t >= 4 && t % 2 == 0) {
+                        if (last_row) {
+                            raw_b[t / 2 - 2] = piece_b(next, 0, t / 2 - 2);
+                        }
+                        raw_a[t / 2 - 2] = last_row ? piece_a(next, 0, t / 2 - 2)
+                                                    : piece_a(here, i + 1, t / 2 - 2);
+                    }
+                    if (j == 1) {
+                        if (t % 2 == 1) {
+                            if (last_row) {
+                                widen_b(0, t / 2);
+                            }
+                            widen_a(t / 2);
+                            if (t / 2 < 2) {
+                                raw_a[t / 2 + 2] = last_row ? piece_a(next, 0, t / 2 + 2)
+                                                            : piece_a(here, i + 1, t / 2 + 2);
+                                if (last_row) {
+                                    raw_b[t / 2 + 2] = piece_b(next, 0, t / 2 + 2);
+                                }
+                            } else if (last_row) {
+                                raw_b[t / 2 - 2] = piece_b(next, 1, t / 2 - 2);
+                            }
+                        }
+                    }
+                    if (c == 0 && t % 2 == 1) {
+                        widen_b(1, t / 2);
+                        if (t / 2 < 2) {
+                            raw_b[t / 2 + 2] = piece_b(here, 1, t / 2 + 2);
+                        }
+                    }
+                } else {
+                    // The next fragments replace this chain's behind its second half.
+                    if (t < 4) {
+                        raw_a[t] = last_row ? piece_a(next, 0, t) : piece_a(here, i + 1, t);
+                        if (last_row) {
+                            raw_b[t] = piece_b(next, 0, t);
                         }
                     }
                 }
+                // The copies one by one: a wavefront that hands over several waits for their addresses
+                // to be taken. (None is left behind the last slice: empty resources.)
+                if (last_row && (j * 8 + t) % kPace == 0 && (j * 8 + t) / kPace < kRounds) {
+                    copy(here, kb + 2, (j * 8 + t) / kPace);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            const float sa = s.scales[row];
+            if constexpr (NJ == 1) {
 #pragma unroll
-            for (int w = 0; w < kWeights; ++w) {
-                const float scale = sa * sb[w];
-#pragma unroll
-                for (int j = 0; j < FN; ++j) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        acc[w][i][j][e] = fmaf(part[w][j][e], scale, acc[w][i][j][e]);
+                for (int q = 0; q < 4; ++q) {
+                    widen_a(q);
+                    if (last_row) {
+                        widen_b(0, q);
                     }
                 }
             }
+            asm volatile("" : "+v"(sums));
+            part_scale = sa[i] * sb[j / FN];
         }
-    };
-    const auto step = [&](Slice& here, Slice& next, int64_t kb) {
-        wait_copies();
-        bare_barrier(); // everyone's copies have landed, and `next` has been read
-        if (kb + 1 < depth_blocks) {
-            copy(next, kb + 1);
-        } else if (p.k % kBlock != 0) {
-            clear(here);
-            __syncthreads();
-        }
-        multiply(here, kb);
     };
 
     if (depth_blocks > 0) {
-        copy(slice0, 0);
+        copy_all(slice0, 0);
+        wait_copies();
+        bare_barrier();
+        if (depth_blocks == 1 && p.k % kBlock != 0) {
+            clear(slice0);
+            __syncthreads();
+        }
+        if (depth_blocks > 1) {
+            copy_all(slice1, 1);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            raw_a[q] = piece_a(slice0, 0, q);
+            widen_a(q);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            raw_b[q] = piece_b(slice0, 0, q);
+            widen_b(0, q);
+        }
+        if constexpr (NJ == 2) {
+            raw_b[0] = piece_b(slice0, 1, 0);
+            raw_b[1] = piece_b(slice0, 1, 1);
+        }
     }
     for (int64_t kb = 0; kb < depth_blocks; kb += 2) {
         step(slice0, slice1, kb);
@@ -273,83 +402,160 @@ __global__ __launch_bounds__(64 * WM * WN) void tile_kernel(Params p) {
             step(slice1, slice0, kb + 1);
         }
     }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+        floatx16& sums = acc[(NJ - 1) / FN][FM - 1][(NJ - 1) % FN];
+        sums[e] = fmaf(part[1][e], part_scale, sums[e]);
+    }
 
-    // The epilogue. Element e of block (i, j) is row 16 i + r16, column 16 j + 4 g + e.
+    wait_copies(); // the epilogue uses the slices' memory
+
+    // The epilogue. Element e of block (i, j) is row 32 i + r32, column 32 j + 8 (e / 4) + 4 half +
+    // e % 4: four neighbouring columns a quad.
     namespace dev = f8::dev;
+    const int64_t row0 = m0 + wm * (BM / WM) + r32;
+    const int64_t col0 = n0 + wn * (BN / WN) + 4 * half;
+    // Whether the tile lies inside the matrix: no test per quad then.
+    const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;
+    if constexpr (!GATED) {
+        if (p.c0 != nullptr) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                const float* line = p.c0 + (row0 + 32 * i) * p.c0_rs + col0;
+                const int64_t left = row0 + 32 * i < p.m ? p.n - col0 : 0;
+#pragma unroll
+                for (int x = 0; x < 4 * FN; ++x) {
+                    const float4 c0 = whole ? mfr::dev::load_loose(line + 8 * x)
+                                            : dev::load_quad(line + 8 * x, left - 8 * x);
+                    floatx16& v = acc[0][i][x / 4];
+                    const int e = x % 4 * 4;
+                    v[e] += p.beta * c0.x, v[e + 1] += p.beta * c0.y;
+                    v[e + 2] += p.beta * c0.z, v[e + 3] += p.beta * c0.w;
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int x = 0; x < 4 * FN; ++x) {
+                const float4 bias = dev::load_quad(p.bias + col0 + 8 * x, p.n - col0 - 8 * x);
+                const int e = x % 4 * 4;
+#pragma unroll
+                for (int i = 0; i < FM; ++i) {
+                    floatx16& v = acc[0][i][x / 4];
+                    v[e] += bias.x, v[e + 1] += bias.y, v[e + 2] += bias.z, v[e + 3] += bias.w;
+                }
+            }
+        }
+    }
+    if (p.act == MFR_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+#pragma unroll
+            for (int x = 0; x < 16 * FN; ++x) {
+                float v = acc[0][i][x / 16][x % 16];
+                acc[0][i][x / 16][x % 16] = silu(v);
+                if (x % 4 == 3) {
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+    } else if (p.act != MFR_ACT_NONE) {
+        // The gelus, in double, are too long to be laid out for every element: a lane's elements
+        // pass through LDS, a block at a time, and a loop takes them one by one.
+        __syncthreads(); // the slices have been read
+        float* const mine = reinterpret_cast<float*>(&slice0) + wave * 16 * 64 + lane;
+        static_assert(sizeof(Slice) >= sizeof(float) * 64 * 16 * WM * WN, "a block fits");
+#pragma unroll
+        for (int b = 0; b < FM * FN; ++b) {
+            floatx16& v = acc[0][b / FN][b % FN];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                mine[64 * e] = v[e];
+            }
+#pragma nounroll
+            for (int e = 0; e < 16; ++e) {
+                mine[64 * e] = mfr::dev::gelu(mine[64 * e], p.act);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                v[e] = mine[64 * e];
+            }
+        }
+    }
     uint32_t top[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int64_t row = m0 + wm * (BM / WM) + 16 * i + r16;
         top[i] = 0;
+        float* const line = p.c + (row0 + 32 * i) * p.c_rs + col0;
+        const int64_t left = row0 + 32 * i < p.m ? p.n - col0 : 0;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t col = n0 + wn * (BN / WN) + 16 * j + 4 * g;
-            floatx4 v = acc[0][i][j];
-            const int64_t count = row < p.m ? p.n - col : 0;
-            if (!GATED && p.c0 != nullptr) {
-                const float4 c0 = dev::load_quad(p.c0 + row * p.c0_rs + col, count);
-                v[0] += p.beta * c0.x, v[1] += p.beta * c0.y;
-                v[2] += p.beta * c0.z, v[3] += p.beta * c0.w;
-            }
-            if (!GATED && p.bias != nullptr) {
-                const float4 bias = dev::load_quad(p.bias + col, p.n - col);
-                v[0] += bias.x, v[1] += bias.y, v[2] += bias.z, v[3] += bias.w;
-            }
+        for (int x = 0; x < 4 * FN; ++x) {
+            floatx16& v = acc[0][i][x / 4];
+            const int e = x % 4 * 4;
+            if constexpr (GATED) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = activate(v[e], p.act);
-                if constexpr (GATED) {
-                    v[e] = v[e] * acc[1][i][j][e];
+                for (int y = e; y < e + 4; ++y) {
+                    v[y] = v[y] * acc[1][i][x / 4][y];
                 }
-                v[e] = e < count ? v[e] : 0.0f;
             }
-            acc[0][i][j] = v;
-            const float4 y = make_float4(v[0], v[1], v[2], v[3]);
-            top[i] = max(top[i], dev::magnitude(y));
+            if (!whole) {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) { // what counts for nothing in the block's scale
+                    v[e + y] = y < left - 8 * x ? v[e + y] : 0.0f;
+                }
+            }
+            const float4 quad = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
             if (p.c != nullptr) {
-                dev::store_quad(p.c + row * p.c_rs + col, y, count);
+                if (whole) {
+                    mfr::dev::store_loose(line + 8 * x, quad);
+                } else {
+                    dev::store_quad(line + 8 * x, quad, left - 8 * x);
+                }
             }
+            top[i] = max(top[i], dev::magnitude(quad));
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     if (p.q.values == nullptr) {
         return;
     }
-    // The largest magnitude of a row's 128 columns: over the lanes of a row, then over the
+    // The largest magnitude of a row's 128 columns: over the two lanes of a row, then over the
     // wavefronts that share the block.
     uint32_t(&tops)[WN][BM] = *reinterpret_cast<uint32_t(*)[WN][BM]>(&slice0);
     __syncthreads(); // the slices have been read
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        top[i] = max(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 16, 64)));
         top[i] = max(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 32, 64)));
-        if (g == 0) {
-            tops[wn][wm * (BM / WM) + 16 * i + r16] = top[i];
+        if (half == 0) {
+            tops[wn][wm * (BM / WM) + 32 * i + r32] = top[i];
         }
     }
     __syncthreads();
     constexpr int kSharing = kBlock / (BN / WN);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        const int in_tile = wm * (BM / WM) + 16 * i + r16;
-        const int64_t row = m0 + in_tile;
+        const int64_t row = row0 + 32 * i;
 #pragma unroll
         for (int w = 0; w < kSharing; ++w) {
-            top[i] = max(top[i], tops[wn / kSharing * kSharing + w][in_tile]);
+            top[i] = max(top[i],
+                         tops[wn / kSharing * kSharing + w][wm * (BM / WM) + 32 * i + r32]);
         }
         const float scale = dev::scale_of(top[i]);
+        const float inverse = 1.0f / scale;
         const int64_t first = n0 + wn / kSharing * kSharing * (BN / WN);
-        if (row < p.m && first < p.n && wn % kSharing == 0 && g == 0) {
+        if (row < p.m && first < p.n && wn % kSharing == 0 && half == 0) {
             p.q.scales[row * p.q.srs + first / kBlock * p.q.scs] = scale;
         }
+        uint8_t* const line = p.q.values + row * p.q.rs + col0;
+        const int64_t left = row < p.m ? p.n - col0 : 0;
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int64_t col = n0 + wn * (BN / WN) + 16 * j + 4 * g;
-            const floatx4 v = acc[0][i][j];
-            if (row < p.m && col < p.n) {
-                dev::store_bytes(p.q.values + row * p.q.rs + col,
-                                 dev::pack(make_float4(v[0], v[1], v[2], v[3]), 1.0f / scale),
-                                 p.n - col);
-            }
+        for (int x = 0; x < 4 * FN; ++x) {
+            const floatx16 v = acc[0][i][x / 4];
+            const int e = x % 4 * 4;
+            dev::store_bytes(line + 8 * x,
+                             dev::pack(make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]), inverse),
+                             left - 8 * x);
         }
     }
 }

@@ -253,7 +253,7 @@ GEMM_SIZES = [(1, 1, 1), (1, 128, 128), (1, 300, 1000), (2, 3, 17), (3, 130, 15)
               (9, 129, 129), (16, 257, 127), (17, 64, 300), (31, 500, 640), (32, 128, 2049),
               (33, 127, 128), (48, 200, 513), (64, 384, 384), (65, 129, 143), (100, 40, 1030),
               (127, 255, 260), (128, 256, 512), (129, 257, 385), (200, 1100, 130), (257, 513, 700),
-              (520, 260, 255), (1000, 30, 64)]
+              (520, 260, 255), (1000, 30, 64), (2100, 2200, 300), (2049, 2305, 129)]
 
 
 @pytest.mark.parametrize("m,n,k", GEMM_SIZES)
@@ -488,7 +488,7 @@ def test_the_other_entry_points_refuse_the_silu(stream):
 def test_offsets_past_32_bits(stream):
     """Rows that lie more than 4 GiB apart in all: the last rows' values and scales are found."""
     rng = np.random.default_rng(14)
-    m, n, k, pitch = 70, 129, 200, 1 << 26  # 70 rows of 64 MiB: 4.4 GiB
+    m, n, k, pitch = 140, 129, 200, 1 << 25  # 140 rows of 32 MiB: 4.4 GiB
     a, sa = exact_operands(rng, m, k, 1)
     b, sb = exact_operands(rng, n, k, 128)
     far = mf.DeviceArray.empty((m, pitch), stream, np.uint8)
