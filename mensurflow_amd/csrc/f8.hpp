@@ -66,6 +66,10 @@ inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int bl
     return m;
 }
 
+// x in 8 bits, a scale per row and 128 columns (mfr_f8_quantize's launch).
+void quantize_rows(const mfr_stream& s, const float* x, int64_t x_rs, int64_t rows, int64_t cols,
+                   const Matrix& q);
+
 } // namespace mfr::f8
 
 namespace mfr::f8::dev {
@@ -99,6 +103,27 @@ __device__ inline void store_bytes(uint8_t* p, uint32_t w, int64_t count) {
     }
     for (int64_t e = 0; e < count; ++e) {
         p[e] = static_cast<uint8_t>(w >> (8 * e));
+    }
+}
+
+// The largest of v over the 32 lanes of a half wavefront, in each of them.
+__device__ inline uint32_t half_max(uint32_t v) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
+    }
+    return v;
+}
+
+// Four columns from `col` on of row r, in 8 bits. 32 lanes hold a block: columns past the row are
+// zeros and count for nothing.
+__device__ inline void write_f8(const Matrix& q, int64_t r, int64_t col, int64_t cols, float4 v) {
+    const float scale = scale_of(half_max(magnitude(v)));
+    if (col < cols) {
+        store_bytes(q.values + r * q.rs + col, pack(v, 1.0f / scale), cols - col);
+        if (col % kBlock == 0) {
+            q.scales[r * q.srs + col / kBlock * q.scs] = scale;
+        }
     }
 }
 

@@ -14,35 +14,14 @@ namespace dev = mfr::f8::dev;
 constexpr int kThreads = 256;
 constexpr int kStep = 4 * kThreads; // columns per workgroup step
 
-// The largest of v over the 32 lanes of a half wavefront, in each of them.
-__device__ inline uint32_t half_max(uint32_t v) {
-#pragma unroll
-    for (int m = 16; m > 0; m >>= 1) {
-        v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, kWave)));
-    }
-    return v;
-}
-
-// Four columns from `col` on of row r, in 8 bits. 32 lanes hold a block: columns past the row are
-// zeros and count for nothing.
-__device__ inline void write_f8(const Matrix& q, int64_t r, int64_t col, int64_t cols, float4 v) {
-    const float scale = dev::scale_of(half_max(dev::magnitude(v)));
-    if (col < cols) {
-        dev::store_bytes(q.values + r * q.rs + col, dev::pack(v, 1.0f / scale), cols - col);
-        if (col % kBlock == 0) {
-            q.scales[r * q.srs + col / kBlock * q.scs] = scale;
-        }
-    }
-}
-
+// A workgroup takes 1024 columns of a row at a time, a thread 4, 32 lanes a block.
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const float* x, int64_t x_rs,
-                                                                 int64_t rows, int64_t cols,
-                                                                 Matrix q) {
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-        for (int64_t c0 = 0; c0 < cols; c0 += kStep) {
-            const int64_t col = c0 + 4 * threadIdx.x;
-            write_f8(q, r, col, cols, dev::load_quad(x + r * x_rs + col, cols - col));
-        }
+                                                                 int64_t groups, int64_t cols,
+                                                                 uint32_t col_groups, Matrix q) {
+    for (int64_t i = blockIdx.x; i < groups; i += gridDim.x) {
+        const int64_t r = i / col_groups;
+        const int64_t col = (i - r * col_groups) * kStep + 4 * threadIdx.x;
+        dev::write_f8(q, r, col, cols, dev::load_quad(x + r * x_rs + col, cols - col));
     }
 }
 
@@ -63,7 +42,7 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(const float* 
         v[i] = dev::load_quad(x + r * x_rs + col, r < rows ? cols - col : 0);
         top = max(top, dev::magnitude(v[i]));
     }
-    tops[threadIdx.x / 32] = half_max(top); // the 32 lanes store one value
+    tops[threadIdx.x / 32] = dev::half_max(top); // the 32 lanes store one value
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) {
@@ -171,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void rms_norm_kernel(NormParams p) {
                 dev::store_quad(p.out + r * p.out_rs + col, y, p.cols - col);
             }
             if (p.q.values != nullptr) {
-                write_f8(p.q, r, col, p.cols, y);
+                dev::write_f8(p.q, r, col, p.cols, y);
             }
         }
     }
@@ -212,6 +191,21 @@ NormParams checked(const mfr_rms_norm_desc* desc) {
 
 } // namespace
 
+namespace mfr::f8 {
+
+void quantize_rows(const mfr_stream& s, const float* x, int64_t x_rs, int64_t rows, int64_t cols,
+                   const Matrix& q) {
+    const int64_t col_groups = (cols + kStep - 1) / kStep;
+    require(col_groups < (int64_t{1} << 32) && rows < (int64_t{1} << 62) / col_groups,
+            "f8_quantize: matrix too large");
+    const int64_t groups = rows * col_groups;
+    quantize_rows_kernel<<<grid_blocks(groups, 1, int64_t{1} << 20), kThreads, 0, s.stream>>>(
+        x, x_rs, groups, cols, static_cast<uint32_t>(col_groups), q);
+    check_launch("quantize_rows_kernel");
+}
+
+} // namespace mfr::f8
+
 extern "C" {
 
 int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float* x, int64_t x_rs,
@@ -231,8 +225,8 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
             return;
         }
         if (out->block_rows == 1) {
-            quantize_rows_kernel<<<mfr::grid_blocks(rows, 1, int64_t{1} << 20), kThreads, 0,
-                                   s.stream>>>(x, x_rs, rows, cols, q);
+            mfr::f8::quantize_rows(s, x, x_rs, rows, cols, q);
+            return;
         } else {
             const int64_t col_blocks = mfr::f8::blocks_of(cols);
             const int64_t blocks = mfr::f8::blocks_of(rows) * col_blocks;

@@ -1,8 +1,14 @@
-// mfr_f8gemm: checks, and the choice of a tile (f8gemm_kernel.hpp).
-#include "f8gemm_kernel.hpp"
+// mfr_f8gemm: checks, and the choice between the tiles (f8gemm_kernel.hpp), the depth in ranges
+// (f8gemm_finish.hpp) and the form for few rows (f8gemm_few.hpp).
+#include "f8gemm_few.hpp"
+#include "f8gemm_finish.hpp"
+
+#include <algorithm>
+#include <limits>
 
 namespace {
 
+using mfr::f8::blocks_of;
 using mfr::f8gemm::Params;
 
 // The descriptor's checks (of shapes, layouts and pointers: no device is needed).
@@ -43,23 +49,198 @@ Params checked(const mfr_f8gemm_desc* desc) {
     return p;
 }
 
-int64_t tiles(const Params& p, int64_t bm, int64_t bn) {
-    return ((p.m + bm - 1) / bm) * ((p.n + bn - 1) / bn);
+// ---- which form ---------------------------------------------------------------------------------
+//
+// The times of a call in microseconds, by what was measured on an MI355X (256 CUs) over m = 1 ..
+// 8192, n = 1024 .. 16384 and k = 1024 .. 8192: a fixed part, and one per block of the depth that a
+// workgroup or wavefront walks, by how many workgroups a CU has. The least of them is taken.
+
+enum class Form { kFew16, kFew32, kFew32Wide, kFew64, kTile64, kTile128 };
+
+// A workgroup's rows and columns, the wavefronts that share the depth, and a wavefront's time per
+// block with one workgroup per CU. Measured, k = 4096 (32 blocks): 16 x 4096 5.8 us and 16 x 16384
+// 18.7; 32 x 4096 8.7; 32 x 16384 18.4 wide (28.5 narrow); 128 x 4096 15.5 in the last form. Gated:
+// 1 x 10240 17.6, 32 x 4096 11.5, 64 x 4096 16.6.
+struct Few {
+    Form form;
+    int64_t rows, cols, waves;
+    double block;
+};
+constexpr double kFewFixed = 2.6;
+constexpr Few kFew[] = {{Form::kFew16, 16, 16, 8, 1.0},
+                        {Form::kFew32, 32, 16, 8, 1.45},
+                        {Form::kFew32Wide, 32, 32, 4, 1.0},
+                        {Form::kFew64, 64, 32, 8, 3.15}};
+constexpr Few kFewGated[] = {{Form::kFew16, 16, 16, 8, 1.5},
+                             {Form::kFew32, 32, 16, 8, 2.3},
+                             {Form::kFew64, 64, 16, 4, 1.7}};
+
+// A tile's workgroups per CU at once, its fixed time, and the time of a block when every CU has
+// them all, or one alone on few CUs. Measured, k = 4096: 64 x 128 25.4 us on 32 CUs, 41.5 with two on
+// each; 128 x 128 37.5 and 67.9 (8192^3 920); gated 46.2 and 97 for two in turn; 52 and 66 (8192 x
+// 10240 x 4096 1160).
+struct Tile {
+    Form form;
+    int64_t rows, at_once;
+    double fixed, full, alone;
+};
+constexpr Tile kTiles[] = {{Form::kTile64, 64, 2, 5.2, 1.2, 0.65},
+                           {Form::kTile128, 128, 2, 6.0, 2.0, 1.0}};
+constexpr Tile kTilesGated[] = {{Form::kTile64, 64, 1, 7.0, 1.4, 1.22},
+                                {Form::kTile128, 128, 1, 8.0, 1.8, 1.38}};
+constexpr int64_t kTileCols = 128;
+
+// The second launch of a depth in ranges and the memory it reads; the second launch of few rows
+// with an 8-bit output.
+constexpr double kFinishFixed = 3.0;
+constexpr double kFinishBytesPerUs = 4e6;
+constexpr double kConvertFixed = 2.6;
+constexpr int64_t kMostPartialBytes = int64_t{256} << 20;
+
+struct Plan {
+    Form form = Form::kTile64;
+    int64_t splits = 1;
+    double time = std::numeric_limits<double>::infinity();
+    int64_t workspace = 0; // bytes
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+Plan choose(const Params& p, int64_t cus, bool workspace) {
+    const bool gated = p.up.values != nullptr;
+    const int64_t blocks = blocks_of(p.k);
+    Plan best;
+    const auto offer = [&](Form form, int64_t splits, double time, int64_t bytes) {
+        if (time < best.time && (bytes == 0 || (workspace && bytes <= kMostPartialBytes))) {
+            best = {form, splits, time, bytes};
+        }
+    };
+    const auto few = [&](const Few& f) {
+        const double groups =
+            static_cast<double>(ceil_div(p.m, f.rows)) * static_cast<double>(ceil_div(p.n, f.cols));
+        double time = kFewFixed + static_cast<double>(ceil_div(blocks, f.waves)) * f.block *
+                                      std::max(1.0, groups / static_cast<double>(cus));
+        int64_t bytes = 0;
+        if (p.q.values != nullptr) {
+            time += kConvertFixed;
+            bytes = p.c != nullptr ? 0 : 4 * p.m * p.n;
+        }
+        if (ceil_div(p.m, f.rows) < 65536) {
+            offer(f.form, 1, time, bytes);
+        }
+    };
+    const auto tiles = [&](const Tile& t) {
+        for (int64_t splits = 1; splits <= 8 && splits <= std::max(blocks, int64_t{1}); splits *= 2) {
+            const int64_t groups = ceil_div(p.m, t.rows) * ceil_div(p.n, kTileCols) * splits;
+            const int64_t slots = cus * t.at_once;
+            const int64_t rest = groups % slots;
+            // One workgroup on a CU takes `alone`; the second of a pair, or the CUs' rivalry when
+            // all are busy, brings that to `full`.
+            const double part =
+                rest == 0 ? 0.0
+                          : std::max(t.alone, t.full * static_cast<double>(rest) /
+                                                  static_cast<double>(slots));
+            double time = t.fixed + static_cast<double>(ceil_div(blocks, splits)) *
+                                        (static_cast<double>(groups / slots) * t.full + part);
+            int64_t bytes = 0;
+            if (splits > 1) {
+                bytes = splits * (gated ? 2 : 1) * 4 * p.m * p.n;
+                time += kFinishFixed + 2.0 * static_cast<double>(bytes) / kFinishBytesPerUs;
+            }
+            offer(t.form, splits, time, bytes);
+        }
+    };
+    if (gated) {
+        for (const Few& f : kFewGated) {
+            few(f);
+        }
+        for (const Tile& t : kTilesGated) {
+            tiles(t);
+        }
+    } else {
+        for (const Few& f : kFew) {
+            few(f);
+        }
+        for (const Tile& t : kTiles) {
+            tiles(t);
+        }
+    }
+    return best;
 }
 
-void run(const mfr_stream& s, const Params& p) {
-    // The small tile where the large one leaves compute units without a tile.
-    const bool large = tiles(p, 128, 128) >= s.compute_units;
-    if (p.up.values != nullptr) {
-        if (large) {
-            mfr::f8gemm::launch_gated<128, 128, 2, 4>(s, p);
-        } else {
-            mfr::f8gemm::launch_gated<64, 128, 1, 4>(s, p);
+void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
+    using namespace mfr::f8gemm;
+    const bool gated = p.up.values != nullptr;
+    switch (plan.form) {
+    case Form::kFew16:
+        gated ? launch_few<1, 1, 8, 2, true>(s, p) : launch_few<1, 1, 8, 2, false>(s, p);
+        break;
+    case Form::kFew32:
+        gated ? launch_few<2, 1, 8, 1, true>(s, p) : launch_few<2, 1, 8, 2, false>(s, p);
+        break;
+    case Form::kFew32Wide:
+        launch_few<2, 2, 4, 2, false>(s, p);
+        break;
+    case Form::kFew64:
+        gated ? launch_few<4, 1, 4, 1, true>(s, p) : launch_few<4, 2, 8, 1, false>(s, p);
+        break;
+    case Form::kTile64:
+        gated ? launch_tiles<64, 128, 1, 4, true>(s, p, plan.splits)
+              : launch_tiles<64, 128, 1, 4, false>(s, p, plan.splits);
+        break;
+    case Form::kTile128:
+        gated ? launch_tiles<128, 128, 2, 4, true>(s, p, plan.splits)
+              : launch_tiles<128, 128, 2, 2, false>(s, p, plan.splits);
+        break;
+    }
+}
+
+bool is_few(Form f) { return f != Form::kTile64 && f != Form::kTile128; }
+
+void run(mfr_stream& s, Params p) {
+    Plan plan = choose(p, s.compute_units, true);
+    std::unique_lock<std::mutex> hold(s.workspace_mutex, std::defer_lock);
+    void* memory = nullptr;
+    if (plan.workspace > 0) {
+        // Held until all kernels are queued: another thread's reserve() may not free the memory.
+        // Under stream capture none is used: a graph would keep its address, which a later call may
+        // free to grow it, and its replays may run beside calls that use it. (The default stream
+        // cannot be asked while another captures: none then, too.)
+        hold.lock();
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s.stream, &capture) != hipSuccess) {
+            (void)hipGetLastError();
+        } else if (capture == hipStreamCaptureStatusNone) {
+            try {
+                memory = s.reserve(static_cast<size_t>(plan.workspace));
+            } catch (const mfr::Error&) {
+                (void)hipGetLastError();
+            }
         }
-    } else if (large) {
-        mfr::f8gemm::launch<128, 128, 2, 2>(s, p);
-    } else {
-        mfr::f8gemm::launch<64, 128, 1, 4>(s, p);
+        if (memory == nullptr) {
+            plan = choose(p, s.compute_units, false);
+        }
+    }
+    if (is_few(plan.form)) {
+        Params sums = p;
+        if (p.c == nullptr) {
+            sums.c = static_cast<float*>(memory);
+            sums.c_rs = p.n;
+        }
+        launch(s, plan, sums);
+        if (p.q.values != nullptr) {
+            mfr::f8::quantize_rows(s, sums.c, sums.c_rs, p.m, p.n, p.q);
+        }
+        return;
+    }
+    p.split_blocks = ceil_div(blocks_of(p.k), plan.splits);
+    if (plan.splits > 1) {
+        p.partial = static_cast<float*>(memory);
+        plan.splits = ceil_div(blocks_of(p.k), p.split_blocks); // none of them empty
+    }
+    launch(s, plan, p);
+    if (p.partial != nullptr) {
+        mfr::f8gemm::launch_finish(s, p, plan.splits);
     }
 }
 

@@ -28,6 +28,11 @@ struct Params {
     float beta;
     int act;
     uint32_t tiles_m, tiles_n;
+    // Where sums are left for finish_kernel (null: the kernel writes the outputs itself): those of
+    // split s and weight w at partial + (s kWeights + w) m n, rows n floats apart. A split is
+    // split_blocks blocks of the depth.
+    float* partial;
+    int64_t split_blocks;
 };
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -155,7 +160,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const int64_t m0 = static_cast<int64_t>(group * group_rows + in_group % rows_here) * BM;
     const int64_t n0 = static_cast<int64_t>(in_group / rows_here) * BN;
 
-    const int64_t depth_blocks = blocks_of(p.k);
+    // This workgroup's blocks of the depth: [first_block, end_block).
+    const int64_t first_block = blockIdx.y * p.split_blocks;
+    const int64_t end_block = min(first_block + p.split_blocks, blocks_of(p.k));
+    const bool ragged = p.k % kBlock != 0 && end_block == blocks_of(p.k);
 
     // Copies of a slice: 8 threads take a row's pieces, kRowStep rows a round. Each round has a
     // resource of its own, made by the scalar unit: it begins at the round's first row and the
@@ -176,7 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         const int64_t rows = (x < kCopiesA ? p.m : p.n) - row;
         int64_t bytes = (min(rows, static_cast<int64_t>(kRowStep)) - 1) * from.rs + row_bytes -
                         kb * kBlock;
-        bytes = rows > 0 && kb < depth_blocks ? bytes : 0;
+        bytes = rows > 0 && kb < end_block ? bytes : 0;
         copy_to_lds<16>(resource(from.values + row * from.rs + kb * kBlock,
                                  static_cast<uint32_t>(bytes)),
                         x < kCopiesA ? offset_a : second ? offset_up : offset_b,
@@ -210,7 +218,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     };
     // Zeros for the depths of the last slice that lie behind k.
     const auto clear = [&](Slice& s) __attribute__((always_inline)) {
-        const int depths = static_cast<int>(p.k - (depth_blocks - 1) * kBlock);
+        const int depths = static_cast<int>(p.k % kBlock);
         for (int i = static_cast<int>(threadIdx.x); i < (BM + kRowsB) * 8; i += kThreads) {
             const int inside = depths - 16 * ((i % 8) ^ (i / 16 % 8));
             uint4* const at = i < BM * 8 ? s.a + i : s.b + (i - BM * 8);
@@ -285,11 +293,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
             if (last_row && j == 0) {
                 wait_copies();
                 bare_barrier();
-                if (kb + 2 == depth_blocks && p.k % kBlock != 0) {
+                if (kb + 2 == end_block && ragged) {
                     clear(next);
                     __syncthreads();
                 }
-                if (kb + 2 < depth_blocks) {
+                if (kb + 2 < end_block) {
                     copy_scales(here, kb + 2);
                 }
             }
@@ -370,16 +378,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         }
     };
 
-    if (depth_blocks > 0) {
-        copy_all(slice0, 0);
+    if (first_block < end_block) {
+        copy_all(slice0, first_block);
         wait_copies();
         bare_barrier();
-        if (depth_blocks == 1 && p.k % kBlock != 0) {
+        if (first_block + 1 == end_block && ragged) {
             clear(slice0);
             __syncthreads();
         }
-        if (depth_blocks > 1) {
-            copy_all(slice1, 1);
+        if (first_block + 1 < end_block) {
+            copy_all(slice1, first_block + 1);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -396,9 +404,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
             raw_b[1] = piece_b(slice0, 1, 1);
         }
     }
-    for (int64_t kb = 0; kb < depth_blocks; kb += 2) {
+    for (int64_t kb = first_block; kb < end_block; kb += 2) {
         step(slice0, slice1, kb);
-        if (kb + 1 < depth_blocks) {
+        if (kb + 1 < end_block) {
             step(slice1, slice0, kb + 1);
         }
     }
@@ -417,6 +425,26 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const int64_t col0 = n0 + wn * (BN / WN) + 4 * half;
     // Whether the tile lies inside the matrix: no test per quad then.
     const bool whole = m0 + BM <= p.m && n0 + BN <= p.n;
+    if (p.partial != nullptr) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            const int64_t row = row0 + 32 * i;
+#pragma unroll
+            for (int w = 0; w < kWeights; ++w) {
+                float* const line =
+                    p.partial +
+                    ((static_cast<int64_t>(blockIdx.y) * kWeights + w) * p.m + row) * p.n + col0;
+#pragma unroll
+                for (int x = 0; x < 4 * FN; ++x) {
+                    const floatx16& v = acc[w][i][x / 4];
+                    const int e = x % 4 * 4;
+                    dev::store_quad(line + 8 * x, make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]),
+                                    row < p.m ? p.n - col0 - 8 * x : 0);
+                }
+            }
+        }
+        return;
+    }
     if constexpr (!GATED) {
         if (p.c0 != nullptr) {
 #pragma unroll
@@ -560,30 +588,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     }
 }
 
-template <int BM, int BN, int WM, int WN> void launch(const mfr_stream& s, Params p) {
+// Tiles of BM x BN outputs (of each projection when GATED), `splits` ranges of the depth.
+template <int BM, int BN, int WM, int WN, bool GATED>
+void launch_tiles(const mfr_stream& s, Params p, int64_t splits) {
     const int64_t tiles_m = (p.m + BM - 1) / BM;
     const int64_t tiles_n = (p.n + BN - 1) / BN;
     require(tiles_m < (int64_t{1} << 31) && tiles_n < (int64_t{1} << 31) &&
-                one_launch(tiles_m * tiles_n, 64 * WM * WN),
+                one_launch(tiles_m * tiles_n * splits, 64 * WM * WN),
             "f8gemm: problem too large for one launch");
     p.tiles_m = static_cast<uint32_t>(tiles_m);
     p.tiles_n = static_cast<uint32_t>(tiles_n);
-    const unsigned grid = static_cast<unsigned>(tiles_m * tiles_n);
-    tile_kernel<BM, BN, WM, WN, false><<<grid, 64 * WM * WN, 0, s.stream>>>(p);
-    check_launch("f8gemm tile_kernel");
-}
-
-// Gated: BN of each projection.
-template <int BM, int BN, int WM, int WN> void launch_gated(const mfr_stream& s, Params p) {
-    const int64_t tiles_m = (p.m + BM - 1) / BM;
-    const int64_t tiles_n = (p.n + BN - 1) / BN;
-    require(tiles_m < (int64_t{1} << 31) && tiles_n < (int64_t{1} << 31) &&
-                one_launch(tiles_m * tiles_n, 64 * WM * WN),
-            "f8gemm: problem too large for one launch");
-    p.tiles_m = static_cast<uint32_t>(tiles_m);
-    p.tiles_n = static_cast<uint32_t>(tiles_n);
-    const unsigned grid = static_cast<unsigned>(tiles_m * tiles_n);
-    tile_kernel<BM, BN, WM, WN, true><<<grid, 64 * WM * WN, 0, s.stream>>>(p);
+    const dim3 grid(static_cast<unsigned>(tiles_m * tiles_n), static_cast<unsigned>(splits));
+    tile_kernel<BM, BN, WM, WN, GATED><<<grid, 64 * WM * WN, 0, s.stream>>>(p);
     check_launch("f8gemm tile_kernel");
 }
 
