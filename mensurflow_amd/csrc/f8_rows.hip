@@ -2,6 +2,7 @@
 // with a scale per block (f8.hpp), in fp32, or in both.
 #include "f8.hpp"
 
+#include <algorithm>
 #include <cmath>
 
 namespace {
@@ -75,6 +76,19 @@ struct NormParams {
     int64_t out_rs;
     Matrix q; // values null: none
     float eps;
+
+    // `count` rows from `first` on.
+    NormParams from(int64_t first, int64_t count) const {
+        NormParams n = *this;
+        n.rows = count;
+        n.x += first * x_rs;
+        n.residual += residual != nullptr ? first * residual_rs : 0;
+        n.sum += sum != nullptr ? first * sum_rs : 0;
+        n.out += out != nullptr ? first * out_rs : 0;
+        n.q.values += q.values != nullptr ? first * q.rs : 0;
+        n.q.scales += q.values != nullptr ? first * q.srs : 0;
+        return n;
+    }
 };
 
 __device__ inline float4 add(float4 a, float4 b) {
@@ -99,61 +113,173 @@ __device__ inline float4 inside(float4 v, int64_t count) {
                        count > 3 ? v.w : 0.0f);
 }
 
-// A workgroup per row, in two passes over it.
-__global__ __launch_bounds__(kThreads) void rms_norm_kernel(NormParams p) {
-    __shared__ double sums[kThreads / kWave];
-    for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
-        const float* x = p.x + r * p.x_rs;
-        const float* residual = p.residual != nullptr ? p.residual + r * p.residual_rs : nullptr;
-        float* sum = p.sum != nullptr ? p.sum + r * p.sum_rs : nullptr;
-        double total = 0.0;
-        for (int64_t col = 4 * threadIdx.x; col < p.cols; col += kStep) {
-            float4 t = dev::load_quad(x + col, p.cols - col);
+// The sum of v over a workgroup of WAVES wavefronts, in each thread: over the lanes by halves, then
+// over the wavefronts in order.
+template <int WAVES> __device__ inline double group_sum(double v, double* sums) {
+    v = mfr::dev::wave_sum(v);
+    if constexpr (WAVES > 1) {
+        if (threadIdx.x % kWave == 0) {
+            sums[threadIdx.x / kWave] = v;
+        }
+        __syncthreads();
+        v = 0.0;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) {
+            v += sums[i];
+        }
+    }
+    return v;
+}
+
+__device__ inline double norm_scale(const NormParams& p, double squares) {
+    return 1.0 / sqrt(squares / static_cast<double>(p.cols) + static_cast<double>(p.eps));
+}
+
+// What follows the sum of squares: four columns of the result, in the forms that are asked for.
+__device__ inline void write_normed(const NormParams& p, int64_t r, int64_t col, float4 t,
+                                    double scale, float4 w) {
+    const int64_t count = p.cols - col;
+    const float4 y = inside(scaled(t, scale, w), count); // behind the row 0 * scale may be NaN
+    if (p.out != nullptr) {
+        dev::store_quad(p.out + r * p.out_rs + col, y, count);
+    }
+    if (p.q.values != nullptr) {
+        dev::write_f8(p.q, r, col, p.cols, y);
+    }
+}
+
+__device__ inline float4 weight_at(const NormParams& p, int64_t col) {
+    return p.weight != nullptr ? dev::load_quad(p.weight + col, p.cols - col)
+                               : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+}
+
+// A row in the registers of THREADS threads, QUADS x 4 columns each: every element is read once,
+// all of a thread's loads before the first use. A workgroup takes one row, or 4 where a wavefront
+// holds a row. Bound by memory; the double arithmetic (2 conversions, a multiply-add and 2
+// products an element) is under a fifth of the vector units' time at that rate.
+template <int THREADS, int QUADS>
+__global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void rms_norm_kernel(
+    NormParams p) {
+    constexpr int kRows = THREADS == kWave ? 4 : 1;
+    __shared__ double sums[THREADS / kWave];
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / THREADS;
+    if (r >= p.rows) {
+        return; // a whole wavefront, where that has a row of its own
+    }
+    const int64_t col0 = 4 * (threadIdx.x % THREADS);
+    const float* x = p.x + r * p.x_rs;
+    float4 t[QUADS];
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+        const int64_t col = col0 + i * 4 * THREADS;
+        t[i] = dev::load_quad(x + col, p.cols - col);
+    }
+    if (p.residual != nullptr) {
+        const float* residual = p.residual + r * p.residual_rs;
+        float4 u[QUADS];
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) {
+            const int64_t col = col0 + i * 4 * THREADS;
+            u[i] = dev::load_quad(residual + col, p.cols - col);
+        }
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) {
+            t[i] = add(t[i], u[i]);
+        }
+    }
+    if (p.sum != nullptr) {
+#pragma unroll
+        for (int i = 0; i < QUADS; ++i) {
+            const int64_t col = col0 + i * 4 * THREADS;
+            dev::store_quad(p.sum + r * p.sum_rs + col, t[i], p.cols - col);
+        }
+    }
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+        total += squares(t[i]);
+    }
+    const double scale = norm_scale(p, group_sum<THREADS / kWave>(total, sums));
+#pragma unroll
+    for (int i = 0; i < QUADS; ++i) {
+        const int64_t col = col0 + i * 4 * THREADS;
+        write_normed(p, r, col, t[i], scale, weight_at(p, col));
+    }
+}
+
+// Rows of any length, a workgroup each, in two passes over them.
+constexpr int kLongThreads = 1024;
+
+__global__ __launch_bounds__(kLongThreads) void rms_norm_long_kernel(NormParams p) {
+    __shared__ double sums[kLongThreads / kWave];
+    const int64_t r = blockIdx.x;
+    const float* x = p.x + r * p.x_rs;
+    const float* residual = p.residual != nullptr ? p.residual + r * p.residual_rs : nullptr;
+    float* sum = p.sum != nullptr ? p.sum + r * p.sum_rs : nullptr;
+    double total = 0.0;
+    for (int64_t col = 4 * threadIdx.x; col < p.cols; col += 4 * kLongThreads) {
+        float4 t = dev::load_quad(x + col, p.cols - col);
+        if (residual != nullptr) {
+            t = add(t, dev::load_quad(residual + col, p.cols - col));
+        }
+        if (sum != nullptr) {
+            dev::store_quad(sum + col, t, p.cols - col);
+        }
+        total += squares(t);
+    }
+    const double scale = norm_scale(p, group_sum<kLongThreads / kWave>(total, sums));
+    for (int64_t c0 = 0; c0 < p.cols; c0 += 4 * kLongThreads) {
+        const int64_t col = c0 + 4 * threadIdx.x;
+        float4 t;
+        if (sum != nullptr) {
+            t = dev::load_quad(sum + col, p.cols - col);
+        } else {
+            t = dev::load_quad(x + col, p.cols - col);
             if (residual != nullptr) {
                 t = add(t, dev::load_quad(residual + col, p.cols - col));
             }
-            if (sum != nullptr) {
-                dev::store_quad(sum + col, t, p.cols - col);
-            }
-            total += squares(t);
         }
-        total = mfr::dev::wave_sum(total);
-        if (threadIdx.x % kWave == 0) {
-            sums[threadIdx.x / kWave] = total;
-        }
-        __syncthreads();
-        total = 0.0;
-#pragma unroll
-        for (int i = 0; i < kThreads / kWave; ++i) {
-            total += sums[i];
-        }
-        __syncthreads(); // `sums` has been read
-        const double scale = 1.0 / sqrt(total / static_cast<double>(p.cols) + p.eps);
-        for (int64_t c0 = 0; c0 < p.cols; c0 += kStep) {
-            const int64_t col = c0 + 4 * threadIdx.x;
-            float4 t;
-            if (sum != nullptr) {
-                t = dev::load_quad(sum + col, p.cols - col);
-            } else {
-                t = dev::load_quad(x + col, p.cols - col);
-                if (residual != nullptr) {
-                    t = add(t, dev::load_quad(residual + col, p.cols - col));
-                }
-            }
-            float4 w = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
-            if (p.weight != nullptr) {
-                w = dev::load_quad(p.weight + col, p.cols - col);
-            }
-            float4 y = scaled(t, scale, w);
-            y = inside(y, p.cols - col); // behind the row 0 * scale may be NaN
-            if (p.out != nullptr) {
-                dev::store_quad(p.out + r * p.out_rs + col, y, p.cols - col);
-            }
-            if (p.q.values != nullptr) {
-                dev::write_f8(p.q, r, col, p.cols, y);
-            }
-        }
+        write_normed(p, r, col, t, scale, weight_at(p, col));
     }
+}
+
+template <int THREADS, int QUADS> void launch_norm(const mfr_stream& s, const NormParams& p) {
+    constexpr int kRows = THREADS == kWave ? 4 : 1;
+    rms_norm_kernel<THREADS, QUADS>
+        <<<static_cast<unsigned>((p.rows + kRows - 1) / kRows), kRows * THREADS, 0, s.stream>>>(p);
+}
+
+// The rows of one launch. A wavefront holds up to 1024 columns; longer rows go over 256 threads
+// where there are rows for every compute unit, over 1024 where there are few and a row's own time
+// counts.
+void norm_rows(const mfr_stream& s, const NormParams& p) {
+    const int64_t quads = (p.cols + 3) / 4;
+    if (quads <= kWave * 4) {
+        if (quads <= kWave) {
+            launch_norm<kWave, 1>(s, p);
+        } else if (quads <= kWave * 2) {
+            launch_norm<kWave, 2>(s, p);
+        } else {
+            launch_norm<kWave, 4>(s, p);
+        }
+    } else if (quads <= 256 * 8 && p.rows > 2 * s.compute_units) {
+        if (quads <= 256 * 2) {
+            launch_norm<256, 2>(s, p);
+        } else if (quads <= 256 * 4) {
+            launch_norm<256, 4>(s, p);
+        } else {
+            launch_norm<256, 8>(s, p);
+        }
+    } else if (quads <= 1024) {
+        launch_norm<1024, 1>(s, p);
+    } else if (quads <= 1024 * 2) {
+        launch_norm<1024, 2>(s, p);
+    } else if (quads <= 1024 * 4) {
+        launch_norm<1024, 4>(s, p);
+    } else {
+        rms_norm_long_kernel<<<static_cast<unsigned>(p.rows), kLongThreads, 0, s.stream>>>(p);
+    }
+    mfr::check_launch("rms_norm_kernel");
 }
 
 // The descriptor's checks (of shapes, layouts and pointers: no device is needed).
@@ -245,9 +371,11 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc) {
         if (p.rows == 0 || p.cols == 0) {
             return;
         }
-        rms_norm_kernel<<<mfr::grid_blocks(p.rows, 1, int64_t{1} << 20), kThreads, 0, s.stream>>>(
-            p);
-        mfr::check_launch("rms_norm_kernel");
+        // 2^21 rows a launch: fewer than 2^32 threads.
+        constexpr int64_t kMostRows = int64_t{1} << 21;
+        for (int64_t r = 0; r < p.rows; r += kMostRows) {
+            norm_rows(s, p.from(r, std::min(p.rows - r, kMostRows)));
+        }
     });
 }
 

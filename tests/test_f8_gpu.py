@@ -141,7 +141,8 @@ def test_empty_matrices(stream):
 # ---- norm -----------------------------------------------------------------------------------------
 
 NORM_SIZES = SIZES + [(3, 1024), (2, 1025), (9, 2048), (2, 4096), (2, 4097), (3, 8192), (2, 8193),
-                      (1, 16384), (2, 16385), (1, 40001), (300, 64)]
+                      (1, 16384), (2, 16385), (1, 40001), (300, 64),
+                      (600, 300), (513, 1100), (520, 2100), (515, 4100), (514, 8200)]
 
 
 def assert_norm(y, t, weight, eps):
@@ -253,7 +254,9 @@ GEMM_SIZES = [(1, 1, 1), (1, 128, 128), (1, 300, 1000), (2, 3, 17), (3, 130, 15)
               (9, 129, 129), (16, 257, 127), (17, 64, 300), (31, 500, 640), (32, 128, 2049),
               (33, 127, 128), (48, 200, 513), (64, 384, 384), (65, 129, 143), (100, 40, 1030),
               (127, 255, 260), (128, 256, 512), (129, 257, 385), (200, 1100, 130), (257, 513, 700),
-              (520, 260, 255), (1000, 30, 64), (2100, 2200, 300), (2049, 2305, 129)]
+              (520, 260, 255), (1000, 30, 64), (2100, 2200, 300), (2049, 2305, 129),
+              (512, 1024, 4096), (600, 1300, 2100), (260, 4100, 900), (40, 8300, 1000),
+              (100, 9000, 300), (700, 700, 3100)]
 
 
 @pytest.mark.parametrize("m,n,k", GEMM_SIZES)
