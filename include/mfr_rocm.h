@@ -399,7 +399,7 @@ int mfr_attention(mfr_stream_t stream, const mfr_attention_desc* desc);
 /* A matrix of e4m3 values (OCP: 4 exponent bits, 3 of mantissa, no infinities, largest 448) with
  * fp32 scales: element (r, c) stands for value(r, c) * scale(r / block_rows, c / 128), scale (i, j)
  * at scales[i * scales_rs + j * scales_cs]. Rows are contiguous and rs bytes apart; the base and rs
- * are multiples of 16 bytes, rs at least the row's length and at most 2^25, scales_rs at most 2^23. A row is read in whole 16-byte pieces,
+ * are multiples of 16 bytes, rs at least the row's length and at most 2^24, scales_rs at most 2^23. A row is read in whole 16-byte pieces,
  * so the bytes between its end and the next multiple of 16 are read (not used, never written).
  * block_rows is 1 (activations: a scale per row and 128 columns) or 128 (weights: one per 128 x 128
  * block). Columns of scales that lie together (scales_rs = 1) suit mfr_f8gemm's loads best. */

@@ -16,8 +16,8 @@ constexpr int kBlock = MFR_F8_BLOCK;
 constexpr float kTop = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;
 
-// A round of 64 rows, and of 64 rows' scales, is addressed with 32 bits.
-constexpr int64_t kMostRowBytes = int64_t{1} << 25;
+// A tile's rows (up to 128), and 64 rows' scales, are addressed with 31 and 32 bits.
+constexpr int64_t kMostRowBytes = int64_t{1} << 24;
 constexpr int64_t kMostScaleStride = int64_t{1} << 23;
 
 constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }

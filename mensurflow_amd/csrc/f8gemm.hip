@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <limits>
+#include <utility>
 
 namespace {
 
@@ -76,18 +77,18 @@ constexpr Few kFewGated[] = {{Form::kFew16, 16, 16, 8, 1.5},
                              {Form::kFew64, 64, 16, 4, 1.7}};
 
 // A tile's workgroups per CU at once, its fixed time, and the time of a block when every CU has
-// them all, or one alone on few CUs. Measured, k = 4096: 64 x 128 25.4 us on 32 CUs, 41.5 with two on
-// each; 128 x 128 37.5 and 67.9 (8192^3 920); gated 46.2 and 97 for two in turn; 52 and 66 (8192 x
-// 10240 x 4096 1160).
+// them all, or one alone on few CUs. Measured, k = 4096: 64 x 128 tiles on 64 CUs 21.8 us, one on
+// every CU 26.8, two 40.1; 128 x 128 31.4 on 32 CUs, 35.1 on 128, 42.2 on all (8192^3, two on each
+// 930); gated 64 x 128 35.4 on 128 CUs (8192 x 10240 x 4096 1520), 128 x 128 49.3 on 64 (1230).
 struct Tile {
     Form form;
     int64_t rows, at_once;
     double fixed, full, alone;
 };
-constexpr Tile kTiles[] = {{Form::kTile64, 64, 2, 5.2, 1.2, 0.65},
-                           {Form::kTile128, 128, 2, 6.0, 2.0, 1.0}};
-constexpr Tile kTilesGated[] = {{Form::kTile64, 64, 1, 7.0, 1.4, 1.22},
-                                {Form::kTile128, 128, 1, 8.0, 1.8, 1.38}};
+constexpr Tile kTiles[] = {{Form::kTile64, 64, 2, 4.5, 1.12, 0.55},
+                           {Form::kTile128, 128, 2, 5.7, 1.8, 0.8}};
+constexpr Tile kTilesGated[] = {{Form::kTile64, 64, 1, 6.0, 1.2, 0.92},
+                                {Form::kTile128, 128, 1, 8.0, 1.92, 1.29}};
 constexpr int64_t kTileCols = 128;
 
 // The second launch of a depth in ranges and the memory it reads; the second launch of few rows
@@ -134,12 +135,10 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
             const int64_t groups = ceil_div(p.m, t.rows) * ceil_div(p.n, kTileCols) * splits;
             const int64_t slots = cus * t.at_once;
             const int64_t rest = groups % slots;
-            // One workgroup on a CU takes `alone`; the second of a pair, or the CUs' rivalry when
-            // all are busy, brings that to `full`.
-            const double part =
-                rest == 0 ? 0.0
-                          : std::max(t.alone, t.full * static_cast<double>(rest) /
-                                                  static_cast<double>(slots));
+            // The second workgroup of a CU, and the CUs' rivalry when all are busy, bring `alone`
+            // to `full`.
+            const double share = static_cast<double>(rest) / static_cast<double>(slots);
+            const double part = rest == 0 ? 0.0 : t.alone + (t.full - t.alone) * share * share;
             double time = t.fixed + static_cast<double>(ceil_div(blocks, splits)) *
                                         (static_cast<double>(groups / slots) * t.full + part);
             int64_t bytes = 0;
@@ -185,20 +184,19 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
         gated ? launch_few<4, 1, 4, 1, true>(s, p) : launch_few<4, 2, 8, 1, false>(s, p);
         break;
     case Form::kTile64:
-        gated ? launch_tiles<64, 128, 1, 4, true>(s, p, plan.splits)
-              : launch_tiles<64, 128, 1, 4, false>(s, p, plan.splits);
+        gated ? launch_tiles<64, 128, 2, 4, 3, true>(s, p, plan.splits)
+              : launch_tiles<64, 128, 1, 4, 2, false>(s, p, plan.splits);
         break;
     case Form::kTile128:
-        gated ? launch_tiles<128, 128, 2, 4, true>(s, p, plan.splits)
-              : launch_tiles<128, 128, 2, 2, false>(s, p, plan.splits);
+        gated ? launch_tiles<128, 128, 2, 4, 2, true>(s, p, plan.splits)
+              : launch_tiles<128, 128, 2, 2, 2, false>(s, p, plan.splits);
         break;
     }
 }
 
 bool is_few(Form f) { return f != Form::kTile64 && f != Form::kTile128; }
 
-void run(mfr_stream& s, Params p) {
-    Plan plan = choose(p, s.compute_units, true);
+void run_region(mfr_stream& s, Params p, Plan plan) {
     std::unique_lock<std::mutex> hold(s.workspace_mutex, std::defer_lock);
     void* memory = nullptr;
     if (plan.workspace > 0) {
@@ -241,6 +239,86 @@ void run(mfr_stream& s, Params p) {
     launch(s, plan, p);
     if (p.partial != nullptr) {
         mfr::f8gemm::launch_finish(s, p, plan.splits);
+    }
+}
+
+// Rows [first, m) or columns [first, n) of the problem, and what comes before them; first a multiple
+// of 128.
+Params rows_from(Params p, int64_t first) {
+    p.m -= first;
+    p.a.values += first * p.a.rs;
+    p.a.scales += first * p.a.srs;
+    p.c += p.c != nullptr ? first * p.c_rs : 0;
+    p.c0 += p.c0 != nullptr ? first * p.c0_rs : 0;
+    p.q.values += p.q.values != nullptr ? first * p.q.rs : 0;
+    p.q.scales += p.q.values != nullptr ? first * p.q.srs : 0;
+    return p;
+}
+
+Params cols_from(Params p, int64_t first) {
+    const int64_t block = first / mfr::f8::kBlock;
+    p.n -= first;
+    for (mfr::f8::Matrix* w : {&p.b, &p.up}) {
+        if (w->values != nullptr) {
+            w->values += first * w->rs;
+            w->scales += block * w->srs;
+        }
+    }
+    p.c += p.c != nullptr ? first : 0;
+    p.c0 += p.c0 != nullptr ? first : 0;
+    p.bias += p.bias != nullptr ? first : 0;
+    p.q.values += p.q.values != nullptr ? first : 0;
+    p.q.scales += p.q.values != nullptr ? block * p.q.scs : 0;
+    return p;
+}
+
+// The problem whole, or, where the model prices that lower, without the rows and columns past the
+// last multiple of 128, which run by themselves: 3 columns more than 32 x 32 tiles of two on each CU
+// cost a third turn of every CU (4093 x 4099 x 1023 58.9 -> 54.0 us). Short calls are not worth the
+// question.
+constexpr double kShortCall = 20.0;
+
+void run(mfr_stream& s, const Params& p) {
+    const auto priced = [&](const Params& x) { return choose(x, s.compute_units, true); };
+    const Plan whole = priced(p);
+    const int64_t m = p.m / 128 * 128;
+    const int64_t n = p.n / 128 * 128;
+    const auto head = [](Params x, int64_t rows, int64_t cols) {
+        x.m = rows;
+        x.n = cols;
+        return x;
+    };
+    double best = whole.time;
+    int64_t rows = p.m;
+    int64_t cols = p.n;
+    for (const auto& [r, c] : {std::pair{p.m, n}, std::pair{m, p.n}, std::pair{m, n}}) {
+        if (whole.time < kShortCall || r == 0 || c == 0 || (r == p.m && c == p.n)) {
+            continue;
+        }
+        double time = priced(head(p, r, c)).time;
+        if (c < p.n) {
+            time += priced(cols_from(head(p, r, p.n), c)).time;
+        }
+        if (r < p.m) {
+            time += priced(rows_from(p, r)).time;
+        }
+        if (time < best) {
+            best = time;
+            rows = r;
+            cols = c;
+        }
+    }
+    if (rows == p.m && cols == p.n) {
+        run_region(s, p, whole);
+        return;
+    }
+    const auto region = [&](const Params& x) { run_region(s, x, priced(x)); };
+    region(head(p, rows, cols));
+    if (cols < p.n) {
+        region(cols_from(head(p, rows, p.n), cols));
+    }
+    if (rows < p.m) {
+        region(rows_from(p, rows));
     }
 }
 

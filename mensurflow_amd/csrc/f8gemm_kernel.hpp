@@ -59,10 +59,13 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
-// The copies into LDS have landed, and the LDS reads before have been done (a later copy may write there).
-__device__ __forceinline__ void wait_copies() {
+// All copies into LDS but the last COPIES have landed, and the LDS reads before have been done (a
+// later copy may write there). s_waitcnt of gfx9: vmcnt in bits 3:0 and 15:14, expcnt 6:4 (left
+// alone), lgkmcnt 11:8.
+template <int COPIES> __device__ __forceinline__ void wait_copies() {
+    static_assert(COPIES < 64, "vmcnt is 6 bits");
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(7 << 4); // vmcnt 0, lgkmcnt 0
+    __builtin_amdgcn_s_waitcnt((COPIES & 15) | (7 << 4) | ((COPIES >> 4) << 14));
 }
 
 // A workgroup barrier that waits for no memory operation by itself.
@@ -85,22 +88,25 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
     return r;
 }
 
-// One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at `offset`
-// go to `to` + 16 l (4 l), `to` the wavefront's. In assembly, because the compiler waits for every
-// such copy that it knows of before any read of LDS once there are more than 8 in a kernel;
-// wait_copies() is what waits here. No register is written.
+// One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at `lane_offset`
+// + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past the resource
+// (its range counts both offsets). In assembly, because the compiler waits for every such copy that
+// it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is what
+// waits here. No register is written.
 template <int BYTES>
-__device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t offset, void* to) {
+__device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, uint32_t offset,
+                                            void* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(to)))));
     if constexpr (BYTES == 16) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
-                     "v"(offset), "s"(from)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
+                         at),
+                     "v"(lane_offset), "s"(from), "s"(offset)
                      : "memory");
     } else {
         static_assert(BYTES == 4, "4 or 16 bytes a lane");
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(at),
-                     "v"(offset), "s"(from)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(at),
+                     "v"(lane_offset), "s"(from), "s"(offset)
                      : "memory");
     }
 }
@@ -116,7 +122,10 @@ __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t offset, void* t
 // operand: a lane then holds quads of neighbouring columns of one row of C. The 64 depths that a lane
 // gives to the 8 instructions are 64 neighbouring ones for both operands: which depth stands where
 // does not matter to a sum as long as it is the same for both.
-template <int BM, int BN, int WM, int WN, bool GATED>
+//
+// SLICES of them lie in LDS: with two, a slice is under way while one is multiplied, which covers
+// memory's latency where two workgroups share a CU; with three, two are.
+template <int BM, int BN, int WM, int WN, int SLICES, bool GATED>
 __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     constexpr int kThreads = 64 * WM * WN;
     constexpr int kWeights = GATED ? 2 : 1;
@@ -136,9 +145,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         float scales[BM];
         float scales_b[kWeights][64]; // of block columns
     };
-    // Two objects, so that the compiler sees that the copy into one does not write the other.
+    static_assert(SLICES == 2 || SLICES == 3, "");
     __shared__ __align__(16) Slice slice0;
     __shared__ __align__(16) Slice slice1;
+    __shared__ __align__(16) Slice slice2;
 
     const int lane = static_cast<int>(threadIdx.x % 64);
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
@@ -165,32 +175,46 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const int64_t end_block = min(first_block + p.split_blocks, blocks_of(p.k));
     const bool ragged = p.k % kBlock != 0 && end_block == blocks_of(p.k);
 
-    // Copies of a slice: 8 threads take a row's pieces, kRowStep rows a round. Each round has a
-    // resource of its own, made by the scalar unit: it begins at the round's first row and the
-    // slice's first depth and ends with the matrix, so that rows past it come as zeros. (A row's
-    // pieces past its end are the next row's; clear() removes them.)
+    // Copies of a slice: 8 threads take a row's pieces, kRowStep rows a round. An operand's resource
+    // begins at the tile's first row and depth and ends with the matrix, so that rows past it come
+    // as zeros. (A row's pieces past its end are the next row's; clear() removes them.) The host
+    // keeps a tile's bytes below kNothing, which lies past every resource.
+    constexpr uint32_t kNothing = 0x80000000u;
     const int64_t row_bytes = (p.k + 15) / 16 * 16;
+    const auto operand = [&](const Matrix& m, int64_t row, int64_t rows) {
+        const int64_t bytes = (rows - row - 1) * m.rs + row_bytes - first_block * kBlock;
+        return resource(m.values + row * m.rs + first_block * kBlock,
+                        static_cast<uint32_t>(min(bytes, static_cast<int64_t>(kNothing))));
+    };
+    const intx4 from_a = operand(p.a, m0, p.m);
+    const intx4 from_b = operand(p.b, n0, p.n);
+    const intx4 from_up = GATED ? operand(p.up, n0, p.n) : intx4{};
+    const uint32_t a_rs = static_cast<uint32_t>(p.a.rs);
+    const uint32_t b_rs = static_cast<uint32_t>(p.b.rs);
+    const uint32_t up_rs = static_cast<uint32_t>(p.up.rs);
     const uint32_t thread_row = threadIdx.x / 8;
     const uint32_t thread_piece = (threadIdx.x ^ (thread_row / 2)) % 8 * 16;
-    const uint32_t offset_a = thread_row * static_cast<uint32_t>(p.a.rs) + thread_piece;
-    const uint32_t offset_b = thread_row * static_cast<uint32_t>(p.b.rs) + thread_piece;
-    const uint32_t offset_up = thread_row * static_cast<uint32_t>(p.up.rs) + thread_piece;
+    const uint32_t offset_a = thread_row * a_rs + thread_piece;
+    const uint32_t offset_b = thread_row * b_rs + thread_piece;
+    const uint32_t offset_up = thread_row * up_rs + thread_piece;
     constexpr int kRounds = kCopiesA + kCopiesB;
+    // Round x of slice kb; zeros for one past the last.
     const auto copy = [&](Slice& to, int64_t kb, int x) __attribute__((always_inline)) {
-        const int i = x < kCopiesA ? x : x - kCopiesA;
-        const bool second = GATED && x >= kCopiesA && i * kRowStep >= BN;
-        const Matrix& from = x < kCopiesA ? p.a : second ? p.up : p.b;
-        const int64_t row = x < kCopiesA ? m0 + i * kRowStep : n0 + i * kRowStep % BN;
-        const int64_t rows = (x < kCopiesA ? p.m : p.n) - row;
-        int64_t bytes = (min(rows, static_cast<int64_t>(kRowStep)) - 1) * from.rs + row_bytes -
-                        kb * kBlock;
-        bytes = rows > 0 && kb < end_block ? bytes : 0;
-        copy_to_lds<16>(resource(from.values + row * from.rs + kb * kBlock,
-                                 static_cast<uint32_t>(bytes)),
-                        x < kCopiesA ? offset_a : second ? offset_up : offset_b,
-                        (x < kCopiesA ? to.a : to.b) + i * kThreads + wave * 64);
+        const uint32_t depth =
+            kb < end_block ? static_cast<uint32_t>(kb - first_block) * kBlock : kNothing;
+        if (x < kCopiesA) {
+            copy_to_lds<16>(from_a, offset_a, depth + x * kRowStep * a_rs,
+                            to.a + x * kThreads + wave * 64);
+            return;
+        }
+        const int i = x - kCopiesA;
+        const bool second = GATED && i * kRowStep >= BN;
+        copy_to_lds<16>(second ? from_up : from_b, second ? offset_up : offset_b,
+                        depth + i * kRowStep % BN * (second ? up_rs : b_rs),
+                        to.b + i * kThreads + wave * 64);
     };
-    // The scales: a wavefront each for 64 rows of A and for the block columns of a weight.
+    // The scales: a wavefront each for 64 rows of A and for the block columns of a weight, read one
+    // by one through a resource that begins at the first of them.
     constexpr int kWaves = WM * WN;
     static_assert(BM / 64 + kWeights <= kWaves, "a wavefront copies one run of scales at most");
     const bool of_a = wave < BM / 64;
@@ -198,19 +222,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const Matrix& scaled = of_a ? p.a : GATED && wave == kWaves - 2 ? p.up : p.b;
     const int64_t first_scale = of_a ? m0 + wave * 64 : n0 / kBlock;
     const int64_t last_scale = (of_a ? p.m : blocks_of(p.n)) - 1 - first_scale;
+    const bool has_scales = (of_a && last_scale >= 0) || of_b;
     const uint32_t scale_offset =
         static_cast<uint32_t>(min(static_cast<int64_t>(of_a ? lane : lane % kBlocksN),
                                   max(last_scale, static_cast<int64_t>(0)))) *
         static_cast<uint32_t>(scaled.srs) * 4;
-    const auto copy_scales = [&](Slice& to, int64_t kb) __attribute__((always_inline)) {
-        if ((of_a && last_scale >= 0) || of_b) {
-            const float* from = scaled.scales + first_scale * scaled.srs + kb * scaled.scs;
-            copy_to_lds<4>(resource(from, 0xffffffffu), scale_offset,
+    // In scalar registers: fetched anew for each slice, they would be waited for.
+    const auto scalar = [](uint64_t v) {
+        const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
+        const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+        return static_cast<uint64_t>(hi) << 32 | lo;
+    };
+    uint64_t scales_at = scalar(reinterpret_cast<uint64_t>(
+        scaled.scales + first_scale * scaled.srs + first_block * scaled.scs));
+    const uint64_t scales_step = scalar(static_cast<uint64_t>(scaled.scs) * 4);
+    // Those of the next slice that has not had any.
+    const auto copy_scales = [&](Slice& to) __attribute__((always_inline)) {
+        if (has_scales) {
+            copy_to_lds<4>(resource(reinterpret_cast<const void*>(scales_at), 0xffffffffu),
+                           scale_offset, 0,
                            of_a ? to.scales + wave * 64 : to.scales_b[kWaves - 1 - wave]);
+            scales_at += scales_step;
         }
     };
     const auto copy_all = [&](Slice& to, int64_t kb) __attribute__((always_inline)) {
-        copy_scales(to, kb);
+        if (kb < end_block) {
+            copy_scales(to);
+        }
 #pragma unroll
         for (int x = 0; x < kRounds; ++x) {
             copy(to, kb, x);
@@ -237,7 +275,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     // The wavefront's blocks of 32 x 32 outputs: FM block rows, and NJ block columns over the weights.
     constexpr int NJ = kWeights * FN;
     constexpr int kChains = FM * NJ;
-    static_assert(kChains % 2 == 0 && NJ <= 2 && FM >= 2, "chains alternate between two results");
+    static_assert(kChains % 2 == 0 && NJ <= 2, "chains alternate between two results");
     floatx16 acc[kWeights][FM][FN] = {};
     const int row_a = wm * (BM / WM) + r32;
     const int row_b = wn * (BN / WN) + r32;
@@ -253,14 +291,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     bf16x8 fb[NJ][8];
     uint4 raw_a[4];
     uint4 raw_b[4];
+    uint4 raw_last[4]; // of B's second block, where the one block row lets none be read later
     const auto widen_a = [&](int q) __attribute__((always_inline)) {
         fa[2 * q] = widen(raw_a[q].x, raw_a[q].y);
         fa[2 * q + 1] = widen(raw_a[q].z, raw_a[q].w);
         asm volatile("" : "+v"(fa[2 * q]), "+v"(fa[2 * q + 1])); // here, not where it is used
     };
-    const auto widen_b = [&](int j, int q) __attribute__((always_inline)) {
-        fb[j][2 * q] = widen(raw_b[q].x, raw_b[q].y);
-        fb[j][2 * q + 1] = widen(raw_b[q].z, raw_b[q].w);
+    const auto widen_b = [&](int j, const uint4 (&raw)[4], int q) __attribute__((always_inline)) {
+        fb[j][2 * q] = widen(raw[q].x, raw[q].y);
+        fb[j][2 * q + 1] = widen(raw[q].z, raw[q].w);
         asm volatile("" : "+v"(fb[j][2 * q]), "+v"(fb[j][2 * q + 1]));
     };
     floatx16 part[2] = {};
@@ -291,14 +330,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
             const int j = c % NJ;
             const bool last_row = i == FM - 1;
             if (last_row && j == 0) {
-                wait_copies();
+                // (Rounds of copies alone are counted: a wavefront with scales to copy as well waits
+                // for one more.)
+                wait_copies<(SLICES - 2) * kRounds>();
                 bare_barrier();
                 if (kb + 2 == end_block && ragged) {
                     clear(next);
                     __syncthreads();
                 }
-                if (kb + 2 < end_block) {
-                    copy_scales(here, kb + 2);
+                if (kb + SLICES < end_block) {
+                    copy_scales(here);
                 }
             }
             floatx16& now = part[c % 2];
@@ -325,27 +366,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
                         raw_a[t / 2 - 2] = last_row ? piece_a(next, 0, t / 2 - 2)
                                                     : piece_a(here, i + 1, t / 2 - 2);
                     }
-                    if (j == 1) {
-                        if (t % 2 == 1) {
+                    if (j == 1 && t % 2 == 1) {
+                        if (last_row) {
+                            widen_b(0, raw_b, t / 2);
+                        }
+                        widen_a(t / 2);
+                        if (t / 2 < 2) {
+                            raw_a[t / 2 + 2] = last_row ? piece_a(next, 0, t / 2 + 2)
+                                                        : piece_a(here, i + 1, t / 2 + 2);
                             if (last_row) {
-                                widen_b(0, t / 2);
+                                raw_b[t / 2 + 2] = piece_b(next, 0, t / 2 + 2);
                             }
-                            widen_a(t / 2);
-                            if (t / 2 < 2) {
-                                raw_a[t / 2 + 2] = last_row ? piece_a(next, 0, t / 2 + 2)
-                                                            : piece_a(here, i + 1, t / 2 + 2);
-                                if (last_row) {
-                                    raw_b[t / 2 + 2] = piece_b(next, 0, t / 2 + 2);
-                                }
-                            } else if (last_row) {
-                                raw_b[t / 2 - 2] = piece_b(next, 1, t / 2 - 2);
-                            }
+                        } else if (last_row && FM > 1) {
+                            raw_b[t / 2 - 2] = piece_b(next, 1, t / 2 - 2);
+                        }
+                        if (FM == 1) {
+                            raw_last[t / 2] = piece_b(next, 1, t / 2);
                         }
                     }
                     if (c == 0 && t % 2 == 1) {
-                        widen_b(1, t / 2);
-                        if (t / 2 < 2) {
-                            raw_b[t / 2 + 2] = piece_b(here, 1, t / 2 + 2);
+                        if constexpr (FM == 1) {
+                            widen_b(1, raw_last, t / 2);
+                        } else {
+                            widen_b(1, raw_b, t / 2);
+                            if (t / 2 < 2) {
+                                raw_b[t / 2 + 2] = piece_b(here, 1, t / 2 + 2);
+                            }
                         }
                     }
                 } else {
@@ -360,7 +406,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
                 // The copies one by one: a wavefront that hands over several waits for their addresses
                 // to be taken. (None is left behind the last slice: empty resources.)
                 if (last_row && (j * 8 + t) % kPace == 0 && (j * 8 + t) / kPace < kRounds) {
-                    copy(here, kb + 2, (j * 8 + t) / kPace);
+                    copy(here, kb + SLICES, (j * 8 + t) / kPace);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -369,7 +415,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
                 for (int q = 0; q < 4; ++q) {
                     widen_a(q);
                     if (last_row) {
-                        widen_b(0, q);
+                        widen_b(0, raw_b, q);
                     }
                 }
             }
@@ -380,14 +426,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
 
     if (first_block < end_block) {
         copy_all(slice0, first_block);
-        wait_copies();
+        copy_all(slice1, first_block + 1);
+        if constexpr (SLICES == 3) {
+            copy_all(slice2, first_block + 2);
+        }
+        wait_copies<(SLICES - 1) * kRounds>();
         bare_barrier();
         if (first_block + 1 == end_block && ragged) {
             clear(slice0);
             __syncthreads();
-        }
-        if (first_block + 1 < end_block) {
-            copy_all(slice1, first_block + 1);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -397,17 +444,29 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             raw_b[q] = piece_b(slice0, 0, q);
-            widen_b(0, q);
+            widen_b(0, raw_b, q);
         }
-        if constexpr (NJ == 2) {
+        if constexpr (NJ == 2 && FM > 1) {
             raw_b[0] = piece_b(slice0, 1, 0);
             raw_b[1] = piece_b(slice0, 1, 1);
+        } else if constexpr (NJ == 2) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                raw_last[q] = piece_b(slice0, 1, q);
+            }
         }
     }
-    for (int64_t kb = first_block; kb < end_block; kb += 2) {
+    for (int64_t kb = first_block; kb < end_block; kb += SLICES) {
         step(slice0, slice1, kb);
         if (kb + 1 < end_block) {
-            step(slice1, slice0, kb + 1);
+            if constexpr (SLICES == 2) {
+                step(slice1, slice0, kb + 1);
+            } else {
+                step(slice1, slice2, kb + 1);
+                if (kb + 2 < end_block) {
+                    step(slice2, slice0, kb + 2);
+                }
+            }
         }
     }
 #pragma unroll
@@ -416,7 +475,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         sums[e] = fmaf(part[1][e], part_scale, sums[e]);
     }
 
-    wait_copies(); // the epilogue uses the slices' memory
+    wait_copies<0>(); // the epilogue uses the slices' memory
 
     // The epilogue. Element e of block (i, j) is row 32 i + r32, column 32 j + 8 (e / 4) + 4 half +
     // e % 4: four neighbouring columns a quad.
@@ -589,7 +648,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
 }
 
 // Tiles of BM x BN outputs (of each projection when GATED), `splits` ranges of the depth.
-template <int BM, int BN, int WM, int WN, bool GATED>
+template <int BM, int BN, int WM, int WN, int SLICES, bool GATED>
 void launch_tiles(const mfr_stream& s, Params p, int64_t splits) {
     const int64_t tiles_m = (p.m + BM - 1) / BM;
     const int64_t tiles_n = (p.n + BN - 1) / BN;
@@ -599,7 +658,7 @@ void launch_tiles(const mfr_stream& s, Params p, int64_t splits) {
     p.tiles_m = static_cast<uint32_t>(tiles_m);
     p.tiles_n = static_cast<uint32_t>(tiles_n);
     const dim3 grid(static_cast<unsigned>(tiles_m * tiles_n), static_cast<unsigned>(splits));
-    tile_kernel<BM, BN, WM, WN, GATED><<<grid, 64 * WM * WN, 0, s.stream>>>(p);
+    tile_kernel<BM, BN, WM, WN, SLICES, GATED><<<grid, 64 * WM * WN, 0, s.stream>>>(p);
     check_launch("f8gemm tile_kernel");
 }
 

@@ -100,7 +100,7 @@ F8 = [
     (dict(rs=232), abi.MFR_E_UNSUPPORTED, "16-byte aligned"),
     (dict(rs=96), abi.MFR_E_INVALID, "overlap"),
     (dict(rs=-208), abi.MFR_E_INVALID, "overlap"),
-    (dict(rs=(1 << 25) + 16), abi.MFR_E_UNSUPPORTED, "too far apart"),
+    (dict(rs=(1 << 24) + 16), abi.MFR_E_UNSUPPORTED, "too far apart"),
     (dict(scales_rs=(1 << 23) + 1), abi.MFR_E_UNSUPPORTED, "too far apart"),
     (dict(scales=None), abi.MFR_E_INVALID, "null pointer"),
     (dict(scales_rs=-1), abi.MFR_E_INVALID, "negative scale strides"),

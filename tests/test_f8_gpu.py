@@ -491,7 +491,7 @@ def test_the_other_entry_points_refuse_the_silu(stream):
 def test_offsets_past_32_bits(stream):
     """Rows that lie more than 4 GiB apart in all: the last rows' values and scales are found."""
     rng = np.random.default_rng(14)
-    m, n, k, pitch = 140, 129, 200, 1 << 25  # 140 rows of 32 MiB: 4.4 GiB
+    m, n, k, pitch = 280, 129, 200, 1 << 24  # 280 rows of 16 MiB: 4.4 GiB
     a, sa = exact_operands(rng, m, k, 1)
     b, sb = exact_operands(rng, n, k, 128)
     far = mf.DeviceArray.empty((m, pitch), stream, np.uint8)
