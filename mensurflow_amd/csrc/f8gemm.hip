@@ -172,24 +172,24 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     const bool gated = p.up.values != nullptr;
     switch (plan.form) {
     case Form::kFew16:
-        gated ? launch_few<1, 1, 8, 2, true>(s, p) : launch_few<1, 1, 8, 2, false>(s, p);
+        (gated ? launch_few<1, 1, 8, 2, true> : launch_few<1, 1, 8, 2, false>)(s, p);
         break;
     case Form::kFew32:
-        gated ? launch_few<2, 1, 8, 1, true>(s, p) : launch_few<2, 1, 8, 2, false>(s, p);
+        (gated ? launch_few<2, 1, 8, 1, true> : launch_few<2, 1, 8, 2, false>)(s, p);
         break;
     case Form::kFew32Wide:
         launch_few<2, 2, 4, 2, false>(s, p);
         break;
     case Form::kFew64:
-        gated ? launch_few<4, 1, 4, 1, true>(s, p) : launch_few<4, 2, 8, 1, false>(s, p);
+        (gated ? launch_few<4, 1, 4, 1, true> : launch_few<4, 2, 8, 1, false>)(s, p);
         break;
     case Form::kTile64:
-        gated ? launch_tiles<64, 128, 2, 4, 3, true>(s, p, plan.splits)
-              : launch_tiles<64, 128, 1, 4, 2, false>(s, p, plan.splits);
+        (gated ? launch_tiles<64, 128, 2, 4, 3, true> : launch_tiles<64, 128, 1, 4, 2, false>)(
+            s, p, plan.splits);
         break;
     case Form::kTile128:
-        gated ? launch_tiles<128, 128, 2, 4, 2, true>(s, p, plan.splits)
-              : launch_tiles<128, 128, 2, 2, 2, false>(s, p, plan.splits);
+        (gated ? launch_tiles<128, 128, 2, 4, 2, true> : launch_tiles<128, 128, 2, 2, 2, false>)(
+            s, p, plan.splits);
         break;
     }
 }

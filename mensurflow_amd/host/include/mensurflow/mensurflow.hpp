@@ -7,6 +7,7 @@
 #include "mensurflow/ops/attention.hpp"
 #include "mensurflow/ops/blas.hpp"
 #include "mensurflow/ops/elementwise.hpp"
+#include "mensurflow/ops/f8.hpp"
 #include "mensurflow/ops/random.hpp"
 #include "mensurflow/ops/reduction.hpp"
 #include "mensurflow/ops/softmax.hpp"

@@ -706,6 +706,9 @@ class RocmBackend final : public Backend {
 
 } // namespace
 
+// For the adapters in other files.
+mfr_stream_t rocm_stream(Stream& stream) { return handle(stream); }
+
 void register_rocm_backend(Registry& registry) { registry.add(std::make_unique<RocmBackend>()); }
 
 } // namespace mensurflow::detail

@@ -6,6 +6,8 @@
 //                dispatch where a device has it;
 //   StridedCopy  packs a strided view on its own device, for Tensor::contiguous();
 //   Attention    fused scaled dot-product attention (mask, causal).
+// And three of the 8-bit serving path, which mensurflow has no counterpart of: RmsNorm, QuantizeF8
+// (keyed by F32, their input) and GemmF8 (keyed by U8, its values).
 // A missing kernel is reported (NotImplemented); dispatch never moves an op to another device on
 // its own.
 #pragma once
@@ -45,7 +47,10 @@ enum class OpId {
     StridedCopy,
     Attention,
     Dot,
-    Sub
+    Sub,
+    RmsNorm,
+    QuantizeF8,
+    GemmF8
 };
 
 // "gemm_strided_batched", "bias_add", ...: the name errors and tuning results use.
@@ -98,6 +103,17 @@ struct OpArgs {
     // wherever j > i; a layout the kernel cannot mask throws NotImplemented.
     bool causal = false;
     bool has_mask = false;
+    // RmsNorm, QuantizeF8 and GemmF8 (backends/rocm/f8.cpp): the optional operands that follow the
+    // fixed ones, in this order, and the outputs. An 8-bit matrix is two tensors, values and
+    // scales; `columns` is the elements of a row of the values' pitched rows (of A in GemmF8).
+    bool has_weight = false;
+    bool has_residual = false;
+    bool has_c = false;
+    bool gated = false;
+    bool has_sum = false; // the first output is x + residual
+    bool f8_out = false;  // the result is in 8 bits
+    int block_rows = 1;
+    std::int64_t columns = 0;
     TuningConfig tuning{}; // filled by dispatch() from an active tuning scope
 };
 

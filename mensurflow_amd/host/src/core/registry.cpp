@@ -24,6 +24,7 @@ struct BackendHook {
 constexpr BackendHook kHooks[] = {
     {register_cpu_backend, false},
     {register_rocm_backend, true},
+    {register_rocm_f8, true},
 };
 
 } // namespace

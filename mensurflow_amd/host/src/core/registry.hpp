@@ -45,5 +45,7 @@ class Registry {
 
 void register_cpu_backend(Registry& registry);
 void register_rocm_backend(Registry& registry);
+// The 8-bit ops of the ROCm device, where that was registered.
+void register_rocm_f8(Registry& registry);
 
 } // namespace mensurflow::detail
