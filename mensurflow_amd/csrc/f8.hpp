@@ -20,6 +20,10 @@ constexpr float kLeastScale = 0x1p-126f;
 constexpr int64_t kMostRowBytes = int64_t{1} << 24;
 constexpr int64_t kMostScaleStride = int64_t{1} << 23;
 
+// Of two values of one type. (HIP's own min and max take 64-bit values for ints in host code.)
+template <typename T> __host__ __device__ constexpr T least(T a, T b) { return b < a ? b : a; }
+template <typename T> __host__ __device__ constexpr T most(T a, T b) { return a < b ? b : a; }
+
 constexpr int64_t blocks_of(int64_t n) { return (n + kBlock - 1) / kBlock; }
 
 // One matrix as a kernel's argument.
@@ -79,7 +83,7 @@ namespace mfr::f8::dev {
 __device__ inline uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 __device__ inline uint32_t magnitude(float4 v) {
-    return max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w)));
+    return most(most(magnitude(v.x), magnitude(v.y)), most(magnitude(v.z), magnitude(v.w)));
 }
 
 // The block's scale from its largest magnitude's bits; NaN stays.
@@ -110,7 +114,7 @@ __device__ inline void store_bytes(uint8_t* p, uint32_t w, int64_t count) {
 __device__ inline uint32_t half_max(uint32_t v) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) {
-        v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
+        v = most(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), m, 64)));
     }
     return v;
 }

@@ -41,13 +41,13 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(const float* 
     for (int i = 0; i < 16; ++i) {
         const int64_t r = row + 8 * i;
         v[i] = dev::load_quad(x + r * x_rs + col, r < rows ? cols - col : 0);
-        top = max(top, dev::magnitude(v[i]));
+        top = mfr::f8::most(top, dev::magnitude(v[i]));
     }
     tops[threadIdx.x / 32] = dev::half_max(top); // the 32 lanes store one value
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kThreads / 32; ++i) {
-        top = max(top, tops[i]);
+        top = mfr::f8::most(top, tops[i]);
     }
     const float scale = dev::scale_of(top);
     const float inverse = 1.0f / scale;

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(64 * WK) void few_rows_kernel(Params p) {
     const float* scales_a[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int64_t row = min(m0 + 16 * i + r16, p.m - 1);
+        const int64_t row = f8::least(m0 + 16 * i + r16, p.m - 1);
         rows_a[i] = p.a.values + row * p.a.rs;
         scales_a[i] = p.a.scales + row * p.a.srs;
     }
@@ -43,10 +43,10 @@ __global__ __launch_bounds__(64 * WK) void few_rows_kernel(Params p) {
         const Matrix& from = w == 1 ? p.up : p.b;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            rows_b[w][j] = from.values + min(n0 + 16 * j + r16, p.n - 1) * from.rs;
+            rows_b[w][j] = from.values + f8::least(n0 + 16 * j + r16, p.n - 1) * from.rs;
         }
         // 16 NT divides 128: one block of columns.
-        scales_b[w] = from.scales + min(n0, p.n - 1) / kBlock * from.srs;
+        scales_b[w] = from.scales + f8::least(n0, p.n - 1) / kBlock * from.srs;
     }
 
     const int64_t depth_blocks = blocks_of(p.k);
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(64 * WK) void few_rows_kernel(Params p) {
     };
     Block ring[DEEP];
     const auto load = [&](Block& to, int64_t kb) __attribute__((always_inline)) {
-        const int64_t at[2] = {min(kb * 8 + g, last_piece) * 16, min(kb * 8 + 4 + g, last_piece) * 16};
+        const int64_t at[2] = {f8::least(kb * 8 + g, last_piece) * 16, f8::least(kb * 8 + 4 + g, last_piece) * 16};
 #pragma unroll
         for (int w = 0; w < kWeights; ++w) {
 #pragma unroll
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(64 * WK) void few_rows_kernel(Params p) {
     // Wavefront wk takes a run of neighbouring blocks.
     const int64_t run = (depth_blocks + WK - 1) / WK;
     const int64_t begin = wk * run;
-    const int64_t end = min(begin + run, depth_blocks);
+    const int64_t end = f8::least(begin + run, depth_blocks);
 #pragma unroll
     for (int d = 0; d < DEEP; ++d) {
         if (begin + d < end) {

@@ -165,14 +165,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         blockIdx.x < per_xcd * 8 ? blockIdx.x % 8 * per_xcd + blockIdx.x / 8 : blockIdx.x;
     const uint32_t group_rows = p.tiles_m < 8 ? p.tiles_m : 8;
     const uint32_t group = logical / (group_rows * p.tiles_n);
-    const uint32_t rows_here = min(group_rows, p.tiles_m - group * group_rows);
+    const uint32_t rows_here = f8::least(group_rows, p.tiles_m - group * group_rows);
     const uint32_t in_group = logical - group * group_rows * p.tiles_n;
     const int64_t m0 = static_cast<int64_t>(group * group_rows + in_group % rows_here) * BM;
     const int64_t n0 = static_cast<int64_t>(in_group / rows_here) * BN;
 
     // This workgroup's blocks of the depth: [first_block, end_block).
     const int64_t first_block = blockIdx.y * p.split_blocks;
-    const int64_t end_block = min(first_block + p.split_blocks, blocks_of(p.k));
+    const int64_t end_block = f8::least(first_block + p.split_blocks, blocks_of(p.k));
     const bool ragged = p.k % kBlock != 0 && end_block == blocks_of(p.k);
 
     // Copies of a slice: 8 threads take a row's pieces, kRowStep rows a round. An operand's resource
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const auto operand = [&](const Matrix& m, int64_t row, int64_t rows) {
         const int64_t bytes = (rows - row - 1) * m.rs + row_bytes - first_block * kBlock;
         return resource(m.values + row * m.rs + first_block * kBlock,
-                        static_cast<uint32_t>(min(bytes, static_cast<int64_t>(kNothing))));
+                        static_cast<uint32_t>(f8::least(bytes, static_cast<int64_t>(kNothing))));
     };
     const intx4 from_a = operand(p.a, m0, p.m);
     const intx4 from_b = operand(p.b, n0, p.n);
@@ -224,8 +224,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     const int64_t last_scale = (of_a ? p.m : blocks_of(p.n)) - 1 - first_scale;
     const bool has_scales = (of_a && last_scale >= 0) || of_b;
     const uint32_t scale_offset =
-        static_cast<uint32_t>(min(static_cast<int64_t>(of_a ? lane : lane % kBlocksN),
-                                  max(last_scale, static_cast<int64_t>(0)))) *
+        static_cast<uint32_t>(f8::least(static_cast<int64_t>(of_a ? lane : lane % kBlocksN),
+                                  f8::most(last_scale, static_cast<int64_t>(0)))) *
         static_cast<uint32_t>(scaled.srs) * 4;
     // In scalar registers: fetched anew for each slice, they would be waited for.
     const auto scalar = [](uint64_t v) {
@@ -600,7 +600,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
                     dev::store_quad(line + 8 * x, quad, left - 8 * x);
                 }
             }
-            top[i] = max(top[i], dev::magnitude(quad));
+            top[i] = f8::most(top[i], dev::magnitude(quad));
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -613,7 +613,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
     __syncthreads(); // the slices have been read
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-        top[i] = max(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 32, 64)));
+        top[i] = f8::most(top[i], static_cast<uint32_t>(__shfl_xor(static_cast<int>(top[i]), 32, 64)));
         if (half == 0) {
             tops[wn][wm * (BM / WM) + 32 * i + r32] = top[i];
         }
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         const int64_t row = row0 + 32 * i;
 #pragma unroll
         for (int w = 0; w < kSharing; ++w) {
-            top[i] = max(top[i],
+            top[i] = f8::most(top[i],
                          tops[wn / kSharing * kSharing + w][wm * (BM / WM) + 32 * i + r32]);
         }
         const float scale = dev::scale_of(top[i]);

@@ -1,6 +1,7 @@
 // The 8-bit ops through the public API: a feed-forward block on the rocm device against doubles,
 // device-resident and from host tensors; what the CPU has no kernel for; the checks of arguments.
 #include "core/dispatcher.hpp"
+#include "oracle_cpu.hpp"
 #include "test_util.hpp"
 
 #include <algorithm>
@@ -170,6 +171,7 @@ void test_checks() {
 
 int main(int argc, char** argv) {
     return test::run("f8_test", argc, argv, [] {
+        test::register_oracle_cpu_kernels(); // normal and uniform
         test_checks();
         test_cpu_has_no_kernels();
         for (const Device device : test::devices()) {
