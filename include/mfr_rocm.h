@@ -399,8 +399,9 @@ int mfr_attention(mfr_stream_t stream, const mfr_attention_desc* desc);
 /* A matrix of e4m3 values (OCP: 4 exponent bits, 3 of mantissa, no infinities, largest 448) with
  * fp32 scales: element (r, c) stands for value(r, c) * scale(r / block_rows, c / 128), scale (i, j)
  * at scales[i * scales_rs + j * scales_cs]. Rows are contiguous and rs bytes apart; the base and rs
- * are multiples of 16 bytes, rs at least the row's length and at most 2^24, scales_rs at most 2^23. A row is read in whole 16-byte pieces,
- * so the bytes between its end and the next multiple of 16 are read (not used, never written).
+ * are multiples of 16 bytes, rs at least the row's length and at most 2^24; scales_rs is at most
+ * 2^23, scales_cs 2^40, and in an input either may be 0. A row is read in whole 16-byte pieces, so
+ * the bytes between its end and the next multiple of 16 are read (not used, never written).
  * block_rows is 1 (activations: a scale per row and 128 columns) or 128 (weights: one per 128 x 128
  * block). Columns of scales that lie together (scales_rs = 1) suit mfr_f8gemm's loads best. */
 typedef struct mfr_f8_matrix {
@@ -428,8 +429,8 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
  * sum = t is written where sum is not NULL (the residual stream for the next block), out = y where
  * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize) where out_f8.values is
  * not NULL; at least one of out and out_f8. residual and weight may be NULL (0 and 1). t is
- * rounded to fp32, the squares are summed in double in an order that depends on cols alone, and y
- * is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
+ * rounded to fp32, the squares are summed in double in an order that depends on rows and cols alone,
+ * and y is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
  * least cols. sum or out may be x or residual itself (the same base and row stride), not one
  * another; other overlaps of outputs with anything are undefined. A NaN in a row makes the row NaN;
  * an infinity becomes NaN and the row's other elements 0, the formula's values. A row of zeros gives
@@ -464,9 +465,12 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
  *
  *   c(i, j) = fl( act(P_B(i, j)) * P_up(i, j) ).
  *
- * The inner sums are of exact products on the 8-bit matrix cores in fp32, the outer ones in fp32 in
- * the order of b (ranges of b where the depth is split, added in order): the same inputs give the
- * same bits on every call. c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8
+ * The inner sums are of exact products on the bf16 matrix cores in fp32 (e4m3 numbers are bf16
+ * numbers), the outer ones in fp32 in the order of b, by ranges of b that are added in order where
+ * the depth is split: the same call gives the same bits every time. Ranges and products of few rows
+ * that end in out_f8 alone go through the stream's workspace; under stream capture, where none is
+ * taken, such a call runs without (slower, and by other ranges than eagerly). A captured product of
+ * few rows that is given c besides out_f8 needs no workspace and runs as it does eagerly. c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8
  * is given, out_f8.values may be NULL where c is: c in 8 bits, as mfr_f8_quantize gives it
  * (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
  * outputs with operands are undefined. k == 0 gives the epilogue of zero products. The product of

@@ -671,7 +671,8 @@ def _f8_desc(m: F8Matrix | None, what: str) -> abi.F8Desc:
         raise ValueError(f"{what}: scales {m.scales.shape}, {blocks} are needed")
     if cols > 1 and m.values.strides[1] != 1:
         raise ValueError(f"{what}: rows need unit stride")
-    d.values, d.rs = m.values.ptr, m.values.strides[0]
+    d.values = m.values.ptr
+    d.rs = m.values.strides[0] if rows > 1 else -(-cols // 16) * 16
     d.scales, (d.scales_rs, d.scales_cs) = m.scales.ptr, m.scales.strides
     d.block_rows = m.block_rows
     return d
@@ -685,7 +686,16 @@ def _rows_of(t: DeviceArray | None, shape, what: str) -> tuple:
         raise ValueError(f"{what}: {t.dtype} {t.shape}, float32 {tuple(shape)} is needed")
     if shape[1] > 1 and t.strides[1] != 1:
         raise ValueError(f"{what}: rows need unit stride")
-    return t.ptr, t.strides[0]
+    # The stride of a single row says nothing.
+    return t.ptr, t.strides[0] if shape[0] > 1 else max(t.strides[0], shape[1])
+
+
+def _one_device(what: str, *operands) -> None:
+    """Refuses arrays and F8Matrix operands (None: not given) of more than one device."""
+    arrays = [a for t in operands if t is not None
+              for a in ((t.values, t.scales) if isinstance(t, F8Matrix) else (t,))]
+    if len({a.stream.device for a in arrays}) > 1:
+        raise ValueError(f"{what}: operands of different devices")
 
 
 def _vector_of(t: DeviceArray | None, length: int, what: str):
@@ -705,6 +715,7 @@ def quantize_f8(x: DeviceArray, block_rows: int = 1, out: F8Matrix | None = None
         out = F8Matrix.empty(rows, cols, x.stream, block_rows)
     if out.shape != x.shape or out.block_rows != block_rows:
         raise ValueError(f"quantize_f8: out is {out.shape} with block_rows {out.block_rows}")
+    _one_device("quantize_f8", x, out)
     d = _f8_desc(out, "quantize_f8: out")
     abi.check(abi.load().mfr_f8_quantize(x.stream.handle, rows, cols, ptr, rs, ctypes.byref(d)),
               "mfr_f8_quantize")
@@ -719,6 +730,7 @@ def rms_norm_desc(x: DeviceArray, weight: DeviceArray | None = None, *,
     many times (rms_norm_run): t = x + residual to `summed`, t / rms(t) * weight to `out` (fp32)
     and `out_f8` (8 bits), whichever are given."""
     rows, cols = x.shape
+    _one_device("rms_norm", x, weight, residual, summed, out, out_f8)
     d = RmsNormDesc()
     d.rows, d.cols, d.eps = rows, cols, eps
     d.x, d.x_rs = _rows_of(x, x.shape, "rms_norm: x")
@@ -772,6 +784,7 @@ def f8gemm_desc(a: F8Matrix, b: F8Matrix, *, up: F8Matrix | None = None, act=ACT
             raise ValueError(f"f8gemm: a is {a.shape}, a weight {w.shape}")
     if out_f8 is not None and out_f8.shape != (m, n):
         raise ValueError(f"f8gemm: out_f8 is {out_f8.shape}, {(m, n)} is needed")
+    _one_device("f8gemm", a, b, up, c0, bias, out, out_f8)
     d = F8GemmDesc()
     d.m, d.n, d.k = m, n, k
     d.a, d.b, d.up = _f8_desc(a, "f8gemm: a"), _f8_desc(b, "f8gemm: b"), _f8_desc(up, "f8gemm: up")
@@ -804,7 +817,8 @@ def gemm_f8_gated(a: F8Matrix, gate: F8Matrix, up: F8Matrix, *, act=ACT_SILU,
                   out: DeviceArray | None = None, out_f8: F8Matrix | None = None):
     """act(a gate^T) * (a up^T), both projections in one kernel: in 8 bits for the next product (a
     new F8Matrix), or to `out` (fp32) and / or `out_f8` where they are given. Returns out_f8 where
-    that is given or made, else out."""
+    that is given or made, else out. A call of few rows that is captured into a graph is faster
+    with both: the sums then need no workspace, which a captured call does not take."""
     if out is None and out_f8 is None:
         out_f8 = F8Matrix.empty(a.shape[0], gate.shape[0], a.stream)
     f8gemm(a.stream, f8gemm_desc(a, gate, up=up, act=act, out=out, out_f8=out_f8))

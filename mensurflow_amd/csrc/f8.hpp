@@ -20,6 +20,11 @@ constexpr float kLeastScale = 0x1p-126f;
 constexpr int64_t kMostRowBytes = int64_t{1} << 24;
 constexpr int64_t kMostScaleStride = int64_t{1} << 23;
 
+// More rows, or column blocks of scales further apart, are no memory's: their products stay inside
+// 64 bits.
+constexpr int64_t kMostRows = int64_t{1} << 40;
+constexpr int64_t kMostScaleStep = int64_t{1} << 40;
+
 // Of two values of one type. (HIP's own min and max take 64-bit values for ints in host code.)
 template <typename T> __host__ __device__ constexpr T least(T a, T b) { return b < a ? b : a; }
 template <typename T> __host__ __device__ constexpr T most(T a, T b) { return a < b ? b : a; }
@@ -49,9 +54,10 @@ inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int bl
         return m;
     }
     require(d.values != nullptr && d.scales != nullptr, at + " has a null pointer");
+    require(rows <= kMostRows, at + " has too many rows");
     require(d.rs >= cols, at + " has rows that overlap");
-    if (d.rs > kMostRowBytes || d.scales_rs > kMostScaleStride) {
-        throw Error(MFR_E_UNSUPPORTED, at + " has rows that lie too far apart");
+    if (d.rs > kMostRowBytes || d.scales_rs > kMostScaleStride || d.scales_cs > kMostScaleStep) {
+        throw Error(MFR_E_UNSUPPORTED, at + " has rows or scales that lie too far apart");
     }
     require(d.scales_rs >= 0 && d.scales_cs >= 0, at + " has negative scale strides");
     if (!aligned16(d.values) || d.rs % 16 != 0) {

@@ -353,14 +353,13 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
         if (out->block_rows == 1) {
             mfr::f8::quantize_rows(s, x, x_rs, rows, cols, q);
             return;
-        } else {
-            const int64_t col_blocks = mfr::f8::blocks_of(cols);
-            const int64_t blocks = mfr::f8::blocks_of(rows) * col_blocks;
-            mfr::require(mfr::one_launch(blocks, kThreads), "f8_quantize: matrix too large");
-            quantize_blocks_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s.stream>>>(
-                x, x_rs, rows, cols, q, col_blocks);
         }
-        mfr::check_launch("f8_quantize kernel");
+        const int64_t col_blocks = mfr::f8::blocks_of(cols);
+        const int64_t blocks = mfr::f8::blocks_of(rows) * col_blocks;
+        mfr::require(mfr::one_launch(blocks, kThreads), "f8_quantize: matrix too large");
+        quantize_blocks_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, s.stream>>>(
+            x, x_rs, rows, cols, q, col_blocks);
+        mfr::check_launch("quantize_blocks_kernel");
     });
 }
 

@@ -12,6 +12,8 @@ namespace {
 using mfr::f8::blocks_of;
 using mfr::f8gemm::Params;
 
+constexpr int64_t kMostOutputs = int64_t{1} << 44;
+
 // The descriptor's checks (of shapes, layouts and pointers: no device is needed).
 Params checked(const mfr_f8gemm_desc* desc) {
     using mfr::require;
@@ -39,6 +41,7 @@ Params checked(const mfr_f8gemm_desc* desc) {
     const bool add = d.c0 != nullptr && d.beta != 0.0f;
     require(d.c != nullptr || d.out_f8.values != nullptr,
             "f8gemm: neither c nor out_f8 is given");
+    require(d.m <= kMostOutputs / d.n, "f8gemm: problem too large");
     require(d.c == nullptr || d.c_rs >= d.n, "f8gemm: c has rows that overlap");
     require(!add || d.c0_rs >= d.n, "f8gemm: c0 has rows that overlap");
     require(!add || d.c0 != d.c || d.c0_rs == d.c_rs,

@@ -102,6 +102,7 @@ F8 = [
     (dict(rs=-208), abi.MFR_E_INVALID, "overlap"),
     (dict(rs=(1 << 24) + 16), abi.MFR_E_UNSUPPORTED, "too far apart"),
     (dict(scales_rs=(1 << 23) + 1), abi.MFR_E_UNSUPPORTED, "too far apart"),
+    (dict(scales_cs=(1 << 40) + 1), abi.MFR_E_UNSUPPORTED, "too far apart"),
     (dict(scales=None), abi.MFR_E_INVALID, "null pointer"),
     (dict(scales_rs=-1), abi.MFR_E_INVALID, "negative scale strides"),
 ]
@@ -204,3 +205,48 @@ def test_python_refuses_shapes_that_disagree():
         mf.f8gemm_desc(bad, matrix(200, 300, 128), out=array((4, 200)))
     with pytest.raises(ValueError):
         mf.quantize_f8(x, 128, out=matrix(4, 100, 1))
+
+
+def test_sizes_past_64_bits_are_refused():
+    """Products of sizes that would leave 64 bits: refused by the sizes, before any launch."""
+    for change in (dict(m=1 << 41), dict(n=1 << 41), dict(m=1 << 30, n=1 << 20)):
+        d = good_gemm(out_f8=None)
+        d.c_rs = 1 << 50
+        for name, value in change.items():
+            setattr(d, name, value)
+        status, message = call("mfr_f8gemm", d)
+        assert status == abi.MFR_E_INVALID and ("too many rows" in message or
+                                                "too large" in message), message
+    lib = abi.load()
+    for block_rows in (1, 128):
+        d = mf._f8_desc(matrix(4, 100, block_rows), "x")
+        assert lib.mfr_f8_quantize(None, 1 << 41, 100, 1 << 24, 100,
+                                   ctypes.byref(d)) == abi.MFR_E_INVALID
+        assert "too many rows" in abi.last_error()
+
+
+def test_a_single_row_has_any_stride():
+    row = array((1, 100), strides=(1, 1))
+    d = mf.rms_norm_desc(row, residual=row, summed=row, out_f8=matrix(1, 100))
+    assert (d.x_rs, d.residual_rs, d.sum_rs) == (100, 100, 100)
+    q = matrix(1, 100)
+    q.values = array((1, 100), np.uint8, (1, 1))
+    assert mf.f8gemm_desc(q, matrix(20, 100, 128), out=array((1, 20))).a.rs == 112
+    for entry, desc in (("mfr_rms_norm", d),
+                        ("mfr_f8gemm", mf.f8gemm_desc(q, matrix(20, 100, 128),
+                                                      out=array((1, 20))))):
+        assert call(entry, desc) == (abi.MFR_E_INVALID, "null stream")
+
+
+def test_python_refuses_operands_of_two_devices():
+    other = SimpleNamespace(device=1, handle=None)
+    x = array((4, 100))
+    far = mf.DeviceArray.wrap(1 << 20, (4, 100), other)
+    far_f8 = mf.F8Matrix(mf.DeviceArray.wrap(1 << 20, (200, 100), other, np.uint8, (112, 1)),
+                         mf.DeviceArray.wrap(1 << 20, (2, 1), other), 128)
+    with pytest.raises(ValueError, match="devices"):
+        mf.rms_norm_desc(x, residual=far, out=x)
+    with pytest.raises(ValueError, match="devices"):
+        mf.quantize_f8(far, out=matrix(4, 100))
+    with pytest.raises(ValueError, match="devices"):
+        mf.f8gemm_desc(matrix(4, 100), far_f8, out=array((4, 200)))
