@@ -2,6 +2,7 @@
 // (f8gemm_finish.hpp) and the form for few rows (f8gemm_few.hpp).
 #include "f8gemm_few.hpp"
 #include "f8gemm_finish.hpp"
+#include "f8gemm_ring.hpp"
 
 #include <algorithm>
 #include <limits>
@@ -59,7 +60,18 @@ Params checked(const mfr_f8gemm_desc* desc) {
 // 8192, n = 1024 .. 16384 and k = 1024 .. 8192: a fixed part, and one per block of the depth that a
 // workgroup or wavefront walks, by how many workgroups a CU has. The least of them is taken.
 
-enum class Form { kFew16, kFew32, kFew32Wide, kFew64, kTile64, kTile128 };
+enum class Form {
+    kFew16,
+    kFew32,
+    kFew32Wide,
+    kFew64,
+    kRing32,
+    kRing32Wide,
+    kRing64,
+    kRing64Pair,
+    kTile64,
+    kTile128
+};
 
 // A workgroup's rows and columns, the wavefronts that share the depth, and a wavefront's time per
 // block with one workgroup per CU. Measured, k = 4096 (32 blocks): 16 x 4096 5.8 us and 16 x 16384
@@ -79,19 +91,42 @@ constexpr Few kFewGated[] = {{Form::kFew16, 16, 16, 8, 1.5},
                              {Form::kFew32, 32, 16, 8, 2.3},
                              {Form::kFew64, 64, 16, 4, 1.7}};
 
-// A tile's workgroups per CU at once, its fixed time, and the time of a block when every CU has
-// them all, or one alone on few CUs. Measured, k = 4096: 64 x 128 tiles on 64 CUs 21.8 us, one on
-// every CU 26.8, two 40.1; 128 x 128 31.4 on 32 CUs, 35.1 on 128, 42.2 on all (8192^3, two on each
-// 930); gated 64 x 128 35.4 on 128 CUs (8192 x 10240 x 4096 1520), 128 x 128 49.3 on 64 (1230).
+// A ring's rows and columns, the slices of a turn, how many share a CU, what a workgroup takes
+// besides its turns, and the time of a turn when every CU has them all, or one alone. Measured, a
+// round of every CU at k = 1024, 4096, 8192: 32 x 32 4.3, 7.9, 13.4 us; 32 x 64 5.4, 9.8, 16.3; 64 x 64
+// 7.6, 14.6, 24.5, two on a CU 9.5, 23, 43; gated, k = 4096: 32 x 32 12, 64 x 32 15.5, two 23.5.
+struct Ring {
+    Form form;
+    int64_t rows, cols, slices, at_once;
+    double start, full, alone;
+};
+constexpr double kRingFixed = 2.0;
+constexpr Ring kRings[] = {{Form::kRing32, 32, 32, 8, 1, 3.0, 1.28, 1.28},
+                           {Form::kRing32Wide, 32, 64, 4, 1, 3.7, 0.78, 0.78},
+                           {Form::kRing64, 64, 64, 3, 1, 4.5, 0.88, 0.88},
+                           {Form::kRing64Pair, 64, 64, 2, 2, 3.0, 1.26, 1.0}};
+constexpr Ring kRingsGated[] = {{Form::kRing32, 32, 32, 4, 1, 3.7, 1.04, 1.04},
+                                {Form::kRing64, 64, 32, 4, 1, 3.5, 1.5, 1.5},
+                                {Form::kRing64Pair, 64, 32, 2, 2, 3.0, 1.28, 0.95}};
+
+// The rate at which a ring's weights come from memory at most (32 x 16384 x 4096).
+constexpr double kBytesPerUs = 4.6e6;
+
+// A tile's workgroups per CU at once, what a round of them takes besides its blocks (the first
+// loads and the outputs, 32 MB a round of the larger tile), and the time of a block when every CU
+// has them all, or one alone on few CUs. Measured, n = 8192, every CU full: 64 x 128 tiles, one round,
+// k = 1024 16.3 us, 2304 27.8; 128 x 128 25.1, 45.4 and 76 at 4096, two rounds of 1024 48.6; gated
+// 64 x 128 37 us a round of k = 4096, 128 x 128 59.
 struct Tile {
     Form form;
     int64_t rows, at_once;
-    double fixed, full, alone;
+    double start, full, alone;
 };
-constexpr Tile kTiles[] = {{Form::kTile64, 64, 2, 4.5, 1.12, 0.55},
-                           {Form::kTile128, 128, 2, 5.7, 1.8, 0.8}};
-constexpr Tile kTilesGated[] = {{Form::kTile64, 64, 1, 6.0, 1.2, 0.92},
-                                {Form::kTile128, 128, 1, 8.0, 1.92, 1.29}};
+constexpr double kTileFixed = 2.5;
+constexpr Tile kTiles[] = {{Form::kTile64, 64, 2, 4.0, 1.2, 0.55},
+                           {Form::kTile128, 128, 2, 6.3, 1.95, 0.8}};
+constexpr Tile kTilesGated[] = {{Form::kTile64, 64, 1, 3.8, 1.1, 0.92},
+                                {Form::kTile128, 128, 1, 6.0, 1.75, 1.29}};
 constexpr int64_t kTileCols = 128;
 
 // The second launch of a depth in ranges and the memory it reads; the second launch of few rows
@@ -120,10 +155,13 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
         }
     };
     const auto few = [&](const Few& f) {
-        const double groups =
-            static_cast<double>(ceil_div(p.m, f.rows)) * static_cast<double>(ceil_div(p.n, f.cols));
+        // The CUs' share of the workgroups: the memory sees the mean, a CU's wavefronts the most;
+        // between them where small workgroups mingle.
+        const int64_t groups = ceil_div(p.m, f.rows) * ceil_div(p.n, f.cols);
+        const double most = static_cast<double>(ceil_div(groups, cus));
+        const double mean = std::max(1.0, static_cast<double>(groups) / static_cast<double>(cus));
         double time = kFewFixed + static_cast<double>(ceil_div(blocks, f.waves)) * f.block *
-                                      std::max(1.0, groups / static_cast<double>(cus));
+                                      (f.rows < 64 ? (most + mean) / 2.0 : most);
         int64_t bytes = 0;
         if (p.q.values != nullptr) {
             time += kConvertFixed;
@@ -133,17 +171,38 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
             offer(f.form, 1, time, bytes);
         }
     };
+    const double weights = (gated ? 2.0 : 1.0) * static_cast<double>(p.n) * static_cast<double>(p.k);
+    const auto ring = [&](const Ring& r) {
+        const int64_t groups = ceil_div(p.m, r.rows) * ceil_div(p.n, r.cols);
+        const int64_t slots = cus * r.at_once;
+        const int64_t rest = groups % slots;
+        const double turns = static_cast<double>(ceil_div(blocks, r.slices));
+        double time = static_cast<double>(groups / slots) * (r.start + turns * r.full);
+        if (rest > 0) {
+            time += r.start + turns * (rest > cus ? r.full : r.alone);
+        }
+        time = kRingFixed + std::max(time, weights / kBytesPerUs);
+        int64_t bytes = 0;
+        if (p.q.values != nullptr) {
+            time += kConvertFixed;
+            bytes = p.c != nullptr ? 0 : 4 * p.m * p.n;
+        }
+        offer(r.form, 1, time, bytes);
+    };
     const auto tiles = [&](const Tile& t) {
         for (int64_t splits = 1; splits <= 8 && splits <= std::max(blocks, int64_t{1}); splits *= 2) {
             const int64_t groups = ceil_div(p.m, t.rows) * ceil_div(p.n, kTileCols) * splits;
             const int64_t slots = cus * t.at_once;
             const int64_t rest = groups % slots;
+            const double walked = static_cast<double>(ceil_div(blocks, splits));
             // The second workgroup of a CU, and the CUs' rivalry when all are busy, bring `alone`
             // to `full`.
             const double share = static_cast<double>(rest) / static_cast<double>(slots);
-            const double part = rest == 0 ? 0.0 : t.alone + (t.full - t.alone) * share * share;
-            double time = t.fixed + static_cast<double>(ceil_div(blocks, splits)) *
-                                        (static_cast<double>(groups / slots) * t.full + part);
+            double time = kTileFixed + static_cast<double>(groups / slots) * (t.start + walked * t.full);
+            if (rest > 0) {
+                time += t.start * (0.5 + 0.5 * share) +
+                        walked * (t.alone + (t.full - t.alone) * share * share);
+            }
             int64_t bytes = 0;
             if (splits > 1) {
                 bytes = splits * (gated ? 2 : 1) * 4 * p.m * p.n;
@@ -156,12 +215,18 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
         for (const Few& f : kFewGated) {
             few(f);
         }
+        for (const Ring& r : kRingsGated) {
+            ring(r);
+        }
         for (const Tile& t : kTilesGated) {
             tiles(t);
         }
     } else {
         for (const Few& f : kFew) {
             few(f);
+        }
+        for (const Ring& r : kRings) {
+            ring(r);
         }
         for (const Tile& t : kTiles) {
             tiles(t);
@@ -186,6 +251,18 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     case Form::kFew64:
         (gated ? launch_few<4, 1, 4, 1, true> : launch_few<4, 2, 8, 1, false>)(s, p);
         break;
+    case Form::kRing32:
+        (gated ? launch_ring<1, 1, 4, 3, true> : launch_ring<1, 1, 8, 2, false>)(s, p);
+        break;
+    case Form::kRing32Wide:
+        launch_ring<1, 2, 4, 3, false>(s, p);
+        break;
+    case Form::kRing64:
+        (gated ? launch_ring<2, 1, 4, 2, true> : launch_ring<2, 2, 3, 3, false>)(s, p);
+        break;
+    case Form::kRing64Pair:
+        (gated ? launch_ring<2, 1, 2, 2, true> : launch_ring<2, 2, 2, 2, false>)(s, p);
+        break;
     case Form::kTile64:
         (gated ? launch_tiles<64, 128, 2, 4, 3, true> : launch_tiles<64, 128, 1, 4, 2, false>)(
             s, p, plan.splits);
@@ -197,6 +274,7 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     }
 }
 
+// Whether the form leaves an 8-bit output to a second launch.
 bool is_few(Form f) { return f != Form::kTile64 && f != Form::kTile128; }
 
 void run_region(mfr_stream& s, Params p, Plan plan) {

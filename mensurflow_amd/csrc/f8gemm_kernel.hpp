@@ -88,9 +88,9 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
     return r;
 }
 
-// One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at `lane_offset`
-// + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past the resource
-// (its range counts both offsets). In assembly, because the compiler waits for every such copy that
+// One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at
+// `lane_offset` + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past
+// the resource (its range counts both offsets). In assembly, because the compiler waits for every such copy that
 // it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is what
 // waits here. No register is written.
 template <int BYTES>
@@ -113,8 +113,8 @@ __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, ui
 
 // A tile of BM x BN outputs (BN of each projection when GATED) by WM x WN wavefronts. Depth slices
 // of one block (128 bytes of a row) are copied to LDS in 16-byte pieces, piece c of row r at place
-// c ^ (r / 2 % 8), so that 16 rows of a fragment lie in different banks (64 of 4 bytes, two rows); while one slice is
-// multiplied the next is on its way.
+// c ^ (r / 2 % 8), so that 16 rows of a fragment lie in different banks (64 of 4 bytes, two rows);
+// while one slice is multiplied the next is on its way.
 //
 // A wavefront keeps its columns' fragments of a slice in registers, as bf16, and takes its rows 32
 // at a time: 8 v_mfma_f32_32x32x16_bf16 give the block's inner sums of 32 x 32 outputs, which the
@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
         float scales[BM];
         float scales_b[kWeights][64]; // of block columns
     };
-    static_assert(SLICES == 2 || SLICES == 3, "");
+    static_assert(SLICES == 2 || SLICES == 3, "the loop takes turns of two or three");
     __shared__ __align__(16) Slice slice0;
     __shared__ __align__(16) Slice slice1;
     __shared__ __align__(16) Slice slice2;

@@ -1,5 +1,5 @@
-"""The forms of mfr_f8gemm that sizes choose between (tiles of 64 and 128 rows, the depth in ranges,
-few rows, strips past a multiple of 128 by themselves), each with every kind of output, and what is
+"""The forms of mfr_f8gemm that sizes choose between (few rows, rings of slices, tiles of 64 and 128
+rows, the depth in ranges, strips past a multiple of 128 by themselves), each with every kind of output, and what is
 queued around them: calls of two threads on one stream, on two streams, a workspace that grows,
 graphs that are replayed between eager calls."""
 import ctypes
@@ -18,10 +18,13 @@ pytestmark = pytest.mark.gpu
 
 # Sums of 9000 products of whole values up to 16 under scales up to 4 stay below 2^22 on average by
 # far; the tests assert it of the magnitudes' sums, which makes every partial sum exact.
-FORMS = [(2, 4683, 454), (17, 2816, 8567), (740, 125, 549),     # few rows; many ranges; one column
-         (99, 2559, 3360), (155, 3457, 2499), (129, 4481, 2757),  # 64-row tiles in ranges
-         (67, 2842, 2664), (74, 4534, 2294), (65, 4507, 4438),    # the gated ones
-         (193, 4382, 7538), (2335, 385, 6024), (1025, 137, 8767),  # 128-row tiles in ranges
+FORMS = [(2, 4683, 454), (740, 125, 549), (35, 5759, 786), (105, 2437, 549),  # few rows
+         (1, 6913, 5450), (3, 8300, 1000), (128, 4100, 1100), (99, 2559, 3360),  # rings
+         (155, 3457, 2499), (258, 6145, 4260), (65, 4507, 4438), (200, 4096, 2048),
+         (39, 4097, 3153), (201, 4674, 4375), (2051, 195, 5841),  # 64-row tiles in ranges
+         (65, 4122, 2921), (268, 1664, 5874), (17, 2816, 8567),  # the gated ones
+         (193, 4382, 7538), (210, 4112, 8909), (2335, 385, 6024),  # 128-row tiles in ranges
+         (2305, 19, 8334), (1025, 137, 8767),                     # the gated ones
          (1349, 2945, 130), (639, 3208, 271),                     # and whole
          (1883, 4353, 777), (1668, 4863, 642), (2304, 1802, 629),  # a strip of columns, of rows
          (2176, 3843, 1335), (2051, 3971, 1064),
@@ -125,7 +128,7 @@ def test_scales_of_stride_zero(stream, m, n, k):
 
 
 # One of each kind that takes the workspace: a depth in ranges, few rows in 8 bits alone.
-SHARED = [(99, 2559, 3360), (4, 4000, 4100), (193, 4382, 2100)]
+SHARED = [(39, 4097, 3153), (4, 4000, 4100), (210, 4112, 8909)]
 
 
 def make_calls(stream, seed):
