@@ -4,7 +4,8 @@ The product is two native libraries built in-tree (``mensurflow_amd/build.py``):
 
 * ``_lib/libmfr_rocm.so``: hand-written HIP kernels behind the C ABI of
   ``include/mfr_rocm.h`` (fp32-MFMA GEMM with a fused epilogue, HBM-bound gemv, softmax,
-  where, bias+gelu, argmax, strided copy);
+  where, bias+gelu, argmax, strided copy; for serving in 8 bits, RMS norm, conversion to e4m3 with
+  block scales, and products of such matrices);
 * ``_lib/libmensurflow.so``: the C++17 host layer that plugs those kernels into mensurflow's
   ``Backend``/``Dispatcher`` API as the ``rocm`` device.
 

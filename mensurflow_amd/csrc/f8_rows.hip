@@ -15,7 +15,8 @@ namespace dev = mfr::f8::dev;
 constexpr int kThreads = 256;
 constexpr int kStep = 4 * kThreads; // columns per workgroup step
 
-// A workgroup takes 1024 columns of a row at a time, a thread 4, 32 lanes a block.
+// A workgroup takes 1024 columns of a row at a time, a thread 4, 32 lanes a block: one read, one
+// write, no LDS. 2000 x 1960: 6.0 us, 3.3 TB/s, of which launch and tail are half.
 __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const float* x, int64_t x_rs,
                                                                  int64_t groups, int64_t cols,
                                                                  uint32_t col_groups, Matrix q) {
@@ -26,7 +27,8 @@ __global__ __launch_bounds__(kThreads) void quantize_rows_kernel(const float* x,
     }
 }
 
-// A workgroup per 128 x 128 block.
+// A workgroup per 128 x 128 block, all of it in registers between the one read and the one write:
+// bound by memory. 16384 x 4096: 62 us, 5.4 TB/s.
 __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(const float* x, int64_t x_rs,
                                                                    int64_t rows, int64_t cols,
                                                                    Matrix q, int64_t col_blocks) {
@@ -156,7 +158,9 @@ __device__ inline float4 weight_at(const NormParams& p, int64_t col) {
 // A row in the registers of THREADS threads, QUADS x 4 columns each: every element is read once,
 // all of a thread's loads before the first use. A workgroup takes one row, or 4 where a wavefront
 // holds a row. Bound by memory; the double arithmetic (2 conversions, a multiply-add and 2
-// products an element) is under a fifth of the vector units' time at that rate.
+// products an element) and the rest take a third of the vector units' time at that rate. With residual,
+// sum and 8 bits: 16384 x 8192 333 us, 5.25 TB/s (two passes over the row 364), 1 x 4096 4.3 us (6.4);
+// fp32 alone, 4093 x 1023 8.5 us (10.8).
 template <int THREADS, int QUADS>
 __global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void rms_norm_kernel(
     NormParams p) {

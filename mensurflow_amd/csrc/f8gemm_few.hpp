@@ -7,6 +7,8 @@
 // bf16 and multiplies: 4 v_mfma_f32_16x16x32_bf16 per 16 x 16 block, added to the outer sum with the
 // two scales. DEEP blocks are in flight. The wavefronts' sums are added through LDS in the order of
 // the depths' runs, so nothing here needs memory of its own and a captured call is like any other.
+// 1 x 4096 x 4096: 6.0 us, launch and 4 blocks a wavefront at memory's latency (tiles 26.7); gated
+// 1 x 10240 x 4096: 17.3 us, 4.9 TB/s.
 #pragma once
 
 #include "f8gemm_kernel.hpp"
@@ -59,7 +61,8 @@ __global__ __launch_bounds__(64 * WK) void few_rows_kernel(Params p) {
     };
     Block ring[DEEP];
     const auto load = [&](Block& to, int64_t kb) __attribute__((always_inline)) {
-        const int64_t at[2] = {f8::least(kb * 8 + g, last_piece) * 16, f8::least(kb * 8 + 4 + g, last_piece) * 16};
+        const int64_t at[2] = {f8::least(kb * 8 + g, last_piece) * 16,
+                               f8::least(kb * 8 + 4 + g, last_piece) * 16};
 #pragma unroll
         for (int w = 0; w < kWeights; ++w) {
 #pragma unroll

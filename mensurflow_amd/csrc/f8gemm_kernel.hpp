@@ -123,6 +123,11 @@ __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, ui
 // gives to the 8 instructions are 64 neighbouring ones for both operands: which depth stands where
 // does not matter to a sum as long as it is the same for both.
 //
+// What bounds it: 8192^3 takes 940 to 980 us by the clock that the power leaves (1120 to 1170
+// TFLOP/s; matrix cores 62 % busy at 1.74 GHz, vector units 58 %; without the copies 13 % less). 4096 x
+// 4096 x 1024 takes 42 us, two rounds of 8 blocks, 12 of them for outputs that nothing runs under.
+// Gated, 8192 x 10240 x 4096 with 8 bits out: 1170 us (1170 TFLOP/s).
+//
 // SLICES of them lie in LDS: with two, a slice is under way while one is multiplied, which covers
 // memory's latency where two workgroups share a CU; with three, two are.
 template <int BM, int BN, int WM, int WN, int SLICES, bool GATED>
