@@ -101,6 +101,7 @@ struct Ring {
     double start, full, alone;
 };
 constexpr double kRingFixed = 2.0;
+constexpr int64_t kMostRingThreads = 768;
 constexpr Ring kRings[] = {{Form::kRing32, 32, 32, 8, 1, 3.0, 1.28, 1.28},
                            {Form::kRing32Wide, 32, 64, 4, 1, 3.7, 0.78, 0.78},
                            {Form::kRing64, 64, 64, 3, 1, 4.5, 0.88, 0.88},
@@ -167,7 +168,7 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
             time += kConvertFixed;
             bytes = p.c != nullptr ? 0 : 4 * p.m * p.n;
         }
-        if (ceil_div(p.m, f.rows) < 65536) {
+        if (ceil_div(p.m, f.rows) < 65536 && mfr::one_launch(groups, 64 * f.waves)) {
             offer(f.form, 1, time, bytes);
         }
     };
@@ -187,7 +188,9 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
             time += kConvertFixed;
             bytes = p.c != nullptr ? 0 : 4 * p.m * p.n;
         }
-        offer(r.form, 1, time, bytes);
+        if (mfr::one_launch(groups, kMostRingThreads)) {
+            offer(r.form, 1, time, bytes);
+        }
     };
     const auto tiles = [&](const Tile& t) {
         for (int64_t splits = 1; splits <= 8 && splits <= std::max(blocks, int64_t{1}); splits *= 2) {

@@ -14,11 +14,20 @@
 
 namespace mfr::f8gemm {
 
+// The wavefronts of a SIMD: of the one workgroup whose ring fits the 160 KB of LDS, or of two.
+constexpr int ring_waves(int wm, int wn, int wk, int turns, bool gated) {
+    const int rows = 32 * wm + 32 * wn * (gated ? 2 : 1);
+    const int bytes = turns * wk * (rows * 128 + (gated ? 3 : 2) * 256);
+    const int waves = wm * wn * wk * (2 * bytes <= 160 * 1024 ? 2 : 1);
+    return (waves + 3) / 4;
+}
+
 // A workgroup: 32 WM rows of A against 32 WN rows of each weight, WK slices of the depth a turn, a
 // wavefront for each 32 x 32 block of each slice. TURNS turns' slices lie in LDS, all but one under
 // way. The wavefronts' sums are added through LDS in the order of their slices.
 template <int WM, int WN, int WK, int TURNS, bool GATED>
-__global__ __launch_bounds__(64 * WM * WN * WK, 2) void ring_kernel(Params p) {
+__global__ __launch_bounds__(64 * WM * WN * WK, ring_waves(WM, WN, WK, TURNS, GATED)) void ring_kernel(
+    Params p) {
     constexpr int kWeights = GATED ? 2 : 1;
     constexpr int kWaves = WM * WN * WK;
     constexpr int kRowsA = 32 * WM;
