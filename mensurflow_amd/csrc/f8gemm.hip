@@ -69,6 +69,7 @@ enum class Form {
     kRing32Wide,
     kRing64,
     kRing64Pair,
+    kRing128,
     kTile64,
     kTile128
 };
@@ -94,7 +95,10 @@ constexpr Few kFewGated[] = {{Form::kFew16, 16, 16, 8, 1.5},
 // A ring's rows and columns, the slices of a turn, how many share a CU, what a workgroup takes
 // besides its turns, and the time of a turn when every CU has them all, or one alone. Measured, a
 // round of every CU at k = 1024, 4096, 8192: 32 x 32 4.3, 7.9, 13.4 us; 32 x 64 5.4, 9.8, 16.3; 64 x 64
-// 7.6, 14.6, 24.5, two on a CU 9.5, 23, 43; gated, k = 4096: 32 x 32 12, 64 x 32 15.5, two 23.5.
+// 7.6, 14.6, 24.5, two on a CU 9.5, 23, 43; gated, k = 4096: 32 x 32 12, 64 x 32 15.5, two 23.5. The
+// one of 128 columns makes 8 bits by itself: 8-bit output of 32 x 16384 x 4096 17.4 us (18.9 with a
+// second launch), of the gated 32 x 14336 x 4096 28.6 (30.2), of few rows without a workspace, 1 x 4096
+// x 4096, 16.7 (64-row tiles 22.1), gated 1 x 10240 x 4096 26.5 (33.5).
 struct Ring {
     Form form;
     int64_t rows, cols, slices, at_once;
@@ -105,10 +109,12 @@ constexpr int64_t kMostRingThreads = 768;
 constexpr Ring kRings[] = {{Form::kRing32, 32, 32, 8, 1, 3.0, 1.28, 1.28},
                            {Form::kRing32Wide, 32, 64, 4, 1, 3.7, 0.78, 0.78},
                            {Form::kRing64, 64, 64, 3, 1, 4.5, 0.88, 0.88},
-                           {Form::kRing64Pair, 64, 64, 2, 2, 3.0, 1.26, 1.0}};
+                           {Form::kRing64Pair, 64, 64, 2, 2, 3.0, 1.26, 1.0},
+                           {Form::kRing128, 32, 128, 2, 1, 3.7, 0.75, 0.75}};
 constexpr Ring kRingsGated[] = {{Form::kRing32, 32, 32, 4, 1, 3.7, 1.04, 1.04},
                                 {Form::kRing64, 64, 32, 4, 1, 3.5, 1.5, 1.5},
-                                {Form::kRing64Pair, 64, 32, 2, 2, 3.0, 1.28, 0.95}};
+                                {Form::kRing64Pair, 64, 32, 2, 2, 3.0, 1.28, 0.95},
+                                {Form::kRing128, 32, 128, 2, 1, 3.7, 1.42, 1.42}};
 
 // The rate at which a ring's weights come from memory at most (32 x 16384 x 4096).
 constexpr double kBytesPerUs = 4.6e6;
@@ -145,6 +151,11 @@ struct Plan {
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Whether the form leaves an 8-bit output to a second launch: several workgroups hold a block.
+bool converts(Form f) {
+    return f != Form::kRing128 && f != Form::kTile64 && f != Form::kTile128;
+}
 
 Plan choose(const Params& p, int64_t cus, bool workspace) {
     const bool gated = p.up.values != nullptr;
@@ -184,7 +195,7 @@ Plan choose(const Params& p, int64_t cus, bool workspace) {
         }
         time = kRingFixed + std::max(time, weights / kBytesPerUs);
         int64_t bytes = 0;
-        if (p.q.values != nullptr) {
+        if (p.q.values != nullptr && converts(r.form)) {
             time += kConvertFixed;
             bytes = p.c != nullptr ? 0 : 4 * p.m * p.n;
         }
@@ -266,6 +277,9 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     case Form::kRing64Pair:
         (gated ? launch_ring<2, 1, 2, 2, true> : launch_ring<2, 2, 2, 2, false>)(s, p);
         break;
+    case Form::kRing128:
+        (gated ? launch_ring<1, 4, 2, 2, true> : launch_ring<1, 4, 2, 3, false>)(s, p);
+        break;
     case Form::kTile64:
         (gated ? launch_tiles<64, 128, 2, 4, 3, true> : launch_tiles<64, 128, 1, 4, 2, false>)(
             s, p, plan.splits);
@@ -277,8 +291,6 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     }
 }
 
-// Whether the form leaves an 8-bit output to a second launch.
-bool is_few(Form f) { return f != Form::kTile64 && f != Form::kTile128; }
 
 void run_region(mfr_stream& s, Params p, Plan plan) {
     std::unique_lock<std::mutex> hold(s.workspace_mutex, std::defer_lock);
@@ -303,7 +315,7 @@ void run_region(mfr_stream& s, Params p, Plan plan) {
             plan = choose(p, s.compute_units, false);
         }
     }
-    if (is_few(plan.form)) {
+    if (converts(plan.form)) {
         Params sums = p;
         if (p.c == nullptr) {
             sums.c = static_cast<float*>(memory);

@@ -255,13 +255,16 @@ __global__ __launch_bounds__(64 * WM * WN * WK, ring_waves(WM, WN, WK, TURNS, GA
         }
         return v;
     };
-    // Quads in the order of rows: a row of a block is 8 lanes'.
-    for (int i = static_cast<int>(threadIdx.x); i < WM * WN * 256; i += 64 * kWaves) {
-        const int block = i / 256; // wn WM + wm
-        const int r = i / 8 % 32;
-        const int at = r * 8 + ((i % 8) ^ (r / 2 % 8));
-        const int64_t row = m0 + block % WM * 32 + r;
-        const int64_t col = n0 + block / WM * 32 + i % 8 * 4;
+    // Quads in the order of rows. With 128 columns half a wavefront holds a row's block, and makes
+    // its 8 bits; otherwise they are another launch's.
+    constexpr int kQuads = 8 * WN;
+    for (int i = static_cast<int>(threadIdx.x); i < kRowsA * kQuads; i += 64 * kWaves) {
+        const int r = i / kQuads;
+        const int quad = i % kQuads;
+        const int block = quad / 8 * WM + r / 32;
+        const int at = r % 32 * 8 + ((quad % 8) ^ (r / 2 % 8));
+        const int64_t row = m0 + r;
+        const int64_t col = n0 + quad * 4;
         const int64_t count = row < p.m ? p.n - col : 0;
         float4 sum = total_of(block, at, 0);
         float v[4] = {sum.x, sum.y, sum.z, sum.w};
@@ -286,8 +289,17 @@ __global__ __launch_bounds__(64 * WM * WN * WK, ring_waves(WM, WN, WK, TURNS, GA
             if constexpr (GATED) {
                 v[e] = v[e] * other[e];
             }
+            v[e] = e < count ? v[e] : 0.0f; // counts for nothing in the block's scale
         }
-        dev::store_quad(p.c + row * p.c_rs + col, make_float4(v[0], v[1], v[2], v[3]), count);
+        const float4 y = make_float4(v[0], v[1], v[2], v[3]);
+        if (p.c != nullptr) {
+            dev::store_quad(p.c + row * p.c_rs + col, y, count);
+        }
+        if constexpr (kRowsB == kBlock) {
+            if (p.q.values != nullptr && row < p.m) {
+                dev::write_f8(p.q, row, col, p.n, y);
+            }
+        }
     }
 }
 

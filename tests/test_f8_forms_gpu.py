@@ -21,9 +21,10 @@ pytestmark = pytest.mark.gpu
 FORMS = [(2, 4683, 454), (740, 125, 549), (35, 5759, 786), (105, 2437, 549),  # few rows
          (1, 6913, 5450), (3, 8300, 1000), (128, 4100, 1100), (99, 2559, 3360),  # rings
          (155, 3457, 2499), (258, 6145, 4260), (65, 4507, 4438), (200, 4096, 2048),
+         (1792, 513, 1878), (30, 14200, 700), (8, 7424, 8399),
          (39, 4097, 3153), (201, 4674, 4375), (2051, 195, 5841),  # 64-row tiles in ranges
          (65, 4122, 2921), (268, 1664, 5874), (17, 2816, 8567),  # the gated ones
-         (193, 4382, 7538), (210, 4112, 8909), (2335, 385, 6024),  # 128-row tiles in ranges
+         (200, 4737, 8536), (210, 4112, 8909), (205, 4824, 6303), (2335, 385, 6024),  # 128-row tiles in ranges
          (2305, 19, 8334), (1025, 137, 8767),                     # the gated ones
          (1349, 2945, 130), (639, 3208, 271),                     # and whole
          (1883, 4353, 777), (1668, 4863, 642), (2304, 1802, 629),  # a strip of columns, of rows
@@ -245,6 +246,36 @@ def test_captured_before_the_workspace_exists_and_beside_calls_that_use_it():
                 check()
         for g in graphs:
             g.close()
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 4100, 2300), (30, 14200, 700), (70, 1000, 2300), (300, 1000, 900)])
+def test_captured_8_bit_outputs_alone(m, n, k):
+    """Without a workspace: exact sums, the plain and the gated product, replayed between eager calls."""
+    rng = np.random.default_rng(m + 1)
+    with mf.Stream(0) as own:
+        a, sa = exact_operands(rng, m, k, 1)
+        b, sb = exact_operands(rng, n, k, 128)
+        p = ref.product(a, sa, b, sb)[0].astype(np.float32)
+        ha, hb = held_of(a, sa, own, 1), held_of(b, sb, own, 128)
+        q, gated = Held(m, n, own), Held(m, n, own)
+
+        def body():
+            mf.gemm_f8(ha.matrix, hb.matrix, out_f8=q.matrix)
+            mf.gemm_f8_gated(ha.matrix, hb.matrix, hb.matrix, act=mf.ACT_NONE, out_f8=gated.matrix)
+
+        graph = Graph(own, body)
+        for _ in range(3):
+            for call in (graph.launch, body):
+                mf.fill(q.store, 1.0)
+                mf.fill(gated.store, 1.0)
+                call()
+                codes, scales = ref.quantize(p)
+                got = q.bytes.numpy()[:m, :n], q.store.numpy()[:, :m].T
+                assert same_codes(got[0], codes) and np.array_equal(got[1], scales)
+                codes, scales = ref.quantize(p * p)
+                got = gated.bytes.numpy()[:m, :n], gated.store.numpy()[:, :m].T
+                assert same_codes(got[0], codes) and np.array_equal(got[1], scales)
+        graph.close()
 
 
 @pytest.mark.parametrize("m", [1, 12, 40])
