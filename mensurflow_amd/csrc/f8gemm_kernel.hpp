@@ -92,7 +92,7 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
 // `lane_offset` + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past
 // the resource (its range counts both offsets). In assembly, because the compiler waits for every such copy that
 // it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is what
-// waits here. No register is written.
+// waits here. No register is written but m0, in which the compiler keeps nothing.
 template <int BYTES>
 __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, uint32_t offset,
                                             void* to) {
