@@ -640,10 +640,12 @@ class F8Matrix:
 
     @classmethod
     def empty(cls, rows: int, cols: int, stream: Stream, block_rows: int = 1) -> "F8Matrix":
-        """Room for [rows, cols]: rows padded to 16 bytes; scales of rows stored [blocks, rows],
-        as mfr_f8gemm reads them best."""
+        """Room for [rows, cols], laid out as mfr_f8gemm reads it best: rows padded to 16 bytes, from
+        1024 on to 128 (a block's bytes are a cache line then); scales of rows stored [blocks,
+        rows]."""
         blocks = -(-cols // abi.F8_BLOCK)
-        values = DeviceArray.empty((rows, -(-cols // 16) * 16), stream, np.uint8)
+        unit = 128 if cols >= 1024 else 16
+        values = DeviceArray.empty((rows, -(-cols // unit) * unit), stream, np.uint8)
         if block_rows == 1:
             scales = DeviceArray.empty((blocks, rows), stream).T
         else:

@@ -14,13 +14,14 @@ namespace mensurflow {
 // A matrix of e4m3 values with a scale per block of block_rows x 128: element (r, c) stands for
 // value * scale.
 struct F8Tensor {
-    Tensor values; // U8 [rows, pitch], pitch = cols rounded up to 16
+    Tensor values; // U8 [rows, pitch], pitch a multiple of 16, at least cols
     Tensor scales; // F32: [ceil(cols / 128), rows] for block_rows 1, else one row per 128 rows
     std::int64_t cols = 0;
     int block_rows = 1; // 1 (activations) or 128 (weights)
 
     std::int64_t rows() const { return values.size(0); }
-    // Undefined contents.
+    // Undefined contents. Rows are padded to 16 bytes, from 1024 columns on to 128: a block's bytes
+    // are a cache line then.
     static F8Tensor empty(std::int64_t rows, std::int64_t cols, int block_rows = 1,
                           Device device = {});
     // A copy on `device`, or *this when it lives there.

@@ -42,10 +42,13 @@ void check_f8(const OpCheck& check, const F8Tensor& t, const char* name, int blo
     if (t.values.dtype() != like.values.dtype() || t.scales.dtype() != like.scales.dtype()) {
         check.fail(std::string(name) + " must be U8 values with F32 scales");
     }
-    const Shape values{t.values.size(0), (t.cols + 15) / 16 * 16};
-    const Shape scales = block_rows == 1 ? Shape{blocks_of(t.cols), values[0]}
-                                         : Shape{blocks_of(values[0]), blocks_of(t.cols)};
-    check_shape(check, t.values, name, values);
+    if (t.cols < 0 || t.values.size(1) < t.cols || t.values.size(1) % 16 != 0) {
+        check.fail(std::string(name) + " has rows of " + std::to_string(t.values.size(1)) +
+                   " bytes for " + std::to_string(t.cols) + " columns");
+    }
+    const std::int64_t rows = t.values.size(0);
+    const Shape scales = block_rows == 1 ? Shape{blocks_of(t.cols), rows}
+                                         : Shape{blocks_of(rows), blocks_of(t.cols)};
     check_shape(check, t.scales, name, scales);
     if (!t.values.is_contiguous() || !t.scales.is_contiguous()) {
         check.fail(std::string(name) + " must be contiguous");
@@ -107,7 +110,8 @@ F8Tensor F8Tensor::empty(std::int64_t rows, std::int64_t cols, int block_rows, D
         OpCheck("F8Tensor").fail("block_rows must be 1 or 128, got " + std::to_string(block_rows));
     }
     F8Tensor out;
-    out.values = Tensor::empty({rows, (cols + 15) / 16 * 16}, DType::U8, device);
+    const std::int64_t unit = cols >= 1024 ? 128 : 16;
+    out.values = Tensor::empty({rows, (cols + unit - 1) / unit * unit}, DType::U8, device);
     out.scales = Tensor::empty(block_rows == 1 ? Shape{blocks_of(cols), rows}
                                                : Shape{blocks_of(rows), blocks_of(cols)},
                                DType::F32, device);

@@ -165,6 +165,18 @@ void test_checks() {
     F8Tensor torn = b;
     torn.scales = Tensor::ones({2, 1});
     test::require_throws<Invalid>([&] { gemm_f8(a, torn); }, "scales' shape");
+    const DType bytes = b.values.dtype();
+    for (const std::int64_t pitch : {16, 24, 33}) {
+        torn = b;
+        torn.values = Tensor::empty({5, pitch}, bytes);
+        test::require_throws<Invalid>([&] { gemm_f8(a, torn); }, "rows of " + std::to_string(pitch));
+    }
+    torn.values = Tensor::empty({5, 64}, bytes); // wider than it need be
+    test::require_throws<detail::NotImplemented>([&] { gemm_f8(a, torn); }, "no kernel on the CPU");
+    test::require(F8Tensor::empty(2, 1023).values.size(1) == 1024 &&
+                      F8Tensor::empty(2, 1030).values.size(1) == 1152 &&
+                      F8Tensor::empty(2, 17).values.size(1) == 32,
+                  "pitches");
 }
 
 } // namespace

@@ -154,3 +154,10 @@ def test_infinities_in_weights_and_sums(stream):
             want = (ref.product(a, sa, b, sb)[0].astype(np.float32) + bias).astype(np.float32)
         assert np.array_equal(np.isnan(got), np.isnan(want))
         assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)])
+
+
+@pytest.mark.parametrize("cols,pitch", [(17, 32), (1023, 1024), (1024, 1024), (1030, 1152)])
+def test_rows_are_padded(stream, cols, pitch):
+    for block_rows in (1, 128):
+        m = mf.F8Matrix.empty(3, cols, stream, block_rows)
+        assert m.values.strides[0] == pitch and m.shape == (3, cols)
