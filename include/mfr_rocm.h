@@ -414,9 +414,9 @@ typedef struct mfr_f8_matrix {
 } mfr_f8_matrix;
 
 /* out = x in 8 bits, x [rows, cols] fp32 with unit column stride and row stride x_rs. For each
- * block (out->block_rows x 128), in fp32:
- *   scale = max(fl(largest magnitude / 448), 2^-126),  value = e4m3(fl(x * fl(1 / scale))),
- * rounded to nearest, ties to even. A block that holds a NaN or an infinity stands for NaN as a
+ * block (out->block_rows x 128), with s = max(largest magnitude / 448, 2^-126):
+ *   scale = fl(s),  value = e4m3(x / s),
+ * the quotient rounded once, to the nearest e4m3 number, ties to even. A block that holds a NaN or an infinity stands for NaN as a
  * whole. A block of zeros has the scale 2^-126. */
 int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float* x, int64_t x_rs,
                     const mfr_f8_matrix* out);
@@ -427,8 +427,8 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
  *   t = x + residual,   y(r, c) = t(r, c) / sqrt(mean_c(t(r, c)^2) + eps) * weight(c)
  *
  * sum = t is written where sum is not NULL (the residual stream for the next block), out = y where
- * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize) where out_f8.values is
- * not NULL; at least one of out and out_f8. residual and weight may be NULL (0 and 1). t is
+ * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize, from y before its
+ * rounding to fp32) where out_f8.values is not NULL; at least one of out and out_f8. residual and weight may be NULL (0 and 1). t is
  * rounded to fp32, the squares are summed in double in an order that depends on rows and cols alone,
  * and y is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
  * least cols. sum or out may be x or residual itself (the same base and row stride), not one

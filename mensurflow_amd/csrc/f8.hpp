@@ -99,10 +99,68 @@ __device__ inline float scale_of(uint32_t top) {
 }
 
 // Four values in e4m3, the first in the low byte (v_cvt_pk_fp8_f32: nearest, ties to even).
-__device__ inline uint32_t pack(float4 v, float inverse) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v.x * inverse, v.y * inverse, 0, false);
-    w = __builtin_amdgcn_cvt_pk_fp8_f32(v.z * inverse, v.w * inverse, w, true);
+__device__ inline uint32_t pack(float4 v) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v.x, v.y, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(v.z, v.w, w, true);
     return static_cast<uint32_t>(w);
+}
+
+// `near`, a float next to or at a number that lies `beyond` (its sign alone counts) past it, as the
+// one of the number's neighbours whose last bit is set; `near` itself if it is the number. A later
+// rounding to fewer bits then goes the number's way.
+__device__ inline float to_odd(float near, float beyond) {
+    const int bits = __float_as_int(near);
+    const int step = (bits ^ __float_as_int(beyond)) >> 31 | 1; // away from zero, or towards it
+    return __int_as_float((beyond > 0.0f || beyond < 0.0f) && (bits & 1) == 0 ? bits + step : bits);
+}
+
+// What takes the values x of a block to x / s, s = max(top / 448, 2^-126) unrounded: the e4m3 value of
+// x is the nearest to that quotient, as if there were no rounding between.
+struct Quotient {
+    float up;      // a power of two that brings top to [4, 8)
+    float top;     // top up
+    float inverse; // 448 / (top up), within 2 units of the last place
+};
+
+__device__ inline Quotient quotient_of(uint32_t top) {
+    if (__uint_as_float(top) < kTop * kLeastScale) {
+        return {0x1p126f, kTop, 1.0f};
+    }
+    if (top >= 0x7f800000u) { // with an infinity, the others are 0; with a NaN, all are NaN
+        return {top == 0x7f800000u ? 0.0f : __uint_as_float(top), 0.0f, 1.0f};
+    }
+    const float up = __uint_as_float((256u - (top >> 23)) << 23);
+    const float at = __uint_as_float(top) * up;
+    return {up, at, kTop * __builtin_amdgcn_rcpf(at)};
+}
+
+// x / s, its last bit as to_odd() has it. p top and 448 x are compared exactly: the first as two
+// floats, their difference then fits one.
+__device__ inline float quotient(float x, const Quotient& by) {
+    const float v = x * by.up;
+    const auto beyond = [&](float p) {
+        const float product = p * by.top;
+        return fmaf(v, kTop, -product) - fmaf(p, by.top, -product);
+    };
+    float p = v * by.inverse;
+    // Within 3 units of the last place; then within one.
+    p = fmaf(beyond(p) * by.inverse, 1.0f / kTop, p);
+    return copysignf(to_odd(p, beyond(p)), x); // -0 + 0 above is 0
+}
+
+// Four values of a block in e4m3. A product with 448 / top, rounded, is within 4 units of the last
+// place of the quotient: where a little less and a little more of it round alike, the quotient does too.
+// Otherwise, 2 values in 10^5, it is taken exactly.
+__device__ inline uint32_t pack(float4 v, const Quotient& by) {
+    const float less = by.up * by.inverse * (1.0f - 0x1p-20f);
+    const float more = by.up * by.inverse * (1.0f + 0x1p-20f);
+    const uint32_t low = pack(make_float4(v.x * less, v.y * less, v.z * less, v.w * less));
+    const uint32_t high = pack(make_float4(v.x * more, v.y * more, v.z * more, v.w * more));
+    if (low == high) {
+        return low;
+    }
+    return pack(make_float4(quotient(v.x, by), quotient(v.y, by), quotient(v.z, by),
+                            quotient(v.w, by)));
 }
 
 // Stores the first `count` (up to 4) bytes of w at p, which is 4-byte aligned.
@@ -128,11 +186,11 @@ __device__ inline uint32_t half_max(uint32_t v) {
 // Four columns from `col` on of row r, in 8 bits. 32 lanes hold a block: columns past the row are
 // zeros and count for nothing.
 __device__ inline void write_f8(const Matrix& q, int64_t r, int64_t col, int64_t cols, float4 v) {
-    const float scale = scale_of(half_max(magnitude(v)));
+    const uint32_t top = half_max(magnitude(v));
     if (col < cols) {
-        store_bytes(q.values + r * q.rs + col, pack(v, 1.0f / scale), cols - col);
+        store_bytes(q.values + r * q.rs + col, pack(v, quotient_of(top)), cols - col);
         if (col % kBlock == 0) {
-            q.scales[r * q.srs + col / kBlock * q.scs] = scale;
+            q.scales[r * q.srs + col / kBlock * q.scs] = scale_of(top);
         }
     }
 }

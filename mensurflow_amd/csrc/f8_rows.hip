@@ -51,17 +51,16 @@ __global__ __launch_bounds__(kThreads) void quantize_blocks_kernel(const float* 
     for (int i = 0; i < kThreads / 32; ++i) {
         top = mfr::f8::most(top, tops[i]);
     }
-    const float scale = dev::scale_of(top);
-    const float inverse = 1.0f / scale;
+    const dev::Quotient by = dev::quotient_of(top);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
         const int64_t r = row + 8 * i;
         if (r < rows && col < cols) {
-            dev::store_bytes(q.values + r * q.rs + col, dev::pack(v[i], inverse), cols - col);
+            dev::store_bytes(q.values + r * q.rs + col, dev::pack(v[i], by), cols - col);
         }
     }
     if (threadIdx.x == 0) {
-        q.scales[rb * q.srs + cb * q.scs] = scale;
+        q.scales[rb * q.srs + cb * q.scs] = dev::scale_of(top);
     }
 }
 
@@ -102,17 +101,42 @@ __device__ inline double squares(float4 v) {
     return fma(x, x, fma(y, y, fma(z, z, w * w)));
 }
 
-// t * scale * weight, rounded once.
-__device__ inline float4 scaled(float4 t, double scale, float4 w) {
-    return make_float4(static_cast<float>(t.x * scale * w.x), static_cast<float>(t.y * scale * w.y),
-                       static_cast<float>(t.z * scale * w.z),
-                       static_cast<float>(t.w * scale * w.w));
-}
-
-// v with zeros behind the first `count` elements.
-__device__ inline float4 inside(float4 v, int64_t count) {
-    return make_float4(count > 0 ? v.x : 0.0f, count > 1 ? v.y : 0.0f, count > 2 ? v.z : 0.0f,
-                       count > 3 ? v.w : 0.0f);
+// Four columns from `col` on of row r in 8 bits, as dev::write_f8, from numbers before their rounding
+// to fp32: no value is on the wrong side of a border between two codes.
+__device__ inline void write_f8(const Matrix& q, int64_t r, int64_t col, int64_t cols,
+                                const double (&y)[4]) {
+    // Magnitudes as bits, a NaN on top (dev::magnitude).
+    uint64_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        top = mfr::f8::most(top, static_cast<uint64_t>(__double_as_longlong(fabs(y[e]))));
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) {
+        top = mfr::f8::most(top, static_cast<uint64_t>(__shfl_xor(
+                                     static_cast<unsigned long long>(top), m, 64)));
+    }
+    if (col >= cols) {
+        return;
+    }
+    const double largest = __longlong_as_double(static_cast<long long>(top));
+    const double least = mfr::f8::kLeastScale;
+    const double top_code = mfr::f8::kTop;
+    const bool clamped = largest < top_code * least;
+    const double by = clamped ? 1.0 / least : top_code / largest;
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const double x = y[e] * by;
+        const float near = static_cast<float>(x);
+        v[e] = dev::to_odd(near, static_cast<float>(x - static_cast<double>(near)));
+    }
+    dev::store_bytes(q.values + r * q.rs + col, dev::pack(make_float4(v[0], v[1], v[2], v[3])),
+                     cols - col);
+    if (col % kBlock == 0) {
+        q.scales[r * q.srs + col / kBlock * q.scs] =
+            static_cast<float>(clamped ? least : largest / top_code);
+    }
 }
 
 // The sum of v over a workgroup of WAVES wavefronts, in each thread: over the lanes by halves, then
@@ -141,12 +165,21 @@ __device__ inline double norm_scale(const NormParams& p, double squares) {
 __device__ inline void write_normed(const NormParams& p, int64_t r, int64_t col, float4 t,
                                     double scale, float4 w) {
     const int64_t count = p.cols - col;
-    const float4 y = inside(scaled(t, scale, w), count); // behind the row 0 * scale may be NaN
+    const float from[4] = {t.x, t.y, t.z, t.w};
+    const float by[4] = {w.x, w.y, w.z, w.w};
+    double y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        y[e] = e < count ? from[e] * scale * by[e] : 0.0; // behind the row 0 * scale may be NaN
+    }
     if (p.out != nullptr) {
-        dev::store_quad(p.out + r * p.out_rs + col, y, count);
+        dev::store_quad(p.out + r * p.out_rs + col,
+                        make_float4(static_cast<float>(y[0]), static_cast<float>(y[1]),
+                                    static_cast<float>(y[2]), static_cast<float>(y[3])),
+                        count);
     }
     if (p.q.values != nullptr) {
-        dev::write_f8(p.q, r, col, p.cols, y);
+        write_f8(p.q, r, col, p.cols, y);
     }
 }
 

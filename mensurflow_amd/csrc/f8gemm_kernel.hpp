@@ -633,11 +633,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
             top[i] = f8::most(top[i],
                          tops[wn / kSharing * kSharing + w][wm * (BM / WM) + 32 * i + r32]);
         }
-        const float scale = dev::scale_of(top[i]);
-        const float inverse = 1.0f / scale;
+        const dev::Quotient by = dev::quotient_of(top[i]);
         const int64_t first = n0 + wn / kSharing * kSharing * (BN / WN);
         if (row < p.m && first < p.n && wn % kSharing == 0 && half == 0) {
-            p.q.scales[row * p.q.srs + first / kBlock * p.q.scs] = scale;
+            p.q.scales[row * p.q.srs + first / kBlock * p.q.scs] = dev::scale_of(top[i]);
         }
         uint8_t* const line = p.q.values + row * p.q.rs + col0;
         const int64_t left = row < p.m ? p.n - col0 : 0;
@@ -646,7 +645,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Params p) {
             const floatx16 v = acc[0][i][x / 4];
             const int e = x % 4 * 4;
             dev::store_bytes(line + 8 * x,
-                             dev::pack(make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]), inverse),
+                             dev::pack(make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]), by),
                              left - 8 * x);
         }
     }

@@ -1,5 +1,5 @@
 """8-bit matrices in numpy, from their definition: e4m3's 256 values, the conversion with block
-scales (fp32 steps, bit for bit), the norm and the block-scaled product in 64 bits."""
+scales (bit for bit), the norm and the block-scaled product in 64 bits."""
 from __future__ import annotations
 
 import numpy as np
@@ -41,8 +41,9 @@ def blocks(n: int) -> int:
 
 
 def quantize(x: np.ndarray, block_rows: int = 1):
-    """(codes, scales) of a float32 matrix: scale = max(fl(top / 448), 2^-126), the code of
-    fl(x * fl(1 / scale)). Blocks with a NaN or an infinity are NaN throughout, or hold NaN and
+    """(codes, scales) of a float32 matrix: s = max(top / 448, 2^-126), the scale fl(s), the codes
+    nearest to x / s (448 x and top are exact in 64 bits, and their quotient is never rounded across
+    a border between codes). Blocks with a NaN or an infinity are NaN throughout, or hold NaN and
     zeros under an infinite scale."""
     x = np.asarray(x, dtype=np.float32)
     rows, cols = x.shape
@@ -58,10 +59,35 @@ def quantize(x: np.ndarray, block_rows: int = 1):
             s = (top / np.float32(448)).astype(np.float32)
             s = np.where(s < np.float32(2.0 ** -126), np.float32(2.0 ** -126), s)
             scales[:, j] = s
-            inverse = (np.float32(1) / s).astype(np.float32)
+            tops = np.repeat(top.astype(np.float64), block_rows)[:rows, None]
+            wide = part.astype(np.float64)
             codes[:, j * BLOCK:(j + 1) * BLOCK] = encode(
-                (part * np.repeat(inverse, block_rows)[:rows, None]).astype(np.float32))
+                np.where(tops < 448 * 2.0 ** -126, wide * 2.0 ** 126, wide * 448 / tops))
     return codes, scales
+
+
+def quantize_exact(y: np.ndarray):
+    """(codes, sure, scales) of a float64 matrix with a scale per row and 128 columns: the codes
+    nearest to y / s, where that is no closer to a border between two codes than 2^-40 of it
+    (elsewhere either may come), and s."""
+    y = np.asarray(y, dtype=np.float64)
+    rows, cols = y.shape
+    codes, sure = np.empty((rows, cols), np.uint8), np.empty((rows, cols), bool)
+    scales = np.empty((rows, blocks(cols)))
+    with np.errstate(all="ignore"):
+        for j in range(blocks(cols)):
+            part = y[:, j * BLOCK:(j + 1) * BLOCK]
+            s = np.abs(part).max(axis=1) / 448
+            s = np.where(s < 2.0 ** -126, 2.0 ** -126, s)
+            scales[:, j] = s
+            v = part / s[:, None]
+            at = slice(j * BLOCK, (j + 1) * BLOCK)
+            codes[:, at] = encode(v)
+            a = np.minimum(np.abs(np.where(np.isnan(v), 0.0, v)), 448.0)
+            i = np.minimum(np.searchsorted(_MIDDLE, a), len(_MIDDLE) - 1)
+            away = np.minimum(np.abs(_MIDDLE[i] - a), np.abs(_MIDDLE[np.maximum(i - 1, 0)] - a))
+            sure[:, at] = away > 2.0 ** -40 * a
+    return codes, sure, scales
 
 
 def dequantize(codes: np.ndarray, scales: np.ndarray, block_rows: int = 1) -> np.ndarray:

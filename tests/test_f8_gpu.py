@@ -79,6 +79,21 @@ def assert_f8(held, y, block_rows=1):
     assert same_codes(codes, want_codes)
 
 
+def assert_norm_f8(held, t, weight, eps):
+    """`held` is the norm in 8 bits, from the 64-bit value: the codes are the nearest ones, the scales
+    rounded once."""
+    codes, scales = held.read()
+    want, sure, exact = ref.quantize_exact(ref.rms_norm(t, weight, eps))
+    nan = np.isnan(exact)
+    assert np.array_equal(np.isnan(scales), nan)
+    with np.errstate(invalid="ignore"):
+        off = np.abs(scales - exact) > ref.EPS32 * (1 + 2.0 ** -10) * exact + 2.0 ** -149
+    assert not np.any(off[~nan])
+    assert same_codes(np.where(sure, codes, 0), np.where(sure, want, 0))
+    values = ref.VALUES[codes[~sure]], ref.VALUES[want[~sure]]
+    assert np.all(np.abs(values[0] - values[1]) <= 0.125 * np.abs(values[1]) + 2.0 ** -9)
+
+
 def sample(rng, rows, cols):
     """Values of widely differing size, rows and blocks of zeros among them."""
     x = rng.standard_normal((rows, cols)) * np.exp(2 * rng.standard_normal((rows, 1)))
@@ -171,7 +186,7 @@ def test_rms_norm(stream, rows, cols):
     y = out.numpy()
     assert same_bits(summed.numpy(), t)
     assert_norm(y, t, w, 1e-6)
-    assert_f8(held, y)
+    assert_norm_f8(held, t, w, 1e-6)
     wide = mf.DeviceArray(out._base.shape, np.float32, stream, _base=out._base, _ptr=out._base._ptr)
     assert np.all(wide.numpy()[:, cols:] == POISON), "written behind the rows"
     # In place: the sum over the residual, the result over x; 8 bits from the sum alone; no weight.
@@ -179,7 +194,7 @@ def test_rms_norm(stream, rows, cols):
     assert same_bits(dr.numpy(), t) and same_bits(dx.numpy(), y)
     again = Held(rows, cols, stream, by_row=True)
     mf.rms_norm_f8(dr, dw, out=again.matrix)
-    assert_f8(again, y)
+    assert_norm_f8(again, t, w, 1e-6)
     assert_norm(mf.rms_norm(dr, eps=0.5).numpy(), t, None, 0.5)
 
 
@@ -210,7 +225,7 @@ def test_rms_norm_extremes(stream, cols):
         assert np.array_equal(np.isnan(want), np.isnan(y))
         assert np.all(np.abs(y - want)[fine] <= ref.EPS32 * (1 + 2.0 ** -10) * np.abs(want[fine])
                       + 2.0 ** -149)
-        assert_f8(held, y)
+        assert_norm_f8(held, x, None, eps)
 
 
 def test_many_rows(stream):
@@ -219,7 +234,7 @@ def test_many_rows(stream):
     held, out = Held(70001, 33, stream), mf.DeviceArray.empty(x.shape, stream)
     mf.rms_norm_run(stream, mf.rms_norm_desc(dev(x, stream), out=out, out_f8=held.matrix))
     assert_norm(out.numpy(), x, None, 1e-6)
-    assert_f8(held, out.numpy())
+    assert_norm_f8(held, x, None, 1e-6)
 
 
 # ---- products -------------------------------------------------------------------------------------
@@ -467,15 +482,23 @@ def test_captured_and_replayed(stream):
             hip_call("hipStreamEndCapture", handle, ctypes.byref(graph))
             hip_call("hipGraphInstantiate", ctypes.byref(run), graph, None, None, ctypes.c_size_t(0))
             for _ in range(3):
-                x.upload(rng.standard_normal((tokens, 512)).astype(np.float32))
+                host = rng.standard_normal((tokens, 512)).astype(np.float32)
+                x.upload(host)
                 block()
-                want, codes = out.numpy(), h.values.numpy()
-                mf.fill(out, 7.0)
-                hip_call("hipGraphLaunch", run, handle)
-                # A captured product may add its ranges of depth in another order.
-                got = out.numpy()
-                assert np.all(np.abs(got - want) <= 2e-5 * np.abs(want).max())
-                assert np.mean(h.values.numpy() != codes) < 0.01
+                codes = h.values.numpy()
+                for launched in (False, True):
+                    if launched:
+                        mf.fill(out, 7.0)
+                        hip_call("hipGraphLaunch", run, handle)
+                    # A captured product may add its ranges of depth in another order, so that a
+                    # code next to a border is another: each is held to its own codes.
+                    again = h.values.numpy()
+                    assert np.mean(again != codes) < 0.01
+                    p, magnitude = ref.product(again, h.scales.numpy(), down.values.numpy(),
+                                               down.scales.numpy())
+                    assert np.all(np.abs(out.numpy() - (host + p)) <=
+                                  ref.product_bound(magnitude, 384) +
+                                  2 * ref.EPS32 * (np.abs(p) + np.abs(host)))
             hip_call("hipGraphExecDestroy", run)
             hip_call("hipGraphDestroy", graph)
 

@@ -8,7 +8,7 @@ import f8_reference as ref
 import mensurflow_amd as mf
 from helpers import same_bits
 from mensurflow_amd import abi
-from test_f8_gpu import (TINY, Held, assert_f8, assert_norm, dev, exact_operands, held_of, pitched,
+from test_f8_gpu import (TINY, Held, assert_f8, assert_norm, assert_norm_f8, dev, exact_operands, held_of, pitched,
                          same_codes, sample)
 
 pytestmark = pytest.mark.gpu
@@ -24,12 +24,11 @@ def test_more_rows_than_a_launch(stream, rows, cols):
     rng = np.random.default_rng(cols)
     x = rng.standard_normal((rows, cols)).astype(np.float32)
     dx = dev(x, stream)
-    out, q = mf.DeviceArray.empty(x.shape, stream), mf.F8Matrix.empty(rows, cols, stream)
-    mf.rms_norm_run(stream, mf.rms_norm_desc(dx, out=out, out_f8=q))
-    y = out.numpy()
-    assert_norm(y, x, None, 1e-6)
-    codes, scales = ref.quantize(y)
-    assert same_codes(q.values.numpy(), codes) and np.array_equal(q.scales.numpy(), scales)
+    out, held = mf.DeviceArray.empty(x.shape, stream), Held(rows, cols, stream)
+    mf.rms_norm_run(stream, mf.rms_norm_desc(dx, out=out, out_f8=held.matrix))
+    assert_norm(out.numpy(), x, None, 1e-6)
+    assert_norm_f8(held, x, None, 1e-6)
+    q = mf.F8Matrix.empty(rows, cols, stream)
     mf.quantize_f8(dx, out=q)
     codes, scales = ref.quantize(x)
     assert same_codes(q.values.numpy(), codes) and np.array_equal(q.scales.numpy(), scales)
@@ -85,9 +84,8 @@ def test_row_offsets_past_32_bits(stream, cols):
     out = far.slice(1, cols, 2 * cols)
     held = Held(rows, cols, stream)
     mf.rms_norm_run(stream, mf.rms_norm_desc(view, eps=1e-5, out=out, out_f8=held.matrix))
-    y = out.numpy()
-    assert_norm(y, x, None, 1e-5)
-    assert_f8(held, y)
+    assert_norm(out.numpy(), x, None, 1e-5)
+    assert_norm_f8(held, x, None, 1e-5)
     far.close()
 
 
@@ -161,3 +159,28 @@ def test_rows_are_padded(stream, cols, pitch):
     for block_rows in (1, 128):
         m = mf.F8Matrix.empty(3, cols, stream, block_rows)
         assert m.values.strides[0] == pitch and m.shape == (3, cols)
+
+
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_values_next_to_the_borders_between_codes(stream, block_rows):
+    """Blocks of random tops (over all of fp32's range) whose other values are the floats nearest to
+    the borders between two codes, and the next floats to either side."""
+    rng = np.random.default_rng(21)
+    rows = 4096
+    tops = np.exp2(rng.uniform(-148, 127, rows // block_rows))
+    tops[::3] *= 448 * 2.0 ** -126 / 2.0 ** -117  # some of them near the least scale
+    tops = np.minimum(tops, np.finfo(np.float32).max).astype(np.float32)
+    by_row = np.repeat(tops, block_rows).astype(np.float64)
+    x = np.empty((rows, 128), np.float32)
+    with np.errstate(over="ignore", under="ignore"):
+        borders = rng.choice(ref._MIDDLE, (rows, 127)) * rng.choice([-1.0, 1.0], (rows, 127))
+        near = (borders * np.maximum(by_row / 448, 2.0 ** -126)[:, None]).astype(np.float32)
+        step = rng.integers(-1, 2, near.shape)
+        near = np.where(step < 0, np.nextafter(near, np.float32(-np.inf)),
+                        np.where(step > 0, np.nextafter(near, np.float32(np.inf)), near))
+    x[:, 1:] = np.clip(near, -by_row[:, None], by_row[:, None])
+    x[:, 0] = by_row
+    codes, scales = ref.quantize(x, block_rows)
+    got = mf.quantize_f8(dev(x, stream), block_rows)
+    assert np.array_equal(got.scales.numpy(), scales)
+    assert same_codes(got.values.numpy(), codes)
