@@ -416,8 +416,8 @@ typedef struct mfr_f8_matrix {
 /* out = x in 8 bits, x [rows, cols] fp32 with unit column stride and row stride x_rs. For each
  * block (out->block_rows x 128), with s = max(largest magnitude / 448, 2^-126):
  *   scale = fl(s),  value = e4m3(x / s),
- * the quotient rounded once, to the nearest e4m3 number, ties to even. A block that holds a NaN or an infinity stands for NaN as a
- * whole. A block of zeros has the scale 2^-126. */
+ * the quotient rounded once, to the nearest e4m3 number, ties to even. A block that holds a NaN or
+ * an infinity stands for NaN as a whole. A block of zeros has the scale 2^-126. */
 int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float* x, int64_t x_rs,
                     const mfr_f8_matrix* out);
 
@@ -428,8 +428,8 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
  *
  * sum = t is written where sum is not NULL (the residual stream for the next block), out = y where
  * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize, from y before its
- * rounding to fp32) where out_f8.values is not NULL; at least one of out and out_f8. residual and weight may be NULL (0 and 1). t is
- * rounded to fp32, the squares are summed in double in an order that depends on rows and cols alone,
+ * rounding to fp32) where out_f8.values is not NULL; at least one of out and out_f8. residual and
+ * weight may be NULL (0 and 1). t is rounded to fp32, the squares are summed in double in an order that depends on rows and cols alone,
  * and y is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
  * least cols. sum or out may be x or residual itself (the same base and row stride), not one
  * another; other overlaps of outputs with anything are undefined. A NaN in a row makes the row NaN;
@@ -466,13 +466,14 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
  *   c(i, j) = fl( act(P_B(i, j)) * P_up(i, j) ).
  *
  * The inner sums are of exact products on the bf16 matrix cores in fp32 (e4m3 numbers are bf16
- * numbers), the outer ones in fp32 in the order of b, by ranges of b that are added in order where
- * the depth is split: the same call gives the same bits every time. Ranges and products of few rows
- * that end in out_f8 alone go through the stream's workspace; under stream capture, where none is
- * taken, such a call runs without (slower, and by other ranges than eagerly). A captured product of
- * few rows that is given c besides out_f8 needs no workspace and runs as it does eagerly. c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8
- * is given, out_f8.values may be NULL where c is: c in 8 bits, as mfr_f8_quantize gives it
- * (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
+ * numbers), the outer ones in fp32, in the order of b or by groups of b whose sums are then added in
+ * an order that the sizes and the outputs fix: the same call gives the same bits every time. Ranges
+ * of the depth, and products of few rows that end in out_f8 alone, go through the stream's
+ * workspace; under stream capture, where none is taken, or where the memory cannot be had, such a
+ * call runs without (slower, and by other groups). A captured product of few rows that is given c
+ * besides out_f8 needs no workspace and runs as it does eagerly. c (fp32, unit column stride, row
+ * stride c_rs) may be NULL where out_f8 is given, out_f8.values may be NULL where c is: c in 8 bits,
+ * as mfr_f8_quantize gives it (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
  * outputs with operands are undefined. k == 0 gives the epilogue of zero products. The product of
  * two scales has to be in fp32's range. act is any MFR_ACT_*. */
 typedef struct mfr_f8gemm_desc {

@@ -149,8 +149,8 @@ __device__ inline float quotient(float x, const Quotient& by) {
 }
 
 // Four values of a block in e4m3. A product with 448 / top, rounded, is within 4 units of the last
-// place of the quotient: where a little less and a little more of it round alike, the quotient does too.
-// Otherwise, 2 values in 10^5, it is taken exactly.
+// place of the quotient: where a little less and a little more of it round alike, the quotient does
+// too. Otherwise, 2 values in 10^5, it is taken exactly.
 __device__ inline uint32_t pack(float4 v, const Quotient& by) {
     const float less = by.up * by.inverse * (1.0f - 0x1p-20f);
     const float more = by.up * by.inverse * (1.0f + 0x1p-20f);
