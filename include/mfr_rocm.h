@@ -429,9 +429,9 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
  * sum = t is written where sum is not NULL (the residual stream for the next block), out = y where
  * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize, from y before its
  * rounding to fp32) where out_f8.values is not NULL; at least one of out and out_f8. residual and
- * weight may be NULL (0 and 1). t is rounded to fp32, the squares are summed in double in an order that depends on rows and cols alone,
- * and y is rounded once from double. Every fp32 matrix has unit column stride and its own row stride, at
- * least cols. sum or out may be x or residual itself (the same base and row stride), not one
+ * weight may be NULL (0 and 1). t is rounded to fp32, the squares are summed in double in an order
+ * that depends on rows and cols alone, and y is rounded once from double. Every fp32 matrix has unit
+ * column stride and its own row stride, at least cols. sum or out may be x or residual itself (the same base and row stride), not one
  * another; other overlaps of outputs with anything are undefined. A NaN in a row makes the row NaN;
  * an infinity becomes NaN and the row's other elements 0, the formula's values. A row of zeros gives
  * zeros where eps > 0, NaN where eps is 0. */
