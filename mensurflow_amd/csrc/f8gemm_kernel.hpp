@@ -92,20 +92,23 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
 // `lane_offset` + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past
 // the resource (its range counts both offsets). In assembly, because the compiler waits for every such copy that
 // it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is what
-// waits here. No register is written but m0, in which the compiler keeps nothing.
+// waits here. No register is written but m0, in which the compiler keeps nothing. Nor does the compiler
+// look into assembly for the hardware's waits: a memory instruction reads a scalar register no sooner
+// than 5 wait states after a vector instruction (a v_readfirstlane or the v_readlane of a spilled
+// scalar) wrote it, and one after m0 was set. The block gives all 5 by itself.
 template <int BYTES>
 __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, uint32_t offset,
                                             void* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)(to)))));
     if constexpr (BYTES == 16) {
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(
                          at),
                      "v"(lane_offset), "s"(from), "s"(offset)
                      : "memory");
     } else {
         static_assert(BYTES == 4, "4 or 16 bytes a lane");
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(at),
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, %3 offen lds" ::"s"(at),
                      "v"(lane_offset), "s"(from), "s"(offset)
                      : "memory");
     }
