@@ -40,7 +40,8 @@ struct Matrix {
 };
 
 // Checks `d` as a [rows, cols] matrix with `block_rows`, and takes it over. An empty matrix may
-// have null pointers.
+// have null pointers and any strides: it is taken over with none, since a kernel forms addresses and
+// a buffer's size from them also where the depth is 0 and nothing is read.
 inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int block_rows,
                       bool output, const char* what, const char* name) {
     const std::string at = std::string(what) + ": " + name;
@@ -49,10 +50,10 @@ inline Matrix checked(const mfr_f8_matrix& d, int64_t rows, int64_t cols, int bl
         throw Error(MFR_E_UNSUPPORTED,
                     at + " is taken with block_rows " + std::to_string(block_rows) + " only");
     }
-    const Matrix m{d.values, d.rs, d.scales, d.scales_rs, d.scales_cs};
     if (rows == 0 || cols == 0) {
-        return m;
+        return {d.values, 0, d.scales, 0, 0};
     }
+    const Matrix m{d.values, d.rs, d.scales, d.scales_rs, d.scales_cs};
     require(d.values != nullptr && d.scales != nullptr, at + " has a null pointer");
     require(rows <= kMostRows, at + " has too many rows");
     require(d.rs >= cols, at + " has rows that overlap");
