@@ -39,7 +39,8 @@ enum {
 /* Activation applied in a GEMM epilogue or by mfr_bias_act.
  * GELU_TANH is mensurflow::gelu(x, approximate=true), GELU_ERF is gelu(x, false). */
 enum { MFR_ACT_NONE = 0, MFR_ACT_GELU_TANH = 1, MFR_ACT_GELU_ERF = 2 };
-/* x / (1 + exp(-x)) in fp32, for mfr_f8gemm alone (the other entry points refuse it). */
+/* x / (1 + exp(-x)) in fp32 within 6 of its roundings, also where exp(-x) leaves fp32 and the result
+ * does not; for mfr_f8gemm alone (the other entry points refuse it). */
 enum { MFR_ACT_SILU = 3 };
 
 /* Opaque stream: a HIP stream on one device plus the workspace its kernels use

@@ -57,7 +57,17 @@ __device__ __forceinline__ bf16x8 widen(uint32_t lo, uint32_t hi) {
     return out;
 }
 
-__device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
+// v / (1 + e^-v). Where e^-v leaves fp32 (from -88.7 on down) the sum is e^-v for all that fp32 holds,
+// and v e^v is taken from e^(v / 2), which is a normal number as long as the result is not 0. That
+// stands behind a branch (gated 1000 x 1960 x 1000 16.3 us, 16.2 without, 16.6 with a select).
+__device__ __forceinline__ float silu(float v) {
+    float y = v / (1.0f + expf(-v));
+    if (__builtin_expect(v < -88.0f, 0)) {
+        const float e = expf(0.5f * v);
+        y = v * e * e;
+    }
+    return y;
+}
 
 // All copies into LDS but the last COPIES have landed, and the LDS reads before have been done (a
 // later copy may write there). s_waitcnt of gfx9: vmcnt in bits 3:0 and 15:14, expcnt 6:4 (left

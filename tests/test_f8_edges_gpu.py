@@ -2,10 +2,11 @@
 import numpy as np
 import pytest
 
+import f8_reference as ref
 import mensurflow_amd as mf
 from helpers import same_bits
 from mensurflow_amd import abi
-from test_f8_gpu import Held, assert_f8, dev, pitched
+from test_f8_gpu import Held, assert_f8, dev, held_of, pitched
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +52,54 @@ def test_gated_products_of_depth_0(stream, stride):
         mf.f8gemm(stream, d)
         assert not np.any(out.numpy())
         assert_f8(held, np.zeros((m, n), np.float32))
+
+
+# ---- the silu where e^-x leaves fp32 ------------------------------------------------------------
+
+# Few rows, rings of slices, tiles of 64 and 128 rows, and a depth in ranges.
+FAR = [(1, 300, 300), (40, 400, 300), (64, 2048, 512), (32, 4096, 1024), (128, 4100, 1100),
+       (300, 1000, 900), (155, 3457, 2499), (17, 2816, 8567), (1349, 2945, 130), (2305, 1818, 972)]
+
+
+def one_product(value, m, n, k, stream):
+    """Operands of the product value(i), exactly, throughout row i, and a weight that doubles it 100
+    times."""
+    a, b = np.zeros((m, k), np.uint8), np.zeros((n, k), np.uint8)
+    a[:, 0] = b[:, 0] = ref.encode(1.0)
+    sa = np.ones((m, ref.blocks(k)), np.float32)
+    sa[:, 0] = value
+    sb = np.ones((-(-n // 128), ref.blocks(k)), np.float32)
+    return (held_of(a, sa, stream, 1), held_of(b, sb, stream, 128),
+            held_of(b, sb * np.float32(2.0 ** 100), stream, 128))
+
+
+@pytest.mark.parametrize("m,n,k", FAR)
+def test_silu_far_below_zero(stream, m, n, k):
+    """Two exponentials within 2^-23 each, two products and the last one, and what a result below the
+    normal numbers is rounded by."""
+    value = np.linspace(-87.5, -104.5, m) if m > 1 else np.full(1, -89.25)
+    value = value.astype(np.float32)
+    value[m // 2] = -88.75
+    a, gate, up = one_product(value, m, n, k, stream)
+    other = value.astype(np.float64)[:, None] * 2.0 ** 100
+    want = ref.silu(value)[:, None] * other
+    y = mf.gemm_f8_gated(a.matrix, gate.matrix, up.matrix,
+                         out=pitched(np.zeros((m, n), np.float32), stream, 1)).numpy()
+    assert np.all(want > 0)
+    assert np.all(np.abs(y - want) <=
+                  (7 + 2.0 ** -10) * ref.EPS32 * want + 2.0 ** -150 * np.abs(other))
+    y = mf.gemm_f8(a.matrix, gate.matrix, act=mf.ACT_SILU).numpy()
+    want = ref.silu(value)[:, None]
+    assert np.all(np.abs(y - want) <= (6 + 2.0 ** -10) * ref.EPS32 * np.abs(want) + 2.0 ** -150)
+
+
+def test_silu_of_the_ends(stream):
+    """Nothing is left of the far negative numbers; infinity stays, and minus infinity is the
+    formula's NaN."""
+    value = np.float32([-300, -1e4, -3e38, -np.inf, np.inf, np.nan, 0.0, 3e38])
+    a, b, _ = one_product(np.where(np.isfinite(value), value, 1), 8, 20, 3, stream)
+    bias = np.zeros((8, 20), np.float32)
+    bias[~np.isfinite(value)] = value[~np.isfinite(value), None]
+    y = mf.gemm_f8(a.matrix, b.matrix, c0=dev(bias, stream), beta=1.0, act=mf.ACT_SILU).numpy()
+    want = np.float32([0, 0, 0, np.nan, np.inf, np.nan, 0, 3e38])
+    assert np.array_equal(y, np.repeat(want[:, None], 20, 1), equal_nan=True)
