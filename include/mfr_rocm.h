@@ -471,8 +471,8 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
  * an order that the sizes and the outputs fix: the same call gives the same bits every time. Ranges
  * of the depth, and products of few rows that end in out_f8 alone, go through the stream's
  * workspace; under stream capture, where none is taken, or where the memory cannot be had, such a
- * call runs without (slower, and by other groups). A captured product of few rows that is given c
- * besides out_f8 needs no workspace and runs as it does eagerly. c (fp32, unit column stride, row
+ * call runs without (slower, and by other groups). A product of at most 64 rows that is given c
+ * besides out_f8 takes no workspace, so a captured one runs as an eager one does. c (fp32, unit column stride, row
  * stride c_rs) may be NULL where out_f8 is given, out_f8.values may be NULL where c is: c in 8 bits,
  * as mfr_f8_quantize gives it (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
  * outputs with operands are undefined. k == 0 gives the epilogue of zero products. The product of

@@ -820,8 +820,9 @@ def gemm_f8_gated(a: F8Matrix, gate: F8Matrix, up: F8Matrix, *, act=ACT_SILU,
                   out: DeviceArray | None = None, out_f8: F8Matrix | None = None):
     """act(a gate^T) * (a up^T), both projections in one kernel: in 8 bits for the next product (a
     new F8Matrix), or to `out` (fp32) and / or `out_f8` where they are given. Returns out_f8 where
-    that is given or made, else out. A call of few rows that is captured into a graph is faster
-    with both: the sums then need no workspace, which a captured call does not take."""
+    that is given or made, else out. A call of at most 64 rows that is captured into a
+    graph is faster with both: the sums then need no workspace, which a captured call does not
+    take."""
     if out is None and out_f8 is None:
         out_f8 = F8Matrix.empty(a.shape[0], gate.shape[0], a.stream)
     f8gemm(a.stream, f8gemm_desc(a, gate, up=up, act=act, out=out, out_f8=out_f8))

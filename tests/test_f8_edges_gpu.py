@@ -6,7 +6,8 @@ import f8_reference as ref
 import mensurflow_amd as mf
 from helpers import same_bits
 from mensurflow_amd import abi
-from test_f8_gpu import Held, assert_f8, dev, held_of, pitched
+from test_f8_forms_gpu import Graph
+from test_f8_gpu import (Held, assert_f8, dev, held_of, pitched, random_operands, same_codes)
 
 pytestmark = pytest.mark.gpu
 
@@ -103,3 +104,36 @@ def test_silu_of_the_ends(stream):
     y = mf.gemm_f8(a.matrix, b.matrix, c0=dev(bias, stream), beta=1.0, act=mf.ACT_SILU).numpy()
     want = np.float32([0, 0, 0, np.nan, np.inf, np.nan, 0, 3e38])
     assert np.array_equal(y, np.repeat(want[:, None], 20, 1), equal_nan=True)
+
+
+# ---- few rows with both outputs, captured -------------------------------------------------------
+
+# Deep and narrow: where the depth in ranges, through the workspace, would be the faster plan.
+DEEP = [(1, 1021, 7891), (1, 6675, 5631), (1, 6731, 7816), (39, 4097, 3153), (64, 1176, 8236),
+        (35, 1510, 8992)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m,n,k", DEEP)
+def test_captured_few_deep_rows_with_both_outputs_run_as_they_do_eagerly(m, n, k, gated):
+    """Real values, whose sums tell the order of summation: the same bits, replayed between eager calls."""
+    rng = np.random.default_rng(m + n)
+    with mf.Stream(0) as own:
+        a = held_of(*random_operands(rng, m, k, 1), own, 1)
+        gate, up = (held_of(*random_operands(rng, n, k, 128), own, 128) for _ in range(2))
+        out, q = mf.DeviceArray.empty((m, n), own), Held(m, n, own)
+
+        def body():
+            if gated:
+                mf.gemm_f8_gated(a.matrix, gate.matrix, up.matrix, out=out, out_f8=q.matrix)
+            else:
+                mf.gemm_f8(a.matrix, gate.matrix, out=out, out_f8=q.matrix)
+
+        body()
+        want, codes = out.numpy(), q.read()[0].copy()
+        graph = Graph(own, body)
+        for call in (graph.launch, graph.launch, body, graph.launch):
+            mf.fill(out, 3.0)
+            call()
+            assert same_bits(out.numpy(), want) and same_codes(q.read()[0], codes)
+        graph.close()
