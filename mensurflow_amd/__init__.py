@@ -693,12 +693,14 @@ def _rows_of(t: DeviceArray | None, shape, what: str) -> tuple:
     return t.ptr, t.strides[0] if shape[0] > 1 else max(t.strides[0], shape[1])
 
 
-def _one_device(what: str, *operands) -> None:
-    """Refuses arrays and F8Matrix operands (None: not given) of more than one device."""
-    arrays = [a for t in operands if t is not None
-              for a in ((t.values, t.scales) if isinstance(t, F8Matrix) else (t,))]
+def _arrays_of(what: str, *operands) -> tuple:
+    """The arrays of operands that are arrays, F8Matrix or None (not given); refuses those of more
+    than one device."""
+    arrays = tuple(a for t in operands if t is not None
+                   for a in ((t.values, t.scales) if isinstance(t, F8Matrix) else (t,)))
     if len({a.stream.device for a in arrays}) > 1:
         raise ValueError(f"{what}: operands of different devices")
+    return arrays
 
 
 def _vector_of(t: DeviceArray | None, length: int, what: str):
@@ -718,7 +720,7 @@ def quantize_f8(x: DeviceArray, block_rows: int = 1, out: F8Matrix | None = None
         out = F8Matrix.empty(rows, cols, x.stream, block_rows)
     if out.shape != x.shape or out.block_rows != block_rows:
         raise ValueError(f"quantize_f8: out is {out.shape} with block_rows {out.block_rows}")
-    _one_device("quantize_f8", x, out)
+    _arrays_of("quantize_f8", x, out)
     d = _f8_desc(out, "quantize_f8: out")
     abi.check(abi.load().mfr_f8_quantize(x.stream.handle, rows, cols, ptr, rs, ctypes.byref(d)),
               "mfr_f8_quantize")
@@ -731,10 +733,11 @@ def rms_norm_desc(x: DeviceArray, weight: DeviceArray | None = None, *,
                   out_f8: F8Matrix | None = None) -> RmsNormDesc:
     """The descriptor of one rms_norm over the rows of x [rows, cols], to be filled once and run
     many times (rms_norm_run): t = x + residual to `summed`, t / rms(t) * weight to `out` (fp32)
-    and `out_f8` (8 bits), whichever are given."""
+    and `out_f8` (8 bits), whichever are given. The descriptor keeps the arrays that it points to
+    (`held`)."""
     rows, cols = x.shape
-    _one_device("rms_norm", x, weight, residual, summed, out, out_f8)
     d = RmsNormDesc()
+    d.held = _arrays_of("rms_norm", x, weight, residual, summed, out, out_f8)
     d.rows, d.cols, d.eps = rows, cols, eps
     d.x, d.x_rs = _rows_of(x, x.shape, "rms_norm: x")
     d.residual, d.residual_rs = _rows_of(residual, x.shape, "rms_norm: residual")
@@ -780,15 +783,16 @@ def f8gemm_desc(a: F8Matrix, b: F8Matrix, *, up: F8Matrix | None = None, act=ACT
                 out: DeviceArray | None = None, out_f8: F8Matrix | None = None) -> F8GemmDesc:
     """The descriptor of one product of 8-bit matrices (mfr_f8gemm_desc), to be filled once and run
     many times (f8gemm): a [m, k] with a scale per row, b and up [n, k] with 128 x 128 blocks; the
-    result goes to `out` (fp32), `out_f8` (8 bits) or both."""
+    result goes to `out` (fp32), `out_f8` (8 bits) or both. The descriptor keeps the arrays that it
+    points to (`held`)."""
     (m, k), n = a.shape, b.shape[0]
     for w in (b, up):
         if w is not None and w.shape != (n, k):
             raise ValueError(f"f8gemm: a is {a.shape}, a weight {w.shape}")
     if out_f8 is not None and out_f8.shape != (m, n):
         raise ValueError(f"f8gemm: out_f8 is {out_f8.shape}, {(m, n)} is needed")
-    _one_device("f8gemm", a, b, up, c0, bias, out, out_f8)
     d = F8GemmDesc()
+    d.held = _arrays_of("f8gemm", a, b, up, c0, bias, out, out_f8)
     d.m, d.n, d.k = m, n, k
     d.a, d.b, d.up = _f8_desc(a, "f8gemm: a"), _f8_desc(b, "f8gemm: b"), _f8_desc(up, "f8gemm: up")
     d.c, d.c_rs = _rows_of(out, (m, n), "f8gemm: out")

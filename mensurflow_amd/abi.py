@@ -99,6 +99,8 @@ class F8Desc(ctypes.Structure):
 class RmsNormDesc(ctypes.Structure):
     """mfr_rms_norm_desc (include/mfr_rocm.h)."""
 
+    held = ()  # the arrays that a filled descriptor points to
+
     _fields_ = [
         ("rows", _i64), ("cols", _i64),
         ("x", _vp), ("x_rs", _i64), ("residual", _vp), ("residual_rs", _i64),
@@ -109,6 +111,8 @@ class RmsNormDesc(ctypes.Structure):
 
 class F8GemmDesc(ctypes.Structure):
     """mfr_f8gemm_desc (include/mfr_rocm.h)."""
+
+    held = ()  # the arrays that a filled descriptor points to
 
     _fields_ = [
         ("m", _i64), ("n", _i64), ("k", _i64),
