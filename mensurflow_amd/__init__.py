@@ -703,6 +703,11 @@ def _arrays_of(what: str, *operands) -> tuple:
     return arrays
 
 
+def _same_device(what: str, stream: Stream, desc) -> None:
+    if desc.held and desc.held[0].stream.device != stream.device:
+        raise ValueError(f"{what}: a stream of another device than the operands'")
+
+
 def _vector_of(t: DeviceArray | None, length: int, what: str):
     if t is None:
         return None
@@ -752,6 +757,7 @@ def rms_norm_desc(x: DeviceArray, weight: DeviceArray | None = None, *,
 
 def rms_norm_run(stream: Stream, desc: RmsNormDesc) -> None:
     """mfr_rms_norm on a filled descriptor."""
+    _same_device("rms_norm", stream, desc)
     abi.check(abi.load().mfr_rms_norm(stream.handle, ctypes.byref(desc)), "mfr_rms_norm")
 
 
@@ -805,6 +811,7 @@ def f8gemm_desc(a: F8Matrix, b: F8Matrix, *, up: F8Matrix | None = None, act=ACT
 
 def f8gemm(stream: Stream, desc: F8GemmDesc) -> None:
     """mfr_f8gemm on a filled descriptor."""
+    _same_device("f8gemm", stream, desc)
     abi.check(abi.load().mfr_f8gemm(stream.handle, ctypes.byref(desc)), "mfr_f8gemm")
 
 

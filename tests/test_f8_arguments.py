@@ -1,10 +1,11 @@
 """What the Python entry points of the 8-bit ops do with their arguments, without a GPU."""
 import weakref
+from types import SimpleNamespace
 
 import pytest
 
 import mensurflow_amd as mf
-from test_f8 import array, call, matrix
+from test_f8 import array, call, good_gemm, good_norm, matrix
 
 
 def owners(operand):
@@ -44,3 +45,12 @@ def test_a_descriptor_keeps_its_arrays(make, operands):
     assert call("mfr_rms_norm" if make is norm else "mfr_f8gemm", desc)[1] == "null stream"
     del desc
     assert {n for n, refs in of.items() if any(r() is not None for r in refs)} == set()
+
+
+@pytest.mark.parametrize("run,desc", [(mf.rms_norm_run, good_norm()), (mf.f8gemm, good_gemm()),
+                                      (mf.f8gemm, good_gemm(gated=True))])
+def test_a_descriptor_is_refused_by_a_stream_of_another_device(run, desc):
+    with pytest.raises(ValueError, match="another device"):
+        run(SimpleNamespace(device=1, handle=None), desc)
+    with pytest.raises(ValueError, match="null stream"):
+        run(SimpleNamespace(device=0, handle=None), desc)
