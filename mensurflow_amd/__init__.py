@@ -643,6 +643,8 @@ class F8Matrix:
         """Room for [rows, cols], laid out as mfr_f8gemm reads it best: rows padded to 16 bytes, from
         1024 on to 128 (a block's bytes are a cache line then); scales of rows stored [blocks,
         rows]."""
+        if block_rows not in (1, abi.F8_BLOCK):
+            raise ValueError(f"F8Matrix: block_rows must be 1 or {abi.F8_BLOCK}, got {block_rows}")
         blocks = -(-cols // abi.F8_BLOCK)
         unit = 128 if cols >= 1024 else 16
         values = DeviceArray.empty((rows, -(-cols // unit) * unit), stream, np.uint8)

@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 
 import mensurflow_amd as mf
-from test_f8 import array, call, good_gemm, good_norm, matrix
+from test_f8 import STREAM, array, call, good_gemm, good_norm, matrix
 
 
 def owners(operand):
@@ -54,3 +54,11 @@ def test_a_descriptor_is_refused_by_a_stream_of_another_device(run, desc):
         run(SimpleNamespace(device=1, handle=None), desc)
     with pytest.raises(ValueError, match="null stream"):
         run(SimpleNamespace(device=0, handle=None), desc)
+
+
+@pytest.mark.parametrize("block_rows", [0, 2, -128])
+def test_room_for_other_blocks_is_refused(block_rows):
+    with pytest.raises(ValueError, match="block_rows"):
+        mf.F8Matrix.empty(4, 100, STREAM, block_rows)
+    with pytest.raises(ValueError, match="block_rows"):
+        mf.quantize_f8(array((4, 100)), block_rows)
