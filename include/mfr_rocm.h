@@ -431,11 +431,12 @@ int mfr_f8_quantize(mfr_stream_t stream, int64_t rows, int64_t cols, const float
  * out is not NULL, out_f8 = y in 8 bits (block_rows 1, as mfr_f8_quantize, from y before its
  * rounding to fp32) where out_f8.values is not NULL; at least one of out and out_f8. residual and
  * weight may be NULL (0 and 1). t is rounded to fp32, the squares are summed in double in an order
- * that depends on rows and cols alone, and y is rounded once from double. Every fp32 matrix has unit
- * column stride and its own row stride, at least cols. sum or out may be x or residual itself (the same base and row stride), not one
- * another; other overlaps of outputs with anything are undefined. A NaN in a row makes the row NaN;
- * an infinity becomes NaN and the row's other elements 0, the formula's values. A row of zeros gives
- * zeros where eps > 0, NaN where eps is 0. */
+ * that depends on rows, cols and the device's number of compute units, and y is rounded once from
+ * double. Every fp32 matrix has unit column stride and its own row stride, at least cols. sum or out
+ * may be x or residual itself (the same base and row stride), not one another; other overlaps of
+ * outputs with anything are undefined. A NaN in a row makes the row NaN; an infinity becomes NaN and
+ * the row's other elements 0, the formula's values. A row of zeros gives zeros where eps > 0, NaN
+ * where eps is 0. */
 typedef struct mfr_rms_norm_desc {
     int64_t rows, cols;
     const float* x;
@@ -468,15 +469,18 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
  *
  * The inner sums are of exact products on the bf16 matrix cores in fp32 (e4m3 numbers are bf16
  * numbers), the outer ones in fp32, in the order of b or by groups of b whose sums are then added in
- * an order that the sizes and the outputs fix: the same call gives the same bits every time. Ranges
- * of the depth, and products of few rows that end in out_f8 alone, go through the stream's
- * workspace; under stream capture, where none is taken, or where the memory cannot be had, such a
- * call runs without (slower, and by other groups). A product of at most 64 rows that is given c
- * besides out_f8 takes no workspace, so a captured one runs as an eager one does. c (fp32, unit column stride, row
- * stride c_rs) may be NULL where out_f8 is given, out_f8.values may be NULL where c is: c in 8 bits,
- * as mfr_f8_quantize gives it (block_rows 1). c0 may equal c (in place); beta == 0 or c0 == NULL skips it. Other overlaps of
- * outputs with operands are undefined. k == 0 gives the epilogue of zero products. The product of
- * two scales has to be in fp32's range. act is any MFR_ACT_*. */
+ * an order that is fixed by the sizes, the outputs that are asked for and the device's number of
+ * compute units: the same call gives the same bits every time. Ranges of the depth, and products of
+ * few rows that end in out_f8 alone, go through the stream's workspace; under stream capture, where
+ * none is taken, or where the memory cannot be had, such a call runs without (slower, and by other
+ * groups). A product of at most 64 rows that is given c besides out_f8 takes no workspace, so a
+ * captured one runs as an eager one does.
+ *
+ * c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8 is given, out_f8.values may
+ * be NULL where c is: c in 8 bits, as mfr_f8_quantize gives it (block_rows 1). c0 may equal c (in
+ * place); beta == 0 or c0 == NULL skips it. Other overlaps of outputs with operands are undefined.
+ * k == 0 gives the epilogue of zero products, and nothing of a, b and up but block_rows is looked at.
+ * The product of two scales has to be in fp32's range. act is any MFR_ACT_*. */
 typedef struct mfr_f8gemm_desc {
     int64_t m, n, k;
     mfr_f8_matrix a;
