@@ -479,7 +479,7 @@ int mfr_rms_norm(mfr_stream_t stream, const mfr_rms_norm_desc* desc);
  * c (fp32, unit column stride, row stride c_rs) may be NULL where out_f8 is given, out_f8.values may
  * be NULL where c is: c in 8 bits, as mfr_f8_quantize gives it (block_rows 1). c0 may equal c (in
  * place); beta == 0 or c0 == NULL skips it. Other overlaps of outputs with operands are undefined.
- * k == 0 gives the epilogue of zero products, and nothing of a, b and up but block_rows is looked at.
+ * k == 0 gives the epilogue of zero products: nothing of a, b and up is read, any strides will do.
  * The product of two scales has to be in fp32's range. act is any MFR_ACT_*. */
 typedef struct mfr_f8gemm_desc {
     int64_t m, n, k;
@@ -497,6 +497,34 @@ typedef struct mfr_f8gemm_desc {
 } mfr_f8gemm_desc;
 
 int mfr_f8gemm(mfr_stream_t stream, const mfr_f8gemm_desc* desc);
+
+/* The forms of mfr_f8gemm: the weights from memory to registers, for 16, 32 or 64 rows a workgroup
+ * (WIDE: 32 columns, else 16); slices of the depth that pass through a ring in LDS, workgroups of 32
+ * or 64 rows (the wide ones and 64: 64 columns, 32 of each weight when gated; PAIR: two workgroups on
+ * a compute unit; 128: 32 rows and 128 columns); tiles of 64 or 128 rows and 128 columns. */
+enum {
+    MFR_F8_NOTHING = 0,
+    MFR_F8_FEW_16 = 1,
+    MFR_F8_FEW_32 = 2,
+    MFR_F8_FEW_32_WIDE = 3,
+    MFR_F8_FEW_64 = 4,
+    MFR_F8_RING_32 = 5,
+    MFR_F8_RING_32_WIDE = 6,
+    MFR_F8_RING_64 = 7,
+    MFR_F8_RING_64_PAIR = 8,
+    MFR_F8_RING_128 = 9,
+    MFR_F8_TILE_64 = 10,
+    MFR_F8_TILE_128 = 11
+};
+
+/* What mfr_f8gemm would run for desc on device `device`, without launching anything: the form and the
+ * ranges of the depth (1: whole) of the main part of the outputs, the number of parts that run by
+ * themselves (up to 3: rows and columns past a multiple of 128), and the bytes of the stream's
+ * workspace that it takes (where that is 0, a captured call runs as an eager one; no ranges are
+ * taken under capture). MFR_F8_NOTHING and zeros when there is nothing to compute. Validates desc as
+ * mfr_f8gemm does. */
+int mfr_f8gemm_plan(int device, const mfr_f8gemm_desc* desc, int32_t* form, int32_t* splits,
+                    int32_t* regions, size_t* workspace);
 
 /* ---- layout ------------------------------------------------------------------------------- */
 

@@ -31,7 +31,8 @@ __all__ = [
     "bias_act", "where", "where_nd", "elementwise", "softmax", "argmax", "strided_copy", "fill", "attention",
     "attention_fused", "attention_composed", "gemm_plan",
     "ACT_SILU", "F8Matrix", "F8GemmDesc", "RmsNormDesc", "quantize_f8", "rms_norm_desc",
-    "rms_norm_run", "rms_norm", "rms_norm_f8", "f8gemm_desc", "f8gemm", "gemm_f8", "gemm_f8_gated",
+    "rms_norm_run", "rms_norm", "rms_norm_f8", "f8gemm_desc", "f8gemm", "f8gemm_plan", "gemm_f8",
+    "gemm_f8_gated",
 ]
 
 
@@ -815,6 +816,19 @@ def f8gemm(stream: Stream, desc: F8GemmDesc) -> None:
     """mfr_f8gemm on a filled descriptor."""
     _same_device("f8gemm", stream, desc)
     abi.check(abi.load().mfr_f8gemm(stream.handle, ctypes.byref(desc)), "mfr_f8gemm")
+
+
+def f8gemm_plan(stream: Stream, desc: F8GemmDesc) -> tuple[int, int, int, int]:
+    """(form, splits, regions, workspace) that f8gemm(stream, desc) would run with
+    (mfr_f8gemm_plan): abi.F8_* and the ranges of the depth (1: whole) of the main part, the parts of
+    the outputs that run by themselves, and the bytes of the stream's workspace that it takes."""
+    _same_device("f8gemm_plan", stream, desc)
+    form, splits, regions = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
+    workspace = ctypes.c_size_t()
+    abi.check(abi.load().mfr_f8gemm_plan(stream.device, ctypes.byref(desc), ctypes.byref(form),
+                                         ctypes.byref(splits), ctypes.byref(regions),
+                                         ctypes.byref(workspace)), "mfr_f8gemm_plan")
+    return form.value, splits.value, regions.value, workspace.value
 
 
 def gemm_f8(a: F8Matrix, b: F8Matrix, *, c0: DeviceArray | None = None, beta=0.0,

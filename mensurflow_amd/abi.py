@@ -44,6 +44,18 @@ STAGE_NEVER = 1
 STAGE_ALWAYS = 2
 MAX_SPLITS = 64
 
+F8_FEW_16 = 1  # the forms of f8gemm (MFR_F8_*)
+F8_FEW_32 = 2
+F8_FEW_32_WIDE = 3
+F8_FEW_64 = 4
+F8_RING_32 = 5
+F8_RING_32_WIDE = 6
+F8_RING_64 = 7
+F8_RING_64_PAIR = 8
+F8_RING_128 = 9
+F8_TILE_64 = 10
+F8_TILE_128 = 11
+
 F8_BLOCK = 128  # MFR_F8_BLOCK: columns (and, of weights, rows) that share a scale
 MAX_BATCH_DIMS = 4
 MAX_COPY_DIMS = 8
@@ -167,6 +179,9 @@ SIGNATURES = {
     "mfr_f8_quantize": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, ctypes.POINTER(F8Desc)]),
     "mfr_rms_norm": (ctypes.c_int, [_vp, ctypes.POINTER(RmsNormDesc)]),
     "mfr_f8gemm": (ctypes.c_int, [_vp, ctypes.POINTER(F8GemmDesc)]),
+    "mfr_f8gemm_plan": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(F8GemmDesc),
+                                       ctypes.POINTER(_i32), ctypes.POINTER(_i32),
+                                       ctypes.POINTER(_i32), ctypes.POINTER(ctypes.c_size_t)]),
     "mfr_strided_copy": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, ctypes.POINTER(_i64),
                                         ctypes.POINTER(_i64)]),
     "mfr_fill": (ctypes.c_int, [_vp, _vp, _i32, _i64, ctypes.c_uint64]),

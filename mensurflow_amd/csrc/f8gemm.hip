@@ -60,18 +60,18 @@ Params checked(const mfr_f8gemm_desc* desc) {
 // 8192, n = 1024 .. 16384 and k = 1024 .. 8192: a fixed part, and one per block of the depth that a
 // workgroup or wavefront walks, by how many workgroups a CU has. The least of them is taken.
 
-enum class Form {
-    kFew16,
-    kFew32,
-    kFew32Wide,
-    kFew64,
-    kRing32,
-    kRing32Wide,
-    kRing64,
-    kRing64Pair,
-    kRing128,
-    kTile64,
-    kTile128
+enum class Form : int32_t {
+    kFew16 = MFR_F8_FEW_16,
+    kFew32 = MFR_F8_FEW_32,
+    kFew32Wide = MFR_F8_FEW_32_WIDE,
+    kFew64 = MFR_F8_FEW_64,
+    kRing32 = MFR_F8_RING_32,
+    kRing32Wide = MFR_F8_RING_32_WIDE,
+    kRing64 = MFR_F8_RING_64,
+    kRing64Pair = MFR_F8_RING_64_PAIR,
+    kRing128 = MFR_F8_RING_128,
+    kTile64 = MFR_F8_TILE_64,
+    kTile128 = MFR_F8_TILE_128
 };
 
 // A workgroup's rows and columns, the wavefronts that share the depth, and a wavefront's time per
@@ -299,6 +299,11 @@ void launch(const mfr_stream& s, const Plan& plan, const Params& p) {
     }
 }
 
+// The ranges of the depth that are not empty.
+int64_t ranges_of(const Params& p, const Plan& plan) {
+    const int64_t blocks = blocks_of(p.k);
+    return plan.splits > 1 ? ceil_div(blocks, ceil_div(blocks, plan.splits)) : 1;
+}
 
 void run_region(mfr_stream& s, Params p, Plan plan) {
     std::unique_lock<std::mutex> hold(s.workspace_mutex, std::defer_lock);
@@ -338,7 +343,7 @@ void run_region(mfr_stream& s, Params p, Plan plan) {
     p.split_blocks = ceil_div(blocks_of(p.k), plan.splits);
     if (plan.splits > 1) {
         p.partial = static_cast<float*>(memory);
-        plan.splits = ceil_div(blocks_of(p.k), p.split_blocks); // none of them empty
+        plan.splits = ranges_of(p, plan);
     }
     launch(s, plan, p);
     if (p.partial != nullptr) {
@@ -376,14 +381,26 @@ Params cols_from(Params p, int64_t first) {
     return p;
 }
 
+// Launches of their own, each part of the outputs.
+struct Region {
+    Params p;
+    Plan plan;
+};
+struct Regions {
+    Region list[3];
+    int count = 0;
+};
+
 // The problem whole, or, where the model prices that lower, without the rows and columns past the
 // last multiple of 128, which run by themselves: 3 columns more than 32 x 32 tiles of two on each CU
 // cost a third turn of every CU (4093 x 4099 x 1023 58.9 -> 54.0 us). Short calls are not worth the
 // question.
 constexpr double kShortCall = 20.0;
 
-void run(mfr_stream& s, const Params& p) {
-    const auto priced = [&](const Params& x) { return choose(x, s.compute_units, true); };
+Regions regions_of(const Params& p, int64_t cus) {
+    const auto priced = [&](const Params& x) { return choose(x, cus, true); };
+    Regions out;
+    const auto add = [&](const Params& x, const Plan& plan) { out.list[out.count++] = {x, plan}; };
     const Plan whole = priced(p);
     const int64_t m = p.m / 128 * 128;
     const int64_t n = p.n / 128 * 128;
@@ -413,10 +430,10 @@ void run(mfr_stream& s, const Params& p) {
         }
     }
     if (rows == p.m && cols == p.n) {
-        run_region(s, p, whole);
-        return;
+        add(p, whole);
+        return out;
     }
-    const auto region = [&](const Params& x) { run_region(s, x, priced(x)); };
+    const auto region = [&](const Params& x) { add(x, priced(x)); };
     region(head(p, rows, cols));
     if (cols < p.n) {
         region(cols_from(head(p, rows, p.n), cols));
@@ -424,6 +441,7 @@ void run(mfr_stream& s, const Params& p) {
     if (rows < p.m) {
         region(rows_from(p, rows));
     }
+    return out;
 }
 
 } // namespace
@@ -437,7 +455,38 @@ int mfr_f8gemm(mfr_stream_t stream, const mfr_f8gemm_desc* desc) {
         if (p.m == 0 || p.n == 0) {
             return;
         }
-        run(s, p);
+        const Regions regions = regions_of(p, s.compute_units);
+        for (int i = 0; i < regions.count; ++i) {
+            run_region(s, regions.list[i].p, regions.list[i].plan);
+        }
+    });
+}
+
+int mfr_f8gemm_plan(int device, const mfr_f8gemm_desc* desc, int32_t* form, int32_t* splits,
+                    int32_t* regions, size_t* workspace) {
+    return mfr::guarded([&] {
+        mfr::require(form != nullptr && splits != nullptr && regions != nullptr &&
+                         workspace != nullptr,
+                     "f8gemm_plan: null argument");
+        const Params p = checked(desc);
+        int cus = 0;
+        const int status = mfr_get_device_info(device, nullptr, 0, nullptr, &cus, nullptr);
+        if (status != MFR_OK) {
+            throw mfr::Error(status, mfr_last_error());
+        }
+        *form = MFR_F8_NOTHING;
+        *splits = *regions = 0;
+        *workspace = 0;
+        if (p.m == 0 || p.n == 0) {
+            return;
+        }
+        const Regions made = regions_of(p, cus);
+        *form = static_cast<int32_t>(made.list[0].plan.form);
+        *splits = static_cast<int32_t>(ranges_of(made.list[0].p, made.list[0].plan));
+        *regions = made.count;
+        for (int i = 0; i < made.count; ++i) {
+            *workspace = std::max(*workspace, static_cast<size_t>(made.list[i].plan.workspace));
+        }
     });
 }
 
