@@ -646,6 +646,8 @@ class F8Matrix:
         rows]."""
         if block_rows not in (1, abi.F8_BLOCK):
             raise ValueError(f"F8Matrix: block_rows must be 1 or {abi.F8_BLOCK}, got {block_rows}")
+        if rows < 0 or cols < 0:
+            raise ValueError(f"F8Matrix: negative dimension in {(rows, cols)}")
         blocks = -(-cols // abi.F8_BLOCK)
         unit = 128 if cols >= 1024 else 16
         values = DeviceArray.empty((rows, -(-cols // unit) * unit), stream, np.uint8)

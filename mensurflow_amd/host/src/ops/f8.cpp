@@ -108,6 +108,9 @@ F8Tensor F8Tensor::empty(std::int64_t rows, std::int64_t cols, int block_rows, D
     if (block_rows != 1 && block_rows != 128) {
         OpCheck("F8Tensor").fail("block_rows must be 1 or 128, got " + std::to_string(block_rows));
     }
+    if (rows < 0 || cols < 0) {
+        OpCheck("F8Tensor").fail("negative dimension in " + to_string(Shape{rows, cols}));
+    }
     F8Tensor out;
     const std::int64_t unit = cols >= 1024 ? 128 : 16;
     out.values = Tensor::empty({rows, (cols + unit - 1) / unit * unit}, DType::U8, device);

@@ -62,3 +62,10 @@ def test_room_for_other_blocks_is_refused(block_rows):
         mf.F8Matrix.empty(4, 100, STREAM, block_rows)
     with pytest.raises(ValueError, match="block_rows"):
         mf.quantize_f8(array((4, 100)), block_rows)
+
+
+@pytest.mark.parametrize("rows,cols", [(4, -5), (4, -16), (4, -1000), (-1, 5)])
+def test_room_for_negative_sizes_is_refused(rows, cols):
+    for block_rows in (1, 128):
+        with pytest.raises(ValueError, match="negative"):
+            mf.F8Matrix.empty(rows, cols, STREAM, block_rows)
