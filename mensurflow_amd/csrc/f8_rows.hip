@@ -190,10 +190,9 @@ __device__ inline float4 weight_at(const NormParams& p, int64_t col) {
 
 // A row in the registers of THREADS threads, QUADS x 4 columns each: every element is read once,
 // all of a thread's loads before the first use. A workgroup takes one row, or 4 where a wavefront
-// holds a row. Bound by memory; the double arithmetic (2 conversions, a multiply-add and 2
-// products an element) and the rest take a third of the vector units' time at that rate. With residual,
-// sum and 8 bits: 16384 x 8192 333 us, 5.25 TB/s (two passes over the row 364), 1 x 4096 4.3 us (6.4);
-// fp32 alone, 4093 x 1023 8.5 us (10.8).
+// holds a row. Bound by memory; the arithmetic, most of it in double, takes 57 % of the vector units'
+// time at that rate with 8 bits out. With residual, sum and 8 bits: 16384 x 8192 335 us, 5.2 TB/s (two
+// passes over the row 364), 1 x 4096 4.4 us (6.4); fp32 alone, 4093 x 1023 8.6 us (10.8).
 template <int THREADS, int QUADS>
 __global__ __launch_bounds__(THREADS == kWave ? 4 * kWave : THREADS) void rms_norm_kernel(
     NormParams p) {

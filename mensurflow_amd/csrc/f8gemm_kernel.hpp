@@ -4,8 +4,8 @@
 // (v_cvt_scalef32_pk_bf16_fp8, two at once, one in the time of an fma). The 8-bit matrix cores run at
 // twice the rate, but add the 8 products of neighbouring depths with what is 2^13 times smaller than
 // the largest of them cut off (found by feeding them powers of two): sums over 128 normal values came
-// out 1.4e-5 off in the 2-norm, whole products 2.3e-5 to 4.2e-5, against 1e-8 and 5e-7 here. That is
-// no fp32 sum, so they are not used.
+// out 1.4e-5 off in the 2-norm, whole products 2.3e-5 to 4.2e-5, against 4e-8 and 7e-8 to 1.3e-7 here.
+// That is no fp32 sum, so they are not used.
 #pragma once
 
 #include "f8.hpp"
@@ -100,9 +100,9 @@ __device__ __forceinline__ intx4 resource(const void* base, uint32_t bytes) {
 
 // One load of a wavefront from global memory straight to LDS: lane l's 16 (or 4) bytes at
 // `lane_offset` + `offset` go to `to` + 16 l (4 l), `to` the wavefront's; zeros where they lie past
-// the resource (its range counts both offsets). In assembly, because the compiler waits for every such copy that
-// it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is what
-// waits here. No register is written but m0, in which the compiler keeps nothing. Nor does the compiler
+// the resource (its range counts both offsets). In assembly, because the compiler waits for every such
+// copy that it knows of before any read of LDS once there are more than 8 in a kernel; wait_copies() is
+// what waits here. No register is written but m0, in which the compiler keeps nothing. Nor does the compiler
 // look into assembly for the hardware's waits: a memory instruction reads a scalar register no sooner
 // than 5 wait states after a vector instruction (a v_readfirstlane or the v_readlane of a spilled
 // scalar) wrote it, and one after m0 was set. The block gives all 5 by itself.
@@ -136,10 +136,10 @@ __device__ __forceinline__ void copy_to_lds(intx4 from, uint32_t lane_offset, ui
 // gives to the 8 instructions are 64 neighbouring ones for both operands: which depth stands where
 // does not matter to a sum as long as it is the same for both.
 //
-// What bounds it: 8192^3 takes 940 to 980 us by the clock that the power leaves (1120 to 1170
-// TFLOP/s; matrix cores 62 % busy at 1.74 GHz, vector units 58 %; without the copies 13 % less). 4096 x
+// What bounds it: 8192^3 takes 935 to 1000 us by the clock that a card's power leaves (1100 to 1175
+// TFLOP/s; matrix cores 60 % busy at 1.80 GHz, vector units 57 %; without the copies 13 % less). 4096 x
 // 4096 x 1024 takes 42 us, two rounds of 8 blocks, 12 of them for outputs that nothing runs under.
-// Gated, 8192 x 10240 x 4096 with 8 bits out: 1170 us (1170 TFLOP/s).
+// Gated, 8192 x 10240 x 4096 with 8 bits out: 1170 to 1250 us (1100 to 1175 TFLOP/s).
 //
 // SLICES of them lie in LDS: with two, a slice is under way while one is multiplied, which covers
 // memory's latency where two workgroups share a CU; with three, two are.

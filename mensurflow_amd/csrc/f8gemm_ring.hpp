@@ -4,7 +4,9 @@
 // pass through a ring in LDS that keeps 64 to 100 KB of copies under way without a register.
 //
 // Measured at 128 x 4096 x 4096: 12.4 us, without the multiplication 11.0, without the copies 10.0;
-// a CU takes 56 GB/s from its L2 (few_rows_kernel, whose wavefronts load for themselves: 16.5 us).
+// a CU's LDS fills at 56 GB/s then, 0.4 of the nominal 64 bytes a clock: a ring of two turns has no copy
+// under way while it waits, and the scalar registers of the offsets are spilled in most of these loops.
+// few_rows_kernel, whose wavefronts load for themselves: 16.5 us.
 // 32 x 16384 x 4096: 14.4 us, 4.8 TB/s of memory (19.9). 128 x 5120 x 4096: 15.4 (28.8). 256 x 4096 x
 // 4096: 16.0 (23.9). Gated, 256 x 2048 x 4096: 17.1 (23.8). Two workgroups on a CU with half the
 // ring each win where one would leave a second round: 128 x 14336 x 4096 25.2 against 30.1.
