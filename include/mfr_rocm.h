@@ -526,6 +526,170 @@ enum {
 int mfr_f8gemm_plan(int device, const mfr_f8gemm_desc* desc, int32_t* form, int32_t* splits,
                     int32_t* regions, size_t* workspace);
 
+/* ---- rotary positions, a paged cache of keys and values, attention against it ----------------
+ *
+ * What a decoder's attention needs around the products, for prompts and for single tokens. The
+ * reference has no such ops; these entry points stand beside mfr_attention, whose scale, sums and
+ * empty rows they follow. Heads are fp32 arrays [rows, heads, d] of unit stride along d, a row the
+ * token of one sequence, with row strides ("ts", from token to token) and head strides ("hs").
+ *
+ * Every count that changes from step to step (lengths, rows of a sequence, page numbers, positions) is
+ * read from device memory when the kernels run: a captured call can be replayed on new ones. No such
+ * value leads a kernel outside the arrays that the descriptor describes: what each means out of its
+ * range is said with it. */
+
+#define MFR_ROTARY_MOST 256
+
+/* Which columns of a head turn together: i and rot / 2 + i, or 2 i and 2 i + 1. */
+enum { MFR_ROTARY_HALVES = 0, MFR_ROTARY_PAIRS = 1 };
+
+/* A rotation by position: the first rot columns of a head (even, 0 .. MFR_ROTARY_MOST; 0: none) form
+ * rot / 2 pairs (a, b), and pair i at position t becomes, with w = t * steps[i] radians,
+ *
+ *   (amplitude (a cos w - b sin w), amplitude (b cos w + a sin w)).
+ *
+ * w and what is left of it past whole turns are taken in double, so that far positions keep their
+ * angle: cosine and sine are within 1e-7 + 2.5e-16 w. The columns from rot on stay as they are.
+ * A plain struct in host memory, copied by the calls that take it. */
+typedef struct mfr_rotary {
+    int32_t rot;
+    int32_t layout;             /* MFR_ROTARY_* */
+    float amplitude;
+    int32_t reserved;
+    double steps[MFR_ROTARY_MOST / 2];
+} mfr_rotary;
+
+/* Fills a rotation: steps[i] = base^(-2 i / rot), scaled for contexts longer than the `original` one:
+ * a pair that turns r = original * step / 2 pi times in it gets
+ *
+ *   step * (g + (1 - g) / factor),   g = (r - slow) / (fast - slow), no less than 0, no more than 1,
+ *
+ * so that fast pairs stay and slow ones are stretched. original 0 (slow and fast unused): every step
+ * is divided by factor; factor 1: steps as they are. No device is needed. */
+int mfr_rotary_init(mfr_rotary* rotary, int32_t rot, int32_t layout, double base, double amplitude,
+                    double factor, double original, double slow, double fast);
+
+/* out = x turned by each row's position: positions[row], or first + row where positions is NULL.
+ * backward != 0 turns by the negative angles, which is the gradient of x from that of out. out may be
+ * x (same strides); other overlaps are undefined, and two places of out are never one. */
+typedef struct mfr_rope_desc {
+    int64_t rows, heads, d;
+    const float* x;
+    int64_t x_ts, x_hs;
+    float* out;                 /* may equal x */
+    int64_t out_ts, out_hs;
+    const int32_t* positions;   /* [rows] or NULL */
+    int64_t first;              /* within 2^31 of 0, with the rows behind it */
+    int32_t backward;
+    int32_t reserved;
+    mfr_rotary rotary;
+} mfr_rope_desc;
+
+int mfr_rope(mfr_stream_t stream, const mfr_rope_desc* desc);
+
+/* Number types of a cache: fp32; bf16; e4m3 with an fp32 scale for each row of d (a token's head), as
+ * mfr_f8_quantize makes them: scale = max(largest magnitude / 448, 2^-126), value = e4m3(x / scale). */
+enum { MFR_KV_F32 = 0, MFR_KV_BF16 = 1, MFR_KV_F8 = 2 };
+
+/* A cache of keys and values in `pages` pages of page_size tokens (a power of two, 16 .. 32768): the
+ * row of d numbers of (page, token in the page, head) starts at base + page * page_stride + token *
+ * token_stride + head * head_stride elements of the cache's type, in k and in v alike. d is a multiple
+ * of 16, at most 128; bases and strides are multiples of 16 bytes, strides 0 or more, token_stride at
+ * most 2^24 bytes, the others 2^40. Scales (MFR_KV_F8; NULL otherwise) are contiguous
+ * [pages, heads, page_size], 16-byte aligned. */
+typedef struct mfr_kv_cache {
+    int32_t type;               /* MFR_KV_* */
+    int32_t page_size;
+    int64_t pages, heads, d;
+    void* k;
+    void* v;
+    int64_t page_stride, token_stride, head_stride;
+    float* k_scales;
+    float* v_scales;
+} mfr_kv_cache;
+
+/* The sequences of a step. Sequence s has the rows starts[s] .. starts[s + 1] - 1 of the arrays of
+ * heads (starts NULL: rows / sequences each, which must be whole), and lengths[s] tokens in the cache
+ * with those rows' included: row i of its n stands at place lengths[s] - n + i. Token j of the sequence
+ * lies in page table[s * table_rs + j / page_size]. In front of every sequence stand the `prefix` tokens
+ * of the pages prefix_pages[0 ..] that all share (0: none); places and lengths do not count them.
+ *
+ * Rows of no sequence (behind the last, say) are neither read nor written. starts outside 0 .. rows, and
+ * ends before their start, are taken as the nearest that are not. A length below 0 counts as 0, one past
+ * width * page_size as that; a place below 0 or past that has no token. A page number outside
+ * 0 .. pages - 1 is no page: nothing is written there, and its tokens count as absent. */
+typedef struct mfr_kv_batch {
+    int64_t rows, sequences;
+    const int32_t* starts;      /* [sequences + 1] or NULL */
+    const int32_t* lengths;     /* [sequences] */
+    const int32_t* table;       /* [sequences, width] */
+    int64_t table_rs, width;    /* width * page_size at most 2^30 */
+    const int32_t* prefix_pages;
+    int64_t prefix;             /* at most 2^30 */
+} mfr_kv_batch;
+
+/* Writes the rows' keys and values to their places in the cache, the keys turned by their position
+ * (positions[row], or prefix + place where positions is NULL), and q turned alike to q_out (q NULL: no
+ * queries; q_out may equal q). Keys and queries are turned in fp32, then keys and values rounded to the
+ * cache's type, to the nearest, ties to even. q_out is written for every row of a sequence, also where
+ * its place is none. k and v have the cache's heads and d. Two rows of one place leave one of the two
+ * there, or in 8 bits a mixture. */
+typedef struct mfr_kv_append_desc {
+    mfr_kv_cache cache;
+    mfr_kv_batch batch;
+    const float* k;
+    int64_t k_ts, k_hs;
+    const float* v;
+    int64_t v_ts, v_hs;
+    const float* q;             /* may be NULL */
+    int64_t q_ts, q_hs;
+    float* q_out;               /* may equal q */
+    int64_t q_out_ts, q_out_hs;
+    int64_t q_heads;
+    const int32_t* positions;   /* [rows] or NULL */
+    mfr_rotary rotary;          /* rot 0: nothing is turned */
+} mfr_kv_append_desc;
+
+int mfr_kv_append(mfr_stream_t stream, const mfr_kv_append_desc* desc);
+
+/* Attention of each row's queries against the cache: q and out [rows, q_heads, d], q_heads a multiple g
+ * of the cache's heads, query head h with head h / g of the cache,
+ *
+ *   out(row, h, :) = sum_j p_j v_j,   p = softmax_j(scale * q(row, h, :) . k_j),
+ *
+ * over the prefix's tokens and, of the row's own sequence, those at or before the row's place (causal 0:
+ * all of its lengths[s]). A row that sees no token gives zeros. scale 0 means fl(1 / sqrt(d)). Scores, the
+ * softmax and its sums are fp32. Caches in bf16 and e4m3 go through the bf16 matrix cores, exact
+ * products of three bf16 parts of each query and weight (parts below 2^-126 are lost); fp32 caches
+ * through the fp32 ones. What lies in the cache behind a sequence's tokens, or is not seen by a row,
+ * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, leaves outputs of
+ * that row NaN or infinite, of no other row.
+ *
+ * The work is cut over the chip by the lengths, as the kernels find them; the same call gives the same
+ * bits. Partial results go through a workspace of mfr_attention_paged_workspace() bytes: `workspace`
+ * (16-byte aligned; calls that overlap in time need one each), or the stream's where it is NULL. A
+ * captured call needs one of its own: MFR_E_INVALID otherwise. */
+typedef struct mfr_attention_paged_desc {
+    mfr_kv_cache cache;
+    mfr_kv_batch batch;
+    const float* q;
+    int64_t q_ts, q_hs;
+    float* out;
+    int64_t out_ts, out_hs;
+    int64_t q_heads;
+    float scale;
+    int32_t causal;
+    void* workspace;            /* may be NULL */
+    size_t workspace_bytes;
+} mfr_attention_paged_desc;
+
+int mfr_attention_paged(mfr_stream_t stream, const mfr_attention_paged_desc* desc);
+
+/* The bytes of workspace that mfr_attention_paged takes for desc on device `device` (0: none is
+ * needed). They depend on the sizes alone, not on what lies in device memory. Validates desc as that
+ * does, but for the workspace. */
+int mfr_attention_paged_workspace(int device, const mfr_attention_paged_desc* desc, size_t* bytes);
+
 /* ---- layout ------------------------------------------------------------------------------- */
 
 #define MFR_MAX_COPY_DIMS 8

@@ -5,7 +5,8 @@ The product is two native libraries built in-tree (``mensurflow_amd/build.py``):
 * ``_lib/libmfr_rocm.so``: hand-written HIP kernels behind the C ABI of
   ``include/mfr_rocm.h`` (fp32-MFMA GEMM with a fused epilogue, HBM-bound gemv, softmax,
   where, bias+gelu, argmax, strided copy; for serving in 8 bits, RMS norm, conversion to e4m3 with
-  block scales, and products of such matrices);
+  block scales, and products of such matrices; rotary positions, a paged cache of keys and values,
+  and attention against it);
 * ``_lib/libmensurflow.so``: the C++17 host layer that plugs those kernels into mensurflow's
   ``Backend``/``Dispatcher`` API as the ``rocm`` device.
 
@@ -22,8 +23,9 @@ from dataclasses import dataclass
 import numpy as np
 
 from . import abi
-from .abi import (ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, ACT_SILU, F8GemmDesc,  # noqa: F401
-                  GemmDesc, RmsNormDesc)
+from .abi import (ACT_GELU_ERF, ACT_GELU_TANH, ACT_NONE, ACT_SILU, ROTARY_HALVES,  # noqa: F401
+                  ROTARY_PAIRS, AttentionPagedDesc, F8GemmDesc, GemmDesc, KvAppendDesc, RmsNormDesc,
+                  RopeDesc, Rotary)
 
 __all__ = [
     "ACT_NONE", "ACT_GELU_TANH", "ACT_GELU_ERF", "GemmDesc", "device_count", "device_info",
@@ -33,6 +35,10 @@ __all__ = [
     "ACT_SILU", "F8Matrix", "F8GemmDesc", "RmsNormDesc", "quantize_f8", "rms_norm_desc",
     "rms_norm_run", "rms_norm", "rms_norm_f8", "f8gemm_desc", "f8gemm", "f8gemm_plan", "gemm_f8",
     "gemm_f8_gated",
+    "ROTARY_HALVES", "ROTARY_PAIRS", "Rotary", "RopeDesc", "KvAppendDesc", "AttentionPagedDesc",
+    "KvCache", "KvBatch", "rotary", "rope_desc", "rope_run", "rope", "kv_append_desc",
+    "kv_append_run", "kv_append", "attention_paged_desc", "attention_paged_workspace",
+    "attention_paged_run", "attention_paged",
 ]
 
 
@@ -856,6 +862,291 @@ def gemm_f8_gated(a: F8Matrix, gate: F8Matrix, up: F8Matrix, *, act=ACT_SILU,
         out_f8 = F8Matrix.empty(a.shape[0], gate.shape[0], a.stream)
     f8gemm(a.stream, f8gemm_desc(a, gate, up=up, act=act, out=out, out_f8=out_f8))
     return out_f8 if out_f8 is not None else out
+
+
+# ---- rotary positions, a paged cache, attention against it ------------------------------------------
+
+
+def rotary(rot: int, base: float = 10000.0, *, layout=ROTARY_HALVES, amplitude: float = 1.0,
+           factor: float = 1.0, original: float = 0.0, slow: float = 1.0,
+           fast: float = 32.0) -> Rotary:
+    """The rotation of the first `rot` columns of a head (mfr_rotary_init): steps base^(-2 i / rot)
+    radians a position, divided by `factor` for longer contexts; where `original`, the context that a
+    model learned, is given, only pairs that turn less than `fast` times in it, and those below `slow`
+    turns in full. Other steps may be written into the result's `steps`."""
+    out = Rotary()
+    abi.check(abi.load().mfr_rotary_init(ctypes.byref(out), rot, layout, base, amplitude, factor,
+                                         original, slow, fast), "mfr_rotary_init")
+    return out
+
+
+def _heads_of(t: DeviceArray, shape, what: str) -> tuple:
+    """(address, row stride, head stride) of float32 heads [rows, heads, d] of unit stride along d."""
+    if t.dtype != np.float32 or t.shape != tuple(shape):
+        raise ValueError(f"{what}: {t.dtype} {t.shape}, float32 {tuple(shape)} is needed")
+    if shape[2] > 1 and t.strides[2] != 1:
+        raise ValueError(f"{what}: heads need unit stride")
+    return t.ptr, t.strides[0], t.strides[1]
+
+
+def _indices_of(t: DeviceArray | None, length: int, what: str):
+    """The address of a contiguous int32 vector of at least `length`; None for None."""
+    if t is None:
+        return None
+    if t.dtype != np.int32 or len(t.shape) != 1 or t.shape[0] < length or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous int32 vector of {length} is needed, got {t.dtype} "
+                         f"{t.shape}")
+    return t.ptr
+
+
+def rope_desc(x: DeviceArray, rotary: Rotary, *, positions: DeviceArray | None = None,
+              first: int = 0, backward: bool = False, out: DeviceArray | None = None) -> RopeDesc:
+    """The descriptor of one rotation of x [rows, heads, d] to `out` (x itself if None), to be filled
+    once and run many times (rope_run): row r stands at positions[r] (int32), or at first + r;
+    backward gives the gradient of x from that of the result. The descriptor keeps the arrays that it
+    points to (`held`)."""
+    if len(x.shape) != 3:
+        raise ValueError(f"rope: x is {x.shape}, [rows, heads, d] is needed")
+    out = x if out is None else out
+    d = RopeDesc()
+    d.held = _arrays_of("rope", x, positions, out)
+    d.rows, d.heads, d.d = x.shape
+    d.x, d.x_ts, d.x_hs = _heads_of(x, x.shape, "rope: x")
+    d.out, d.out_ts, d.out_hs = _heads_of(out, x.shape, "rope: out")
+    if positions is not None and positions.shape != x.shape[:1]:
+        raise ValueError(f"rope: {positions.shape} positions, {x.shape[:1]} are needed")
+    d.positions = _indices_of(positions, x.shape[0], "rope: positions")
+    d.first, d.backward, d.rotary = first, 1 if backward else 0, rotary
+    return d
+
+
+def rope_run(stream: Stream, desc: RopeDesc) -> None:
+    """mfr_rope on a filled descriptor."""
+    _same_device("rope", stream, desc)
+    abi.check(abi.load().mfr_rope(stream.handle, ctypes.byref(desc)), "mfr_rope")
+
+
+def rope(x: DeviceArray, rotary: Rotary, *, positions: DeviceArray | None = None, first: int = 0,
+         backward: bool = False, out: DeviceArray | None = None) -> DeviceArray:
+    """x [rows, heads, d] turned by its rows' positions, in a new array or `out` (which may be x)."""
+    if out is None:
+        out = DeviceArray.empty(x.shape, x.stream)
+    rope_run(x.stream, rope_desc(x, rotary, positions=positions, first=first, backward=backward,
+                                 out=out))
+    return out
+
+
+_KV_TYPES = {np.dtype(np.float32): abi.KV_F32, np.dtype(np.uint16): abi.KV_BF16,
+             np.dtype(np.uint8): abi.KV_F8}
+
+
+@dataclass
+class KvCache:
+    """A paged cache (mfr_kv_cache): `k` and `v` of one shape [pages, heads, page, d] and the same
+    strides, unit stride along d, float32, uint16 (the bits of bf16) or uint8 (the codes of e4m3);
+    with uint8, `k_scales` and `v_scales`, contiguous float32 arrays [pages, heads, page]."""
+    k: DeviceArray
+    v: DeviceArray
+    k_scales: DeviceArray | None = None
+    v_scales: DeviceArray | None = None
+
+    @classmethod
+    def empty(cls, pages: int, page: int, heads: int, d: int, stream: Stream,
+              dtype=np.float32) -> "KvCache":
+        """Room for `pages` pages of `page` tokens. Contents are undefined."""
+        dtype = np.dtype(dtype)
+        if dtype not in _KV_TYPES:
+            raise ValueError(f"KvCache: float32, uint16 (bf16) or uint8 (e4m3), got {dtype}")
+        if min(pages, page, heads, d) < 0:
+            raise ValueError(f"KvCache: negative dimension in {(pages, page, heads, d)}")
+        k, v = (DeviceArray.empty((pages, heads, page, d), stream, dtype) for _ in range(2))
+        if _KV_TYPES[dtype] != abi.KV_F8:
+            return cls(k, v)
+        return cls(k, v, *(DeviceArray.empty((pages, heads, page), stream) for _ in range(2)))
+
+    @property
+    def stream(self) -> Stream:
+        return self.k.stream
+
+    def _arrays(self) -> tuple:
+        return self.k, self.v, self.k_scales, self.v_scales
+
+
+@dataclass
+class KvBatch:
+    """The sequences of a step (mfr_kv_batch), int32 arrays in device memory: `lengths` [sequences],
+    tokens of each with this step's; `pages` [sequences, width], the pages that hold them; `starts`
+    [sequences + 1], the rows of each (None: the same number each); `prefix` tokens in
+    `prefix_pages` that all sequences share, in front of their own."""
+    lengths: DeviceArray
+    pages: DeviceArray
+    starts: DeviceArray | None = None
+    prefix: int = 0
+    prefix_pages: DeviceArray | None = None
+
+    def _arrays(self) -> tuple:
+        return self.lengths, self.pages, self.starts, self.prefix_pages
+
+
+def _cache_desc(cache: KvCache, what: str) -> abi.KvCacheDesc:
+    k, v = cache.k, cache.v
+    d = abi.KvCacheDesc()
+    if len(k.shape) != 4 or v.shape != k.shape or v.dtype != k.dtype or k.dtype not in _KV_TYPES:
+        raise ValueError(f"{what}: k is {k.dtype} {k.shape}, v {v.dtype} {v.shape}; both [pages, "
+                         "heads, page, d] in float32, uint16 (bf16) or uint8 (e4m3) are needed")
+    if v.strides != k.strides or (k.shape[3] > 1 and k.strides[3] != 1):
+        raise ValueError(f"{what}: k and v need the same strides, 1 along d")
+    d.type = _KV_TYPES[k.dtype]
+    d.pages, d.heads, d.page_size, d.d = k.shape
+    d.page_stride, d.head_stride, d.token_stride = k.strides[:3]
+    d.k, d.v = k.ptr, v.ptr
+    for name in ("k_scales", "v_scales"):
+        t = getattr(cache, name)
+        if (t is not None) != (d.type == abi.KV_F8):
+            raise ValueError(f"{what}: {name} belong to a cache in uint8, and only there")
+        if t is not None:
+            if t.dtype != np.float32 or t.shape != k.shape[:3] or not t.is_contiguous():
+                raise ValueError(f"{what}: {name} are {t.dtype} {t.shape}, contiguous float32 "
+                                 f"{k.shape[:3]} is needed")
+            setattr(d, name, t.ptr)
+    return d
+
+
+def _batch_desc(batch: KvBatch, rows: int, page: int, what: str) -> abi.KvBatchDesc:
+    d = abi.KvBatchDesc()
+    table = batch.pages
+    if len(table.shape) != 2 or table.dtype != np.int32 or (table.shape[1] > 1 and
+                                                            table.strides[1] != 1):
+        raise ValueError(f"{what}: pages are {table.dtype} {table.shape}, int32 [sequences, width] of "
+                         "unit stride is needed")
+    d.rows, (d.sequences, d.width) = rows, table.shape
+    d.table, d.table_rs = table.ptr, table.strides[0]
+    if batch.lengths.shape != table.shape[:1]:
+        raise ValueError(f"{what}: {batch.lengths.shape} lengths for {d.sequences} sequences")
+    d.lengths = _indices_of(batch.lengths, d.sequences, f"{what}: lengths")
+    if batch.starts is not None and batch.starts.shape != (d.sequences + 1,):
+        raise ValueError(f"{what}: {batch.starts.shape} starts for {d.sequences} sequences")
+    d.starts = _indices_of(batch.starts, d.sequences + 1, f"{what}: starts")
+    d.prefix = batch.prefix
+    if batch.prefix > 0:
+        if batch.prefix_pages is None:
+            raise ValueError(f"{what}: a prefix without its pages")
+        d.prefix_pages = _indices_of(batch.prefix_pages, -(-batch.prefix // max(page, 1)),
+                                     f"{what}: prefix_pages")
+    return d
+
+
+def _kv_held(what: str, cache: KvCache, batch: KvBatch, *operands) -> tuple:
+    return _arrays_of(what, *cache._arrays(), *batch._arrays(), *operands)
+
+
+def kv_append_desc(cache: KvCache, batch: KvBatch, k: DeviceArray, v: DeviceArray, *,
+                   rotary: Rotary | None = None, positions: DeviceArray | None = None,
+                   q: DeviceArray | None = None, q_out: DeviceArray | None = None) -> KvAppendDesc:
+    """The descriptor of one mfr_kv_append, to be filled once and run many times (kv_append_run): k
+    and v [rows, heads, d] to the cache, k turned by `rotary` on the way, and q [rows, q_heads, d]
+    with it to `q_out` (q itself if None). The descriptor keeps the arrays that it points to
+    (`held`)."""
+    if len(k.shape) != 3:
+        raise ValueError(f"kv_append: k is {k.shape}, [rows, heads, d] is needed")
+    if q is None and q_out is not None:
+        raise ValueError("kv_append: q_out without q")
+    rows = k.shape[0]
+    d = KvAppendDesc()
+    q_out = q if q_out is None else q_out
+    d.held = _kv_held("kv_append", cache, batch, k, v, q, q_out, positions)
+    d.cache = _cache_desc(cache, "kv_append")
+    d.batch = _batch_desc(batch, rows, d.cache.page_size, "kv_append")
+    shape = (rows, d.cache.heads, d.cache.d)
+    d.k, d.k_ts, d.k_hs = _heads_of(k, shape, "kv_append: k")
+    d.v, d.v_ts, d.v_hs = _heads_of(v, shape, "kv_append: v")
+    if q is not None:
+        if len(q.shape) != 3:
+            raise ValueError(f"kv_append: q is {q.shape}, [rows, heads, d] is needed")
+        shape = (rows, q.shape[1], d.cache.d)
+        d.q_heads = q.shape[1]
+        d.q, d.q_ts, d.q_hs = _heads_of(q, shape, "kv_append: q")
+        d.q_out, d.q_out_ts, d.q_out_hs = _heads_of(q_out, shape, "kv_append: q_out")
+    d.positions = _indices_of(positions, rows, "kv_append: positions")
+    if rotary is not None:
+        d.rotary = rotary
+    return d
+
+
+def kv_append_run(stream: Stream, desc: KvAppendDesc) -> None:
+    """mfr_kv_append on a filled descriptor."""
+    _same_device("kv_append", stream, desc)
+    abi.check(abi.load().mfr_kv_append(stream.handle, ctypes.byref(desc)), "mfr_kv_append")
+
+
+def kv_append(cache: KvCache, batch: KvBatch, k: DeviceArray, v: DeviceArray, *,
+              rotary: Rotary | None = None, positions: DeviceArray | None = None,
+              q: DeviceArray | None = None, q_out: DeviceArray | None = None) -> DeviceArray | None:
+    """The step's keys and values into the cache, the keys turned by `rotary`; the queries turned with
+    them, in a new array or `q_out` (which may be q), where they are given. Rows of no sequence of a new
+    array are undefined."""
+    if q is not None and q_out is None:
+        q_out = DeviceArray.empty(q.shape, q.stream)
+    kv_append_run(cache.stream, kv_append_desc(cache, batch, k, v, rotary=rotary,
+                                               positions=positions, q=q, q_out=q_out))
+    return q_out
+
+
+def attention_paged_desc(q: DeviceArray, cache: KvCache, batch: KvBatch, *, scale: float = 0.0,
+                         causal: bool = True, out: DeviceArray,
+                         workspace: DeviceArray | None = None) -> AttentionPagedDesc:
+    """The descriptor of one mfr_attention_paged, to be filled once and run many times
+    (attention_paged_run): q [rows, q_heads, d] against the cache, to `out`. `workspace`, a uint8 array
+    of attention_paged_workspace() bytes, is needed by calls that are captured into a graph. The
+    descriptor keeps the arrays that it points to (`held`)."""
+    if len(q.shape) != 3:
+        raise ValueError(f"attention_paged: q is {q.shape}, [rows, heads, d] is needed")
+    d = AttentionPagedDesc()
+    d.held = _kv_held("attention_paged", cache, batch, q, out, workspace)
+    d.cache = _cache_desc(cache, "attention_paged")
+    d.batch = _batch_desc(batch, q.shape[0], d.cache.page_size, "attention_paged")
+    shape = (q.shape[0], q.shape[1], d.cache.d)
+    d.q_heads = q.shape[1]
+    d.q, d.q_ts, d.q_hs = _heads_of(q, shape, "attention_paged: q")
+    d.out, d.out_ts, d.out_hs = _heads_of(out, shape, "attention_paged: out")
+    d.scale, d.causal = scale, 1 if causal else 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("attention_paged: a contiguous workspace is needed")
+        d.workspace = workspace.ptr
+        d.workspace_bytes = workspace.size * workspace.dtype.itemsize
+    return d
+
+
+def attention_paged_workspace(stream: Stream, desc: AttentionPagedDesc) -> int:
+    """The bytes of workspace that attention_paged_run(stream, desc) takes
+    (mfr_attention_paged_workspace)."""
+    _same_device("attention_paged_workspace", stream, desc)
+    size = ctypes.c_size_t()
+    abi.check(abi.load().mfr_attention_paged_workspace(stream.device, ctypes.byref(desc),
+                                                       ctypes.byref(size)),
+              "mfr_attention_paged_workspace")
+    return size.value
+
+
+def attention_paged_run(stream: Stream, desc: AttentionPagedDesc) -> None:
+    """mfr_attention_paged on a filled descriptor."""
+    _same_device("attention_paged", stream, desc)
+    abi.check(abi.load().mfr_attention_paged(stream.handle, ctypes.byref(desc)),
+              "mfr_attention_paged")
+
+
+def attention_paged(q: DeviceArray, cache: KvCache, batch: KvBatch, *, scale: float = 0.0,
+                    causal: bool = True, out: DeviceArray | None = None,
+                    workspace: DeviceArray | None = None) -> DeviceArray:
+    """softmax(scale q k^T) v of each row's queries q [rows, q_heads, d] against the batch's shared
+    prefix and its sequence's tokens up to the row's own (all of them where causal is False). Rows of
+    no sequence of a new array are undefined."""
+    if out is None:
+        out = DeviceArray.empty(q.shape, q.stream)
+    attention_paged_run(q.stream, attention_paged_desc(q, cache, batch, scale=scale, causal=causal,
+                                                       out=out, workspace=workspace))
+    return out
 
 
 def attention_fused(q: DeviceArray, k: DeviceArray, v: DeviceArray,

@@ -57,6 +57,12 @@ F8_TILE_64 = 10
 F8_TILE_128 = 11
 
 F8_BLOCK = 128  # MFR_F8_BLOCK: columns (and, of weights, rows) that share a scale
+ROTARY_HALVES = 0  # MFR_ROTARY_*: columns i and rot / 2 + i turn together, or 2 i and 2 i + 1
+ROTARY_PAIRS = 1
+ROTARY_MOST = 256  # columns of a head that turn, at most
+KV_F32 = 0  # MFR_KV_*: the number types of a paged cache
+KV_BF16 = 1
+KV_F8 = 2
 MAX_BATCH_DIMS = 4
 MAX_COPY_DIMS = 8
 SGEMM_SCRATCH_BYTES = 64 << 20  # MFR_SGEMM_SCRATCH_BYTES: mfr_sgemm_noalloc's fixed scratch
@@ -66,6 +72,7 @@ _i32 = ctypes.c_int32
 _vp = ctypes.c_void_p
 _f32 = ctypes.c_float
 _size = ctypes.c_size_t
+_f64 = ctypes.c_double
 
 
 class GemmDesc(ctypes.Structure):
@@ -134,6 +141,75 @@ class F8GemmDesc(ctypes.Structure):
     ]
 
 
+class Rotary(ctypes.Structure):
+    """mfr_rotary (include/mfr_rocm.h)."""
+
+    _fields_ = [("rot", _i32), ("layout", _i32), ("amplitude", _f32), ("reserved", _i32),
+                ("steps", _f64 * (ROTARY_MOST // 2))]
+
+
+class RopeDesc(ctypes.Structure):
+    """mfr_rope_desc (include/mfr_rocm.h)."""
+
+    held = ()  # the arrays that a filled descriptor points to
+
+    _fields_ = [
+        ("rows", _i64), ("heads", _i64), ("d", _i64),
+        ("x", _vp), ("x_ts", _i64), ("x_hs", _i64),
+        ("out", _vp), ("out_ts", _i64), ("out_hs", _i64),
+        ("positions", _vp), ("first", _i64), ("backward", _i32), ("reserved", _i32),
+        ("rotary", Rotary),
+    ]
+
+
+class KvCacheDesc(ctypes.Structure):
+    """mfr_kv_cache (include/mfr_rocm.h)."""
+
+    _fields_ = [
+        ("type", _i32), ("page_size", _i32), ("pages", _i64), ("heads", _i64), ("d", _i64),
+        ("k", _vp), ("v", _vp),
+        ("page_stride", _i64), ("token_stride", _i64), ("head_stride", _i64),
+        ("k_scales", _vp), ("v_scales", _vp),
+    ]
+
+
+class KvBatchDesc(ctypes.Structure):
+    """mfr_kv_batch (include/mfr_rocm.h)."""
+
+    _fields_ = [
+        ("rows", _i64), ("sequences", _i64), ("starts", _vp), ("lengths", _vp), ("table", _vp),
+        ("table_rs", _i64), ("width", _i64), ("prefix_pages", _vp), ("prefix", _i64),
+    ]
+
+
+class KvAppendDesc(ctypes.Structure):
+    """mfr_kv_append_desc (include/mfr_rocm.h)."""
+
+    held = ()  # the arrays that a filled descriptor points to
+
+    _fields_ = [
+        ("cache", KvCacheDesc), ("batch", KvBatchDesc),
+        ("k", _vp), ("k_ts", _i64), ("k_hs", _i64), ("v", _vp), ("v_ts", _i64), ("v_hs", _i64),
+        ("q", _vp), ("q_ts", _i64), ("q_hs", _i64),
+        ("q_out", _vp), ("q_out_ts", _i64), ("q_out_hs", _i64), ("q_heads", _i64),
+        ("positions", _vp), ("rotary", Rotary),
+    ]
+
+
+class AttentionPagedDesc(ctypes.Structure):
+    """mfr_attention_paged_desc (include/mfr_rocm.h)."""
+
+    held = ()  # the arrays that a filled descriptor points to
+
+    _fields_ = [
+        ("cache", KvCacheDesc), ("batch", KvBatchDesc),
+        ("q", _vp), ("q_ts", _i64), ("q_hs", _i64),
+        ("out", _vp), ("out_ts", _i64), ("out_hs", _i64),
+        ("q_heads", _i64), ("scale", _f32), ("causal", _i32),
+        ("workspace", _vp), ("workspace_bytes", _size),
+    ]
+
+
 # name -> (restype, argtypes). Every symbol the header declares is here; tests check that the
 # library exports each of them.
 SIGNATURES = {
@@ -182,6 +258,14 @@ SIGNATURES = {
     "mfr_f8gemm_plan": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(F8GemmDesc),
                                        ctypes.POINTER(_i32), ctypes.POINTER(_i32),
                                        ctypes.POINTER(_i32), ctypes.POINTER(ctypes.c_size_t)]),
+    "mfr_rotary_init": (ctypes.c_int, [ctypes.POINTER(Rotary), _i32, _i32, _f64, _f64, _f64, _f64,
+                                       _f64, _f64]),
+    "mfr_rope": (ctypes.c_int, [_vp, ctypes.POINTER(RopeDesc)]),
+    "mfr_kv_append": (ctypes.c_int, [_vp, ctypes.POINTER(KvAppendDesc)]),
+    "mfr_attention_paged": (ctypes.c_int, [_vp, ctypes.POINTER(AttentionPagedDesc)]),
+    "mfr_attention_paged_workspace": (ctypes.c_int, [ctypes.c_int,
+                                                     ctypes.POINTER(AttentionPagedDesc),
+                                                     ctypes.POINTER(_size)]),
     "mfr_strided_copy": (ctypes.c_int, [_vp, _vp, _vp, _i32, _i32, ctypes.POINTER(_i64),
                                         ctypes.POINTER(_i64)]),
     "mfr_fill": (ctypes.c_int, [_vp, _vp, _i32, _i64, ctypes.c_uint64]),

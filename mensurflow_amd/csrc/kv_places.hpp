@@ -1,0 +1,96 @@
+// Where the rows of a step stand (mfr_kv_batch): which sequence a row belongs to, which tokens it has,
+// which page holds a token. Everything read from device memory passes these functions, and none of
+// what they give leads outside the arrays. No HIP header, so that the CPU tests run them on any values.
+#pragma once
+
+#include <cstdint>
+
+#if defined(__HIPCC__)
+#define MFR_KV_BOTH __host__ __device__ inline
+#else
+#define MFR_KV_BOTH inline
+#endif
+
+namespace mfr::kv {
+
+struct Batch {
+    int32_t rows, sequences;
+    int32_t each;               // rows of every sequence, where starts is null
+    const int32_t* starts;
+    const int32_t* lengths;
+    const int32_t* table;
+    int64_t table_rs;
+    int32_t width;              // entries of a table's row
+    int32_t page_log2;          // tokens of a page
+    int32_t pages;              // of the cache
+    const int32_t* prefix_pages;
+    int32_t prefix;             // tokens
+};
+
+struct Span {
+    int32_t first, count;
+};
+
+MFR_KV_BOTH int32_t within(int32_t v, int32_t low, int32_t high) {
+    return v < low ? low : v > high ? high : v;
+}
+
+MFR_KV_BOTH int32_t capacity_of(const Batch& b) { return b.width << b.page_log2; }
+
+// The rows of sequence s, inside 0 .. rows.
+MFR_KV_BOTH Span span_of(const Batch& b, int32_t s) {
+    if (b.starts == nullptr) {
+        return {s * b.each, b.each};
+    }
+    const int32_t first = within(b.starts[s], 0, b.rows);
+    return {first, within(b.starts[s + 1], first, b.rows) - first};
+}
+
+// The tokens of sequence s that its table has room for.
+MFR_KV_BOTH int32_t length_of(const Batch& b, int32_t s) {
+    return within(b.lengths[s], 0, capacity_of(b));
+}
+
+// The place of a sequence's first row of `count`: below 0, or past the table, it has none.
+MFR_KV_BOTH int64_t first_place(const Batch& b, int32_t s, int32_t count) {
+    return static_cast<int64_t>(b.lengths[s]) - count;
+}
+
+// The sequence of a row, -1 if it has none.
+MFR_KV_BOTH int32_t sequence_of(const Batch& b, int32_t row) {
+    if (b.starts == nullptr) {
+        return row / b.each;
+    }
+    // The last sequence that starts at or before the row (empty ones of the same start come first).
+    int32_t low = 0, high = b.sequences;
+    while (high - low > 1) {
+        const int32_t mid = low + (high - low) / 2;
+        if (b.starts[mid] <= row) {
+            low = mid;
+        } else {
+            high = mid;
+        }
+    }
+    const Span span = span_of(b, low);
+    return row >= span.first && row - span.first < span.count ? low : -1;
+}
+
+// A page number that the cache has, or -1.
+MFR_KV_BOTH int32_t page_checked(const Batch& b, int32_t page) {
+    return page >= 0 && page < b.pages ? page : -1;
+}
+
+// The page of token `place` of sequence s, -1 if it has none.
+MFR_KV_BOTH int32_t page_of(const Batch& b, int32_t s, int64_t place) {
+    if (place < 0 || place >= capacity_of(b)) {
+        return -1;
+    }
+    return page_checked(b, b.table[s * b.table_rs + (place >> b.page_log2)]);
+}
+
+// The page of token `place` of the prefix, 0 <= place < prefix.
+MFR_KV_BOTH int32_t prefix_page_of(const Batch& b, int32_t place) {
+    return page_checked(b, b.prefix_pages[place >> b.page_log2]);
+}
+
+} // namespace mfr::kv
