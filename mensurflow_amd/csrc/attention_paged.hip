@@ -1,170 +1,124 @@
-// mfr_attention_paged: attention of a step's rows against a paged cache (kv.hpp).
-//
-// The plain form: a workgroup per row and query head; 32 lanes hold a token's row, 4 columns each, so 8
-// tokens go at a time, each lane group with its own running softmax; they are joined through LDS.
-#include "kv.hpp"
+// mfr_attention_paged: checks, the choice of the form, workspace and launches.
+#include "attention_paged.hpp"
 
 #include <algorithm>
 #include <cmath>
 
 namespace {
 
-using mfr::kv::Batch;
-using mfr::kv::Cache;
-using mfr::kv::Heads;
+using mfr::paged::Params;
 
-struct PagedParams {
-    Cache cache;
-    Batch batch;
-    Heads q;
-    float* out;
-    int64_t out_ts, out_hs;
-    int32_t q_heads, group;
-    float scale;
-    int32_t causal;
+// One launch over the prefix or over the sequences' own tokens.
+struct Launch {
+    Params p;
+    size_t parts; // rows of parts
 };
 
-constexpr float kLog2e = 1.4426950408889634f;
+struct Plan {
+    Launch shared, own;
+    bool has_prefix;
+    size_t bytes;
+};
 
-template <int TYPE>
-__device__ inline float4 load_row(const uint8_t* row, const float* scale, int c) {
-    if constexpr (TYPE == MFR_KV_F32) {
-        return *reinterpret_cast<const float4*>(row + 4 * c);
-    } else if constexpr (TYPE == MFR_KV_BF16) {
-        const uint2 w = *reinterpret_cast<const uint2*>(row + 2 * c);
-        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                           __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
-    } else {
-        const int w = *reinterpret_cast<const int*>(row + c);
-        const float s = *scale;
-        return make_float4(__builtin_amdgcn_cvt_f32_fp8(w, 0) * s,
-                           __builtin_amdgcn_cvt_f32_fp8(w, 1) * s,
-                           __builtin_amdgcn_cvt_f32_fp8(w, 2) * s,
-                           __builtin_amdgcn_cvt_f32_fp8(w, 3) * s);
-    }
+size_t aligned(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+size_t parts_bytes(size_t rows, int depth) {
+    return aligned(rows * depth * sizeof(float)) + aligned(rows * 2 * sizeof(float));
 }
 
-template <int TYPE> __global__ __launch_bounds__(256) void attention_paged_kernel(PagedParams p) {
-    __shared__ float4 values[8][32];
-    __shared__ float tops[8], sums[8];
-    const int64_t blocks = static_cast<int64_t>(p.batch.rows) * p.q_heads;
-    const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
-    const int c = 4 * lane;
-    const bool live = c < p.cache.d;
-    for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
-        const int32_t row = static_cast<int32_t>(b / p.q_heads);
-        const int32_t head = static_cast<int32_t>(b - static_cast<int64_t>(row) * p.q_heads);
-        const int32_t seq = mfr::kv::sequence_of(p.batch, row);
-        if (seq < 0) {
-            continue;
-        }
-        const mfr::kv::Span span = mfr::kv::span_of(p.batch, seq);
-        int64_t seen = mfr::kv::length_of(p.batch, seq);
-        if (p.causal != 0) {
-            const int64_t place =
-                mfr::kv::first_place(p.batch, seq, span.count) + (row - span.first);
-            seen = place + 1 < seen ? (place < 0 ? 0 : place + 1) : seen;
-        }
-        const int64_t kv_head = head / p.group;
-        float4 q = make_float4(0.f, 0.f, 0.f, 0.f), acc = q;
-        if (live) {
-            q = mfr::dev::load_loose(p.q.p + row * p.q.ts + head * p.q.hs + c);
-        }
-        float top = -INFINITY, sum = 0.0f;
-        const int64_t prefix = p.batch.prefix;
-        for (int64_t j = part; j < prefix + seen; j += 8) {
-            const int64_t place = j < prefix ? j : j - prefix;
-            const int32_t page = j < prefix
-                                     ? mfr::kv::prefix_page_of(p.batch, static_cast<int32_t>(j))
-                                     : mfr::kv::page_of(p.batch, seq, place);
-            if (page < 0) {
-                continue;
-            }
-            const int64_t slot = place & ((1 << p.cache.page_log2) - 1);
-            const int64_t at = page * p.cache.page_stride + slot * p.cache.token_stride +
-                               kv_head * p.cache.head_stride;
-            const int64_t scale_at =
-                ((page * p.cache.heads + kv_head) << p.cache.page_log2) + slot;
-            float4 k = make_float4(0.f, 0.f, 0.f, 0.f), v = k;
-            if (live) {
-                k = load_row<TYPE>(p.cache.k + at, p.cache.k_scales + scale_at, c);
-                v = load_row<TYPE>(p.cache.v + at, p.cache.v_scales + scale_at, c);
-            }
-            float s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w)));
-#pragma unroll
-            for (int m = 16; m > 0; m >>= 1) {
-                s += __shfl_xor(s, m, 64);
-            }
-            s = p.scale * s * kLog2e;
-            const float most = fmaxf(top, s);
-            const float reference = most == -INFINITY ? 0.0f : most;
-            const float shrink = __builtin_amdgcn_exp2f(top - reference);
-            const float w = __builtin_amdgcn_exp2f(s - reference);
-            top = most;
-            sum = fmaf(sum, shrink, w);
-            acc.x = fmaf(acc.x, shrink, w * v.x);
-            acc.y = fmaf(acc.y, shrink, w * v.y);
-            acc.z = fmaf(acc.z, shrink, w * v.z);
-            acc.w = fmaf(acc.w, shrink, w * v.w);
-        }
-        values[part][lane] = acc;
-        if (lane == 0) {
-            tops[part] = top;
-            sums[part] = sum;
-        }
-        __syncthreads();
-        if (part == 0 && live) {
-            float most = -INFINITY;
-            for (int i = 0; i < 8; ++i) {
-                most = fmaxf(most, tops[i]);
-            }
-            float total = 0.0f;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = 0; i < 8; ++i) {
-                const float w = tops[i] == -INFINITY ? 0.0f
-                                                     : __builtin_amdgcn_exp2f(tops[i] - most);
-                total = fmaf(w, sums[i], total);
-                v.x = fmaf(w, values[i][lane].x, v.x);
-                v.y = fmaf(w, values[i][lane].y, v.y);
-                v.z = fmaf(w, values[i][lane].z, v.z);
-                v.w = fmaf(w, values[i][lane].w, v.w);
-            }
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            mfr::dev::store_loose(p.out + row * p.out_ts + head * p.out_hs + c,
-                                  make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
-        }
-        __syncthreads();
-    }
+mfr::paged::Parts parts_at(uint8_t* at, size_t rows, int depth) {
+    return {reinterpret_cast<float*>(at),
+            reinterpret_cast<float*>(at + aligned(rows * depth * sizeof(float)))};
 }
 
-// The descriptor's checks (of shapes, layouts and pointers: no device is needed).
-PagedParams checked(const mfr_attention_paged_desc* desc) {
+Launch launch_of(Params p, int32_t type, int shared, int cus) {
+    mfr::kv::Work& w = p.work;
+    w.shared = shared;
+    const int64_t sequences = mfr::kv::sequences_of(w);
+    const int64_t rows = static_cast<int64_t>(w.batch.rows) * w.group;
+    // Rows of a sequence, on average: one tile of 16 where they fit.
+    w.tile_rows = rows <= 16 * sequences ? 16 : 32;
+    w.unit = type == MFR_KV_F32 ? 64 : 128;
+    const int64_t tokens =
+        shared != 0 ? w.batch.prefix : static_cast<int64_t>(mfr::kv::capacity_of(w.batch));
+    const int64_t units = std::max<int64_t>(1, (tokens + w.unit - 1) / w.unit);
+    const int64_t items = (rows / w.tile_rows + sequences) * w.heads;
+    const int64_t wanted = static_cast<int64_t>(cus) * (w.tile_rows == 16 ? 2 : 1);
+    p.groups = static_cast<int32_t>(items >= wanted ? wanted : std::min(wanted, items * units));
+    return {p, 2 * static_cast<size_t>(p.groups) * static_cast<size_t>(w.tile_rows)};
+}
+
+// The descriptor's checks (of shapes, layouts and pointers: no device is needed), and the plan of a call
+// on a device of `cus` compute units. The workspace: the parts of one launch after the other, then what
+// the prefix gave.
+Plan planned(const mfr_attention_paged_desc* desc, int cus) {
     using mfr::require;
     require(desc != nullptr, "attention_paged: null descriptor");
     const mfr_attention_paged_desc& d = *desc;
-    PagedParams p{};
+    Params p{};
     p.cache = mfr::kv::checked(d.cache, false, "attention_paged");
-    p.batch = mfr::kv::checked(d.batch, d.cache, "attention_paged");
+    p.work.batch = mfr::kv::checked(d.batch, d.cache, "attention_paged");
     require(d.q_heads >= 1 && d.q_heads % d.cache.heads == 0,
             "attention_paged: q's heads are no multiple of the cache's");
     mfr::kv::supported(d.q_heads <= mfr::kv::kMostHeads, "attention_paged: too many heads");
     require(std::isfinite(d.scale), "attention_paged: scale is not finite");
-    if (p.batch.rows > 0) {
-        mfr::kv::check_heads(d.q, d.q_ts, d.q_hs, d.batch.rows, d.q_heads, d.cache.d, false,
-                             "attention_paged: q");
-        mfr::kv::check_heads(d.out, d.out_ts, d.out_hs, d.batch.rows, d.q_heads, d.cache.d, true,
-                             "attention_paged: out");
+    Plan plan{};
+    if (p.work.batch.rows == 0) {
+        return plan;
     }
+    mfr::kv::check_heads(d.q, d.q_ts, d.q_hs, d.batch.rows, d.q_heads, d.cache.d, false,
+                         "attention_paged: q");
+    mfr::kv::check_heads(d.out, d.out_ts, d.out_hs, d.batch.rows, d.q_heads, d.cache.d, true,
+                         "attention_paged: out");
+    // Rows of an item, and of parts, are counted in 32 bits.
+    mfr::kv::supported(d.batch.rows * d.q_heads < (int64_t{1} << 30),
+                       "attention_paged: too many rows");
+    if (d.cache.pages == 0) { // no token is anywhere, and no address may be read
+        p.work.batch.width = 0;
+        p.work.batch.prefix = 0;
+    }
+    p.work.heads = p.cache.heads;
+    p.work.group = static_cast<int32_t>(d.q_heads / d.cache.heads);
     p.q = {d.q, d.q_ts, d.q_hs};
     p.out = d.out;
     p.out_ts = d.out_ts;
     p.out_hs = d.out_hs;
     p.q_heads = static_cast<int32_t>(d.q_heads);
-    p.group = static_cast<int32_t>(d.q_heads / d.cache.heads);
-    p.scale = d.scale != 0.0f ? d.scale
-                              : static_cast<float>(1.0 / std::sqrt(static_cast<double>(d.cache.d)));
     p.causal = d.causal;
-    return p;
+    const float scale =
+        d.scale != 0.0f ? d.scale : static_cast<float>(1.0 / std::sqrt(static_cast<double>(d.cache.d)));
+    p.scale = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+    p.depth = d.cache.d <= 64 ? 64 : 128;
+    plan.has_prefix = p.work.batch.prefix > 0;
+    plan.own = launch_of(p, d.cache.type, 0, cus);
+    plan.bytes = parts_bytes(plan.own.parts, p.depth);
+    if (plan.has_prefix) {
+        Params shared = p;
+        shared.causal = 0;
+        plan.shared = launch_of(shared, d.cache.type, 1, cus);
+        const size_t rows = static_cast<size_t>(d.batch.rows) * static_cast<size_t>(d.q_heads);
+        plan.bytes = std::max(plan.bytes, parts_bytes(plan.shared.parts, p.depth)) +
+                     parts_bytes(rows, p.depth);
+    }
+    return plan;
+}
+
+void run(Plan& plan, const mfr_attention_paged_desc& d, uint8_t* workspace, hipStream_t stream) {
+    const int depth = plan.own.p.depth;
+    if (plan.has_prefix) {
+        const size_t rows = static_cast<size_t>(d.batch.rows) * static_cast<size_t>(d.q_heads);
+        const mfr::paged::Parts prefix =
+            parts_at(workspace + plan.bytes - parts_bytes(rows, depth), rows, depth);
+        plan.own.p.prefix = plan.shared.p.prefix = prefix;
+    }
+    for (Launch* l : {&plan.shared, &plan.own}) {
+        if (l == &plan.shared && !plan.has_prefix) {
+            continue;
+        }
+        l->p.parts = parts_at(workspace, l->parts, depth);
+        mfr::paged::launch_few(l->p, d.cache.type, stream);
+        mfr::paged::launch_join(l->p, stream);
+    }
 }
 
 } // namespace
@@ -173,28 +127,46 @@ extern "C" {
 
 int mfr_attention_paged(mfr_stream_t stream, const mfr_attention_paged_desc* desc) {
     return mfr::guarded([&] {
-        const PagedParams p = checked(desc);
+        (void)planned(desc, 256); // before the stream is looked at
         auto& s = mfr::stream_of(stream);
-        if (p.batch.rows == 0) {
+        Plan plan = planned(desc, s.compute_units);
+        if (desc->batch.rows == 0 || desc->batch.sequences == 0) {
             return;
         }
-        const unsigned grid = static_cast<unsigned>(
-            std::min<int64_t>(static_cast<int64_t>(p.batch.rows) * p.q_heads, 1 << 20));
-        switch (desc->cache.type) {
-        case MFR_KV_F32: attention_paged_kernel<MFR_KV_F32><<<grid, 256, 0, s.stream>>>(p); break;
-        case MFR_KV_BF16: attention_paged_kernel<MFR_KV_BF16><<<grid, 256, 0, s.stream>>>(p); break;
-        default: attention_paged_kernel<MFR_KV_F8><<<grid, 256, 0, s.stream>>>(p); break;
+        if (desc->workspace != nullptr) {
+            mfr::require(mfr::aligned16(desc->workspace) && desc->workspace_bytes >= plan.bytes,
+                         "attention_paged: the workspace is too small (" +
+                             std::to_string(plan.bytes) + " bytes) or not 16-byte aligned");
+            run(plan, *desc, static_cast<uint8_t*>(desc->workspace), s.stream);
+            return;
         }
-        mfr::check_launch("attention_paged_kernel");
+        // A graph would keep the address of the stream's workspace, which a later call may free to grow
+        // it, and its replays may run beside calls that use it. (A stream that cannot be asked is
+        // taken as one that captures.)
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(s.stream, &capture) != hipSuccess) {
+            (void)hipGetLastError();
+            capture = hipStreamCaptureStatusActive;
+        }
+        mfr::require(capture == hipStreamCaptureStatusNone,
+                     "attention_paged: a captured call needs a workspace of its own (" +
+                         std::to_string(plan.bytes) + " bytes)");
+        // Held until the last launch is queued: another thread's reserve() may not free it before.
+        const std::lock_guard<std::mutex> hold(s.workspace_mutex);
+        run(plan, *desc, static_cast<uint8_t*>(s.reserve(plan.bytes)), s.stream);
     });
 }
 
 int mfr_attention_paged_workspace(int device, const mfr_attention_paged_desc* desc, size_t* bytes) {
     return mfr::guarded([&] {
-        (void)device;
-        (void)checked(desc);
+        (void)planned(desc, 256);
         mfr::require(bytes != nullptr, "attention_paged: null result");
-        *bytes = 0;
+        int cus = 0;
+        if (const int status =
+                mfr_get_device_info(device, nullptr, 0, nullptr, &cus, nullptr)) {
+            throw mfr::Error(status, mfr_last_error());
+        }
+        *bytes = planned(desc, cus).bytes;
     });
 }
 

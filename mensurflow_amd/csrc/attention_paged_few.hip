@@ -1,0 +1,885 @@
+// mfr_attention_paged for items of few rows (one query, or a few drafted ones, of the query heads that
+// share a head of the cache): bound by reading the cache once.
+//
+// A wavefront takes KEYS tokens at a time straight from memory into the operands of the matrix cores,
+// with no LDS between, and the four of a workgroup take turns along the item's tokens, each with its own
+// running softmax; they join through LDS at the item's end.
+//   - S^T = K Q^T by 16 x 16 products: the A operand of K is a lane's 16 bytes of its token's row (the
+//     depth in the order that the loads give, the queries cut alike), so a lane gets 4 tokens' scores
+//     of one row of the item.
+//   - O^T += V^T P^T: those scores are the B operand already, for tokens in the order in which lanes hold
+//     them. A lane loads D / 16 neighbouring columns of each of its 4 tokens; column j of all lanes'
+//     pieces is an A operand, made by byte permutations inside the lane, and the output's columns come
+//     out in that order.
+// bf16 and e4m3 numbers are exact in bf16. Queries, and weights (times the scales of the values), are
+// cut into three bf16 parts, so that products and sums are fp32's; fp32 caches use the fp32 products.
+#include "attention_paged.hpp"
+
+namespace {
+
+using namespace mfr::paged;
+namespace dev = mfr::paged::dev;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float exp2_native(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// The largest of v over the four lanes of one row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float row_max(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    v = fmaxf(a, b);
+    mfr::dev::swap_pair<false>(v, a, b);
+    return fmaxf(a, b);
+}
+
+__device__ __forceinline__ float row_sum(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    v = a + b;
+    mfr::dev::swap_pair<false>(v, a, b);
+    return a + b;
+}
+
+// Two floats cut into three bf16 parts each (the leading 8 bits of what is left, so that no part
+// overflows), packed with x in the low half.
+__device__ __forceinline__ void cut_pair(float x, float y, uint32_t& p0, uint32_t& p1,
+                                         uint32_t& p2) {
+    const auto high = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+    const auto pack = [](float u, float v) {
+        return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
+    };
+    p0 = pack(x, y);
+    x -= high(x);
+    y -= high(y);
+    p1 = pack(x, y);
+    x -= high(x);
+    y -= high(y);
+    p2 = pack(x, y);
+}
+
+// Two e4m3 numbers of a half of w as bf16.
+template <bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+
+template <int TYPE> constexpr int kBytes = TYPE == MFR_KV_F32 ? 4 : TYPE == MFR_KV_BF16 ? 2 : 1;
+
+// TILES: tokens of a step, in tiles of 16. PIECES: 16-byte pieces of a token's row that a lane loads.
+// VBYTES: bytes of a token's values that a lane loads.
+template <int TYPE, int D> struct Form {
+    static constexpr int kTiles = TYPE == MFR_KV_F32 ? 1 : 2;
+    static constexpr int kKeys = 16 * kTiles;
+    static constexpr int kPieces = D * kBytes<TYPE> / 64;
+    static constexpr int kValueBytes = D * kBytes<TYPE> / 16;
+    static constexpr int kColumns = D / 16;                       // of the values that a lane loads
+    static constexpr int kValueWords = (kValueBytes + 3) / 4;
+    static constexpr int kSteps = D / 32;                         // of depth, bf16 products
+};
+
+// The loads of a step: keys, values and scales of 16 tokens each tile.
+template <int TYPE, int D> struct Keys {
+    uint4 k[Form<TYPE, D>::kTiles][Form<TYPE, D>::kPieces];
+    float4 scale[Form<TYPE, D>::kTiles];
+};
+template <int TYPE, int D> struct Values {
+    uint32_t v[Form<TYPE, D>::kTiles][4][Form<TYPE, D>::kValueWords];
+    float4 scale[Form<TYPE, D>::kTiles];
+};
+
+// A lane's constant place in the loads.
+struct Lanes {
+    int row;               // of the item's tile, and token of a key tile: lane % 16
+    int quad;              // lane / 16
+    uint32_t key_at;       // bytes from a tile's first token to the lane's first piece of its key
+    uint32_t value_at;     // to the lane's columns of its first value
+    uint32_t token_stride;
+};
+
+// The first token of a tile of 16 in memory: in bytes, and its place among the scales.
+struct TileAt {
+    int64_t at;
+    int64_t scale_at;
+    bool there;            // its page is one of the cache's
+};
+
+// Of RT tiles of 16 rows: scores or weights (lane: its row, tokens 4 quad + r of each tile), and weighted
+// values (lane: its row, column j of rows 4 quad + r of the pieces).
+template <int TYPE, int D, int RT> using Scores = floatx4[RT][Form<TYPE, D>::kTiles];
+template <int TYPE, int D, int RT> using Sums = floatx4[RT][Form<TYPE, D>::kColumns];
+template <int TYPE, int D> using Tiles = TileAt[Form<TYPE, D>::kTiles];
+template <int TYPE, int D> using There = bool[Form<TYPE, D>::kTiles];
+
+// The running softmax of a lane's row.
+struct Running {
+    float top = -INFINITY;
+    float sum = 0.0f; // this lane's share
+    int32_t seen;     // tokens that the row sees
+};
+template <int RT> using Rows = Running[RT];
+
+template <int TYPE, int D, int RT> struct Segment {
+    using F = Form<TYPE, D>;
+    const Params& p;
+    const Shape& shape;
+    const int32_t seq, head;
+    const Lanes& lanes;
+
+    // A tile that no token of the sequence is in is taken as the last one that has some.
+    __device__ __forceinline__ TileAt tile_at(int32_t token) const {
+        const Batch& b = p.work.batch;
+        const int32_t first = min(token, (shape.tokens - 1) & ~15);
+        const int32_t* pages = p.work.shared != 0 ? b.prefix_pages : b.table + seq * b.table_rs;
+        const int32_t page = __builtin_amdgcn_readfirstlane(pages[first >> b.page_log2]);
+        const bool there = mfr::kv::page_checked(b, page) >= 0;
+        const int64_t number = there ? page : 0;
+        const int32_t slot = first & ((1 << b.page_log2) - 1);
+        return {number * p.cache.page_stride + head * p.cache.head_stride +
+                    static_cast<int64_t>(slot) * p.cache.token_stride,
+                ((number * p.cache.heads + head) << b.page_log2) + slot, there};
+    }
+
+    __device__ __forceinline__ void load_keys(Keys<TYPE, D>& to, const Tiles<TYPE, D>& at) const {
+        const int row_bytes = p.cache.d * kBytes<TYPE>;
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+            const uint8_t* base = p.cache.k + at[t].at;
+#pragma unroll
+            for (int i = 0; i < F::kPieces; ++i) {
+                to.k[t][i] = make_uint4(0, 0, 0, 0);
+                if (64 * i + 16 * lanes.quad < row_bytes) {
+                    to.k[t][i] =
+                        *reinterpret_cast<const uint4*>(base + (lanes.key_at + 64 * i));
+                }
+            }
+            if constexpr (TYPE == MFR_KV_F8) {
+                to.scale[t] = *reinterpret_cast<const float4*>(p.cache.k_scales + at[t].scale_at +
+                                                               4 * lanes.quad);
+            }
+        }
+    }
+
+    __device__ __forceinline__ void load_values(Values<TYPE, D>& to,
+                                                const Tiles<TYPE, D>& at) const {
+        const int row_bytes = p.cache.d * kBytes<TYPE>;
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+            const uint8_t* base = p.cache.v + at[t].at;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t from = lanes.value_at + r * lanes.token_stride;
+                auto& v = to.v[t][r];
+                if constexpr (TYPE == MFR_KV_F32) {
+#pragma unroll
+                    for (int i = 0; i < F::kValueWords / 4; ++i) {
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (256 * i + 16 * lanes.row < row_bytes) {
+                            w = *reinterpret_cast<const uint4*>(base + (from + 256 * i));
+                        }
+                        v[4 * i] = w.x;
+                        v[4 * i + 1] = w.y;
+                        v[4 * i + 2] = w.z;
+                        v[4 * i + 3] = w.w;
+                    }
+                } else {
+                    constexpr int kWords = F::kValueWords;
+                    struct alignas(4 * kWords) Piece {
+                        uint32_t w[kWords];
+                    };
+                    Piece piece{};
+                    if (F::kValueBytes * lanes.row < row_bytes) {
+                        piece = *reinterpret_cast<const Piece*>(base + from);
+                    }
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        v[i] = piece.w[i];
+                    }
+                }
+            }
+            if constexpr (TYPE == MFR_KV_F8) {
+                to.scale[t] = *reinterpret_cast<const float4*>(p.cache.v_scales + at[t].scale_at +
+                                                               4 * lanes.quad);
+            }
+        }
+    }
+};
+
+// The queries of an item's rows as B operands: three bf16 parts, or fp32.
+template <int TYPE, int D, int RT> struct Queries {
+    static constexpr int kSteps = Form<TYPE, D>::kSteps;
+    uint4 part[RT][3][kSteps];
+};
+template <int D, int RT> struct Queries<MFR_KV_F32, D, RT> {
+    float4 q[RT][D / 16];
+};
+
+template <int TYPE, int D, int RT>
+__device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Params& p,
+                                             const Shape& shape, int32_t head, int32_t tile,
+                                             const Lanes& lanes) {
+    const int32_t rows = shape.span.count * p.work.group;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int32_t rr = tile * (16 * RT) + 16 * rt + lanes.row;
+        const int32_t i = rr / p.work.group;
+        const float* q = p.q.p + (shape.span.first + static_cast<int64_t>(i)) * p.q.ts +
+                         (head * p.work.group + (rr - i * p.work.group)) * p.q.hs;
+        const auto quad = [&](int c) {
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (rr < rows && c < p.cache.d) {
+                v = mfr::dev::load_loose(q + c);
+            }
+            return v;
+        };
+        if constexpr (TYPE == MFR_KV_F32) {
+#pragma unroll
+            for (int s = 0; s < D / 16; ++s) {
+                to.q[rt][s] = quad(16 * s + 4 * lanes.quad);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < Form<TYPE, D>::kSteps; ++s) {
+                // The depths of piece s of a key: 8 neighbours, or in 8 bits half of 16.
+                const int c = TYPE == MFR_KV_BF16 ? 32 * s + 8 * lanes.quad
+                                                  : 64 * (s / 2) + 16 * lanes.quad + 8 * (s % 2);
+                const float4 a = quad(c), b = quad(c + 4);
+                auto& part = to.part[rt];
+                cut_pair(a.x, a.y, part[0][s].x, part[1][s].x, part[2][s].x);
+                cut_pair(a.z, a.w, part[0][s].y, part[1][s].y, part[2][s].y);
+                cut_pair(b.x, b.y, part[0][s].z, part[1][s].z, part[2][s].z);
+                cut_pair(b.z, b.w, part[0][s].w, part[1][s].w, part[2][s].w);
+            }
+        }
+    }
+}
+
+// Scores of a step's tokens, unscaled.
+template <int TYPE, int D, int RT>
+__device__ __forceinline__ void scores_of(Scores<TYPE, D, RT>& s,
+                                          const Keys<TYPE, D>& keys,
+                                          const Queries<TYPE, D, RT>& queries) {
+    using F = Form<TYPE, D>;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+            s[rt][t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    }
+    if constexpr (TYPE == MFR_KV_F32) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            const float k[4] = {__uint_as_float(keys.k[0][i].x), __uint_as_float(keys.k[0][i].y),
+                                __uint_as_float(keys.k[0][i].z), __uint_as_float(keys.k[0][i].w)};
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const float4 q = queries.q[rt][i];
+                s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0], q.x, s[rt][0], 0, 0, 0);
+                s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[1], q.y, s[rt][0], 0, 0, 0);
+                s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[2], q.z, s[rt][0], 0, 0, 0);
+                s[rt][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[3], q.w, s[rt][0], 0, 0, 0);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int step = 0; step < F::kSteps; ++step) {
+            bf16x8 k[F::kTiles];
+#pragma unroll
+            for (int t = 0; t < F::kTiles; ++t) {
+                if constexpr (TYPE == MFR_KV_BF16) {
+                    k[t] = __builtin_bit_cast(bf16x8, keys.k[t][step]);
+                } else {
+                    const uint4 w = keys.k[t][step / 2];
+                    const uint32_t lo = step % 2 == 0 ? w.x : w.z, hi = step % 2 == 0 ? w.y : w.w;
+                    k[t] = __builtin_bit_cast(bf16x8,
+                                              make_uint4(widen<false>(lo), widen<true>(lo),
+                                                         widen<false>(hi), widen<true>(hi)));
+                }
+            }
+            // The smallest parts first.
+#pragma unroll
+            for (int part = 2; part >= 0; --part) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const bf16x8 q = __builtin_bit_cast(bf16x8, queries.part[rt][part][step]);
+#pragma unroll
+                    for (int t = 0; t < F::kTiles; ++t) {
+                        s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t], q, s[rt][t], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ float element(const float4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// Scores to weights (not yet times the values' scales); the output so far is rescaled where a
+// maximum moved. EDGE: some row does not see some token; `first` is the step's first token.
+template <int TYPE, int D, int RT, bool EDGE>
+__device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
+                                             Sums<TYPE, D, RT>& acc,
+                                             Rows<RT>& run, const Keys<TYPE, D>& keys,
+                                             float scale, int32_t first, const Lanes& lanes,
+                                             const There<TYPE, D>& there) {
+    using F = Form<TYPE, D>;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float v = s[rt][t][r] * scale;
+                if constexpr (TYPE == MFR_KV_F8) {
+                    v *= element(keys.scale[t], r);
+                }
+                if constexpr (EDGE) {
+                    const int32_t token = first + 16 * t + 4 * lanes.quad + r;
+                    v = there[t] && token < run[rt].seen ? v : -INFINITY;
+                }
+                s[rt][t][r] = v;
+                most = fmaxf(most, v);
+            }
+        }
+        most = fmaxf(run[rt].top, row_max(most));
+        // Nothing seen yet: any finite reference gives weights of 0.
+        const float reference = most == -INFINITY ? 0.0f : most;
+        if (__any(most != run[rt].top)) {
+            const float shrink = exp2_native(run[rt].top - reference);
+            run[rt].top = most;
+            run[rt].sum *= shrink;
+#pragma unroll
+            for (int j = 0; j < F::kColumns; ++j) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc[rt][j][r] *= shrink;
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float w = exp2_native(s[rt][t][r] - reference);
+                run[rt].sum += w;
+                s[rt][t][r] = w;
+            }
+        }
+    }
+}
+
+// Column j of the values as an A operand of bf16 products; tokens r of tile t whose bit 4 t + r of
+// `keep` is clear are zeros.
+template <int TYPE, int D>
+__device__ __forceinline__ bf16x8 column_of(const Values<TYPE, D>& values, int j,
+                                            uint32_t keep = ~0u) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { // tokens 2 (i % 2), 2 (i % 2) + 1 of tile i / 2
+        constexpr int kPerWord = TYPE == MFR_KV_BF16 ? 2 : 4;
+        uint32_t a = values.v[i / 2][2 * (i % 2)][j / kPerWord];
+        uint32_t b = values.v[i / 2][2 * (i % 2) + 1][j / kPerWord];
+        a = (keep >> (2 * i) & 1u) != 0 ? a : 0u;
+        b = (keep >> (2 * i + 1) & 1u) != 0 ? b : 0u;
+        if constexpr (TYPE == MFR_KV_BF16) {
+            w[i] = __builtin_amdgcn_perm(b, a, j % 2 == 0 ? 0x05040100u : 0x07060302u);
+        } else {
+            const uint32_t both =
+                __builtin_amdgcn_perm(b, a, j % 4 < 2 ? 0x05010400u : 0x07030602u);
+            w[i] = j % 2 == 0 ? widen<false>(both) : widen<true>(both);
+        }
+    }
+    return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// Whether a value that the lane loaded is an infinity or NaN.
+template <int TYPE, int D> __device__ __forceinline__ bool odd_values(const Values<TYPE, D>& values) {
+    using F = Form<TYPE, D>;
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int i = 0; i < F::kValueWords; ++i) {
+                const uint32_t w = values.v[t][r][i];
+                if constexpr (TYPE == MFR_KV_F32) {
+                    odd |= (w & 0x7f800000u) == 0x7f800000u;
+                } else if constexpr (TYPE == MFR_KV_BF16) {
+                    odd |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        odd |= ((w >> (8 * e)) & 0x7fu) == 0x7fu;
+                    }
+                }
+            }
+        }
+    }
+    return odd;
+}
+
+// Leaves the values of tokens before `seen` (from the step's first), zeros for the others.
+template <int TYPE, int D>
+__device__ __forceinline__ void keep_values(Values<TYPE, D>& values, int32_t seen,
+                                            const Lanes& lanes,
+                                            const There<TYPE, D>& there) {
+    using F = Form<TYPE, D>;
+#pragma unroll
+    for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool keep = there[t] && 16 * t + 4 * lanes.quad + r < seen;
+#pragma unroll
+            for (int i = 0; i < F::kValueWords; ++i) {
+                values.v[t][r][i] = keep ? values.v[t][r][i] : 0u;
+            }
+        }
+    }
+}
+
+// The weights of a tile of rows as B operands of bf16 products.
+struct Cut {
+    bf16x8 part[3];
+};
+__device__ __forceinline__ Cut cut_weights(const floatx4& a, const floatx4& b) {
+    uint4 cut[3];
+    cut_pair(a[0], a[1], cut[0].x, cut[1].x, cut[2].x);
+    cut_pair(a[2], a[3], cut[0].y, cut[1].y, cut[2].y);
+    cut_pair(b[0], b[1], cut[0].z, cut[1].z, cut[2].z);
+    cut_pair(b[2], b[3], cut[0].w, cut[1].w, cut[2].w);
+    return {__builtin_bit_cast(bf16x8, cut[0]), __builtin_bit_cast(bf16x8, cut[1]),
+            __builtin_bit_cast(bf16x8, cut[2])};
+}
+
+// sums + the products of one column, the smallest parts first.
+__device__ __forceinline__ floatx4 add_column(floatx4 sums, bf16x8 column, const Cut& w) {
+#pragma unroll
+    for (int i = 2; i >= 0; --i) {
+        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(column, w.part[i], sums, 0, 0, 0);
+    }
+    return sums;
+}
+
+// acc += V^T P^T.
+template <int TYPE, int D, int RT>
+__device__ __forceinline__ void add_values(Sums<TYPE, D, RT>& acc, const Scores<TYPE, D, RT>& w,
+                                           const Values<TYPE, D>& values) {
+    using F = Form<TYPE, D>;
+    if constexpr (TYPE == MFR_KV_F32) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int j = 0; j < F::kColumns; ++j) {
+                const float v = __uint_as_float(values.v[0][r][j]);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    acc[rt][j] =
+                        __builtin_amdgcn_mfma_f32_16x16x4f32(v, w[rt][0][r], acc[rt][j], 0, 0, 0);
+                }
+            }
+        }
+    } else {
+        Cut cut[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            cut[rt] = cut_weights(w[rt][0], w[rt][1]);
+        }
+#pragma unroll
+        for (int j = 0; j < F::kColumns; ++j) {
+            const bf16x8 v = column_of<TYPE, D>(values, j);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                acc[rt][j] = add_column(acc[rt][j], v, cut[rt]);
+            }
+        }
+    }
+}
+
+// A step that some row does not see whole. Where a token that only some rows see has values that are
+// no numbers, they must not meet the others' weights of 0: each row then adds its own, with the tokens
+// that it does not see cleared, and the other rows' sums stay.
+template <int TYPE, int D, int RT>
+__device__ __forceinline__ void add_edge_values(Sums<TYPE, D, RT>& acc,
+                                                const Scores<TYPE, D, RT>& w,
+                                                Values<TYPE, D>& values, const Rows<RT>& run,
+                                                int32_t tokens, int32_t first, const Lanes& lanes,
+                                                const There<TYPE, D>& there) {
+    using F = Form<TYPE, D>;
+    keep_values<TYPE, D>(values, tokens - first, lanes, there);
+    if (!__any(odd_values<TYPE, D>(values))) {
+        add_values<TYPE, D, RT>(acc, w, values);
+        return;
+    }
+#pragma unroll 1
+    for (int row = 0; row < 16; ++row) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int32_t seen = __builtin_amdgcn_readlane(run[rt].seen, row) - first;
+            uint32_t keep = 0;
+#pragma unroll
+            for (int i = 0; i < 4 * F::kTiles; ++i) {
+                keep |= 16 * (i / 4) + 4 * lanes.quad + i % 4 < seen ? 1u << i : 0u;
+            }
+            if constexpr (TYPE == MFR_KV_F32) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                    for (int j = 0; j < F::kColumns; ++j) {
+                        const float v =
+                            __uint_as_float((keep >> r & 1u) != 0 ? values.v[0][r][j] : 0u);
+                        const floatx4 sums = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                            v, w[rt][0][r], acc[rt][j], 0, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            acc[rt][j][e] = lanes.row == row ? sums[e] : acc[rt][j][e];
+                        }
+                    }
+                }
+            } else {
+                const Cut cut = cut_weights(w[rt][0], w[rt][1]);
+#pragma unroll
+                for (int j = 0; j < F::kColumns; ++j) {
+                    const floatx4 sums =
+                        add_column(acc[rt][j], column_of<TYPE, D>(values, j, keep), cut);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        acc[rt][j][e] = lanes.row == row ? sums[e] : acc[rt][j][e];
+                    }
+                }
+            }
+        }
+    }
+}
+
+// Weights times the scales of the values, in 8 bits; 0 for tokens that the row does not see, whatever
+// their scales are.
+template <int TYPE, int D, int RT, bool EDGE>
+__device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w,
+                                              const Values<TYPE, D>& values,
+                                              const Rows<RT>& run, int32_t first,
+                                              const Lanes& lanes,
+                                              const There<TYPE, D>& there) {
+    if constexpr (TYPE == MFR_KV_F8) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int t = 0; t < Form<TYPE, D>::kTiles; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float v = w[rt][t][r] * element(values.scale[t], r);
+                    const int32_t token = first + 16 * t + 4 * lanes.quad + r;
+                    w[rt][t][r] = !EDGE || (there[t] && token < run[rt].seen) ? v : 0.0f;
+                }
+            }
+        }
+    }
+}
+
+// The first of four neighbouring columns that a lane holds in acc[4 q ..][r].
+template <int TYPE, int D> __device__ __forceinline__ int column_at(int quad, int r, int q) {
+    return TYPE == MFR_KV_F32 ? 16 * quad + 4 * r + 64 * q
+                              : Form<TYPE, D>::kColumns * (4 * quad + r) + 4 * q;
+}
+
+template <int TYPE, int D, int RT>
+__global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few_kernel(Params p) {
+    using F = Form<TYPE, D>;
+    constexpr int kPitch = D + 4;
+    __shared__ float joined[kWaves][16][kPitch];
+    __shared__ float stats[kWaves][16][2];
+    const int64_t index = blockIdx.x;
+    const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t chunk) {
+        return index * chunk < total ? index * chunk : int64_t{-1};
+    });
+    if (place.seq < 0) {
+        return;
+    }
+    const int lane = threadIdx.x % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x / 64));
+    Lanes lanes;
+    lanes.row = lane % 16;
+    lanes.quad = lane / 16;
+    lanes.token_stride = p.cache.token_stride;
+    lanes.key_at = lanes.row * p.cache.token_stride + 16 * lanes.quad;
+    lanes.value_at = 4 * lanes.quad * p.cache.token_stride +
+                     (TYPE == MFR_KV_F32 ? 16 : F::kValueBytes) * lanes.row;
+    const int64_t begin = index * place.chunk;
+    const int64_t end = begin + place.chunk < place.total ? begin + place.chunk : place.total;
+    int32_t seq = place.seq;
+    int64_t base = place.base;
+    Shape shape = mfr::kv::shape_of(p.work, seq);
+    for (int64_t at = begin; at < end;) {
+        while (at >= base + shape.count) { // the next sequence that has units
+            base += shape.count;
+            shape = mfr::kv::shape_of(p.work, ++seq);
+        }
+        const Item item = mfr::kv::item_of(shape, base, at);
+        const int64_t item_end = item.begin + shape.units;
+        const int32_t units = static_cast<int32_t>((item_end < end ? item_end : end) - at);
+
+        Rows<RT> run;
+        const int32_t rows = shape.span.count * p.work.group;
+        const int32_t row0 = item.tile * (16 * RT);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int32_t rr = min(row0 + 16 * rt + lanes.row, rows - 1);
+            run[rt].seen = mfr::kv::seen_by(shape, rr / p.work.group, p.causal != 0);
+        }
+        // Tokens that every row sees, and that some row sees.
+        const int32_t all_see = mfr::kv::seen_by(shape, row0 / p.work.group, p.causal != 0);
+        const int32_t some_see = mfr::kv::seen_by(
+            shape, (min(row0 + 16 * RT, rows) - 1) / p.work.group, p.causal != 0);
+        Queries<TYPE, D, RT> queries;
+        load_queries<TYPE, D, RT>(queries, p, shape, item.head, item.tile, lanes);
+        Sums<TYPE, D, RT> acc;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int j = 0; j < F::kColumns; ++j) {
+                acc[rt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+        const Segment<TYPE, D, RT> segment{p, shape, seq, item.head, lanes};
+        // This wavefront's tokens: a step of every unit.
+        constexpr int kUnit = kWaves * F::kKeys;
+        int32_t first = item.first * kUnit + wave * F::kKeys;
+        const int32_t last = min(some_see, (item.first + units) * kUnit);
+        if (first < last) {
+            Tiles<TYPE, D> tiles;
+            Keys<TYPE, D> keys;
+            Values<TYPE, D> values;
+            const auto tiles_of = [&](int32_t token, Tiles<TYPE, D>& to) {
+#pragma unroll
+                for (int t = 0; t < F::kTiles; ++t) {
+                    to[t] = segment.tile_at(token + 16 * t);
+                }
+            };
+            // Whether a step is one that every row sees whole, in pages that are there.
+            const auto plain = [&](int32_t token) {
+                bool there = token + F::kKeys <= all_see;
+#pragma unroll
+                for (int t = 0; t < F::kTiles; ++t) {
+                    there = there && tiles[t].there;
+                }
+                return there;
+            };
+            tiles_of(first, tiles);
+            segment.load_keys(keys, tiles);
+            segment.load_values(values, tiles);
+            while (first < last && plain(first)) {
+                // The next step's keys are under way from the scores on, its values from the end;
+                // behind the last step the same ones are loaded again.
+                tiles_of(first + kUnit < last ? first + kUnit : first, tiles);
+                Scores<TYPE, D, RT> s;
+                scores_of<TYPE, D, RT>(s, keys, queries);
+                softmax_step<TYPE, D, RT, false>(s, acc, run, keys, p.scale, first, lanes, {});
+                segment.load_keys(keys, tiles);
+                scale_weights<TYPE, D, RT, false>(s, values, run, first, lanes, {});
+                add_values<TYPE, D, RT>(acc, s, values);
+                segment.load_values(values, tiles);
+                first += kUnit;
+            }
+            while (first < last) {
+                There<TYPE, D> there;
+#pragma unroll
+                for (int t = 0; t < F::kTiles; ++t) {
+                    there[t] = tiles[t].there;
+                }
+                Scores<TYPE, D, RT> s;
+                scores_of<TYPE, D, RT>(s, keys, queries);
+                softmax_step<TYPE, D, RT, true>(s, acc, run, keys, p.scale, first, lanes, there);
+                scale_weights<TYPE, D, RT, true>(s, values, run, first, lanes, there);
+                add_edge_values<TYPE, D, RT>(acc, s, values, run, shape.tokens, first, lanes, there);
+                first += kUnit;
+                if (first < last) {
+                    tiles_of(first, tiles);
+                    segment.load_keys(keys, tiles);
+                    segment.load_values(values, tiles);
+                }
+            }
+        }
+        // The wavefronts' parts, joined: 16 threads a row, 4 columns each and 64 further on.
+        const bool whole = item.first == 0 && units == shape.units;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            __syncthreads(); // the rows before have been read
+#pragma unroll
+            for (int q = 0; q < F::kColumns / 4; ++q) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    *reinterpret_cast<float4*>(
+                        &joined[wave][lanes.row][column_at<TYPE, D>(lanes.quad, r, q)]) =
+                        make_float4(acc[rt][4 * q][r], acc[rt][4 * q + 1][r],
+                                    acc[rt][4 * q + 2][r], acc[rt][4 * q + 3][r]);
+                }
+            }
+            const float sum = row_sum(run[rt].sum);
+            if (lanes.quad == 0) {
+                stats[wave][lanes.row][0] = run[rt].top;
+                stats[wave][lanes.row][1] = sum;
+            }
+            __syncthreads();
+            const int row = threadIdx.x / 16;
+            const int32_t rr = row0 + 16 * rt + row;
+            if (rr < rows) {
+                float top = stats[0][row][0];
+#pragma unroll
+                for (int i = 1; i < kWaves; ++i) {
+                    top = fmaxf(top, stats[i][row][0]);
+                }
+                float weight[kWaves], total = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kWaves; ++i) {
+                    weight[i] = dev::part_weight(stats[i][row][0], top);
+                    total = fmaf(weight[i], stats[i][row][1], total);
+                }
+                const int32_t i = rr / p.work.group;
+                const int32_t head = item.head * p.work.group + (rr - i * p.work.group);
+                const int64_t part = mfr::kv::part_of(index, place.chunk, item.begin) * (16 * RT) +
+                                     16 * rt + row;
+#pragma unroll
+                for (int c0 = 0; c0 < D; c0 += 64) {
+                    const int c = c0 + 4 * (threadIdx.x % 16);
+                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < kWaves; ++w) {
+                        v = dev::add_scaled(v, *reinterpret_cast<const float4*>(&joined[w][row][c]),
+                                            weight[w]);
+                    }
+                    if (whole) {
+                        dev::finish(p, shape.span.first + static_cast<int64_t>(i), head, c, v, top,
+                                    total);
+                    } else {
+                        *reinterpret_cast<float4*>(p.parts.values + part * D + c) = v;
+                        if (c == 0) {
+                            *reinterpret_cast<float2*>(p.parts.stats + 2 * part) =
+                                make_float2(top, total);
+                        }
+                    }
+                }
+            }
+        }
+        at += units;
+    }
+}
+
+// Joins the parts of the items that were cut: workgroup x looks at the end of chunk x, and takes the
+// item that began in it and goes on, rows y, y + gridDim.y, ... of it. 32 lanes hold a part's row, 8 parts
+// at a time, so a long list of parts has its loads in flight together.
+__global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p) {
+    __shared__ float4 values[8][32];
+    __shared__ float tops[8], sums[8];
+    const int64_t index = blockIdx.x;
+    const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t chunk) {
+        // The last unit of a chunk that another one follows.
+        return (index + 1) * chunk < total ? (index + 1) * chunk - 1 : int64_t{-1};
+    });
+    if (place.seq < 0) {
+        return;
+    }
+    const Shape shape = mfr::kv::shape_of(p.work, place.seq);
+    const int64_t edge = (index + 1) * place.chunk;
+    const Item item = mfr::kv::item_of(shape, place.base, edge - 1);
+    const int64_t end = item.begin + shape.units;
+    if (item.begin < index * place.chunk || end <= edge) {
+        return;
+    }
+    const int64_t last = (end - 1) / place.chunk; // the chunk of its last unit
+    const int count = static_cast<int>(last - index) + 1;
+    const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    const int c = 4 * lane;
+    const int32_t rows = shape.span.count * p.work.group;
+    const int32_t row0 = item.tile * p.work.tile_rows;
+    const int32_t here = min(p.work.tile_rows, rows - row0);
+    for (int32_t r = blockIdx.y; r < here; r += gridDim.y) {
+        float top = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+        for (int i = group; i < count; i += 8) {
+            const int64_t part =
+                mfr::kv::part_of(index + i, place.chunk, item.begin) * p.work.tile_rows + r;
+            const float2 stats = *reinterpret_cast<const float2*>(p.parts.stats + 2 * part);
+            float4 other = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (c < p.depth) {
+                other = *reinterpret_cast<const float4*>(p.parts.values + part * p.depth + c);
+            }
+            const float most = fmaxf(top, stats.x);
+            const float a = dev::part_weight(top, most), b = dev::part_weight(stats.x, most);
+            sum = fmaf(b, stats.y, a * sum);
+            v = dev::add_scaled(dev::scaled(v, a), other, b);
+            top = most;
+        }
+        __syncthreads(); // the row before has been read
+        values[group][lane] = v;
+        if (lane == 0) {
+            tops[group] = top;
+            sums[group] = sum;
+        }
+        __syncthreads();
+        if (group == 0 && c < p.depth) {
+            float most = tops[0];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) {
+                most = fmaxf(most, tops[i]);
+            }
+            float total = 0.0f;
+            float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float w = dev::part_weight(tops[i], most);
+                total = fmaf(w, sums[i], total);
+                all = dev::add_scaled(all, values[i][lane], w);
+            }
+            const int32_t rr = row0 + r;
+            const int32_t i = rr / p.work.group;
+            dev::finish(p, shape.span.first + static_cast<int64_t>(i),
+                        item.head * p.work.group + (rr - i * p.work.group), c, all, most, total);
+        }
+    }
+}
+
+template <int TYPE, int D> void launch_rows(const Params& p, hipStream_t stream) {
+    const unsigned grid = static_cast<unsigned>(p.groups);
+    if (p.work.tile_rows == 16) {
+        attention_paged_few_kernel<TYPE, D, 1><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+        attention_paged_few_kernel<TYPE, D, 2><<<grid, kThreads, 0, stream>>>(p);
+    }
+    mfr::check_launch("attention_paged_few_kernel");
+}
+
+template <int TYPE> void launch_depth(const Params& p, hipStream_t stream) {
+    if (p.depth == 64) {
+        launch_rows<TYPE, 64>(p, stream);
+    } else {
+        launch_rows<TYPE, 128>(p, stream);
+    }
+}
+
+} // namespace
+
+namespace mfr::paged {
+
+void launch_few(const Params& p, int32_t type, hipStream_t stream) {
+    switch (type) {
+    case MFR_KV_F32: launch_depth<MFR_KV_F32>(p, stream); break;
+    case MFR_KV_BF16: launch_depth<MFR_KV_BF16>(p, stream); break;
+    default: launch_depth<MFR_KV_F8>(p, stream); break;
+    }
+}
+
+void launch_join(const Params& p, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(p.groups),
+                    static_cast<unsigned>(p.work.tile_rows < 8 ? p.work.tile_rows : 8));
+    attention_paged_join_kernel<<<grid, kThreads, 0, stream>>>(p);
+    check_launch("attention_paged_join_kernel");
+}
+
+} // namespace mfr::paged

@@ -23,8 +23,9 @@ def call(entry, desc):
     return getattr(abi.load(), entry)(None, ctypes.byref(desc)), abi.last_error()
 
 
-def test_places():
-    run_cpp("kv_places_test")
+@pytest.mark.parametrize("name", ["kv_places_test", "kv_work_test"])
+def test_places_and_work(name):
+    run_cpp(name)
 
 
 # ---- rotations ------------------------------------------------------------------------------------
