@@ -36,14 +36,15 @@ Launch launch_of(Params p, int32_t type, int shared, int cus) {
     w.shared = shared;
     const int64_t sequences = mfr::kv::sequences_of(w);
     const int64_t rows = static_cast<int64_t>(w.batch.rows) * w.group;
-    // Rows of a sequence, on average: one tile of 16 where they fit.
-    w.tile_rows = rows <= 16 * sequences ? 16 : 32;
-    w.unit = type == MFR_KV_F32 ? 64 : 128;
+    // Rows of a sequence, on average.
+    const bool many = type != MFR_KV_F32 && rows > 32 * sequences;
+    w.tile_rows = many ? mfr::paged::kManyRows : rows <= 16 * sequences ? 16 : 32;
+    w.unit = many || type == MFR_KV_F32 ? 64 : 128;
     const int64_t tokens =
         shared != 0 ? w.batch.prefix : static_cast<int64_t>(mfr::kv::capacity_of(w.batch));
     const int64_t units = std::max<int64_t>(1, (tokens + w.unit - 1) / w.unit);
     const int64_t items = (rows / w.tile_rows + sequences) * w.heads;
-    const int64_t wanted = static_cast<int64_t>(cus) * (w.tile_rows == 16 ? 2 : 1);
+    const int64_t wanted = static_cast<int64_t>(cus) * (w.tile_rows == 32 ? 1 : 2);
     p.groups = static_cast<int32_t>(items >= wanted ? wanted : std::min(wanted, items * units));
     return {p, 2 * static_cast<size_t>(p.groups) * static_cast<size_t>(w.tile_rows)};
 }
@@ -116,7 +117,11 @@ void run(Plan& plan, const mfr_attention_paged_desc& d, uint8_t* workspace, hipS
             continue;
         }
         l->p.parts = parts_at(workspace, l->parts, depth);
-        mfr::paged::launch_few(l->p, d.cache.type, stream);
+        if (l->p.work.tile_rows == mfr::paged::kManyRows) {
+            mfr::paged::launch_tiles(l->p, d.cache.type, stream);
+        } else {
+            mfr::paged::launch_few(l->p, d.cache.type, stream);
+        }
         mfr::paged::launch_join(l->p, stream);
     }
 }

@@ -16,7 +16,7 @@ using kv::Work;
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr float kLog2e = 1.4426950408889634f;
+template <int TYPE> constexpr int kBytes = TYPE == MFR_KV_F32 ? 4 : TYPE == MFR_KV_BF16 ? 2 : 1;
 
 // Unnormalised results of rows: weighted values [row][depth], and the running maximum (of base-2
 // scores) and sum [row][2].
@@ -42,13 +42,134 @@ struct Params {
     Parts prefix;
 };
 
-// The launches (attention_paged_few.hip, attention_paged_tiles.hip): `p` filled but for nothing.
+// The forms: tiles of 16 or 32 rows (attention_paged_few.hip), and of 128 rows, not in fp32
+// (attention_paged_tiles.hip).
+constexpr int32_t kManyRows = 128;
+
 void launch_few(const Params& p, int32_t type, hipStream_t stream);
+void launch_tiles(const Params& p, int32_t type, hipStream_t stream);
 void launch_join(const Params& p, hipStream_t stream);
 
 } // namespace mfr::paged
 
 namespace mfr::paged::dev {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ float exp2_native(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Two floats cut into three bf16 parts each (the leading 8 bits of what is left, so that no part
+// overflows), packed with x in the low half.
+__device__ __forceinline__ void cut_pair(float x, float y, uint32_t& p0, uint32_t& p1,
+                                         uint32_t& p2) {
+    const auto high = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
+    const auto pack = [](float u, float v) {
+        return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
+    };
+    p0 = pack(x, y);
+    x -= high(x);
+    y -= high(y);
+    p1 = pack(x, y);
+    x -= high(x);
+    y -= high(y);
+    p2 = pack(x, y);
+}
+
+// Two e4m3 numbers of a half of w as bf16.
+template <bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
+    return __builtin_bit_cast(uint32_t,
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+
+// The largest of v over the four lanes of one row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float row_max(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    v = fmaxf(a, b);
+    mfr::dev::swap_pair<false>(v, a, b);
+    return fmaxf(a, b);
+}
+
+// Over two lanes, l and l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    return fmaxf(a, b);
+}
+
+__device__ __forceinline__ float sum_halves(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    return a + b;
+}
+
+__device__ __forceinline__ float row_sum(float v) {
+    float a, b;
+    mfr::dev::swap_pair<true>(v, a, b);
+    v = a + b;
+    mfr::dev::swap_pair<false>(v, a, b);
+    return a + b;
+}
+
+// The running softmax of a lane's row.
+struct Running {
+    float top = -INFINITY;
+    float sum = 0.0f; // this lane's share
+    int32_t seen;     // tokens that the row sees
+};
+// The weights of a tile of rows as B operands of bf16 products.
+struct Cut {
+    bf16x8 part[3];
+};
+__device__ __forceinline__ Cut cut_weights(const floatx4& a, const floatx4& b) {
+    uint4 cut[3];
+    cut_pair(a[0], a[1], cut[0].x, cut[1].x, cut[2].x);
+    cut_pair(a[2], a[3], cut[0].y, cut[1].y, cut[2].y);
+    cut_pair(b[0], b[1], cut[0].z, cut[1].z, cut[2].z);
+    cut_pair(b[2], b[3], cut[0].w, cut[1].w, cut[2].w);
+    return {__builtin_bit_cast(bf16x8, cut[0]), __builtin_bit_cast(bf16x8, cut[1]),
+            __builtin_bit_cast(bf16x8, cut[2])};
+}
+
+// sums + the products of one column, the smallest parts first.
+__device__ __forceinline__ floatx4 add_column(floatx4 sums, bf16x8 column, const Cut& w) {
+#pragma unroll
+    for (int i = 2; i >= 0; --i) {
+        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(column, w.part[i], sums, 0, 0, 0);
+    }
+    return sums;
+}
+
+// Pairs of values that some rows do not see, so that infinities and NaN must not meet their weights of
+// 0: zeros in place of these, and ones where they were. Products of the ones with `ones` of the tokens
+// that a row sees count those that it does see. bf16, or fp16 (TYPE MFR_KV_F8 of the tiles).
+template <int TYPE = MFR_KV_BF16> struct Exponent {
+    static constexpr uint32_t kMask = 0x7f80u, kOne = 0x3f80u;
+};
+template <> struct Exponent<MFR_KV_F8> {
+    static constexpr uint32_t kMask = 0x7c00u, kOne = 0x3c00u;
+};
+template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint32_t ones(bool x, bool y) {
+    constexpr uint32_t kOne = Exponent<TYPE>::kOne;
+    return (x ? kOne : 0u) | (y ? kOne << 16 : 0u);
+}
+template <int TYPE> __device__ __forceinline__ uint32_t odd_of(uint32_t w) {
+    constexpr uint32_t kMask = Exponent<TYPE>::kMask;
+    return ((w & kMask) == kMask ? 0xffffu : 0u) |
+           ((w & kMask << 16) == kMask << 16 ? 0xffff0000u : 0u);
+}
+template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint4 odd_ones(const uint4& w) {
+    const uint32_t one = ones<TYPE>(true, true);
+    return make_uint4(odd_of<TYPE>(w.x) & one, odd_of<TYPE>(w.y) & one, odd_of<TYPE>(w.z) & one,
+                      odd_of<TYPE>(w.w) & one);
+}
+template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint4 without_odd(const uint4& w) {
+    return make_uint4(w.x & ~odd_of<TYPE>(w.x), w.y & ~odd_of<TYPE>(w.y), w.z & ~odd_of<TYPE>(w.z),
+                      w.w & ~odd_of<TYPE>(w.w));
+}
 
 // The sum of v over the workgroup, and over the threads before this one.
 struct Scan {
@@ -76,6 +197,54 @@ __device__ inline Scan scan_of(int64_t v, int64_t* waves) {
     }
     return s;
 }
+
+// A number at a uniform address in memory that this launch does not write, through the scalar cache: its
+// wait is not one for the loads of keys and values that are under way.
+__device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+        reinterpret_cast<uintptr_t>(p));
+}
+
+// A uniform address as the scalar part of a load's address, whatever it was made of: the compiler would
+// else fold it into 64 bits a lane.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+    const uint64_t at = reinterpret_cast<uintptr_t>(p);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(at));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32));
+    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Where 16 tokens lie: in bytes from the cache's base, and their place among the scales.
+struct TileAt {
+    int64_t at;
+    int64_t scale_at;
+    bool there; // their page is one of the cache's; another one's place is given otherwise
+};
+
+// The pages of a sequence (or the prefix), and one head of them.
+struct Pages {
+    const int32_t* table;
+    int32_t most; // the first token of the last 16 that hold some
+    int32_t head;
+
+    __device__ __forceinline__ Pages(const Params& p, const Shape& shape, int32_t seq, int32_t head)
+        : table(p.work.shared != 0 ? p.work.batch.prefix_pages
+                                   : p.work.batch.table + seq * p.work.batch.table_rs),
+          most((shape.tokens - 1) & ~15), head(head) {}
+
+    // The number of the page of 16 tokens; ones behind the last are taken as the last.
+    __device__ __forceinline__ int32_t page(const Params& p, int32_t token) const {
+        return uniform_load(table + (min(token, most) >> p.work.batch.page_log2));
+    }
+    __device__ __forceinline__ TileAt at(const Params& p, int32_t token, int32_t page) const {
+        const bool there = mfr::kv::page_checked(p.work.batch, page) >= 0;
+        const int64_t number = there ? page : 0;
+        const int32_t slot = min(token, most) & ((1 << p.cache.page_log2) - 1);
+        return {number * p.cache.page_stride + head * p.cache.head_stride +
+                    static_cast<int64_t>(slot) * p.cache.token_stride,
+                ((number * p.cache.heads + head) << p.cache.page_log2) + slot, there};
+    }
+};
 
 // Where in the work a workgroup starts.
 struct Place {

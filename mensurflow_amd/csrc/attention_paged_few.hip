@@ -18,55 +18,8 @@
 namespace {
 
 using namespace mfr::paged;
+using namespace mfr::paged::dev;
 namespace dev = mfr::paged::dev;
-
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float exp2_native(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// The largest of v over the four lanes of one row (l, l ^ 16, l ^ 32, l ^ 48).
-__device__ __forceinline__ float row_max(float v) {
-    float a, b;
-    mfr::dev::swap_pair<true>(v, a, b);
-    v = fmaxf(a, b);
-    mfr::dev::swap_pair<false>(v, a, b);
-    return fmaxf(a, b);
-}
-
-__device__ __forceinline__ float row_sum(float v) {
-    float a, b;
-    mfr::dev::swap_pair<true>(v, a, b);
-    v = a + b;
-    mfr::dev::swap_pair<false>(v, a, b);
-    return a + b;
-}
-
-// Two floats cut into three bf16 parts each (the leading 8 bits of what is left, so that no part
-// overflows), packed with x in the low half.
-__device__ __forceinline__ void cut_pair(float x, float y, uint32_t& p0, uint32_t& p1,
-                                         uint32_t& p2) {
-    const auto high = [](float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); };
-    const auto pack = [](float u, float v) {
-        return __builtin_amdgcn_perm(__float_as_uint(v), __float_as_uint(u), 0x07060302u);
-    };
-    p0 = pack(x, y);
-    x -= high(x);
-    y -= high(y);
-    p1 = pack(x, y);
-    x -= high(x);
-    y -= high(y);
-    p2 = pack(x, y);
-}
-
-// Two e4m3 numbers of a half of w as bf16.
-template <bool HIGH> __device__ __forceinline__ uint32_t widen(uint32_t w) {
-    return __builtin_bit_cast(uint32_t,
-                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
-}
-
-template <int TYPE> constexpr int kBytes = TYPE == MFR_KV_F32 ? 4 : TYPE == MFR_KV_BF16 ? 2 : 1;
 
 // TILES: tokens of a step, in tiles of 16. PIECES: 16-byte pieces of a token's row that a lane loads.
 // VBYTES: bytes of a token's values that a lane loads.
@@ -96,14 +49,8 @@ struct Lanes {
     int quad;              // lane / 16
     uint32_t key_at;       // bytes from a tile's first token to the lane's first piece of its key
     uint32_t value_at;     // to the lane's columns of its first value
-    uint32_t token_stride;
-};
-
-// The first token of a tile of 16 in memory: in bytes, and its place among the scales.
-struct TileAt {
-    int64_t at;
-    int64_t scale_at;
-    bool there;            // its page is one of the cache's
+    uint32_t key_most;     // the last piece's distance from the first, of a row of fewer than D
+    uint32_t value_most;   // likewise, in fp32
 };
 
 // Of RT tiles of 16 rows: scores or weights (lane: its row, tokens 4 quad + r of each tile), and weighted
@@ -113,47 +60,25 @@ template <int TYPE, int D, int RT> using Sums = floatx4[RT][Form<TYPE, D>::kColu
 template <int TYPE, int D> using Tiles = TileAt[Form<TYPE, D>::kTiles];
 template <int TYPE, int D> using There = bool[Form<TYPE, D>::kTiles];
 
-// The running softmax of a lane's row.
-struct Running {
-    float top = -INFINITY;
-    float sum = 0.0f; // this lane's share
-    int32_t seen;     // tokens that the row sees
-};
 template <int RT> using Rows = Running[RT];
 
-template <int TYPE, int D, int RT> struct Segment {
+// FULL: rows of D.
+template <int TYPE, int D, bool FULL> struct Segment {
     using F = Form<TYPE, D>;
     const Params& p;
-    const Shape& shape;
-    const int32_t seq, head;
     const Lanes& lanes;
 
-    // A tile that no token of the sequence is in is taken as the last one that has some.
-    __device__ __forceinline__ TileAt tile_at(int32_t token) const {
-        const Batch& b = p.work.batch;
-        const int32_t first = min(token, (shape.tokens - 1) & ~15);
-        const int32_t* pages = p.work.shared != 0 ? b.prefix_pages : b.table + seq * b.table_rs;
-        const int32_t page = __builtin_amdgcn_readfirstlane(pages[first >> b.page_log2]);
-        const bool there = mfr::kv::page_checked(b, page) >= 0;
-        const int64_t number = there ? page : 0;
-        const int32_t slot = first & ((1 << b.page_log2) - 1);
-        return {number * p.cache.page_stride + head * p.cache.head_stride +
-                    static_cast<int64_t>(slot) * p.cache.token_stride,
-                ((number * p.cache.heads + head) << b.page_log2) + slot, there};
-    }
-
+    // Addresses are a uniform part and 32 bits of the lane's. Lanes past a row's end load its last piece
+    // again: the queries are zeros there, and those columns of the output are not written.
     __device__ __forceinline__ void load_keys(Keys<TYPE, D>& to, const Tiles<TYPE, D>& at) const {
-        const int row_bytes = p.cache.d * kBytes<TYPE>;
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
-            const uint8_t* base = p.cache.k + at[t].at;
+            const uint8_t* base = uniform(p.cache.k + at[t].at);
 #pragma unroll
             for (int i = 0; i < F::kPieces; ++i) {
-                to.k[t][i] = make_uint4(0, 0, 0, 0);
-                if (64 * i + 16 * lanes.quad < row_bytes) {
-                    to.k[t][i] =
-                        *reinterpret_cast<const uint4*>(base + (lanes.key_at + 64 * i));
-                }
+                const uint32_t from = FULL ? lanes.key_at + 64 * i
+                                           : lanes.key_at + min(64u * i, lanes.key_most);
+                to.k[t][i] = *reinterpret_cast<const uint4*>(base + from);
             }
             if constexpr (TYPE == MFR_KV_F8) {
                 to.scale[t] = *reinterpret_cast<const float4*>(p.cache.k_scales + at[t].scale_at +
@@ -164,21 +89,19 @@ template <int TYPE, int D, int RT> struct Segment {
 
     __device__ __forceinline__ void load_values(Values<TYPE, D>& to,
                                                 const Tiles<TYPE, D>& at) const {
-        const int row_bytes = p.cache.d * kBytes<TYPE>;
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
-            const uint8_t* base = p.cache.v + at[t].at;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint32_t from = lanes.value_at + r * lanes.token_stride;
+                const uint8_t* base =
+                    uniform(p.cache.v + at[t].at + static_cast<int64_t>(r) * p.cache.token_stride);
                 auto& v = to.v[t][r];
                 if constexpr (TYPE == MFR_KV_F32) {
 #pragma unroll
                     for (int i = 0; i < F::kValueWords / 4; ++i) {
-                        uint4 w = make_uint4(0, 0, 0, 0);
-                        if (256 * i + 16 * lanes.row < row_bytes) {
-                            w = *reinterpret_cast<const uint4*>(base + (from + 256 * i));
-                        }
+                        const uint32_t from = FULL ? lanes.value_at + 256 * i
+                                                   : lanes.value_at + min(256u * i, lanes.value_most);
+                        const uint4 w = *reinterpret_cast<const uint4*>(base + from);
                         v[4 * i] = w.x;
                         v[4 * i + 1] = w.y;
                         v[4 * i + 2] = w.z;
@@ -189,10 +112,7 @@ template <int TYPE, int D, int RT> struct Segment {
                     struct alignas(4 * kWords) Piece {
                         uint32_t w[kWords];
                     };
-                    Piece piece{};
-                    if (F::kValueBytes * lanes.row < row_bytes) {
-                        piece = *reinterpret_cast<const Piece*>(base + from);
-                    }
+                    const Piece piece = *reinterpret_cast<const Piece*>(base + lanes.value_at);
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
                         v[i] = piece.w[i];
@@ -216,7 +136,7 @@ template <int D, int RT> struct Queries<MFR_KV_F32, D, RT> {
     float4 q[RT][D / 16];
 };
 
-template <int TYPE, int D, int RT>
+template <int TYPE, int D, int RT, bool FULL>
 __device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Params& p,
                                              const Shape& shape, int32_t head, int32_t tile,
                                              const Lanes& lanes) {
@@ -229,7 +149,7 @@ __device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Par
                          (head * p.work.group + (rr - i * p.work.group)) * p.q.hs;
         const auto quad = [&](int c) {
             float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (rr < rows && c < p.cache.d) {
+            if (rr < rows && (FULL || c < p.cache.d)) {
                 v = mfr::dev::load_loose(q + c);
             }
             return v;
@@ -320,31 +240,39 @@ __device__ __forceinline__ float element(const float4& v, int i) {
 }
 
 // Scores to weights (not yet times the values' scales); the output so far is rescaled where a
-// maximum moved. EDGE: some row does not see some token; `first` is the step's first token.
-template <int TYPE, int D, int RT, bool EDGE>
+// maximum moved. `edge` (uniform): some row does not see some token; `first` is the step's first token.
+template <int TYPE, int D, int RT>
 __device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
                                              Sums<TYPE, D, RT>& acc,
                                              Rows<RT>& run, const Keys<TYPE, D>& keys,
                                              float scale, int32_t first, const Lanes& lanes,
-                                             const There<TYPE, D>& there) {
+                                             bool edge, const There<TYPE, D>& there) {
     using F = Form<TYPE, D>;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[rt][t][r] *= TYPE == MFR_KV_F8 ? element(keys.scale[t], r) * scale : scale;
+            }
+        }
+        if (edge) {
+#pragma unroll
+            for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t token = first + 16 * t + 4 * lanes.quad + r;
+                    s[rt][t][r] = there[t] && token < run[rt].seen ? s[rt][t][r] : -INFINITY;
+                }
+            }
+        }
         float most = -INFINITY;
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float v = s[rt][t][r] * scale;
-                if constexpr (TYPE == MFR_KV_F8) {
-                    v *= element(keys.scale[t], r);
-                }
-                if constexpr (EDGE) {
-                    const int32_t token = first + 16 * t + 4 * lanes.quad + r;
-                    v = there[t] && token < run[rt].seen ? v : -INFINITY;
-                }
-                s[rt][t][r] = v;
-                most = fmaxf(most, v);
+                most = fmaxf(most, s[rt][t][r]);
             }
         }
         most = fmaxf(run[rt].top, row_max(most));
@@ -374,19 +302,15 @@ __device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
     }
 }
 
-// Column j of the values as an A operand of bf16 products; tokens r of tile t whose bit 4 t + r of
-// `keep` is clear are zeros.
+// Column j of the values as an A operand of bf16 products.
 template <int TYPE, int D>
-__device__ __forceinline__ bf16x8 column_of(const Values<TYPE, D>& values, int j,
-                                            uint32_t keep = ~0u) {
+__device__ __forceinline__ bf16x8 column_of(const Values<TYPE, D>& values, int j) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { // tokens 2 (i % 2), 2 (i % 2) + 1 of tile i / 2
         constexpr int kPerWord = TYPE == MFR_KV_BF16 ? 2 : 4;
-        uint32_t a = values.v[i / 2][2 * (i % 2)][j / kPerWord];
-        uint32_t b = values.v[i / 2][2 * (i % 2) + 1][j / kPerWord];
-        a = (keep >> (2 * i) & 1u) != 0 ? a : 0u;
-        b = (keep >> (2 * i + 1) & 1u) != 0 ? b : 0u;
+        const uint32_t a = values.v[i / 2][2 * (i % 2)][j / kPerWord];
+        const uint32_t b = values.v[i / 2][2 * (i % 2) + 1][j / kPerWord];
         if constexpr (TYPE == MFR_KV_BF16) {
             w[i] = __builtin_amdgcn_perm(b, a, j % 2 == 0 ? 0x05040100u : 0x07060302u);
         } else {
@@ -444,29 +368,6 @@ __device__ __forceinline__ void keep_values(Values<TYPE, D>& values, int32_t see
     }
 }
 
-// The weights of a tile of rows as B operands of bf16 products.
-struct Cut {
-    bf16x8 part[3];
-};
-__device__ __forceinline__ Cut cut_weights(const floatx4& a, const floatx4& b) {
-    uint4 cut[3];
-    cut_pair(a[0], a[1], cut[0].x, cut[1].x, cut[2].x);
-    cut_pair(a[2], a[3], cut[0].y, cut[1].y, cut[2].y);
-    cut_pair(b[0], b[1], cut[0].z, cut[1].z, cut[2].z);
-    cut_pair(b[2], b[3], cut[0].w, cut[1].w, cut[2].w);
-    return {__builtin_bit_cast(bf16x8, cut[0]), __builtin_bit_cast(bf16x8, cut[1]),
-            __builtin_bit_cast(bf16x8, cut[2])};
-}
-
-// sums + the products of one column, the smallest parts first.
-__device__ __forceinline__ floatx4 add_column(floatx4 sums, bf16x8 column, const Cut& w) {
-#pragma unroll
-    for (int i = 2; i >= 0; --i) {
-        sums = __builtin_amdgcn_mfma_f32_16x16x32_bf16(column, w.part[i], sums, 0, 0, 0);
-    }
-    return sums;
-}
-
 // acc += V^T P^T.
 template <int TYPE, int D, int RT>
 __device__ __forceinline__ void add_values(Sums<TYPE, D, RT>& acc, const Scores<TYPE, D, RT>& w,
@@ -502,55 +403,64 @@ __device__ __forceinline__ void add_values(Sums<TYPE, D, RT>& acc, const Scores<
     }
 }
 
-// A step that some row does not see whole. Where a token that only some rows see has values that are
-// no numbers, they must not meet the others' weights of 0: each row then adds its own, with the tokens
-// that it does not see cleared, and the other rows' sums stay.
+// Before a step that some row does not see whole: zeros for values of tokens that there are not. Where
+// others are no numbers, rows that see one become NaN in its column, and then there are zeros in their
+// place: they must not meet the weights of 0 of rows that do not see them.
 template <int TYPE, int D, int RT>
-__device__ __forceinline__ void add_edge_values(Sums<TYPE, D, RT>& acc,
-                                                const Scores<TYPE, D, RT>& w,
-                                                Values<TYPE, D>& values, const Rows<RT>& run,
-                                                int32_t tokens, int32_t first, const Lanes& lanes,
-                                                const There<TYPE, D>& there) {
+__device__ __forceinline__ void settle_values(Sums<TYPE, D, RT>& acc, Values<TYPE, D>& values,
+                                              const Rows<RT>& run, int32_t tokens, int32_t first,
+                                              const Lanes& lanes, const There<TYPE, D>& there) {
     using F = Form<TYPE, D>;
     keep_values<TYPE, D>(values, tokens - first, lanes, there);
     if (!__any(odd_values<TYPE, D>(values))) {
-        add_values<TYPE, D, RT>(acc, w, values);
         return;
     }
-#pragma unroll 1
-    for (int row = 0; row < 16; ++row) {
+    const auto sees = [&](int rt, int i) {
+        return there[i / 4] && first + 16 * (i / 4) + 4 * lanes.quad + i % 4 < run[rt].seen;
+    };
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int32_t seen = __builtin_amdgcn_readlane(run[rt].seen, row) - first;
-            uint32_t keep = 0;
+    for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
-            for (int i = 0; i < 4 * F::kTiles; ++i) {
-                keep |= 16 * (i / 4) + 4 * lanes.quad + i % 4 < seen ? 1u << i : 0u;
-            }
+        for (int j = 0; j < F::kColumns; ++j) {
+            floatx4 count{0.0f, 0.0f, 0.0f, 0.0f};
             if constexpr (TYPE == MFR_KV_F32) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                    for (int j = 0; j < F::kColumns; ++j) {
-                        const float v =
-                            __uint_as_float((keep >> r & 1u) != 0 ? values.v[0][r][j] : 0u);
-                        const floatx4 sums = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                            v, w[rt][0][r], acc[rt][j], 0, 0, 0);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            acc[rt][j][e] = lanes.row == row ? sums[e] : acc[rt][j][e];
-                        }
-                    }
+                    const bool odd = (values.v[0][r][j] & 0x7f800000u) == 0x7f800000u;
+                    count = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                        odd ? 1.0f : 0.0f, sees(rt, r) ? 1.0f : 0.0f, count, 0, 0, 0);
                 }
             } else {
-                const Cut cut = cut_weights(w[rt][0], w[rt][1]);
+                const uint4 v = __builtin_bit_cast(uint4, column_of<TYPE, D>(values, j));
+                const uint4 seen =
+                    make_uint4(ones(sees(rt, 0), sees(rt, 1)), ones(sees(rt, 2), sees(rt, 3)),
+                               ones(sees(rt, 4), sees(rt, 5)), ones(sees(rt, 6), sees(rt, 7)));
+                count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd_ones(v)),
+                                                                __builtin_bit_cast(bf16x8, seen),
+                                                                count, 0, 0, 0);
+            }
 #pragma unroll
-                for (int j = 0; j < F::kColumns; ++j) {
-                    const floatx4 sums =
-                        add_column(acc[rt][j], column_of<TYPE, D>(values, j, keep), cut);
+            for (int e = 0; e < 4; ++e) {
+                acc[rt][j][e] = count[e] > 0.0f ? NAN : acc[rt][j][e];
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        acc[rt][j][e] = lanes.row == row ? sums[e] : acc[rt][j][e];
+    for (int t = 0; t < F::kTiles; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+#pragma unroll
+            for (int i = 0; i < F::kValueWords; ++i) {
+                uint32_t& w = values.v[t][r][i];
+                if constexpr (TYPE == MFR_KV_F32) {
+                    w = (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
+                } else if constexpr (TYPE == MFR_KV_BF16) {
+                    w &= ~odd_of<MFR_KV_BF16>(w);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        w = (w >> e & 0x7fu) == 0x7fu ? w & ~(0xffu << e) : w;
                     }
                 }
             }
@@ -560,11 +470,11 @@ __device__ __forceinline__ void add_edge_values(Sums<TYPE, D, RT>& acc,
 
 // Weights times the scales of the values, in 8 bits; 0 for tokens that the row does not see, whatever
 // their scales are.
-template <int TYPE, int D, int RT, bool EDGE>
+template <int TYPE, int D, int RT>
 __device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w,
                                               const Values<TYPE, D>& values,
                                               const Rows<RT>& run, int32_t first,
-                                              const Lanes& lanes,
+                                              const Lanes& lanes, bool edge,
                                               const There<TYPE, D>& there) {
     if constexpr (TYPE == MFR_KV_F8) {
 #pragma unroll
@@ -573,9 +483,20 @@ __device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w,
             for (int t = 0; t < Form<TYPE, D>::kTiles; ++t) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float v = w[rt][t][r] * element(values.scale[t], r);
-                    const int32_t token = first + 16 * t + 4 * lanes.quad + r;
-                    w[rt][t][r] = !EDGE || (there[t] && token < run[rt].seen) ? v : 0.0f;
+                    w[rt][t][r] *= element(values.scale[t], r);
+                }
+            }
+        }
+        if (edge) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int t = 0; t < Form<TYPE, D>::kTiles; ++t) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int32_t token = first + 16 * t + 4 * lanes.quad + r;
+                        w[rt][t][r] = there[t] && token < run[rt].seen ? w[rt][t][r] : 0.0f;
+                    }
                 }
             }
         }
@@ -588,7 +509,7 @@ template <int TYPE, int D> __device__ __forceinline__ int column_at(int quad, in
                               : Form<TYPE, D>::kColumns * (4 * quad + r) + 4 * q;
 }
 
-template <int TYPE, int D, int RT>
+template <int TYPE, int D, int RT, bool FULL>
 __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few_kernel(Params p) {
     using F = Form<TYPE, D>;
     constexpr int kPitch = D + 4;
@@ -606,10 +527,14 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
     Lanes lanes;
     lanes.row = lane % 16;
     lanes.quad = lane / 16;
-    lanes.token_stride = p.cache.token_stride;
-    lanes.key_at = lanes.row * p.cache.token_stride + 16 * lanes.quad;
-    lanes.value_at = 4 * lanes.quad * p.cache.token_stride +
-                     (TYPE == MFR_KV_F32 ? 16 : F::kValueBytes) * lanes.row;
+    const int row_bytes = p.cache.d * kBytes<TYPE>;
+    const int key_piece = min(16 * lanes.quad, row_bytes - 16);
+    constexpr int kPiece = TYPE == MFR_KV_F32 ? 16 : F::kValueBytes;
+    const int value_piece = min(kPiece * lanes.row, row_bytes - kPiece);
+    lanes.key_at = lanes.row * p.cache.token_stride + key_piece;
+    lanes.value_at = 4 * lanes.quad * p.cache.token_stride + value_piece;
+    lanes.key_most = row_bytes - 16 - key_piece;
+    lanes.value_most = row_bytes - kPiece - value_piece;
     const int64_t begin = index * place.chunk;
     const int64_t end = begin + place.chunk < place.total ? begin + place.chunk : place.total;
     int32_t seq = place.seq;
@@ -637,7 +562,7 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
         const int32_t some_see = mfr::kv::seen_by(
             shape, (min(row0 + 16 * RT, rows) - 1) / p.work.group, p.causal != 0);
         Queries<TYPE, D, RT> queries;
-        load_queries<TYPE, D, RT>(queries, p, shape, item.head, item.tile, lanes);
+        load_queries<TYPE, D, RT, FULL>(queries, p, shape, item.head, item.tile, lanes);
         Sums<TYPE, D, RT> acc;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -646,7 +571,8 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
                 acc[rt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
-        const Segment<TYPE, D, RT> segment{p, shape, seq, item.head, lanes};
+        const Segment<TYPE, D, FULL> segment{p, lanes};
+        const Pages pages(p, shape, seq, item.head);
         // This wavefront's tokens: a step of every unit.
         constexpr int kUnit = kWaves * F::kKeys;
         int32_t first = item.first * kUnit + wave * F::kKeys;
@@ -655,54 +581,50 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
             Tiles<TYPE, D> tiles;
             Keys<TYPE, D> keys;
             Values<TYPE, D> values;
-            const auto tiles_of = [&](int32_t token, Tiles<TYPE, D>& to) {
+            // Page numbers are read a step before they are used.
+            int32_t numbers[F::kTiles];
+            const auto numbers_of = [&](int32_t token) {
 #pragma unroll
                 for (int t = 0; t < F::kTiles; ++t) {
-                    to[t] = segment.tile_at(token + 16 * t);
+                    numbers[t] = pages.page(p, token + 16 * t);
                 }
             };
-            // Whether a step is one that every row sees whole, in pages that are there.
-            const auto plain = [&](int32_t token) {
-                bool there = token + F::kKeys <= all_see;
+            const auto tiles_of = [&](int32_t token) {
 #pragma unroll
                 for (int t = 0; t < F::kTiles; ++t) {
-                    there = there && tiles[t].there;
+                    tiles[t] = pages.at(p, token + 16 * t, numbers[t]);
                 }
-                return there;
             };
-            tiles_of(first, tiles);
+            numbers_of(first);
+            tiles_of(first);
+            numbers_of(first + kUnit);
             segment.load_keys(keys, tiles);
             segment.load_values(values, tiles);
-            while (first < last && plain(first)) {
-                // The next step's keys are under way from the scores on, its values from the end;
-                // behind the last step the same ones are loaded again.
-                tiles_of(first + kUnit < last ? first + kUnit : first, tiles);
-                Scores<TYPE, D, RT> s;
-                scores_of<TYPE, D, RT>(s, keys, queries);
-                softmax_step<TYPE, D, RT, false>(s, acc, run, keys, p.scale, first, lanes, {});
-                segment.load_keys(keys, tiles);
-                scale_weights<TYPE, D, RT, false>(s, values, run, first, lanes, {});
-                add_values<TYPE, D, RT>(acc, s, values);
-                segment.load_values(values, tiles);
-                first += kUnit;
-            }
-            while (first < last) {
+            // The next step's keys are under way from the scores on, its values from the end; behind the
+            // last step there is something to load all the same. One code for steps that some row does not
+            // see whole and the others: a second one, run once at an item's end, takes longer to come into
+            // the instruction cache than to run.
+#pragma unroll 1
+            for (; first < last; first += kUnit) {
                 There<TYPE, D> there;
+                bool edge = first + F::kKeys > all_see;
 #pragma unroll
                 for (int t = 0; t < F::kTiles; ++t) {
                     there[t] = tiles[t].there;
+                    edge = edge || !there[t];
                 }
+                tiles_of(first + kUnit);
+                numbers_of(first + 2 * kUnit);
                 Scores<TYPE, D, RT> s;
                 scores_of<TYPE, D, RT>(s, keys, queries);
-                softmax_step<TYPE, D, RT, true>(s, acc, run, keys, p.scale, first, lanes, there);
-                scale_weights<TYPE, D, RT, true>(s, values, run, first, lanes, there);
-                add_edge_values<TYPE, D, RT>(acc, s, values, run, shape.tokens, first, lanes, there);
-                first += kUnit;
-                if (first < last) {
-                    tiles_of(first, tiles);
-                    segment.load_keys(keys, tiles);
-                    segment.load_values(values, tiles);
+                softmax_step<TYPE, D, RT>(s, acc, run, keys, p.scale, first, lanes, edge, there);
+                segment.load_keys(keys, tiles);
+                scale_weights<TYPE, D, RT>(s, values, run, first, lanes, edge, there);
+                if (edge) {
+                    settle_values<TYPE, D, RT>(acc, values, run, shape.tokens, first, lanes, there);
                 }
+                add_values<TYPE, D, RT>(acc, s, values);
+                segment.load_values(values, tiles);
             }
         }
         // The wavefronts' parts, joined: 16 threads a row, 4 columns each and 64 further on.
@@ -771,11 +693,13 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
 }
 
 // Joins the parts of the items that were cut: workgroup x looks at the end of chunk x, and takes the
-// item that began in it and goes on, rows y, y + gridDim.y, ... of it. 32 lanes hold a part's row, 8 parts
-// at a time, so a long list of parts has its loads in flight together.
+// item that began in it and goes on, rows 8 y .. 8 y + 7 of it. 32 lanes hold a part's row; they take a row's
+// parts in order, or, where an item has few rows, share them (a part in `split`) and join through LDS.
+constexpr int kJoinRows = 8;
+
 __global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p) {
-    __shared__ float4 values[8][32];
-    __shared__ float tops[8], sums[8];
+    __shared__ float4 values[kJoinRows][32];
+    __shared__ float2 stats[kJoinRows];
     const int64_t index = blockIdx.x;
     const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t chunk) {
         // The last unit of a chunk that another one follows.
@@ -791,66 +715,97 @@ __global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p
     if (item.begin < index * place.chunk || end <= edge) {
         return;
     }
+    const int32_t rows = shape.span.count * p.work.group;
+    const int32_t row0 = item.tile * p.work.tile_rows + kJoinRows * static_cast<int32_t>(blockIdx.y);
+    const int32_t here = min(kJoinRows, min((item.tile + 1) * p.work.tile_rows, rows) - row0);
+    if (here <= 0) {
+        return;
+    }
     const int64_t last = (end - 1) / place.chunk; // the chunk of its last unit
     const int count = static_cast<int>(last - index) + 1;
+    const int split = here <= 1 ? 8 : here <= 2 ? 4 : here <= 4 ? 2 : 1;
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+    const int32_t r = group / split;
     const int c = 4 * lane;
-    const int32_t rows = shape.span.count * p.work.group;
-    const int32_t row0 = item.tile * p.work.tile_rows;
-    const int32_t here = min(p.work.tile_rows, rows - row0);
-    for (int32_t r = blockIdx.y; r < here; r += gridDim.y) {
-        float top = -INFINITY, sum = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-        for (int i = group; i < count; i += 8) {
-            const int64_t part =
-                mfr::kv::part_of(index + i, place.chunk, item.begin) * p.work.tile_rows + r;
-            const float2 stats = *reinterpret_cast<const float2*>(p.parts.stats + 2 * part);
-            float4 other = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (c < p.depth) {
-                other = *reinterpret_cast<const float4*>(p.parts.values + part * p.depth + c);
+    const int64_t first = mfr::kv::part_of(index, place.chunk, item.begin); // the others' are 2 apart
+    const int64_t row = row0 - item.tile * p.work.tile_rows + r;
+    float top = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < here) {
+        constexpr int kAtOnce = 8;
+        for (int i0 = group % split; i0 < count; i0 += kAtOnce * split) {
+            float2 stat[kAtOnce];
+            float4 value[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int i = i0 + k * split;
+                stat[k] = make_float2(-INFINITY, 0.0f);
+                value[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (i < count) {
+                    const int64_t part = (i == 0 ? first : 2 * (index + i)) * p.work.tile_rows + row;
+                    stat[k] = *reinterpret_cast<const float2*>(p.parts.stats + 2 * part);
+                    if (c < p.depth) {
+                        value[k] = *reinterpret_cast<const float4*>(p.parts.values + part * p.depth + c);
+                    }
+                }
             }
-            const float most = fmaxf(top, stats.x);
-            const float a = dev::part_weight(top, most), b = dev::part_weight(stats.x, most);
-            sum = fmaf(b, stats.y, a * sum);
-            v = dev::add_scaled(dev::scaled(v, a), other, b);
+            float most = top;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                most = fmaxf(most, stat[k].x);
+            }
+            const float a = dev::part_weight(top, most);
+            sum *= a;
+            v = dev::scaled(v, a);
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const float b = dev::part_weight(stat[k].x, most);
+                sum = fmaf(b, stat[k].y, sum);
+                v = dev::add_scaled(v, value[k], b);
+            }
             top = most;
         }
-        __syncthreads(); // the row before has been read
+    }
+    if (split > 1) { // the whole workgroup
         values[group][lane] = v;
         if (lane == 0) {
-            tops[group] = top;
-            sums[group] = sum;
+            stats[group] = make_float2(top, sum);
         }
         __syncthreads();
-        if (group == 0 && c < p.depth) {
-            float most = tops[0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) {
-                most = fmaxf(most, tops[i]);
-            }
-            float total = 0.0f;
-            float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float w = dev::part_weight(tops[i], most);
-                total = fmaf(w, sums[i], total);
-                all = dev::add_scaled(all, values[i][lane], w);
-            }
-            const int32_t rr = row0 + r;
-            const int32_t i = rr / p.work.group;
-            dev::finish(p, shape.span.first + static_cast<int64_t>(i),
-                        item.head * p.work.group + (rr - i * p.work.group), c, all, most, total);
+        if (group % split != 0) {
+            return;
         }
+#pragma unroll 1
+        for (int k = 1; k < split; ++k) {
+            const float2 other = stats[group + k];
+            const float most = fmaxf(top, other.x);
+            const float a = dev::part_weight(top, most), b = dev::part_weight(other.x, most);
+            sum = fmaf(b, other.y, a * sum);
+            v = dev::add_scaled(dev::scaled(v, a), values[group + k][lane], b);
+            top = most;
+        }
+    }
+    if (r < here && c < p.depth) {
+        const int32_t i = (row0 + r) / p.work.group;
+        dev::finish(p, shape.span.first + static_cast<int64_t>(i),
+                    item.head * p.work.group + (row0 + r - i * p.work.group), c, v, top, sum);
     }
 }
 
 template <int TYPE, int D> void launch_rows(const Params& p, hipStream_t stream) {
     const unsigned grid = static_cast<unsigned>(p.groups);
     if (p.work.tile_rows == 16) {
-        attention_paged_few_kernel<TYPE, D, 1><<<grid, kThreads, 0, stream>>>(p);
+        if (p.cache.d == D) {
+            attention_paged_few_kernel<TYPE, D, 1, true><<<grid, kThreads, 0, stream>>>(p);
+        } else {
+            attention_paged_few_kernel<TYPE, D, 1, false><<<grid, kThreads, 0, stream>>>(p);
+        }
     } else {
-        attention_paged_few_kernel<TYPE, D, 2><<<grid, kThreads, 0, stream>>>(p);
+        if (p.cache.d == D) {
+            attention_paged_few_kernel<TYPE, D, 2, true><<<grid, kThreads, 0, stream>>>(p);
+        } else {
+            attention_paged_few_kernel<TYPE, D, 2, false><<<grid, kThreads, 0, stream>>>(p);
+        }
     }
     mfr::check_launch("attention_paged_few_kernel");
 }
@@ -877,7 +832,7 @@ void launch_few(const Params& p, int32_t type, hipStream_t stream) {
 
 void launch_join(const Params& p, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(p.groups),
-                    static_cast<unsigned>(p.work.tile_rows < 8 ? p.work.tile_rows : 8));
+                    static_cast<unsigned>((p.work.tile_rows + kJoinRows - 1) / kJoinRows));
     attention_paged_join_kernel<<<grid, kThreads, 0, stream>>>(p);
     check_launch("attention_paged_join_kernel");
 }
