@@ -114,6 +114,13 @@ __device__ __forceinline__ float row_sum(float v) {
     return a + b;
 }
 
+// A workgroup barrier that waits for this wavefront's LDS accesses only: loads from memory stay under way.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // The running softmax of a lane's row.
 struct Running {
     float top = -INFINITY;
@@ -143,32 +150,28 @@ __device__ __forceinline__ floatx4 add_column(floatx4 sums, bf16x8 column, const
     return sums;
 }
 
-// Pairs of values that some rows do not see, so that infinities and NaN must not meet their weights of
-// 0: zeros in place of these, and ones where they were. Products of the ones with `ones` of the tokens
-// that a row sees count those that it does see. bf16, or fp16 (TYPE MFR_KV_F8 of the tiles).
-template <int TYPE = MFR_KV_BF16> struct Exponent {
-    static constexpr uint32_t kMask = 0x7f80u, kOne = 0x3f80u;
-};
-template <> struct Exponent<MFR_KV_F8> {
-    static constexpr uint32_t kMask = 0x7c00u, kOne = 0x3c00u;
-};
-template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint32_t ones(bool x, bool y) {
-    constexpr uint32_t kOne = Exponent<TYPE>::kOne;
-    return (x ? kOne : 0u) | (y ? kOne << 16 : 0u);
+// Whether any of the numbers of a cache in a word is an infinity or NaN, and the word with zeros for
+// those: values that some rows do not see must not meet their weights of 0. (Rows that see one are made
+// NaN through their sum.)
+template <int TYPE> __device__ __forceinline__ bool is_odd(uint32_t w) {
+    if constexpr (TYPE == MFR_KV_F32) {
+        return (w & 0x7f800000u) == 0x7f800000u;
+    } else if constexpr (TYPE == MFR_KV_BF16) {
+        return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+    } else { // a byte of 0x7f or 0xff: 0x01 is carried into its top bit
+        return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
+    }
 }
-template <int TYPE> __device__ __forceinline__ uint32_t odd_of(uint32_t w) {
-    constexpr uint32_t kMask = Exponent<TYPE>::kMask;
-    return ((w & kMask) == kMask ? 0xffffu : 0u) |
-           ((w & kMask << 16) == kMask << 16 ? 0xffff0000u : 0u);
-}
-template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint4 odd_ones(const uint4& w) {
-    const uint32_t one = ones<TYPE>(true, true);
-    return make_uint4(odd_of<TYPE>(w.x) & one, odd_of<TYPE>(w.y) & one, odd_of<TYPE>(w.z) & one,
-                      odd_of<TYPE>(w.w) & one);
-}
-template <int TYPE = MFR_KV_BF16> __device__ __forceinline__ uint4 without_odd(const uint4& w) {
-    return make_uint4(w.x & ~odd_of<TYPE>(w.x), w.y & ~odd_of<TYPE>(w.y), w.z & ~odd_of<TYPE>(w.z),
-                      w.w & ~odd_of<TYPE>(w.w));
+template <int TYPE> __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
+    if constexpr (TYPE == MFR_KV_F32) {
+        return is_odd<TYPE>(w) ? 0u : w;
+    } else if constexpr (TYPE == MFR_KV_BF16) {
+        return ((w & 0x7f80u) == 0x7f80u ? 0u : w & 0xffffu) |
+               ((w & 0x7f800000u) == 0x7f800000u ? 0u : w & 0xffff0000u);
+    } else {
+        const uint32_t tops = ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        return w & ~((tops >> 7) * 0xffu);
+    }
 }
 
 // The sum of v over the workgroup, and over the threads before this one.
@@ -205,16 +208,23 @@ __device__ __forceinline__ int32_t uniform_load(const int32_t* p) {
         reinterpret_cast<uintptr_t>(p));
 }
 
-// A uniform address as the scalar part of a load's address, whatever it was made of: the compiler would
-// else fold it into 64 bits a lane.
-__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
-    const uint64_t at = reinterpret_cast<uintptr_t>(p);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(at));
-    const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<int>(at >> 32));
-    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi) << 32 | lo);
+// A lane's address in memory (and not anywhere: a flat load counts as one from LDS too, and every wait for
+// LDS would wait for it), which the compiler takes as it is: a load's uniform offset is added to it in one
+// instruction then, instead of all its terms one by one.
+typedef const __attribute__((address_space(1))) uint8_t* GlobalBytes;
+__device__ __forceinline__ GlobalBytes lane_address(const void* p, uint32_t lane_offset) {
+    uint64_t at = reinterpret_cast<uintptr_t>(p) + lane_offset;
+    asm volatile("" : "+v"(at));
+    return reinterpret_cast<GlobalBytes>(at);
+}
+// T from `offset` bytes behind it, aligned to its size.
+template <typename T> __device__ __forceinline__ T load_at(GlobalBytes base, int64_t offset) {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T) / 4)));
+    const Words w = *reinterpret_cast<const __attribute__((address_space(1))) Words*>(base + offset);
+    return __builtin_bit_cast(T, w);
 }
 
-// Where 16 tokens lie: in bytes from the cache's base, and their place among the scales.
+// Where 16 tokens lie: in bytes from a head's first row, and from the first scale.
 struct TileAt {
     int64_t at;
     int64_t scale_at;
@@ -237,12 +247,12 @@ struct Pages {
         return uniform_load(table + (min(token, most) >> p.work.batch.page_log2));
     }
     __device__ __forceinline__ TileAt at(const Params& p, int32_t token, int32_t page) const {
-        const bool there = mfr::kv::page_checked(p.work.batch, page) >= 0;
+        // (kv::page_checked without a branch.)
+        const bool there = static_cast<uint32_t>(page) < static_cast<uint32_t>(p.work.batch.pages);
         const int64_t number = there ? page : 0;
         const int32_t slot = min(token, most) & ((1 << p.cache.page_log2) - 1);
-        return {number * p.cache.page_stride + head * p.cache.head_stride +
-                    static_cast<int64_t>(slot) * p.cache.token_stride,
-                ((number * p.cache.heads + head) << p.cache.page_log2) + slot, there};
+        return {number * p.cache.page_stride + static_cast<int64_t>(slot) * p.cache.token_stride,
+                4 * (((number * p.cache.heads + head) << p.cache.page_log2) + slot), there};
     }
 };
 

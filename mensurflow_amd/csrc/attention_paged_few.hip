@@ -67,22 +67,31 @@ template <int TYPE, int D, bool FULL> struct Segment {
     using F = Form<TYPE, D>;
     const Params& p;
     const Lanes& lanes;
+    // From a tile's first token to the lane's first piece of its key, to the lane's columns of its first
+    // value, and to its four scales.
+    GlobalBytes keys, values, key_scales, value_scales;
 
-    // Addresses are a uniform part and 32 bits of the lane's. Lanes past a row's end load its last piece
-    // again: the queries are zeros there, and those columns of the output are not written.
+    __device__ __forceinline__ Segment(const Params& params, const Lanes& l, int32_t head)
+        : p(params), lanes(l) {
+        const int64_t at = head * p.cache.head_stride;
+        keys = lane_address(p.cache.k + at, lanes.key_at);
+        values = lane_address(p.cache.v + at, lanes.value_at);
+        key_scales = lane_address(p.cache.k_scales, 16 * lanes.quad);
+        value_scales = lane_address(p.cache.v_scales, 16 * lanes.quad);
+    }
+
+    // Lanes past a row's end load its last piece again: the queries are zeros there, and those columns of
+    // the output are not written.
     __device__ __forceinline__ void load_keys(Keys<TYPE, D>& to, const Tiles<TYPE, D>& at) const {
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
-            const uint8_t* base = uniform(p.cache.k + at[t].at);
 #pragma unroll
             for (int i = 0; i < F::kPieces; ++i) {
-                const uint32_t from = FULL ? lanes.key_at + 64 * i
-                                           : lanes.key_at + min(64u * i, lanes.key_most);
-                to.k[t][i] = *reinterpret_cast<const uint4*>(base + from);
+                to.k[t][i] = load_at<uint4>(keys + at[t].at,
+                                            FULL ? 64 * i : min(64u * i, lanes.key_most));
             }
             if constexpr (TYPE == MFR_KV_F8) {
-                to.scale[t] = *reinterpret_cast<const float4*>(p.cache.k_scales + at[t].scale_at +
-                                                               4 * lanes.quad);
+                to.scale[t] = load_at<float4>(key_scales, at[t].scale_at);
             }
         }
     }
@@ -93,35 +102,35 @@ template <int TYPE, int D, bool FULL> struct Segment {
         for (int t = 0; t < F::kTiles; ++t) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint8_t* base =
-                    uniform(p.cache.v + at[t].at + static_cast<int64_t>(r) * p.cache.token_stride);
+                const GlobalBytes base =
+                    values + (at[t].at + static_cast<int64_t>(r) * p.cache.token_stride);
                 auto& v = to.v[t][r];
                 if constexpr (TYPE == MFR_KV_F32) {
 #pragma unroll
                     for (int i = 0; i < F::kValueWords / 4; ++i) {
-                        const uint32_t from = FULL ? lanes.value_at + 256 * i
-                                                   : lanes.value_at + min(256u * i, lanes.value_most);
-                        const uint4 w = *reinterpret_cast<const uint4*>(base + from);
+                        const uint4 w =
+                            load_at<uint4>(base, FULL ? 256 * i : min(256u * i, lanes.value_most));
                         v[4 * i] = w.x;
                         v[4 * i + 1] = w.y;
                         v[4 * i + 2] = w.z;
                         v[4 * i + 3] = w.w;
                     }
+                } else if constexpr (F::kValueWords == 4) {
+                    const uint4 w = load_at<uint4>(base, 0);
+                    v[0] = w.x;
+                    v[1] = w.y;
+                    v[2] = w.z;
+                    v[3] = w.w;
+                } else if constexpr (F::kValueWords == 2) {
+                    const uint2 w = load_at<uint2>(base, 0);
+                    v[0] = w.x;
+                    v[1] = w.y;
                 } else {
-                    constexpr int kWords = F::kValueWords;
-                    struct alignas(4 * kWords) Piece {
-                        uint32_t w[kWords];
-                    };
-                    const Piece piece = *reinterpret_cast<const Piece*>(base + lanes.value_at);
-#pragma unroll
-                    for (int i = 0; i < kWords; ++i) {
-                        v[i] = piece.w[i];
-                    }
+                    v[0] = load_at<uint32_t>(base, 0);
                 }
             }
             if constexpr (TYPE == MFR_KV_F8) {
-                to.scale[t] = *reinterpret_cast<const float4*>(p.cache.v_scales + at[t].scale_at +
-                                                               4 * lanes.quad);
+                to.scale[t] = load_at<float4>(value_scales, at[t].scale_at);
             }
         }
     }
@@ -238,6 +247,9 @@ __device__ __forceinline__ void scores_of(Scores<TYPE, D, RT>& s,
 __device__ __forceinline__ float element(const float4& v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
+__device__ __forceinline__ float& element(float4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
 
 // Scores to weights (not yet times the values' scales); the output so far is rescaled where a
 // maximum moved. `edge` (uniform): some row does not see some token; `first` is the step's first token.
@@ -275,12 +287,14 @@ __device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
                 most = fmaxf(most, s[rt][t][r]);
             }
         }
-        most = fmaxf(run[rt].top, row_max(most));
-        // Nothing seen yet: any finite reference gives weights of 0.
-        const float reference = most == -INFINITY ? 0.0f : most;
-        if (__any(most != run[rt].top)) {
-            const float shrink = exp2_native(run[rt].top - reference);
-            run[rt].top = most;
+        // Weights are taken against a reference that follows the maximum in steps: it moves, and the output
+        // so far with it, where the maximum has grown by more than 2^8, so that few steps do.
+        most = row_max(most);
+        if (__any(most > run[rt].top + 8.0f)) {
+            const float top = fmaxf(run[rt].top, most);
+            float shrink = run[rt].top == -INFINITY ? 0.0f : exp2_native(run[rt].top - top);
+            asm volatile("" : "+v"(shrink)); // no products with it ahead of the branch
+            run[rt].top = top;
             run[rt].sum *= shrink;
 #pragma unroll
             for (int j = 0; j < F::kColumns; ++j) {
@@ -290,6 +304,8 @@ __device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
                 }
             }
         }
+        // Nothing seen yet: any finite reference gives weights of 0.
+        const float reference = run[rt].top == -INFINITY ? 0.0f : run[rt].top;
 #pragma unroll
         for (int t = 0; t < F::kTiles; ++t) {
 #pragma unroll
@@ -320,52 +336,6 @@ __device__ __forceinline__ bf16x8 column_of(const Values<TYPE, D>& values, int j
         }
     }
     return __builtin_bit_cast(bf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-}
-
-// Whether a value that the lane loaded is an infinity or NaN.
-template <int TYPE, int D> __device__ __forceinline__ bool odd_values(const Values<TYPE, D>& values) {
-    using F = Form<TYPE, D>;
-    bool odd = false;
-#pragma unroll
-    for (int t = 0; t < F::kTiles; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-#pragma unroll
-            for (int i = 0; i < F::kValueWords; ++i) {
-                const uint32_t w = values.v[t][r][i];
-                if constexpr (TYPE == MFR_KV_F32) {
-                    odd |= (w & 0x7f800000u) == 0x7f800000u;
-                } else if constexpr (TYPE == MFR_KV_BF16) {
-                    odd |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        odd |= ((w >> (8 * e)) & 0x7fu) == 0x7fu;
-                    }
-                }
-            }
-        }
-    }
-    return odd;
-}
-
-// Leaves the values of tokens before `seen` (from the step's first), zeros for the others.
-template <int TYPE, int D>
-__device__ __forceinline__ void keep_values(Values<TYPE, D>& values, int32_t seen,
-                                            const Lanes& lanes,
-                                            const There<TYPE, D>& there) {
-    using F = Form<TYPE, D>;
-#pragma unroll
-    for (int t = 0; t < F::kTiles; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const bool keep = there[t] && 16 * t + 4 * lanes.quad + r < seen;
-#pragma unroll
-            for (int i = 0; i < F::kValueWords; ++i) {
-                values.v[t][r][i] = keep ? values.v[t][r][i] : 0u;
-            }
-        }
-    }
 }
 
 // acc += V^T P^T.
@@ -403,79 +373,45 @@ __device__ __forceinline__ void add_values(Sums<TYPE, D, RT>& acc, const Scores<
     }
 }
 
-// Before a step that some row does not see whole: zeros for values of tokens that there are not. Where
-// others are no numbers, rows that see one become NaN in its column, and then there are zeros in their
-// place: they must not meet the weights of 0 of rows that do not see them.
+// Before a step that some row does not see whole: zeros for values of tokens that there are not, and for
+// ones that are no numbers, which must not meet the weights of 0 of rows that do not see them. Rows that
+// do see one become NaN through their sum.
 template <int TYPE, int D, int RT>
-__device__ __forceinline__ void settle_values(Sums<TYPE, D, RT>& acc, Values<TYPE, D>& values,
-                                              const Rows<RT>& run, int32_t tokens, int32_t first,
-                                              const Lanes& lanes, const There<TYPE, D>& there) {
+__device__ __forceinline__ void settle_values(Values<TYPE, D>& values, Rows<RT>& run, int32_t tokens,
+                                              int32_t first, const Lanes& lanes,
+                                              const There<TYPE, D>& there) {
     using F = Form<TYPE, D>;
-    keep_values<TYPE, D>(values, tokens - first, lanes, there);
-    if (!__any(odd_values<TYPE, D>(values))) {
-        return;
-    }
-    const auto sees = [&](int rt, int i) {
-        return there[i / 4] && first + 16 * (i / 4) + 4 * lanes.quad + i % 4 < run[rt].seen;
-    };
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int j = 0; j < F::kColumns; ++j) {
-            floatx4 count{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (TYPE == MFR_KV_F32) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool odd = (values.v[0][r][j] & 0x7f800000u) == 0x7f800000u;
-                    count = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                        odd ? 1.0f : 0.0f, sees(rt, r) ? 1.0f : 0.0f, count, 0, 0, 0);
-                }
-            } else {
-                const uint4 v = __builtin_bit_cast(uint4, column_of<TYPE, D>(values, j));
-                const uint4 seen =
-                    make_uint4(ones(sees(rt, 0), sees(rt, 1)), ones(sees(rt, 2), sees(rt, 3)),
-                               ones(sees(rt, 4), sees(rt, 5)), ones(sees(rt, 6), sees(rt, 7)));
-                count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd_ones(v)),
-                                                                __builtin_bit_cast(bf16x8, seen),
-                                                                count, 0, 0, 0);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                acc[rt][j][e] = count[e] > 0.0f ? NAN : acc[rt][j][e];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
 #pragma unroll
     for (int t = 0; t < F::kTiles; ++t) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
+            const int32_t token = first + 16 * t + 4 * lanes.quad + r;
+            const bool keep = there[t] && token < tokens;
+            bool odd = false;
 #pragma unroll
             for (int i = 0; i < F::kValueWords; ++i) {
-                uint32_t& w = values.v[t][r][i];
-                if constexpr (TYPE == MFR_KV_F32) {
-                    w = (w & 0x7f800000u) == 0x7f800000u ? 0u : w;
-                } else if constexpr (TYPE == MFR_KV_BF16) {
-                    w &= ~odd_of<MFR_KV_BF16>(w);
-                } else {
+                const uint32_t w = keep ? values.v[t][r][i] : 0u;
+                odd |= is_odd<TYPE>(w);
+                values.v[t][r][i] = without_odd<TYPE>(w);
+            }
+            if constexpr (TYPE == MFR_KV_F8) { // (values under a scale that is none are none)
+                float& scale = element(values.scale[t], r);
+                odd |= keep && !(fabsf(scale) < INFINITY);
+                scale = fabsf(scale) < INFINITY ? scale : 0.0f;
+            }
+            // The token's columns are in the 16 lanes of the quad, and so are the rows.
+            const uint64_t lanes_odd = __ballot(odd) >> (16 * lanes.quad) & 0xffffu;
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8) {
-                        w = (w >> e & 0x7fu) == 0x7fu ? w & ~(0xffu << e) : w;
-                    }
-                }
+            for (int rt = 0; rt < RT; ++rt) {
+                run[rt].sum = lanes_odd != 0 && token < run[rt].seen ? NAN : run[rt].sum;
             }
         }
     }
 }
 
-// Weights times the scales of the values, in 8 bits; 0 for tokens that the row does not see, whatever
-// their scales are.
+// Weights times the scales of the values, in 8 bits.
 template <int TYPE, int D, int RT>
-__device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w,
-                                              const Values<TYPE, D>& values,
-                                              const Rows<RT>& run, int32_t first,
-                                              const Lanes& lanes, bool edge,
-                                              const There<TYPE, D>& there) {
+__device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w, Values<TYPE, D>& values) {
     if constexpr (TYPE == MFR_KV_F8) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -484,19 +420,6 @@ __device__ __forceinline__ void scale_weights(Scores<TYPE, D, RT>& w,
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     w[rt][t][r] *= element(values.scale[t], r);
-                }
-            }
-        }
-        if (edge) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                for (int t = 0; t < Form<TYPE, D>::kTiles; ++t) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int32_t token = first + 16 * t + 4 * lanes.quad + r;
-                        w[rt][t][r] = there[t] && token < run[rt].seen ? w[rt][t][r] : 0.0f;
-                    }
                 }
             }
         }
@@ -571,7 +494,7 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
                 acc[rt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
-        const Segment<TYPE, D, FULL> segment{p, lanes};
+        const Segment<TYPE, D, FULL> segment(p, lanes, item.head);
         const Pages pages(p, shape, seq, item.head);
         // This wavefront's tokens: a step of every unit.
         constexpr int kUnit = kWaves * F::kKeys;
@@ -619,10 +542,10 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
                 scores_of<TYPE, D, RT>(s, keys, queries);
                 softmax_step<TYPE, D, RT>(s, acc, run, keys, p.scale, first, lanes, edge, there);
                 segment.load_keys(keys, tiles);
-                scale_weights<TYPE, D, RT>(s, values, run, first, lanes, edge, there);
                 if (edge) {
-                    settle_values<TYPE, D, RT>(acc, values, run, shape.tokens, first, lanes, there);
+                    settle_values<TYPE, D, RT>(values, run, shape.tokens, first, lanes, there);
                 }
+                scale_weights<TYPE, D, RT>(s, values);
                 add_values<TYPE, D, RT>(acc, s, values);
                 segment.load_values(values, tiles);
             }

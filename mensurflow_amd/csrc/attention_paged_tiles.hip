@@ -1,9 +1,15 @@
 // mfr_attention_paged for items of many rows (a prefix that a batch shares, pieces of prompts), caches in
 // bf16 and e4m3: bound by the matrix cores.
 //
-// A workgroup's four wavefronts hold 32 rows each and walk the item's tokens together, 64 at a time: the
-// keys, then the values of the next 64 come into registers under the products of these, are turned into
-// the operands' layouts there, and go to the other of two buffers in LDS.
+// A workgroup's four wavefronts, one a SIMD, hold 32 rows each and walk the item's tokens together, 64 at
+// a time, through three buffers in LDS: one that is multiplied, one that is written, and one that a
+// wavefront behind may still read. There is no second wavefront to fill a SIMD's pauses, so that every
+// stretch of products has vector work of another 32 tokens between them, chunk by chunk (a barrier to the
+// compiler's scheduling ends each): scores of the next 32 beside the weights of these, weights times
+// values beside the maximum of the next scores and the turning of the next tile into the operands'
+// layouts, whose numbers come into registers a whole tile ahead. (Two wavefronts a SIMD of half the
+// registers, without this, ran the matrix cores at a fifth of their rate: each waited for its own
+// results, and what spilled came back behind the loads that were under way.)
 //   - S^T = K Q^T by 32 x 32 x 16 products: a wavefront keeps the parts of its queries in registers; keys
 //     lie by 16-byte pieces. Row 8 g + 4 h + r of a product (h: the half of the lanes that gets its scores,
 //     r < 4) is token 16 (g / 2) + 8 h + 4 (g % 2) + r, so that a lane's scores of 16 tokens are of 8
@@ -35,7 +41,7 @@ template <int D> struct Shared {
     uint4 keys[D / 8][kKeys + 4];       // 16-byte pieces of tokens; the pad turns the banks
     uint4 values[kKeys / 8][4][D / 4];  // [8 tokens][column % 4][column / 4]
     float scales[3][kKeys];             // keys', values', log2 of the values'
-    int odd[kWaves];                    // at edges: whether 16 tokens have values that are no numbers
+    uint32_t odd[kWaves];               // at edges: tokens of 16 with values that are no numbers
 };
 constexpr int kAllThere = 15; // a bit for each 16 tokens whose page is one of the cache's
 
@@ -60,35 +66,13 @@ template <bool HIGH> __device__ __forceinline__ uint32_t widen_half(uint32_t w) 
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
 }
 
-// Eight floats (up to 2^16 in fp16) cut into their parts.
-template <int TYPE> struct Parts8 {
-    uint4 part[kParts<TYPE>];
-};
-template <int TYPE>
-__device__ __forceinline__ Parts8<TYPE> cut(float a, float b, float c, float d, float e, float f,
-                                            float g, float h) {
-    Parts8<TYPE> to;
-    if constexpr (TYPE == MFR_KV_BF16) {
-        cut_pair(a, b, to.part[0].x, to.part[1].x, to.part[2].x);
-        cut_pair(c, d, to.part[0].y, to.part[1].y, to.part[2].y);
-        cut_pair(e, f, to.part[0].z, to.part[1].z, to.part[2].z);
-        cut_pair(g, h, to.part[0].w, to.part[1].w, to.part[2].w);
-    } else {
-        const auto round = [](float u, float v) { // towards zero: no overflow
-            return __builtin_bit_cast(halfx2, __builtin_amdgcn_cvt_pkrtz(u, v));
-        };
-        const auto pair = [&](float x, float y, uint32_t& p0, uint32_t& p1) {
-            const halfx2 h0 = round(x, y);
-            p0 = __builtin_bit_cast(uint32_t, h0);
-            p1 = __builtin_bit_cast(uint32_t, round(fmaf(static_cast<float>(h0[0]), -1.0f, x),
-                                                    fmaf(static_cast<float>(h0[1]), -1.0f, y)));
-        };
-        pair(a, b, to.part[0].x, to.part[1].x);
-        pair(c, d, to.part[0].y, to.part[1].y);
-        pair(e, f, to.part[0].z, to.part[1].z);
-        pair(g, h, to.part[0].w, to.part[1].w);
-    }
-    return to;
+// Two floats (up to 2^16) cut into two fp16 parts each, towards zero, so that none overflows.
+__device__ __forceinline__ void cut_halves(float x, float y, uint32_t& p0, uint32_t& p1) {
+    const halfx2 h = __builtin_bit_cast(halfx2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    p0 = __builtin_bit_cast(uint32_t, h);
+    p1 = __builtin_bit_cast(uint32_t,
+                            __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.0f, x),
+                                                       fmaf(static_cast<float>(h[1]), -1.0f, y)));
 }
 
 // A thread's share of a tile on its way from memory to LDS.
@@ -104,118 +88,129 @@ template <int TYPE, int D> struct StagedValues {
 
 template <int TYPE, int D> struct Loader {
     using T = Tile<TYPE, D>;
+    static constexpr int kTokens = kThreads / T::kRowPieces; // of the workgroup's loads of keys
+    static constexpr int kWaveTokens = 64 / T::kRowPieces;
+
     const Params& p;
     const Shape& shape;
     const Pages& pages;
     const int wave, lane;
+    // From a tile's first token to the lane's piece of its keys (of 16 tokens' pieces) and values (of its
+    // 16 tokens), and to the scales: 16 lanes of the keys', 16 of the values', and the same again.
+    GlobalBytes keys, values, scales;
 
-    // The page numbers of a tile's tokens, 16 by 16.
+    __device__ __forceinline__ Loader(const Params& params, const Shape& of, const Pages& at, int w,
+                                      int l)
+        : p(params), shape(of), pages(at), wave(w), lane(l) {
+        const int row_bytes = p.cache.d * kBytes<TYPE>;
+        keys = lane_address(p.cache.k + at.head * p.cache.head_stride,
+                            (wave * kWaveTokens % 16 + lane / T::kRowPieces) * p.cache.token_stride +
+                                min(16 * (lane % T::kRowPieces), row_bytes - 16));
+        values = lane_address(p.cache.v + at.head * p.cache.head_stride,
+                              8 * (lane / 32) * p.cache.token_stride +
+                                  min(T::kValueBytes * (lane % (D / 4)), row_bytes - T::kValueBytes));
+        scales = lane_address((lane & 16) != 0 ? p.cache.v_scales : p.cache.k_scales, 4 * (lane % 16));
+    }
+
+    // The page numbers of a tile: of this wavefront's pieces of the keys and of its values, and whether
+    // they are all there, 16 tokens a bit.
     struct Numbers {
-        int32_t page[4];
+        int32_t key[T::kPieces];
+        int32_t value;
+        int there;
     };
+    // The tokens, of 16, that piece i of this wavefront's keys is among.
+    __device__ __forceinline__ int key_tile(int i) const {
+        return kTokens == 16 ? i : kTokens == 32 ? 2 * i + wave / 2 : 4 * i + wave;
+    }
     __device__ __forceinline__ Numbers numbers(int32_t first) const {
         Numbers n;
 #pragma unroll
+        for (int i = 0; i < T::kPieces; ++i) {
+            n.key[i] = pages.page(p, first + 16 * key_tile(i));
+        }
+        n.value = pages.page(p, first + 16 * wave);
+        n.there = 0;
+#pragma unroll
         for (int i = 0; i < 4; ++i) {
-            n.page[i] = pages.page(p, first + 16 * i);
+            const uint32_t page = static_cast<uint32_t>(pages.page(p, first + 16 * i));
+            n.there |= page < static_cast<uint32_t>(p.work.batch.pages) ? 1 << i : 0;
         }
         return n;
     }
 
-    __device__ __forceinline__ int there(const Numbers& n) const {
-        int bits = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            bits |= mfr::kv::page_checked(p.work.batch, n.page[i]) >= 0 ? 1 << i : 0;
-        }
-        return bits;
-    }
-    // (Not an array's element: its index is not known before the run.)
-    __device__ __forceinline__ static int32_t page_of(const Numbers& n, int i) {
-        return i == 0 ? n.page[0] : i == 1 ? n.page[1] : i == 2 ? n.page[2] : n.page[3];
-    }
-
-    // Addresses are a uniform part and 32 bits of the lane's. Lanes past a row's end load its last piece
-    // again: the queries are zeros there, and those columns of the output are not written.
-    __device__ __forceinline__ void load_keys(StagedKeys<TYPE, D>& to, int32_t first,
-                                              const Numbers& n) const {
-        constexpr int kTokens = kThreads / T::kRowPieces; // of the workgroup's loads
-        constexpr int kWaveTokens = 64 / T::kRowPieces;
-        const uint32_t lane_at = lane / T::kRowPieces * p.cache.token_stride +
-                                 min(16 * (lane % T::kRowPieces), p.cache.d * kBytes<TYPE> - 16);
-#pragma unroll
-        for (int i = 0; i < T::kPieces; ++i) {
-            const int32_t token = i * kTokens + wave * kWaveTokens;
-            const TileAt at = pages.at(p, first + (token & ~15), page_of(n, token / 16));
-            const uint8_t* base = uniform(
-                p.cache.k + at.at + static_cast<int64_t>(token & 15) * p.cache.token_stride);
-            to.k[i] = *reinterpret_cast<const uint4*>(base + lane_at);
-        }
+    // Lanes past a row's end load its last piece again: the queries are zeros there, and those columns of
+    // the output are not written. Piece i of the keys.
+    __device__ __forceinline__ void load_key(StagedKeys<TYPE, D>& to, int i, int32_t first,
+                                             const Numbers& n) const {
+        to.k[i] = load_at<uint4>(keys, pages.at(p, first + 16 * key_tile(i), n.key[i]).at);
     }
 
     // Values: this wavefront's 16 tokens, a thread 8 of them and four columns (at a depth of 64 half of the
-    // threads load what the others do).
-    __device__ __forceinline__ void load_values(StagedValues<TYPE, D>& to, int32_t first,
+    // threads load what the others do). Token r of them.
+    __device__ __forceinline__ TileAt values_at(StagedValues<TYPE, D>& to, int32_t first,
                                                 const Numbers& n) const {
-        const TileAt at = pages.at(p, first + 16 * wave, page_of(n, wave));
+        const TileAt at = pages.at(p, first + 16 * wave, n.value);
         to.first = first;
         to.there = at.there;
-        const int half = lane / 32;
-        const uint32_t lane_at = 8 * half * p.cache.token_stride +
-                                 min(T::kValueBytes * (lane % (D / 4)),
-                                     p.cache.d * kBytes<TYPE> - T::kValueBytes);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const uint8_t* from =
-                uniform(p.cache.v + at.at + static_cast<int64_t>(r) * p.cache.token_stride) + lane_at;
-            if constexpr (T::kValueBytes == 8) {
-                const uint2 w = *reinterpret_cast<const uint2*>(from);
-                to.v[r][0] = w.x;
-                to.v[r][1] = w.y;
-            } else {
-                to.v[r][0] = *reinterpret_cast<const uint32_t*>(from);
-            }
-        }
         if constexpr (TYPE == MFR_KV_F8) {
-            to.scale = 0.0f;
-            if (half == 0) {
-                const float* scales = lane < 16 ? p.cache.k_scales : p.cache.v_scales;
-                to.scale = scales[at.scale_at + lane % 16];
-            }
+            to.scale = load_at<float>(scales, at.scale_at);
+        }
+        return at;
+    }
+    __device__ __forceinline__ void load_value(StagedValues<TYPE, D>& to, int r, const TileAt& at) const {
+        const int64_t from = at.at + static_cast<int64_t>(r) * p.cache.token_stride;
+        if constexpr (T::kValueBytes == 8) {
+            const uint2 w = load_at<uint2>(values, from);
+            to.v[r][0] = w.x;
+            to.v[r][1] = w.y;
+        } else {
+            to.v[r][0] = load_at<uint32_t>(values, from);
         }
     }
 
-    // What was loaded, turned into the operands' layouts, to a buffer that nothing reads.
-    __device__ __forceinline__ void store_keys(const StagedKeys<TYPE, D>& from, Shared<D>& to) const {
-        constexpr int kWaveTokens = 64 / T::kRowPieces;
-        constexpr int kTokens = kThreads / T::kRowPieces;
+    __device__ __forceinline__ void load(StagedKeys<TYPE, D>& k, StagedValues<TYPE, D>& v,
+                                         int32_t first, const Numbers& n) const {
 #pragma unroll
         for (int i = 0; i < T::kPieces; ++i) {
-            const int token = i * kTokens + wave * kWaveTokens + lane / T::kRowPieces;
-            const int piece = lane % T::kRowPieces;
-            if constexpr (TYPE == MFR_KV_BF16) {
-                to.keys[piece][token] = from.k[i];
-            } else {
-                const uint4 w = from.k[i];
-                to.keys[2 * piece][token] =
-                    make_uint4(widen_half<false>(w.x), widen_half<true>(w.x), widen_half<false>(w.y),
-                               widen_half<true>(w.y));
-                to.keys[2 * piece + 1][token] =
-                    make_uint4(widen_half<false>(w.z), widen_half<true>(w.z), widen_half<false>(w.w),
-                               widen_half<true>(w.w));
-            }
+            load_key(k, i, first, n);
+        }
+        const TileAt at = values_at(v, first, n);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            load_value(v, r, at);
         }
     }
 
-    // Values of tokens that there are not are zeros; `edge`: some row does not see some token.
-    __device__ __forceinline__ void store_values(StagedValues<TYPE, D>& from, Shared<D>& to,
-                                                 bool edge) const {
+    // What was loaded, turned into the operands' layouts, to a buffer that nothing reads: a piece of the
+    // keys, ...
+    __device__ __forceinline__ void store_key(const StagedKeys<TYPE, D>& from, int i,
+                                              Shared<D>& to) const {
+        const int token = i * kTokens + wave * kWaveTokens + lane / T::kRowPieces;
+        const int piece = lane % T::kRowPieces;
+        if constexpr (TYPE == MFR_KV_BF16) {
+            to.keys[piece][token] = from.k[i];
+        } else {
+            const uint4 w = from.k[i];
+            to.keys[2 * piece][token] =
+                make_uint4(widen_half<false>(w.x), widen_half<true>(w.x), widen_half<false>(w.y),
+                           widen_half<true>(w.y));
+            to.keys[2 * piece + 1][token] =
+                make_uint4(widen_half<false>(w.z), widen_half<true>(w.z), widen_half<false>(w.w),
+                           widen_half<true>(w.w));
+        }
+    }
+
+    // ... what the columns of the values need before (zeros for tokens that there are not, and, where some
+    // row does not see some token, for numbers that are none), ...
+    __device__ __forceinline__ void settle(StagedValues<TYPE, D>& from, Shared<D>& to,
+                                           bool edge) const {
         const int half = lane / 32;
         if (from.first + kKeys > shape.tokens || !from.there) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                const int32_t token = from.first + 16 * wave + 8 * half + r;
-                const bool keep = from.there && token < shape.tokens;
+                const bool keep =
+                    from.there && from.first + 16 * wave + 8 * half + r < shape.tokens;
 #pragma unroll
                 for (int i = 0; i < T::kValueBytes / 4; ++i) {
                     from.v[r][i] = keep ? from.v[r][i] : 0u;
@@ -223,53 +218,74 @@ template <int TYPE, int D> struct Loader {
             }
         }
         if (edge) {
-            bool odd = false;
+            // Values under a scale that is no number are none. (Their tokens: 16 lanes of the scales.)
+            uint64_t bad = 0;
+            if constexpr (TYPE == MFR_KV_F8) {
+                const bool mine = (lane & 16) != 0 && !(fabsf(from.scale) < INFINITY);
+                bad = __ballot(mine && lane < 32) >> 16;
+                from.scale = mine ? 1.0f : from.scale;
+            }
+            uint32_t tokens = 0;
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
+                const bool under = (bad >> (8 * half + r) & 1) != 0;
+                bool odd = under;
 #pragma unroll
                 for (int i = 0; i < T::kValueBytes / 4; ++i) {
-                    const uint32_t w = from.v[r][i];
-                    if constexpr (TYPE == MFR_KV_BF16) {
-                        odd |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            odd |= ((w >> (8 * e)) & 0x7fu) == 0x7fu;
-                        }
-                    }
+                    odd |= is_odd<TYPE>(from.v[r][i]);
+                    from.v[r][i] = under ? 0u : without_odd<TYPE>(from.v[r][i]);
+                }
+                const uint64_t lanes = __ballot(odd);
+                tokens |= static_cast<uint32_t>(lanes) != 0 ? 1u << r : 0u;
+                tokens |= static_cast<uint32_t>(lanes >> 32) != 0 ? 0x100u << r : 0u;
+            }
+            if (lane == 0) {
+                to.odd[wave] = tokens;
+            }
+        }
+        if constexpr (TYPE == MFR_KV_F8) {
+            if (half == 0) {
+                to.scales[lane / 16][16 * wave + lane % 16] = from.scale;
+                if (lane >= 16) {
+                    // No further down, so that a weight over its value's scale stays inside fp32: values
+                    // under a scale of 2^-96 lose bits.
+                    to.scales[2][16 * wave + lane % 16] =
+                        fmaxf(__builtin_amdgcn_logf(from.scale), -96.0f);
                 }
             }
-            const int any = __any(odd) ? 1 : 0;
-            if (lane == 0) {
-                to.odd[wave] = any;
+        }
+    }
+
+    // ... and column j of this thread's 8 tokens.
+    __device__ __forceinline__ void store_value(const StagedValues<TYPE, D>& from, int j,
+                                                Shared<D>& to) const {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            constexpr int kPerWord = TYPE == MFR_KV_BF16 ? 2 : 4;
+            const uint32_t a = from.v[2 * i][j / kPerWord], b = from.v[2 * i + 1][j / kPerWord];
+            if constexpr (TYPE == MFR_KV_BF16) {
+                w[i] = __builtin_amdgcn_perm(b, a, j % 2 == 0 ? 0x05040100u : 0x07060302u);
+            } else {
+                const uint32_t both =
+                    __builtin_amdgcn_perm(b, a, j % 4 < 2 ? 0x05010400u : 0x07030602u);
+                w[i] = j % 2 == 0 ? widen_half<false>(both) : widen_half<true>(both);
             }
         }
-        if (TYPE == MFR_KV_F8 && half == 0) {
-            to.scales[lane / 16][16 * wave + lane % 16] = from.scale;
-            if (lane >= 16) {
-                // No further down, so that a weight over its value's scale stays inside fp32: values under
-                // a scale of 2^-96 lose bits.
-                to.scales[2][16 * wave + lane % 16] =
-                    fmaxf(__builtin_amdgcn_logf(from.scale), -96.0f);
-            }
+        to.values[2 * wave + lane / 32][j][lane % (D / 4)] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+
+    // All of it.
+    __device__ __forceinline__ void store(const StagedKeys<TYPE, D>& k, StagedValues<TYPE, D>& v,
+                                          Shared<D>& to, bool edge) const {
+#pragma unroll
+        for (int i = 0; i < T::kPieces; ++i) {
+            store_key(k, i, to);
         }
-        // Column j of the 8 tokens.
+        settle(v, to, edge);
 #pragma unroll
         for (int j = 0; j < T::kColumns; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                constexpr int kPerWord = TYPE == MFR_KV_BF16 ? 2 : 4;
-                const uint32_t a = from.v[2 * i][j / kPerWord], b = from.v[2 * i + 1][j / kPerWord];
-                if constexpr (TYPE == MFR_KV_BF16) {
-                    w[i] = __builtin_amdgcn_perm(b, a, j % 2 == 0 ? 0x05040100u : 0x07060302u);
-                } else {
-                    const uint32_t both =
-                        __builtin_amdgcn_perm(b, a, j % 4 < 2 ? 0x05010400u : 0x07030602u);
-                    w[i] = j % 2 == 0 ? widen_half<false>(both) : widen_half<true>(both);
-                }
-            }
-            to.values[2 * wave + half][j][lane % (D / 4)] = make_uint4(w[0], w[1], w[2], w[3]);
+            store_value(v, j, to);
         }
     }
 };
@@ -308,16 +324,24 @@ __device__ __forceinline__ float load_queries(Queries<TYPE, D>& to, const Params
         const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         const int shift = max(-112, min(14 - exponent, 126));
         by = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        rest = p.scale / by;
+        // Above 0, so that scores of tokens that are not seen stay -infinity.
+        rest = fmaxf(fabsf(p.scale) / by, 0x1p-126f);
+        by = copysignf(by, p.scale);
     }
 #pragma unroll
     for (int s = 0; s < D / 16; ++s) {
         const float4 a = scaled(quad(16 * s + 8 * half), by);
         const float4 b = scaled(quad(16 * s + 8 * half + 4), by);
-        const Parts8<TYPE> w = cut<TYPE>(a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w);
-#pragma unroll
-        for (int part = 0; part < kParts<TYPE>; ++part) {
-            to[part][s] = w.part[part];
+        if constexpr (TYPE == MFR_KV_BF16) {
+            cut_pair(a.x, a.y, to[0][s].x, to[1][s].x, to[2][s].x);
+            cut_pair(a.z, a.w, to[0][s].y, to[1][s].y, to[2][s].y);
+            cut_pair(b.x, b.y, to[0][s].z, to[1][s].z, to[2][s].z);
+            cut_pair(b.z, b.w, to[0][s].w, to[1][s].w, to[2][s].w);
+        } else {
+            cut_halves(a.x, a.y, to[0][s].x, to[1][s].x);
+            cut_halves(a.z, a.w, to[0][s].y, to[1][s].y);
+            cut_halves(b.x, b.y, to[0][s].z, to[1][s].z);
+            cut_halves(b.z, b.w, to[0][s].w, to[1][s].w);
         }
     }
     return rest;
@@ -325,83 +349,184 @@ __device__ __forceinline__ float load_queries(Queries<TYPE, D>& to, const Params
 
 template <int D> using Sums = floatx16[D / 32];
 
-// 32 tokens of a tile. Element 4 g + r of the scores: token 16 (g / 2) + 8 half + 4 (g % 2) + r of them.
-// `edge` (uniform): some row does not see some token, or a page is not there. One code for both: a second
-// one, run once at an item's end, takes longer to come into the instruction cache than to run.
+// Scores of 32 tokens: element e is token token_of(e) + 8 half of them.
+__device__ __forceinline__ constexpr int token_of(int e) {
+    return 16 * (e / 8) + 4 * (e / 4 % 2) + e % 4;
+}
+
+// Where a wavefront reads 32 tokens of a tile.
+template <int TYPE, int D> struct Reader {
+    const Shared<D>& tile;
+    const int sub, lane;
+
+    __device__ __forceinline__ uint4 key(int i) const {
+        const int m = lane % 32;
+        const int token = 32 * sub + 16 * (m / 16) + 8 * (m / 4 % 2) + 4 * (m / 8 % 2) + m % 4;
+        return (&tile.keys[lane / 32][token])[i * 2 * (kKeys + 4)];
+    }
+    // Of tokens 16 q + 8 half on, block b of the columns.
+    __device__ __forceinline__ uint4 value(int q, int b) const {
+        return (&tile.values[4 * sub + lane / 32][0][0] + lane % 32)[q * 2 * D + 32 * b];
+    }
+    __device__ __forceinline__ float scale(int which, int e) const {
+        return (&tile.scales[which][32 * sub + 8 * (lane / 32)])[token_of(e)];
+    }
+};
+
+// Weights of 32 tokens as B operands: pairs of them, in parts.
+template <int TYPE> struct Weights {
+    uint32_t pair[kParts<TYPE>][8];
+
+    __device__ __forceinline__ void cut(float x, float y, int i) {
+        if constexpr (TYPE == MFR_KV_BF16) {
+            cut_pair(x, y, pair[0][i], pair[1][i], pair[2][i]);
+        } else {
+            cut_halves(x, y, pair[0][i], pair[1][i]);
+        }
+    }
+    __device__ __forceinline__ uint4 operand(int part, int q) const {
+        return make_uint4(pair[part][4 * q], pair[part][4 * q + 1], pair[part][4 * q + 2],
+                          pair[part][4 * q + 3]);
+    }
+};
+
+// Fragments of keys or values on their way from LDS, four products ahead.
+struct Fragments {
+    uint4 at[4];
+};
+
+// The scales of a lane's 16 tokens, in 8 bits.
+template <int TYPE> struct Scales {
+    float of[TYPE == MFR_KV_F8 ? 16 : 1];
+
+    template <int D> __device__ __forceinline__ void load(const Reader<TYPE, D>& from, int which) {
+        if constexpr (TYPE == MFR_KV_F8) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                of[e] = from.scale(which, e);
+            }
+        }
+    }
+};
+
+// The next scores, whose first keys are in `keys`, and beside them the weights of these: a chunk of 16
+// depths' products has 256 / D weights between them. The first values come into `values`.
 template <int TYPE, int D>
-__device__ __forceinline__ void step(Sums<D>& acc, Running& run, const Queries<TYPE, D>& queries,
-                                     float rest, const Shared<D>& tile, int sub, int32_t first,
-                                     int lane, bool edge, int there) {
-    const int half = lane / 32, m = lane % 32;
-    // The keys of product row m; this half's tokens.
-    const int token = 32 * sub + 16 * (m / 16) + 8 * (m / 4 % 2) + 4 * (m / 8 % 2) + m % 4;
-    const int mine = 32 * sub + 8 * half;
-    floatx16 s;
+__device__ __forceinline__ void scores_and_weights(floatx16& next, Fragments& keys,
+                                                   const Reader<TYPE, D>& ahead,
+                                                   const Queries<TYPE, D>& queries,
+                                                   Weights<TYPE>& weights, const floatx16& s,
+                                                   Fragments& values, const Reader<TYPE, D>& from,
+                                                   Running& run, float reference, float rest) {
+    constexpr int kChunks = D / 16, kEach = 16 / kChunks;
+    Scales<TYPE> by;
+    by.load(from, 1);
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-        s[e] = 0.0f;
+        next[e] = 0.0f;
     }
-    // A piece of the keys is read under the products of the ones before; the barriers keep the compiler
-    // from reading all of them at once, for which there are no registers.
-    const uint4* pieces = &tile.keys[half][token];
-    constexpr int kPitch = 2 * (kKeys + 4);
-    uint4 k[2] = {pieces[0], pieces[kPitch]};
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const uint4 now = k[i % 2];
-        if (i + 2 < D / 16) {
-            k[i % 2] = pieces[(i + 2) * kPitch];
+    for (int i = 0; i < kChunks; ++i) {
+        const uint4 now = keys.at[i % 4];
+        if (i + 4 < kChunks) {
+            keys.at[i % 4] = ahead.key(i + 4);
+        } else {
+            const int j = i + 4 - kChunks;
+            values.at[j] = from.value(j / (D / 32), j % (D / 32));
         }
         // The smallest parts first.
 #pragma unroll
         for (int part = kParts<TYPE> - 1; part >= 0; --part) {
-            s = product<TYPE>(now, queries[part][i], s);
+            next = product<TYPE>(now, queries[part][i], next);
+        }
+#pragma unroll
+        for (int e = kEach * i; e < kEach * (i + 1); e += 2) {
+            float w[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(TYPE == MFR_KV_F8 ? fmaf(s[e + j], rest, -reference)
+                                                                : s[e + j] - reference);
+            }
+            run.sum += w[0] + w[1];
+            if constexpr (TYPE == MFR_KV_F8) {
+                w[0] *= by.of[e];
+                w[1] *= by.of[e + 1];
+            }
+            weights.cut(w[0], w[1], e / 2);
         }
         __builtin_amdgcn_sched_barrier(0);
     }
-    const auto token_of = [&](int e) { return 16 * (e / 8) + 4 * (e / 4 % 2) + e % 4; };
-    const auto visible = [&](int e) {
-        const int at = mine + token_of(e);
-        return first + at < run.seen && (there >> (at / 16) & 1) != 0;
-    };
-    const auto scales_of = [&](int which, int g) {
-        return *reinterpret_cast<const float4*>(&tile.scales[which][mine + token_of(4 * g)]);
-    };
-    // Base-2 scores, and the largest; in 8 bits of what a weight is times its value's scale.
-    if constexpr (TYPE == MFR_KV_F8) {
+}
+
+// Weights times values, whose first are in `values`, and beside them the next scores' maximum and, chunk by
+// chunk, `other(chunk)`. In 8 bits scores are multiplied by their keys' scales (times `rest` they are base-2
+// scores then), and the maximum is of what a weight is times its value's scale.
+template <int TYPE, int D, typename Other>
+__device__ __forceinline__ void add_values(Sums<D>& acc, const Weights<TYPE>& weights,
+                                           Fragments& values, const Reader<TYPE, D>& from,
+                                           floatx16& next, float& most, const Reader<TYPE, D>& ahead,
+                                           float rest, Other other) {
+    constexpr int kBlocks = D / 32, kChunks = 2 * kBlocks, kEach = 16 / kChunks;
+    Scales<TYPE> by, up;
+    by.load(ahead, 0);
+    up.load(ahead, 2);
+    most = -INFINITY;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 by = scaled(scales_of(0, g), rest);
-            s[4 * g] *= by.x;
-            s[4 * g + 1] *= by.y;
-            s[4 * g + 2] *= by.z;
-            s[4 * g + 3] *= by.w;
+    for (int i = 0; i < kChunks; ++i) {
+        const uint4 now = values.at[i % 4];
+        if (i + 4 < kChunks) {
+            values.at[i % 4] = from.value((i + 4) / kBlocks, (i + 4) % kBlocks);
         }
+#pragma unroll
+        for (int part = kParts<TYPE> - 1; part >= 0; --part) {
+            acc[i % kBlocks] = product<TYPE>(now, weights.operand(part, i / kBlocks), acc[i % kBlocks]);
+        }
+#pragma unroll
+        for (int e = kEach * i; e < kEach * (i + 1); ++e) {
+            if constexpr (TYPE == MFR_KV_F8) {
+                next[e] *= by.of[e];
+                most = fmaxf(most, fmaf(next[e], rest, up.of[e]));
+            } else {
+                most = fmaxf(most, next[e]);
+            }
+        }
+        other(i);
+        __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+// What the scores that are ready need before they become weights: tokens that a row does not see (`edge`,
+// uniform: there are some), the running maximum, and the output so far rescaled where it moved. Returns
+// the reference of the weights.
+template <int TYPE, int D>
+__device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>& acc, Running& run,
+                                               const Reader<TYPE, D>& from, float rest, int32_t first,
+                                               bool edge, int there) {
     if (edge) {
+        const int mine = 32 * from.sub + 8 * (from.lane / 32);
+        most = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            s[e] = visible(e) ? s[e] : -INFINITY;
+            const int at = mine + token_of(e);
+            const bool sees = first + at < run.seen && (there >> (at / 16) & 1) != 0;
+            s[e] = sees ? s[e] : -INFINITY;
+            const float t = TYPE == MFR_KV_F8 ? fmaf(s[e], rest, from.scale(2, e)) : s[e];
+            most = fmaxf(most, sees ? t : -INFINITY);
+            // A value that is no number was taken out, and makes the row NaN.
+            const bool odd = sees && (from.tile.odd[at / 16] >> (at % 16) & 1) != 0;
+            run.sum = odd ? NAN : run.sum;
         }
     }
-    float most = -INFINITY;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        float4 up = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if constexpr (TYPE == MFR_KV_F8) {
-            up = scales_of(2, g);
-        }
-        most = fmaxf(fmaxf(most, s[4 * g] + up.x), s[4 * g + 1] + up.y);
-        most = fmaxf(fmaxf(most, s[4 * g + 2] + up.z), s[4 * g + 3] + up.w);
-    }
-    // In 8 bits the reference is 2^15 below the largest.
-    most = max_halves(most) - (TYPE == MFR_KV_F8 ? 15.0f : 0.0f);
-    most = fmaxf(run.top, most);
-    // Nothing seen yet: any finite reference gives weights of 0.
-    const float reference = most == -INFINITY ? 0.0f : most;
-    if (__any(most != run.top)) {
-        const float shrink = __builtin_amdgcn_exp2f(run.top - reference);
-        run.top = most;
+    // Weights are taken against a reference that follows the maximum in steps: it moves, and the output so
+    // far with it, where the maximum has grown by more than 2^8, so that few steps do. In 8 bits it is
+    // 2^7 below the maximum then: fp16 holds weights up to 2^15.
+    constexpr float kBelow = TYPE == MFR_KV_F8 ? 7.0f : 0.0f;
+    most = max_halves(most) - kBelow;
+    if (__any(most > run.top + 8.0f)) {
+        const float top = fmaxf(run.top, most);
+        float shrink = run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top);
+        asm volatile("" : "+v"(shrink)); // no products with it ahead of the branch
+        run.top = top;
         run.sum *= shrink;
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
@@ -411,92 +536,13 @@ __device__ __forceinline__ void step(Sums<D>& acc, Running& run, const Queries<T
             }
         }
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        s[e] = __builtin_amdgcn_exp2f(s[e] - reference);
-    }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) { // a short chain of sums
-        run.sum += (s[4 * g] + s[4 * g + 1]) + (s[4 * g + 2] + s[4 * g + 3]);
-    }
-    if constexpr (TYPE == MFR_KV_F8) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const float4 by = scales_of(1, g);
-            s[4 * g] *= by.x;
-            s[4 * g + 1] *= by.y;
-            s[4 * g + 2] *= by.z;
-            s[4 * g + 3] *= by.w;
-        }
-        if (edge) { // a scale that is not seen may be anything
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = visible(e) ? s[e] : 0.0f;
-            }
-        }
-    }
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-        const Parts8<TYPE> weights =
-            cut<TYPE>(s[8 * q], s[8 * q + 1], s[8 * q + 2], s[8 * q + 3], s[8 * q + 4], s[8 * q + 5],
-                      s[8 * q + 6], s[8 * q + 7]);
-        const uint4* values = &tile.values[4 * sub + 2 * q + half][0][0] + m;
-        uint4 v[2] = {values[0], values[32]};
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-            const uint4 now = v[b % 2];
-            if (b + 2 < D / 32) {
-                v[b % 2] = values[32 * (b + 2)];
-            }
-#pragma unroll
-            for (int part = kParts<TYPE> - 1; part >= 0; --part) {
-                acc[b] = product<TYPE>(now, weights.part[part], acc[b]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-}
-
-// A tile with values that are no numbers, some of which some rows do not see: these must not meet the
-// weights of 0 of such rows. Rows that see one become NaN in its column, and then there are zeros in their
-// place. All wavefronts.
-template <int TYPE, int D>
-__device__ __forceinline__ void settle_odd(Sums<D>& acc, const Running& run, Shared<D>& tile,
-                                           int32_t first, int lane, int there) {
-    const int half = lane / 32;
-#pragma unroll 1
-    for (int group = 0; group < kKeys / 16; ++group) {
-        const int at = first + 16 * group + 8 * half;
-        const auto sees = [&](int i) { return at + i < run.seen && (there >> group & 1) != 0; };
-        const uint4 seen = make_uint4(ones<TYPE>(sees(0), sees(1)), ones<TYPE>(sees(2), sees(3)),
-                                      ones<TYPE>(sees(4), sees(5)), ones<TYPE>(sees(6), sees(7)));
-        const uint4* values = &tile.values[2 * group + half][0][0] + lane % 32;
-#pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-            floatx16 count;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                count[e] = 0.0f;
-            }
-            count = product<TYPE>(odd_ones<TYPE>(values[32 * b]), seen, count);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                acc[b][e] = count[e] > 0.0f ? NAN : acc[b][e];
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
-    __syncthreads();
-    uint4* const values = &tile.values[0][0][0];
-#pragma unroll 1
-    for (int i = threadIdx.x; i < kKeys * D / 8; i += kThreads) {
-        values[i] = without_odd<TYPE>(values[i]);
-    }
-    __syncthreads();
+    // Nothing seen yet: any finite reference gives weights of 0.
+    const float reference = run.top == -INFINITY ? 0.0f : run.top;
+    return reference;
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kThreads, 2) void attention_paged_tiles_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Params p) {
     extern __shared__ uint4 lds[];
     Shared<D>* const tiles = reinterpret_cast<Shared<D>*>(lds);
     const int64_t index = blockIdx.x;
@@ -550,40 +596,111 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_tiles_kernel(Para
         const int32_t last = min(group_some, (item.first + units) * kKeys);
         if (first < last) {
             const Pages pages(p, shape, seq, item.head);
-            const Loader<TYPE, D> loader{p, shape, pages, wave, lane};
+            const Loader<TYPE, D> loader(p, shape, pages, wave, lane);
             typename Loader<TYPE, D>::Numbers numbers = loader.numbers(first);
             StagedKeys<TYPE, D> keys;
             StagedValues<TYPE, D> values;
-            loader.load_keys(keys, first, numbers);
-            loader.load_values(values, first, numbers);
-            int there = loader.there(numbers);
+            loader.load(keys, values, first, numbers);
+            int there = numbers.there; // of the tile, and of the one that is under way
             numbers = loader.numbers(first + kKeys);
-            loader.store_keys(keys, tiles[0]);
-            loader.store_values(values, tiles[0], first + kKeys > group_all);
+            loader.store(keys, values, tiles[0], first + kKeys > group_all);
+            loader.load(keys, values, first + kKeys, numbers);
+            int there_next = numbers.there;
+            numbers = loader.numbers(first + 2 * kKeys);
             __syncthreads();
-            // The next tile's keys are on their way under the first half of this one, its values under the
-            // second, so that the registers hold one of the two; behind the last tile there is something to
-            // load all the same.
-            for (int buffer = 0; first < last; buffer ^= 1) {
-                const int32_t next = first + kKeys;
-                const bool edge = next > group_all || there != kAllThere;
-                if (edge) {
-                    const int4 f = *reinterpret_cast<const int4*>(tiles[buffer].odd);
-                    if (__builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w) != 0) {
-                        settle_odd<TYPE, D>(acc, run, tiles[buffer], first, lane, there);
+            // The first 32 tokens' scores, as they stand after add_values.
+            floatx16 s0, s1;
+            float most = -INFINITY;
+            {
+                const Reader<TYPE, D> from{tiles[0], 0, lane};
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    s0[e] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint4 k = from.key(i);
+#pragma unroll
+                    for (int part = kParts<TYPE> - 1; part >= 0; --part) {
+                        s0 = product<TYPE>(k, queries[part][i], s0);
                     }
                 }
-                loader.load_keys(keys, next, numbers);
-                step<TYPE, D>(acc, run, queries, rest, tiles[buffer], 0, first, lane, edge, there);
-                loader.store_keys(keys, tiles[buffer ^ 1]);
-                loader.load_values(values, next, numbers);
-                step<TYPE, D>(acc, run, queries, rest, tiles[buffer], 1, first, lane, edge, there);
-                loader.store_values(values, tiles[buffer ^ 1], next + kKeys > group_all);
-                there = loader.there(numbers);
-                numbers = loader.numbers(next + kKeys);
-                first = next;
-                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if constexpr (TYPE == MFR_KV_F8) {
+                        s0[e] *= from.scale(0, e);
+                        most = fmaxf(most, fmaf(s0[e], rest, from.scale(2, e)));
+                    } else {
+                        most = fmaxf(most, s0[e]);
+                    }
+                }
             }
+            Fragments keys_ahead, values_ahead;
+            const auto first_keys = [&](const Reader<TYPE, D>& from) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    keys_ahead.at[i] = from.key(i);
+                }
+            };
+            first_keys(Reader<TYPE, D>{tiles[0], 1, lane});
+            Weights<TYPE> weights;
+#pragma unroll 1
+            for (int buffer = 0; first < last; first += kKeys) {
+                Shared<D>& tile = tiles[buffer];
+                buffer = buffer == 2 ? 0 : buffer + 1;
+                Shared<D>& other = tiles[buffer];
+                const bool edge = first + kKeys > group_all || there != kAllThere;
+                const Reader<TYPE, D> low{tile, 0, lane}, high{tile, 1, lane}, ahead{other, 0, lane};
+                loader.settle(values, other, first + 2 * kKeys > group_all);
+                float reference =
+                    settle_scores<TYPE, D>(s0, most, acc, run, low, rest, first, edge, there);
+                scores_and_weights<TYPE, D>(s1, keys_ahead, high, queries, weights, s0, values_ahead, low,
+                                            run, reference, rest);
+                // The next tile's pieces and columns, in the chunks that there are.
+                constexpr int kPieces = Tile<TYPE, D>::kPieces;
+                constexpr int kStores = kPieces + Tile<TYPE, D>::kColumns, kChunks = D / 16;
+                add_values<TYPE, D>(
+                    acc, weights, values_ahead, low, s1, most, high, rest, [&](int chunk) {
+#pragma unroll
+                        for (int i = chunk * kStores / kChunks; i < (chunk + 1) * kStores / kChunks;
+                             ++i) {
+                            if (i < kPieces) {
+                                loader.store_key(keys, i, other);
+                            } else {
+                                loader.store_value(values, i - kPieces, other);
+                            }
+                        }
+                    });
+                lds_barrier();
+                first_keys(ahead);
+                reference =
+                    settle_scores<TYPE, D>(s1, most, acc, run, high, rest, first, edge, there);
+                scores_and_weights<TYPE, D>(s0, keys_ahead, ahead, queries, weights, s1, values_ahead,
+                                            high, run, reference, rest);
+                // Loads of the tile behind the next, and the first keys of the next half.
+                const TileAt at = loader.values_at(values, first + 2 * kKeys, numbers);
+                constexpr int kLoads = kPieces + 8;
+                const Reader<TYPE, D> behind{other, 1, lane};
+                add_values<TYPE, D>(
+                    acc, weights, values_ahead, high, s0, most, ahead, rest, [&](int chunk) {
+#pragma unroll
+                        for (int i = chunk * kLoads / kChunks; i < (chunk + 1) * kLoads / kChunks; ++i) {
+                            if (i < kPieces) {
+                                loader.load_key(keys, i, first + 2 * kKeys, numbers);
+                            } else {
+                                loader.load_value(values, i - kPieces, at);
+                            }
+                        }
+                        if (chunk >= kChunks - 4) {
+                            const int i = chunk + 4 - kChunks;
+                            keys_ahead.at[i] = behind.key(i);
+                        }
+                    });
+                there = there_next;
+                there_next = numbers.there;
+                numbers = loader.numbers(first + 3 * kKeys);
+            }
+            __syncthreads(); // the tiles have been read
         }
         // Results to rows in LDS, in place of the tiles, and from there to memory in whole rows.
         const float sum = sum_halves(run.sum);
@@ -630,9 +747,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_paged_tiles_kernel(Para
 }
 
 template <int TYPE, int D> void launch(const Params& p, hipStream_t stream) {
-    constexpr unsigned kBytesOfLds = 2 * sizeof(Shared<D>);
-    static_assert(kBytesOfLds >= kManyRows * (D + 4) * sizeof(float), "room for the results");
-    static_assert(2 * kBytesOfLds <= 160 * 1024, "two workgroups a compute unit");
+    constexpr unsigned kBytesOfLds = 3 * sizeof(Shared<D>);
+    static_assert(kBytesOfLds <= 160 * 1024 && kBytesOfLds >= kManyRows * (D + 4) * sizeof(float), "room for the results");
     mfr::check(hipFuncSetAttribute(
                    reinterpret_cast<const void*>(attention_paged_tiles_kernel<TYPE, D>),
                    hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBytesOfLds)),
