@@ -36,11 +36,14 @@ template <int TYPE, int D> struct Tile {
     static constexpr int kValueBytes = kColumns * kBytes<TYPE>;
 };
 
+// Tokens of a tile and one more: pieces of a row, which a thread's neighbours write, are in different banks.
+constexpr int kPitch = kKeys + 1;
+
 // A tile in LDS.
 template <int D> struct Shared {
-    uint4 keys[D / 8][kKeys + 4];       // 16-byte pieces of tokens; the pad turns the banks
+    uint4 keys[D / 8][kPitch];          // 16-byte pieces of tokens
     uint4 values[kKeys / 8][4][D / 4];  // [8 tokens][column % 4][column / 4]
-    float scales[3][kKeys];             // keys', values', log2 of the values'
+    float scales[4][kKeys];             // keys', values', log2 of the values', nothing
     uint32_t odd[kWaves];               // at edges: tokens of 16 with values that are no numbers
 };
 constexpr int kAllThere = 15; // a bit for each 16 tokens whose page is one of the cache's
@@ -201,58 +204,49 @@ template <int TYPE, int D> struct Loader {
         }
     }
 
-    // ... what the columns of the values need before (zeros for tokens that there are not, and, where some
-    // row does not see some token, for numbers that are none), ...
-    __device__ __forceinline__ void settle(StagedValues<TYPE, D>& from, Shared<D>& to,
-                                           bool edge) const {
-        const int half = lane / 32;
-        if (from.first + kKeys > shape.tokens || !from.there) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const bool keep =
-                    from.there && from.first + 16 * wave + 8 * half + r < shape.tokens;
-#pragma unroll
-                for (int i = 0; i < T::kValueBytes / 4; ++i) {
-                    from.v[r][i] = keep ? from.v[r][i] : 0u;
-                }
-            }
-        }
-        if (edge) {
-            // Values under a scale that is no number are none. (Their tokens: 16 lanes of the scales.)
-            uint64_t bad = 0;
-            if constexpr (TYPE == MFR_KV_F8) {
-                const bool mine = (lane & 16) != 0 && !(fabsf(from.scale) < INFINITY);
-                bad = __ballot(mine && lane < 32) >> 16;
-                from.scale = mine ? 1.0f : from.scale;
-            }
-            uint32_t tokens = 0;
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const bool under = (bad >> (8 * half + r) & 1) != 0;
-                bool odd = under;
-#pragma unroll
-                for (int i = 0; i < T::kValueBytes / 4; ++i) {
-                    odd |= is_odd<TYPE>(from.v[r][i]);
-                    from.v[r][i] = under ? 0u : without_odd<TYPE>(from.v[r][i]);
-                }
-                const uint64_t lanes = __ballot(odd);
-                tokens |= static_cast<uint32_t>(lanes) != 0 ? 1u << r : 0u;
-                tokens |= static_cast<uint32_t>(lanes >> 32) != 0 ? 0x100u << r : 0u;
-            }
-            if (lane == 0) {
-                to.odd[wave] = tokens;
-            }
-        }
+    // ... the scales (lanes write what others write too, and one row that nothing reads, rather than take a
+    // branch), ...
+    __device__ __forceinline__ void store_scales(const StagedValues<TYPE, D>& from,
+                                                 Shared<D>& to) const {
         if constexpr (TYPE == MFR_KV_F8) {
-            if (half == 0) {
-                to.scales[lane / 16][16 * wave + lane % 16] = from.scale;
-                if (lane >= 16) {
-                    // No further down, so that a weight over its value's scale stays inside fp32: values
-                    // under a scale of 2^-96 lose bits.
-                    to.scales[2][16 * wave + lane % 16] =
-                        fmaxf(__builtin_amdgcn_logf(from.scale), -96.0f);
-                }
+            const int which = lane >> 4 & 1;
+            to.scales[which][16 * wave + lane % 16] = from.scale;
+            // No further down, so that a weight over its value's scale stays inside fp32: values under a
+            // scale of 2^-96 lose bits.
+            to.scales[3 - which][16 * wave + lane % 16] =
+                fmaxf(__builtin_amdgcn_logf(from.scale), -96.0f);
+        }
+    }
+
+    // ... what the values need before where some row does not see some token of the tile, or a page is
+    // not there (zeros for tokens that there are not, and for numbers that are none), ...
+    __device__ __forceinline__ void settle(StagedValues<TYPE, D>& from, Shared<D>& to) const {
+        const int half = lane / 32;
+        // Values under a scale that is no number are none. (Their tokens: 16 lanes of the scales.)
+        uint64_t bad = 0;
+        if constexpr (TYPE == MFR_KV_F8) {
+            const bool mine = (lane & 16) != 0 && !(fabsf(from.scale) < INFINITY);
+            bad = __ballot(mine && lane < 32) >> 16;
+            from.scale = mine ? 1.0f : from.scale;
+        }
+        uint32_t tokens = 0;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const bool keep = from.there && from.first + 16 * wave + 8 * half + r < shape.tokens;
+            const bool under = (bad >> (8 * half + r) & 1) != 0;
+            bool odd = keep && under;
+#pragma unroll
+            for (int i = 0; i < T::kValueBytes / 4; ++i) {
+                const uint32_t w = keep && !under ? from.v[r][i] : 0u;
+                odd |= is_odd<TYPE>(w);
+                from.v[r][i] = without_odd<TYPE>(w);
             }
+            const uint64_t lanes = __ballot(odd);
+            tokens |= static_cast<uint32_t>(lanes) != 0 ? 1u << r : 0u;
+            tokens |= static_cast<uint32_t>(lanes >> 32) != 0 ? 0x100u << r : 0u;
+        }
+        if (lane == 0) {
+            to.odd[wave] = tokens;
         }
     }
 
@@ -282,7 +276,10 @@ template <int TYPE, int D> struct Loader {
         for (int i = 0; i < T::kPieces; ++i) {
             store_key(k, i, to);
         }
-        settle(v, to, edge);
+        if (edge) {
+            settle(v, to);
+        }
+        store_scales(v, to);
 #pragma unroll
         for (int j = 0; j < T::kColumns; ++j) {
             store_value(v, j, to);
@@ -362,7 +359,7 @@ template <int TYPE, int D> struct Reader {
     __device__ __forceinline__ uint4 key(int i) const {
         const int m = lane % 32;
         const int token = 32 * sub + 16 * (m / 16) + 8 * (m / 4 % 2) + 4 * (m / 8 % 2) + m % 4;
-        return (&tile.keys[lane / 32][token])[i * 2 * (kKeys + 4)];
+        return (&tile.keys[lane / 32][token])[i * 2 * kPitch];
     }
     // Of tokens 16 q + 8 half on, block b of the columns.
     __device__ __forceinline__ uint4 value(int q, int b) const {
@@ -503,19 +500,29 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
                                                const Reader<TYPE, D>& from, float rest, int32_t first,
                                                bool edge, int there) {
     if (edge) {
-        const int mine = 32 * from.sub + 8 * (from.lane / 32);
+        const int half = from.lane / 32;
+        const int32_t left = run.seen - first - 32 * from.sub - 8 * half; // tokens of this half's
+        Scales<TYPE> up;
+        up.load(from, 2);
+        const uint32_t* tokens = &from.tile.odd[2 * from.sub];
+        const uint32_t odd = (tokens[0] >> (8 * half) & 0xffu) | (tokens[1] >> (8 * half) & 0xffu) << 8;
+        const uint32_t pages = there >> (2 * from.sub);
+        const uint32_t here = ((pages & 1) != 0 ? 0xffu : 0u) | ((pages & 2) != 0 ? 0xff00u : 0u);
+        uint32_t sees = 0; // element e: bit e, as in `odd`
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sees |= token_of(e) < left ? 1u << e : 0u;
+        }
+        sees &= here;
         most = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            const int at = mine + token_of(e);
-            const bool sees = first + at < run.seen && (there >> (at / 16) & 1) != 0;
-            s[e] = sees ? s[e] : -INFINITY;
-            const float t = TYPE == MFR_KV_F8 ? fmaf(s[e], rest, from.scale(2, e)) : s[e];
-            most = fmaxf(most, sees ? t : -INFINITY);
-            // A value that is no number was taken out, and makes the row NaN.
-            const bool odd = sees && (from.tile.odd[at / 16] >> (at % 16) & 1) != 0;
-            run.sum = odd ? NAN : run.sum;
+            const float t = TYPE == MFR_KV_F8 ? fmaf(s[e], rest, up.of[TYPE == MFR_KV_F8 ? e : 0]) : s[e];
+            most = (sees >> e & 1) != 0 ? fmaxf(most, t) : most;
+            s[e] = (sees >> e & 1) != 0 ? s[e] : -INFINITY;
         }
+        // A value that is no number was taken out, and makes the row NaN.
+        run.sum = (sees & odd) != 0 ? NAN : run.sum;
     }
     // Weights are taken against a reference that follows the maximum in steps: it moves, and the output so
     // far with it, where the maximum has grown by more than 2^8, so that few steps do. In 8 bits it is
@@ -603,7 +610,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
             loader.load(keys, values, first, numbers);
             int there = numbers.there; // of the tile, and of the one that is under way
             numbers = loader.numbers(first + kKeys);
-            loader.store(keys, values, tiles[0], first + kKeys > group_all);
+            loader.store(keys, values, tiles[0], first + kKeys > group_all || there != kAllThere);
             loader.load(keys, values, first + kKeys, numbers);
             int there_next = numbers.there;
             numbers = loader.numbers(first + 2 * kKeys);
@@ -651,7 +658,9 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
                 Shared<D>& other = tiles[buffer];
                 const bool edge = first + kKeys > group_all || there != kAllThere;
                 const Reader<TYPE, D> low{tile, 0, lane}, high{tile, 1, lane}, ahead{other, 0, lane};
-                loader.settle(values, other, first + 2 * kKeys > group_all);
+                if (first + 2 * kKeys > group_all || there_next != kAllThere) {
+                    loader.settle(values, other);
+                }
                 float reference =
                     settle_scores<TYPE, D>(s0, most, acc, run, low, rest, first, edge, there);
                 scores_and_weights<TYPE, D>(s1, keys_ahead, high, queries, weights, s0, values_ahead, low,
@@ -664,6 +673,9 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
 #pragma unroll
                         for (int i = chunk * kStores / kChunks; i < (chunk + 1) * kStores / kChunks;
                              ++i) {
+                            if (i == 0) {
+                                loader.store_scales(values, other);
+                            }
                             if (i < kPieces) {
                                 loader.store_key(keys, i, other);
                             } else {
