@@ -174,25 +174,32 @@ template <int TYPE> __device__ __forceinline__ uint32_t without_odd(uint32_t w) 
     }
 }
 
-// The sum of v over the workgroup, and over the threads before this one.
 struct Scan {
     int64_t total, before;
 };
 
-__device__ inline Scan scan_of(int64_t v, int64_t* waves) {
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+// The sum of v over the wavefront, and over the lanes before this one.
+__device__ inline Scan wave_scan(int64_t v) {
+    const int lane = threadIdx.x % 64;
     int64_t upto = v;
 #pragma unroll
     for (int step = 1; step < 64; step *= 2) {
         const int64_t other = __shfl_up(static_cast<long long>(upto), step, 64);
         upto += lane >= step ? other : 0;
     }
+    return {__shfl(static_cast<long long>(upto), 63, 64), upto - v};
+}
+
+// The same over the workgroup.
+__device__ inline Scan scan_of(int64_t v, int64_t* waves) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const Scan own = wave_scan(v);
     __syncthreads(); // `waves` of a call before has been read
     if (lane == 63) {
-        waves[wave] = upto;
+        waves[wave] = own.total;
     }
     __syncthreads();
-    Scan s{0, upto - v};
+    Scan s{0, own.before};
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
         s.before += i < wave ? waves[i] : 0;
@@ -264,13 +271,36 @@ struct Place {
 };
 
 // Finds the sequence that holds unit `at(total, chunk)` of the list, for all threads; seq -1 where `at`
-// gives a negative place. A sequence a thread, in rounds.
+// gives a negative place. Up to 64 sequences are each wavefront's own matter, a lane each; more are a
+// thread's each, in rounds.
 template <typename At>
 __device__ inline Place find(const Work& w, int32_t groups, At at) {
-    __shared__ int64_t waves[kWaves];
-    __shared__ int64_t found[2];
     const int32_t sequences = kv::sequences_of(w);
     Place p{};
+    p.seq = -1;
+    if (sequences <= 64) {
+        int64_t mine = 0;
+        Scan scan;
+        if (sequences == 1) {
+            mine = kv::shape_of(w, 0).count;
+            scan = {mine, 0};
+        } else {
+            const int32_t lane = threadIdx.x % 64;
+            mine = lane < sequences ? kv::shape_of(w, lane).count : 0;
+            scan = wave_scan(mine);
+        }
+        p.total = scan.total;
+        p.chunk = kv::chunk_of(p.total, groups);
+        const int64_t target = at(p.total, p.chunk);
+        if (target >= 0) {
+            const uint64_t here = __ballot(scan.before <= target && target < scan.before + mine);
+            p.seq = sequences == 1 ? 0 : static_cast<int32_t>(__builtin_ctzll(here));
+            p.base = sequences == 1 ? 0 : __shfl(static_cast<long long>(scan.before), p.seq, 64);
+        }
+        return p;
+    }
+    __shared__ int64_t waves[kWaves];
+    __shared__ int64_t found[2];
     Scan first{};
     int64_t mine = 0;
     for (int32_t s0 = 0; s0 < sequences; s0 += kThreads) {
@@ -285,7 +315,6 @@ __device__ inline Place find(const Work& w, int32_t groups, At at) {
     }
     p.chunk = kv::chunk_of(p.total, groups);
     const int64_t target = at(p.total, p.chunk);
-    p.seq = -1;
     if (target < 0) {
         return p;
     }

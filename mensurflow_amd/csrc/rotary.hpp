@@ -1,9 +1,9 @@
 // Rotation by position (mfr_rotary), for the kernels that turn queries and keys.
 //
-// A workgroup works on one token at a time: the cosines and sines of its rot / 2 angles are made once,
-// into LDS, for all heads of the token. A lane holds 4 columns of a head from 4 lane on and loads its
-// pairs' other halves as well, so that every layout has one form; the second loads find the first ones'
-// lines in the L1 cache.
+// A wavefront works on one token at a time: the cosines and sines of its rot / 2 angles are made once,
+// into LDS, for all heads that it has of the token. Columns that turn together are in one lane: a piece of
+// a head is two times 4 columns, those of four pairs where any of them turns, so that every number is
+// loaded once and a head may be turned in place.
 #pragma once
 
 #include "common.hpp"
@@ -19,7 +19,7 @@ struct Rotary {
     int32_t rot;
     int32_t pairs; // neighbours turn together
     float amplitude;
-    int32_t quads; // no four columns straddle a half's, the rotated part's or the head's end
+    int32_t quads; // no four columns of a piece straddle a half's, the turned part's or the head's end
     double turns[kMostPairs]; // a position, in whole turns
 };
 
@@ -42,6 +42,11 @@ inline Rotary checked(const mfr_rotary& r, int64_t d, const char* what) {
         out.turns[i] = r.steps[i] / 6.283185307179586476925;
     }
     return out;
+}
+
+// Pieces (dev::piece_of) of a head's first `columns`.
+inline int32_t pieces_of(const Rotary& r, int32_t columns) {
+    return r.pairs != 0 ? (columns + 7) / 8 : (r.rot / 2 + 3) / 4 + (columns - r.rot + 7) / 8;
 }
 
 } // namespace mfr::rotary
@@ -70,64 +75,90 @@ __device__ inline float2 angle_of(double position, double turns) {
     return make_float2(quarter == 1 || quarter == 2 ? -a : a, quarter >= 2 ? -b : b);
 }
 
-// The angles of a token into `table` [rot / 2], by all threads of the workgroup. A barrier has to
-// follow.
-__device__ inline void fill_angles(const Rotary& r, int64_t position, bool backward, float2* table,
-                                   int threads) {
-    for (int i = threadIdx.x; i < r.rot / 2; i += threads) {
+// The angles of a token into the wavefront's `table` [rot / 2].
+__device__ inline void fill_angles(const Rotary& r, int64_t position, bool backward, float2* table) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    for (int i = threadIdx.x % 64; i < r.rot / 2; i += 64) {
         const float2 t = angle_of(static_cast<double>(position), r.turns[i]);
         table[i] = make_float2(r.amplitude * t.x, r.amplitude * (backward ? -t.y : t.y));
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 }
 
-// One column: own * cos +- other * sin.
-__device__ inline float turned(float own, float other, float2 t, bool first) {
-    return first ? fmaf(own, t.x, -(other * t.y)) : fmaf(own, t.x, other * t.y);
-}
+// na columns of a head from a on, and nb from b on (each up to 4, nb perhaps 0).
+struct Piece {
+    int32_t a, b, na, nb;
+    int32_t angles; // from here on are its pairs'; -1: nothing turns
+};
 
-// Up to 4 columns from c on (c < d, a multiple of 4) of the head of d columns at x, turned. QUADS:
-// Rotary::quads.
-template <bool QUADS>
-__device__ inline float4 turned_quad(const float* x, int c, int d, const Rotary& r,
-                                     const float2* table) {
-    const int half = r.rot / 2;
-    if constexpr (QUADS) {
-        float4 v = mfr::dev::load_loose(x + c);
-        if (c < r.rot) {
-            if (r.pairs != 0) {
-                const float2 t0 = table[c / 2], t1 = table[c / 2 + 1];
-                return make_float4(turned(v.x, v.y, t0, true), turned(v.y, v.x, t0, false),
-                                   turned(v.z, v.w, t1, true), turned(v.w, v.z, t1, false));
-            }
-            const bool first = c < half;
-            const float4 o = mfr::dev::load_loose(x + (first ? c + half : c - half));
-            const float2* t = table + (first ? c : c - half);
-            v = make_float4(turned(v.x, o.x, t[0], first), turned(v.y, o.y, t[1], first),
-                            turned(v.z, o.z, t[2], first), turned(v.w, o.w, t[3], first));
-        }
-        return v;
-    } else {
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int at = c + e;
-            v[e] = at < d ? x[at] : 0.0f;
-            if (at < r.rot) {
-                const bool first = r.pairs != 0 ? at % 2 == 0 : at < half;
-                const int step = r.pairs != 0 ? 1 : half;
-                const int pair = r.pairs != 0 ? at / 2 : first ? at : at - half;
-                v[e] = turned(v[e], x[first ? at + step : at - step], table[pair], first);
-            }
-        }
-        return make_float4(v[0], v[1], v[2], v[3]);
+// Piece i of a head's first `columns`, which hold at least all that turn. Past the last one na <= 0.
+__device__ inline Piece piece_of(const Rotary& r, int32_t i, int32_t columns) {
+    const int32_t half = r.rot / 2;
+    const int32_t turning = (half + 3) / 4;
+    if (r.pairs == 0 && i < turning) {
+        const int32_t n = min(4, half - 4 * i);
+        return {4 * i, half + 4 * i, n, n, 4 * i};
     }
+    const int32_t a = r.pairs != 0 ? 8 * i : r.rot + 8 * (i - turning);
+    return {a, a + 4, min(4, columns - a), max(0, min(4, columns - a - 4)), a < r.rot ? 4 * i : -1};
 }
 
-// Between a wavefront's loads of a head and its stores over it: no store is moved up into one side of
-// a branch whose other side still loads.
-__device__ inline void loads_before_stores() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_wave_barrier();
+// The numbers of a piece of a head at x. QUADS: Rotary::quads, and whole quads of columns.
+struct Numbers {
+    float4 a, b;
+};
+template <bool QUADS>
+__device__ inline float4 load_columns(const float* x, int32_t n) {
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if constexpr (QUADS) {
+        if (n > 0) {
+            v = mfr::dev::load_loose(x);
+        }
+    } else {
+        v.x = n > 0 ? x[0] : 0.0f;
+        v.y = n > 1 ? x[1] : 0.0f;
+        v.z = n > 2 ? x[2] : 0.0f;
+        v.w = n > 3 ? x[3] : 0.0f;
+    }
+    return v;
+}
+template <bool QUADS>
+__device__ inline Numbers load_piece(const float* x, const Piece& p) {
+    return {load_columns<QUADS>(x + p.a, p.na), load_columns<QUADS>(x + p.b, p.nb)};
+}
+
+// A pair turned, or as it is.
+struct Pair {
+    float own, other;
+};
+__device__ inline Pair turned(float own, float other, float2 t, bool turns) {
+    return {turns ? fmaf(own, t.x, -(other * t.y)) : own,
+            turns ? fmaf(other, t.x, own * t.y) : other};
+}
+
+// Columns past the piece's stay zeros.
+template <bool QUADS>
+__device__ inline Numbers turned_piece(const Numbers& v, const Piece& p, const Rotary& r,
+                                       const float2* table) {
+    if (p.angles < 0) {
+        return v;
+    }
+    const float2* t = table + p.angles;
+    if (r.pairs != 0) {
+        const bool a = p.a < r.rot, b = p.b < r.rot;
+        const Pair p0 = turned(v.a.x, v.a.y, t[0], a);
+        const Pair p1 = turned(v.a.z, v.a.w, t[1], QUADS ? a : p.a + 2 < r.rot);
+        const Pair p2 = turned(v.b.x, v.b.y, t[2], b);
+        const Pair p3 = turned(v.b.z, v.b.w, t[3], QUADS ? b : p.b + 2 < r.rot);
+        return {make_float4(p0.own, p0.other, p1.own, p1.other),
+                make_float4(p2.own, p2.other, p3.own, p3.other)};
+    }
+    const Pair p0 = turned(v.a.x, v.b.x, t[0], true);
+    const Pair p1 = turned(v.a.y, v.b.y, t[1], QUADS || p.na > 1);
+    const Pair p2 = turned(v.a.z, v.b.z, t[2], QUADS || p.na > 2);
+    const Pair p3 = turned(v.a.w, v.b.w, t[3], QUADS || p.na > 3);
+    return {make_float4(p0.own, p1.own, p2.own, p3.own),
+            make_float4(p0.other, p1.other, p2.other, p3.other)};
 }
 
 } // namespace mfr::rotary::dev

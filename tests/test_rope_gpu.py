@@ -152,3 +152,18 @@ def test_many_rows(stream):
     x = rng.standard_normal((rows, 1, 8)).astype(np.float32)
     want, off = ref.turn(x, np.arange(rows), ref.steps(8), mf.ROTARY_PAIRS)
     check(mf.rope(dev(x, stream), mf.rotary(8, layout=mf.ROTARY_PAIRS)).numpy(), want, off, "many")
+
+
+def test_many_heads(stream):
+    """So many heads of a token that few tokens are taken at once."""
+    rng = np.random.default_rng(9)
+    x = rng.standard_normal((40, 1 << 18, 8)).astype(np.float32)
+    got = mf.rope(dev(x, stream), mf.rotary(8), first=5).numpy()
+    for h in (0, 1, 70000, (1 << 18) - 1):
+        want, off = ref.turn(x[:, h:h + 1], np.arange(40) + 5, ref.steps(8), mf.ROTARY_HALVES)
+        check(got[:, h:h + 1], want, off, h)
+    one = rng.standard_normal((300, 1, 8)).astype(np.float32)
+    wide = dev(one, stream).expand((300, 1 << 17, 8))
+    got = mf.rope(wide, mf.rotary(8)).numpy()
+    want, off = ref.turn(one, np.arange(300), ref.steps(8), mf.ROTARY_HALVES)
+    check(got, np.broadcast_to(want, got.shape), np.broadcast_to(off, got.shape), "one for all")
