@@ -44,7 +44,8 @@ Launch launch_of(Params p, int32_t type, int shared, int cus) {
         shared != 0 ? w.batch.prefix : static_cast<int64_t>(mfr::kv::capacity_of(w.batch));
     const int64_t units = std::max<int64_t>(1, (tokens + w.unit - 1) / w.unit);
     const int64_t items = (rows / w.tile_rows + sequences) * w.heads;
-    const int64_t wanted = static_cast<int64_t>(cus) * (w.tile_rows == 16 ? 2 : 1);
+    const int64_t wanted =
+        static_cast<int64_t>(cus) * mfr::paged::per_unit(type, p.depth, w.tile_rows);
     p.groups = static_cast<int32_t>(items >= wanted ? wanted : std::min(wanted, items * units));
     return {p, 2 * static_cast<size_t>(p.groups) * static_cast<size_t>(w.tile_rows)};
 }

@@ -46,6 +46,17 @@ struct Params {
 // (attention_paged_tiles.hip).
 constexpr int32_t kManyRows = 128;
 
+// Workgroups that a compute unit holds at once, by the registers of the forms.
+constexpr int per_unit(int32_t type, int depth, int32_t tile_rows) {
+    if (tile_rows == kManyRows) {
+        return 1;
+    }
+    if (tile_rows == 32) {
+        return type == MFR_KV_F32 && depth == 128 ? 1 : 2;
+    }
+    return depth == 64 ? 3 : 2;
+}
+
 void launch_few(const Params& p, int32_t type, hipStream_t stream);
 void launch_tiles(const Params& p, int32_t type, hipStream_t stream);
 void launch_join(const Params& p, hipStream_t stream);
@@ -270,11 +281,19 @@ struct Place {
     int64_t base; // of the sequence, in the list of units
 };
 
+// A number that is the same in all lanes, known to be so: what is found from it is in scalar registers.
+__device__ __forceinline__ int32_t uniform(int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t low = uniform(static_cast<int32_t>(v));
+    const uint32_t high = uniform(static_cast<int32_t>(v >> 32));
+    return static_cast<int64_t>(static_cast<uint64_t>(high) << 32 | low);
+}
+
 // Finds the sequence that holds unit `at(total, chunk)` of the list, for all threads; seq -1 where `at`
 // gives a negative place. Up to 64 sequences are each wavefront's own matter, a lane each; more are a
 // thread's each, in rounds.
 template <typename At>
-__device__ inline Place find(const Work& w, int32_t groups, At at) {
+__device__ inline Place find_any(const Work& w, int32_t groups, At at) {
     const int32_t sequences = kv::sequences_of(w);
     Place p{};
     p.seq = -1;
@@ -337,9 +356,14 @@ __device__ inline Place find(const Work& w, int32_t groups, At at) {
         }
     }
     __syncthreads();
-    p.seq = __builtin_amdgcn_readfirstlane(static_cast<int>(found[0]));
+    p.seq = static_cast<int32_t>(found[0]);
     p.base = found[1];
     return p;
+}
+template <typename At>
+__device__ inline Place find(const Work& w, int32_t groups, At at) {
+    const Place p = find_any(w, groups, at);
+    return {uniform(p.total), uniform(p.chunk), uniform(p.seq), uniform(p.base)};
 }
 
 // exp2(m - top), 0 for a part that saw nothing (m = -inf, also where every part did).

@@ -15,6 +15,8 @@
 // cut into three bf16 parts, so that products and sums are fp32's; fp32 caches use the fp32 products.
 #include "attention_paged.hpp"
 
+#include <type_traits>
+
 namespace {
 
 using namespace mfr::paged;
@@ -136,19 +138,30 @@ template <int TYPE, int D, bool FULL> struct Segment {
     }
 };
 
-// The queries of an item's rows as B operands: three bf16 parts, or fp32.
+// The queries of an item's rows as B operands: three bf16 parts, or fp32. Where the registers that they
+// take let one more workgroup run on a compute unit, the parts lie in LDS, once for the workgroup's
+// wavefronts, which read them at every step (24 rows a sequence on up to 4096 tokens in 8 bits: 121 us and
+// 153 in registers; 4 rows of 64 on up to 8191: 70 and 74). With one tile of rows of 128 that is not so, and
+// they stay in registers: no barrier holds an item's first loads back then (256 sequences of up to 1023
+// tokens in 8 bits 103 us and 108 in LDS).
+template <int TYPE, int D, int RT>
+constexpr bool kQueriesInLds = TYPE != MFR_KV_F32 && (D == 64 || RT == 2);
+
 template <int TYPE, int D, int RT> struct Queries {
-    static constexpr int kSteps = Form<TYPE, D>::kSteps;
-    uint4 part[RT][3][kSteps];
+    static constexpr int kLanes = kQueriesInLds<TYPE, D, RT> ? 64 : 1;
+    uint4 part[RT][3][Form<TYPE, D>::kSteps][kLanes];
 };
 template <int D, int RT> struct Queries<MFR_KV_F32, D, RT> {
     float4 q[RT][D / 16];
 };
 
+// By every wavefront for itself, but into LDS, where each takes some steps of the depth, and a barrier has to
+// follow.
 template <int TYPE, int D, int RT, bool FULL>
 __device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Params& p,
                                              const Shape& shape, int32_t head, int32_t tile,
-                                             const Lanes& lanes) {
+                                             const Lanes& lanes, int wave) {
+    constexpr bool kLds = kQueriesInLds<TYPE, D, RT>;
     const int32_t rows = shape.span.count * p.work.group;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -169,17 +182,26 @@ __device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Par
                 to.q[rt][s] = quad(16 * s + 4 * lanes.quad);
             }
         } else {
+            static_assert(!kLds || Form<TYPE, D>::kSteps <= kWaves);
 #pragma unroll
-            for (int s = 0; s < Form<TYPE, D>::kSteps; ++s) {
+            for (int j = 0; j < (kLds ? 1 : Form<TYPE, D>::kSteps); ++j) {
+                const int s = kLds ? wave : j;
+                if (kLds && s >= Form<TYPE, D>::kSteps) {
+                    break;
+                }
                 // The depths of piece s of a key: 8 neighbours, or in 8 bits half of 16.
                 const int c = TYPE == MFR_KV_BF16 ? 32 * s + 8 * lanes.quad
                                                   : 64 * (s / 2) + 16 * lanes.quad + 8 * (s % 2);
                 const float4 a = quad(c), b = quad(c + 4);
-                auto& part = to.part[rt];
-                cut_pair(a.x, a.y, part[0][s].x, part[1][s].x, part[2][s].x);
-                cut_pair(a.z, a.w, part[0][s].y, part[1][s].y, part[2][s].y);
-                cut_pair(b.x, b.y, part[0][s].z, part[1][s].z, part[2][s].z);
-                cut_pair(b.z, b.w, part[0][s].w, part[1][s].w, part[2][s].w);
+                uint4 part[3];
+                cut_pair(a.x, a.y, part[0].x, part[1].x, part[2].x);
+                cut_pair(a.z, a.w, part[0].y, part[1].y, part[2].y);
+                cut_pair(b.x, b.y, part[0].z, part[1].z, part[2].z);
+                cut_pair(b.z, b.w, part[0].w, part[1].w, part[2].w);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    to.part[rt][i][s][kLds ? 16 * lanes.quad + lanes.row : 0] = part[i];
+                }
             }
         }
     }
@@ -189,8 +211,9 @@ __device__ __forceinline__ void load_queries(Queries<TYPE, D, RT>& to, const Par
 template <int TYPE, int D, int RT>
 __device__ __forceinline__ void scores_of(Scores<TYPE, D, RT>& s,
                                           const Keys<TYPE, D>& keys,
-                                          const Queries<TYPE, D, RT>& queries) {
+                                          const Queries<TYPE, D, RT>& queries, const Lanes& lanes) {
     using F = Form<TYPE, D>;
+    const int lane = kQueriesInLds<TYPE, D, RT> ? 16 * lanes.quad + lanes.row : 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -233,7 +256,8 @@ __device__ __forceinline__ void scores_of(Scores<TYPE, D, RT>& s,
             for (int part = 2; part >= 0; --part) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-                    const bf16x8 q = __builtin_bit_cast(bf16x8, queries.part[rt][part][step]);
+                    const bf16x8 q =
+                        __builtin_bit_cast(bf16x8, queries.part[rt][part][step][lane]);
 #pragma unroll
                     for (int t = 0; t < F::kTiles; ++t) {
                         s[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[t], q, s[rt][t], 0, 0, 0);
@@ -433,11 +457,12 @@ template <int TYPE, int D> __device__ __forceinline__ int column_at(int quad, in
 }
 
 template <int TYPE, int D, int RT, bool FULL>
-__global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, (per_unit(TYPE, D, 16 * RT))) void attention_paged_few_kernel(Params p) {
     using F = Form<TYPE, D>;
     constexpr int kPitch = D + 4;
     __shared__ float joined[kWaves][16][kPitch];
     __shared__ float stats[kWaves][16][2];
+    __shared__ std::conditional_t<kQueriesInLds<TYPE, D, RT>, Queries<TYPE, D, RT>, int> held;
     const int64_t index = blockIdx.x;
     const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t chunk) {
         return index * chunk < total ? index * chunk : int64_t{-1};
@@ -484,8 +509,20 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
         const int32_t all_see = mfr::kv::seen_by(shape, row0 / p.work.group, p.causal != 0);
         const int32_t some_see = mfr::kv::seen_by(
             shape, (min(row0 + 16 * RT, rows) - 1) / p.work.group, p.causal != 0);
-        Queries<TYPE, D, RT> queries;
-        load_queries<TYPE, D, RT, FULL>(queries, p, shape, item.head, item.tile, lanes);
+        // (What is in LDS of the item before was read before the barriers at its end.)
+        constexpr bool kLds = kQueriesInLds<TYPE, D, RT>;
+        std::conditional_t<kLds, int, Queries<TYPE, D, RT>> own;
+        auto& queries = [&]() -> auto& {
+            if constexpr (kLds) {
+                return held;
+            } else {
+                return own;
+            }
+        }();
+        load_queries<TYPE, D, RT, FULL>(queries, p, shape, item.head, item.tile, lanes, wave);
+        if constexpr (kLds) {
+            __syncthreads();
+        }
         Sums<TYPE, D, RT> acc;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -537,9 +574,19 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
                     edge = edge || !there[t];
                 }
                 tiles_of(first + kUnit);
-                numbers_of(first + 2 * kUnit);
+                if constexpr (!kLds) {
+                    numbers_of(first + 2 * kUnit);
+                }
                 Scores<TYPE, D, RT> s;
-                scores_of<TYPE, D, RT>(s, keys, queries);
+                if constexpr (kLds) { // queries do not move into registers ahead of the loop
+                    asm volatile("" ::: "memory");
+                }
+                scores_of<TYPE, D, RT>(s, keys, queries, lanes);
+                if constexpr (kLds) { // behind the reads from LDS, which would wait for these
+                    __builtin_amdgcn_sched_barrier(0);
+                    numbers_of(first + 2 * kUnit);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
                 softmax_step<TYPE, D, RT>(s, acc, run, keys, p.scale, first, lanes, edge, there);
                 segment.load_keys(keys, tiles);
                 if (edge) {
@@ -615,48 +662,78 @@ __global__ __launch_bounds__(kThreads, RT == 1 ? 2 : 1) void attention_paged_few
     }
 }
 
-// Joins the parts of the items that were cut: workgroup x looks at the end of chunk x, and takes the
-// item that began in it and goes on, rows 8 y .. 8 y + 7 of it. 32 lanes hold a part's row; they take a row's
-// parts in order, or, where an item has few rows, share them (a part in `split`) and join through LDS.
+// Joins the parts of the items that were cut, rows 8 y .. 8 y + 7 of one a workgroup: of item x, where the
+// items are those of the prefix and no more than chunks, otherwise of the one that began in chunk x and goes
+// on behind it (if there is one). 32 lanes
+// hold a part's row; they take a row's parts in order, or, where an item has few rows, share them (a part in
+// `split`) and join through LDS. Workgroups go to the chip's dies in turn. Items of many rows that begin in
+// every 8th or 16th chunk would all go to one die: each takes neighbouring ones instead (16 items of 128
+// rows in 16 parts each: 5.6 us, 22 from one die). Items of few rows go where their first part was written
+// and may still be in a cache (256 sequences in 512 chunks: 6.4 us, 8.3 elsewhere).
 constexpr int kJoinRows = 8;
+constexpr int kDies = 8;
 
-__global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p) {
+__global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p, uint32_t count,
+                                                                       bool by_item) {
     __shared__ float4 values[kJoinRows][32];
     __shared__ float2 stats[kJoinRows];
-    const int64_t index = blockIdx.x;
-    const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t chunk) {
-        // The last unit of a chunk that another one follows.
-        return (index + 1) * chunk < total ? (index + 1) * chunk - 1 : int64_t{-1};
-    });
-    if (place.seq < 0) {
+    const uint32_t pieces = static_cast<uint32_t>(p.work.tile_rows + kJoinRows - 1) / kJoinRows;
+    uint32_t x, y;
+    if (p.work.tile_rows == kManyRows) {
+        const uint32_t per_die = (count * pieces + kDies - 1) / kDies;
+        const uint32_t at = blockIdx.x % kDies * per_die + blockIdx.x / kDies;
+        x = at / pieces;
+        y = at - x * pieces;
+    } else {
+        y = blockIdx.x / count;
+        x = blockIdx.x - y * count;
+    }
+    if (x >= count || y >= pieces) {
         return;
     }
-    const Shape shape = mfr::kv::shape_of(p.work, place.seq);
-    const int64_t edge = (index + 1) * place.chunk;
-    const Item item = mfr::kv::item_of(shape, place.base, edge - 1);
+    int64_t index = x, chunk;
+    Shape shape;
+    Item item;
+    if (by_item) {
+        shape = mfr::kv::shape_of(p.work, 0);
+        chunk = mfr::kv::chunk_of(shape.count, p.groups);
+        item = mfr::kv::item_of(shape, 0, index * shape.units);
+        index = mfr::kv::quotient(item.begin, chunk);
+    } else {
+        const dev::Place place = dev::find(p.work, p.groups, [&](int64_t total, int64_t length) {
+            // The last unit of a chunk that another one follows.
+            return (index + 1) * length < total ? (index + 1) * length - 1 : int64_t{-1};
+        });
+        if (place.seq < 0) {
+            return;
+        }
+        chunk = place.chunk;
+        shape = mfr::kv::shape_of(p.work, place.seq);
+        item = mfr::kv::item_of(shape, place.base, (index + 1) * chunk - 1);
+    }
     const int64_t end = item.begin + shape.units;
-    if (item.begin < index * place.chunk || end <= edge) {
+    if (item.begin < index * chunk || end <= (index + 1) * chunk) {
         return;
     }
     const int32_t rows = shape.span.count * p.work.group;
-    const int32_t row0 = item.tile * p.work.tile_rows + kJoinRows * static_cast<int32_t>(blockIdx.y);
+    const int32_t row0 = item.tile * p.work.tile_rows + kJoinRows * static_cast<int32_t>(y);
     const int32_t here = min(kJoinRows, min((item.tile + 1) * p.work.tile_rows, rows) - row0);
     if (here <= 0) {
         return;
     }
-    const int64_t last = (end - 1) / place.chunk; // the chunk of its last unit
-    const int count = static_cast<int>(last - index) + 1;
+    const int64_t last = mfr::kv::quotient(end - 1, chunk); // the chunk of its last unit
+    const int parts = static_cast<int>(last - index) + 1;
     const int split = here <= 1 ? 8 : here <= 2 ? 4 : here <= 4 ? 2 : 1;
     const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
     const int32_t r = group / split;
     const int c = 4 * lane;
-    const int64_t first = mfr::kv::part_of(index, place.chunk, item.begin); // the others' are 2 apart
+    const int64_t first = mfr::kv::part_of(index, chunk, item.begin); // the others' are 2 apart
     const int64_t row = row0 - item.tile * p.work.tile_rows + r;
     float top = -INFINITY, sum = 0.0f;
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (r < here) {
         constexpr int kAtOnce = 8;
-        for (int i0 = group % split; i0 < count; i0 += kAtOnce * split) {
+        for (int i0 = group % split; i0 < parts; i0 += kAtOnce * split) {
             float2 stat[kAtOnce];
             float4 value[kAtOnce];
 #pragma unroll
@@ -664,7 +741,7 @@ __global__ __launch_bounds__(kThreads) void attention_paged_join_kernel(Params p
                 const int i = i0 + k * split;
                 stat[k] = make_float2(-INFINITY, 0.0f);
                 value[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (i < count) {
+                if (i < parts) {
                     const int64_t part = (i == 0 ? first : 2 * (index + i)) * p.work.tile_rows + row;
                     stat[k] = *reinterpret_cast<const float2*>(p.parts.stats + 2 * part);
                     if (c < p.depth) {
@@ -754,9 +831,17 @@ void launch_few(const Params& p, int32_t type, hipStream_t stream) {
 }
 
 void launch_join(const Params& p, hipStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(p.groups),
-                    static_cast<unsigned>((p.work.tile_rows + kJoinRows - 1) / kJoinRows));
-    attention_paged_join_kernel<<<grid, kThreads, 0, stream>>>(p);
+    int64_t count = p.groups;
+    bool by_item = false;
+    if (p.work.shared != 0) { // known here
+        const int64_t items = static_cast<int64_t>(kv::shape_of(p.work, 0).tiles) * p.work.heads;
+        by_item = items <= count;
+        count = by_item ? items : count;
+    }
+    const int64_t pieces = (p.work.tile_rows + kJoinRows - 1) / kJoinRows;
+    const unsigned blocks = static_cast<unsigned>((count * pieces + kDies - 1) / kDies * kDies);
+    attention_paged_join_kernel<<<blocks, kThreads, 0, stream>>>(p, static_cast<uint32_t>(count),
+                                                              by_item);
     check_launch("attention_paged_join_kernel");
 }
 

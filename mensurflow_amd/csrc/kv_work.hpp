@@ -42,9 +42,10 @@ MFR_KV_BOTH Shape shape_of(const Work& w, int32_t s) {
         p.tokens = w.batch.prefix;
         p.first_place = 0;
     } else {
+        const int32_t length = w.batch.lengths[s]; // under way with the starts
         p.span = span_of(w.batch, s);
-        p.tokens = length_of(w.batch, s);
-        p.first_place = first_place(w.batch, s, p.span.count);
+        p.tokens = within(length, 0, capacity_of(w.batch));
+        p.first_place = static_cast<int64_t>(length) - p.span.count;
     }
     p.tiles = (p.span.count * w.group + w.tile_rows - 1) / w.tile_rows;
     p.units = p.tokens > 0 ? (p.tokens - 1) / w.unit + 1 : 1;
@@ -52,9 +53,13 @@ MFR_KV_BOTH Shape shape_of(const Work& w, int32_t s) {
     return p;
 }
 
+MFR_KV_BOTH int64_t quotient(int64_t a, int64_t b) { // a not below 0, b above; most often of 32 bits
+    return ((a | b) >> 32) == 0 ? static_cast<uint32_t>(a) / static_cast<uint32_t>(b) : a / b;
+}
+
 // The chunk that each of `groups` workgroups takes.
 MFR_KV_BOTH int64_t chunk_of(int64_t total, int32_t groups) {
-    return total > 0 ? (total - 1) / groups + 1 : 1;
+    return total > 0 ? quotient(total - 1, groups) + 1 : 1;
 }
 
 // An item from the place of one of its units in the list.
@@ -66,10 +71,10 @@ struct Item {
 
 MFR_KV_BOTH Item item_of(const Shape& p, int64_t base, int64_t at) {
     const int64_t off = at - base;
-    const int64_t item = off / p.units;
+    const int64_t item = quotient(off, p.units);
     Item i;
     i.first = static_cast<int32_t>(off - item * p.units);
-    i.head = static_cast<int32_t>(item / p.tiles);
+    i.head = static_cast<int32_t>(quotient(item, p.tiles));
     i.tile = static_cast<int32_t>(item - static_cast<int64_t>(i.head) * p.tiles);
     i.begin = at - i.first;
     return i;
