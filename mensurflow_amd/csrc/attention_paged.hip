@@ -36,8 +36,11 @@ Launch launch_of(Params p, int32_t type, int shared, int cus) {
     w.shared = shared;
     const int64_t sequences = mfr::kv::sequences_of(w);
     const int64_t rows = static_cast<int64_t>(w.batch.rows) * w.group;
-    // Rows of a sequence, on average.
-    const bool many = type != MFR_KV_F32 && rows > 32 * sequences;
+    // By the rows of a sequence, on average. 32 sequences of up to 4096 tokens, 8 heads of 128, us in tiles
+    // of 16, 32 and 128 rows, bf16 (8 bits): 16 rows 83, 88, 202 (60, 74, 202); 24 rows 120, 94, 202 (94, 80,
+    // 202); 64 rows 248, 167, 221 (183, 148, 228); 96 rows -, 225, 241 (-, 189, 244); 128 rows -, 317, 263
+    // (-, 275, 264).
+    const bool many = type != MFR_KV_F32 && rows > 96 * sequences;
     w.tile_rows = many ? mfr::paged::kManyRows : rows <= 16 * sequences ? 16 : 32;
     w.unit = many || type == MFR_KV_F32 ? 64 : 128;
     const int64_t tokens =
