@@ -21,9 +21,10 @@ constexpr const char* kOpNames[] = {
     "matmul",  "gelu",     "where",       "bias_add", "argmax", "gemm_strided_batched",
     "uniform", "normal",   "softmax",     "gemm",    "strided_copy", "attention",
     "dot",     "sub",      "rms_norm",    "quantize_f8", "gemm_f8",
+    "rope",    "kv_append", "attention_paged",
 };
 constexpr std::size_t kOpCount = sizeof(kOpNames) / sizeof(kOpNames[0]);
-static_assert(kOpCount == static_cast<std::size_t>(OpId::GemmF8) + 1, "a name for every op");
+static_assert(kOpCount == static_cast<std::size_t>(OpId::AttentionPaged) + 1, "a name for every op");
 
 constexpr std::size_t kDeviceTypeCount = static_cast<std::size_t>(DeviceType::ROCm) + 1;
 constexpr std::size_t kDTypeCount = static_cast<std::size_t>(DType::Bool) + 1;

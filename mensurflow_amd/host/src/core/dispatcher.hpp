@@ -7,7 +7,8 @@
 //   StridedCopy  packs a strided view on its own device, for Tensor::contiguous();
 //   Attention    fused scaled dot-product attention (mask, causal).
 // And three of the 8-bit serving path, which mensurflow has no counterpart of: RmsNorm, QuantizeF8
-// (keyed by F32, their input) and GemmF8 (keyed by U8, its values).
+// (keyed by F32, their input) and GemmF8 (keyed by U8, its values); and Rope, KvAppend and
+// AttentionPaged, a decoder's attention over a paged cache (keyed by F32, their first input).
 // A missing kernel is reported (NotImplemented); dispatch never moves an op to another device on
 // its own.
 #pragma once
@@ -50,7 +51,10 @@ enum class OpId {
     Sub,
     RmsNorm,
     QuantizeF8,
-    GemmF8
+    GemmF8,
+    Rope,
+    KvAppend,
+    AttentionPaged
 };
 
 // "gemm_strided_batched", "bias_add", ...: the name errors and tuning results use.
@@ -81,6 +85,8 @@ inline bool operator==(const TuningConfig& a, const TuningConfig& b) {
     return a.size == b.size && a.values == b.values;
 }
 inline bool operator!=(const TuningConfig& a, const TuningConfig& b) { return !(a == b); }
+
+struct KvArgs;
 
 // One call's operands and scalars. Ops validate before they dispatch, so a kernel may take the
 // shapes as agreeing and every tensor as living on its device.
@@ -114,6 +120,8 @@ struct OpArgs {
     bool f8_out = false;  // the result is in 8 bits
     int block_rows = 1;
     std::int64_t columns = 0;
+    // Rope, KvAppend and AttentionPaged: the rest of their arguments (core/kv_args.hpp), alive for the call.
+    const KvArgs* kv = nullptr;
     TuningConfig tuning{}; // filled by dispatch() from an active tuning scope
 };
 

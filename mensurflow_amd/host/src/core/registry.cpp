@@ -25,6 +25,7 @@ constexpr BackendHook kHooks[] = {
     {register_cpu_backend, false},
     {register_rocm_backend, true},
     {register_rocm_f8, true},
+    {register_rocm_kv, true},
 };
 
 } // namespace
