@@ -499,7 +499,7 @@ template <int TYPE, int D>
 __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>& acc, Running& run,
                                                const Reader<TYPE, D>& from, float rest, int32_t first,
                                                bool edge, int there) {
-    if (edge) {
+    if (__builtin_expect(edge, 0)) {
         const int half = from.lane / 32;
         const int32_t left = run.seen - first - 32 * from.sub - 8 * half; // tokens of this half's
         Scales<TYPE> up;
@@ -529,7 +529,7 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
     // 2^7 below the maximum then: fp16 holds weights up to 2^15.
     constexpr float kBelow = TYPE == MFR_KV_F8 ? 7.0f : 0.0f;
     most = max_halves(most) - kBelow;
-    if (__any(most > run.top + 8.0f)) {
+    if (__builtin_expect(__any(most > run.top + 8.0f), 0)) {
         const float top = fmaxf(run.top, most);
         float shrink = run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top);
         asm volatile("" : "+v"(shrink)); // no products with it ahead of the branch
@@ -658,7 +658,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
                 Shared<D>& other = tiles[buffer];
                 const bool edge = first + kKeys > group_all || there != kAllThere;
                 const Reader<TYPE, D> low{tile, 0, lane}, high{tile, 1, lane}, ahead{other, 0, lane};
-                if (first + 2 * kKeys > group_all || there_next != kAllThere) {
+                if (__builtin_expect(first + 2 * kKeys > group_all || there_next != kAllThere, 0)) {
                     loader.settle(values, other);
                 }
                 float reference =
