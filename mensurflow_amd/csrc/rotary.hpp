@@ -19,7 +19,7 @@ struct Rotary {
     int32_t rot;
     int32_t pairs; // neighbours turn together
     float amplitude;
-    int32_t quads; // no four columns of a piece straddle a half's, the turned part's or the head's end
+    int32_t quads; // a piece is whole quads of columns, at multiples of 4
     double turns[kMostPairs]; // a position, in whole turns
 };
 
@@ -36,7 +36,7 @@ inline Rotary checked(const mfr_rotary& r, int64_t d, const char* what) {
     out.rot = r.rot;
     out.pairs = r.layout == MFR_ROTARY_PAIRS;
     out.amplitude = r.amplitude;
-    out.quads = d % 4 == 0 && r.rot % (out.pairs != 0 ? 4 : 8) == 0;
+    out.quads = d % 4 == 0 && (out.pairs != 0 || r.rot % 8 == 0);
     for (int i = 0; i < r.rot / 2; ++i) {
         require(std::abs(r.steps[i]) <= 1e6, at + "has steps past 10^6 or not finite");
         out.turns[i] = r.steps[i] / 6.283185307179586476925;
@@ -85,7 +85,8 @@ __device__ inline void fill_angles(const Rotary& r, int64_t position, bool backw
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 }
 
-// na columns of a head from a on, and nb from b on (each up to 4, nb perhaps 0).
+// na columns of a head from a on, and nb from b on (each up to 4, nb perhaps 0). Where pieces are whole quads
+// (Rotary::quads) a quad is taken whole if it has any of them: what does not turn is written as it was.
 struct Piece {
     int32_t a, b, na, nb;
     int32_t angles; // from here on are its pairs'; -1: nothing turns
@@ -147,9 +148,9 @@ __device__ inline Numbers turned_piece(const Numbers& v, const Piece& p, const R
     if (r.pairs != 0) {
         const bool a = p.a < r.rot, b = p.b < r.rot;
         const Pair p0 = turned(v.a.x, v.a.y, t[0], a);
-        const Pair p1 = turned(v.a.z, v.a.w, t[1], QUADS ? a : p.a + 2 < r.rot);
+        const Pair p1 = turned(v.a.z, v.a.w, t[1], p.a + 2 < r.rot);
         const Pair p2 = turned(v.b.x, v.b.y, t[2], b);
-        const Pair p3 = turned(v.b.z, v.b.w, t[3], QUADS ? b : p.b + 2 < r.rot);
+        const Pair p3 = turned(v.b.z, v.b.w, t[3], p.b + 2 < r.rot);
         return {make_float4(p0.own, p0.other, p1.own, p1.other),
                 make_float4(p2.own, p2.other, p3.own, p3.other)};
     }
