@@ -249,16 +249,18 @@ struct TileAt {
     bool there; // their page is one of the cache's; another one's place is given otherwise
 };
 
-// The pages of a sequence (or the prefix), and one head of them.
+// The pages of a sequence (or the prefix), and one head of them, for the tokens in front of `last`: loads that
+// run ahead of the work's end get the last 16 of those again, from a cache (one query against 4096 tokens
+// read 32 MiB of 16 without this).
 struct Pages {
     const int32_t* table;
-    int32_t most; // the first token of the last 16 that hold some
+    int32_t most; // the first token of the last 16
     int32_t head;
 
-    __device__ __forceinline__ Pages(const Params& p, const Shape& shape, int32_t seq, int32_t head)
+    __device__ __forceinline__ Pages(const Params& p, int32_t last, int32_t seq, int32_t head)
         : table(p.work.shared != 0 ? p.work.batch.prefix_pages
                                    : p.work.batch.table + seq * p.work.batch.table_rs),
-          most((shape.tokens - 1) & ~15), head(head) {}
+          most((last - 1) & ~15), head(head) {}
 
     // The number of the page of 16 tokens; ones behind the last are taken as the last.
     __device__ __forceinline__ int32_t page(const Params& p, int32_t token) const {

@@ -532,11 +532,11 @@ __global__ __launch_bounds__(kThreads, (per_unit(TYPE, D, 16 * RT))) void attent
             }
         }
         const Segment<TYPE, D, FULL> segment(p, lanes, item.head);
-        const Pages pages(p, shape, seq, item.head);
         // This wavefront's tokens: a step of every unit.
         constexpr int kUnit = kWaves * F::kKeys;
         int32_t first = item.first * kUnit + wave * F::kKeys;
         const int32_t last = min(some_see, (item.first + units) * kUnit);
+        const Pages pages(p, last, seq, item.head);
         if (first < last) {
             Tiles<TYPE, D> tiles;
             Keys<TYPE, D> keys;

@@ -602,7 +602,7 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
         int32_t first = item.first * kKeys;
         const int32_t last = min(group_some, (item.first + units) * kKeys);
         if (first < last) {
-            const Pages pages(p, shape, seq, item.head);
+            const Pages pages(p, last, seq, item.head);
             const Loader<TYPE, D> loader(p, shape, pages, wave, lane);
             typename Loader<TYPE, D>::Numbers numbers = loader.numbers(first);
             StagedKeys<TYPE, D> keys;
