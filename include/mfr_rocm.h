@@ -614,7 +614,7 @@ typedef struct mfr_kv_cache {
  * lies in page table[s * table_rs + j / page_size]. In front of every sequence stand the `prefix` tokens
  * of the pages prefix_pages[0 ..] that all share (0: none); places and lengths do not count them.
  *
- * Rows of no sequence (behind the last, say) are neither read nor written. starts outside 0 .. rows, and
+ * Rows of no sequence (behind the last, say) are not written, and may hold anything. starts outside 0 .. rows, and
  * ends before their start, are taken as the nearest that are not. A length below 0 counts as 0, one past
  * width * page_size as that; a place below 0 or past that has no token. A page number outside
  * 0 .. pages - 1 is no page: nothing is written there, and its tokens count as absent. */
@@ -665,8 +665,8 @@ int mfr_kv_append(mfr_stream_t stream, const mfr_kv_append_desc* desc);
  * counted; over the prefix the rows of all sequences), e4m3 caches go through the fp16 ones in two parts: a
  * number of a query is held to 2^-22 of itself or 2^-39 of the query's largest then, a weight times its
  * value's scale to 2^-22 or 2^-31 of the row's largest, less under scales below 2^-96. What lies in the cache behind a sequence's tokens, or is not seen by a row,
- * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, leaves outputs of
- * that row NaN or infinite, of no other row.
+ * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, may leave outputs of
+ * that row NaN or infinite, of no other row (a score of -infinity is a weight of 0).
  *
  * The work is cut over the chip by the lengths, as the kernels find them; the same call gives the same
  * bits. Partial results go through a workspace of mfr_attention_paged_workspace() bytes: `workspace`

@@ -220,7 +220,7 @@ template <int TYPE, int D> struct Loader {
             // No further down, so that a weight over its value's scale stays inside fp32: values under a
             // scale of 2^-96 lose bits.
             to.scales[3 - which][16 * wave + lane % 16] =
-                fmaxf(__builtin_amdgcn_logf(from.scale), -96.0f);
+                fmaxf(__builtin_amdgcn_logf(fabsf(from.scale)), -96.0f);
         }
     }
 

@@ -98,6 +98,33 @@ def test_many_rows_before_a_token_of_no_number(stream, held, which, bad, in_valu
         assert not np.isfinite(got[sees]).all(axis=-1).any()
 
 
+@pytest.mark.parametrize("counts", [MANY, [(1, 300), (3, 40)]])
+def test_scales_of_any_sign(stream, counts):
+    """A cache that another program filled may have scales below 0, and rows of zeros a scale of 0."""
+    rng = np.random.default_rng(22)
+    p, q = case(rng, stream, counts, 2, 2, 64, "e4m3", prefix=40)
+    for scales in (p.ks, p.vs):
+        scales *= rng.choice(np.float32([-1, 1, 1, 0]), scales.shape)
+    check(p, q, run(p, q))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -90, 2.0 ** 100])
+@pytest.mark.parametrize("counts", [MANY, [(1, 300), (3, 40)]])
+def test_small_and_large_values(stream, counts, scale):
+    """Values under one small or large scale, some rows of zeros among them."""
+    rng = np.random.default_rng(23)
+    p, q = case(rng, stream, counts, 2, 2, 64, "e4m3", prefix=40)
+    seen = np.isfinite(p.vs)
+    p.vs[seen] = scale
+    p.v[np.logical_and(seen, rng.random(seen.shape) < 0.2)] = 0
+    if scale < 2.0 ** -96:      # parts of weights under fp16's least number: those values lose bits
+        got, (want, _) = run(p, q), p.attend(q)
+        there = ~np.isnan(want)
+        assert np.all(np.abs(got[there]) <= 448 * scale)
+        return
+    check(p, q, run(p, q))
+
+
 @pytest.mark.parametrize("held", HELD)
 def test_many_sequences(stream, held):
     """More sequences than a workgroup looks at together, most of them empty, and one long one."""
