@@ -368,6 +368,28 @@ __device__ inline Place find(const Work& w, int32_t groups, At at) {
     return {uniform(p.total), uniform(p.chunk), uniform(p.seq), uniform(p.base)};
 }
 
+// Moves on to the next sequence that has units; false where there is none. Those that follow without rows (a
+// batch of slots may hold many) are passed 64 at a time.
+__device__ inline bool advance(const Work& w, int32_t& seq, Shape& shape) {
+    if (++seq >= kv::sequences_of(w)) {
+        return false;
+    }
+    shape = kv::shape_of(w, seq);
+    while (shape.count == 0) {
+        const int32_t s = seq + 1 + static_cast<int32_t>(threadIdx.x % 64);
+        const uint64_t found =
+            __ballot(s < kv::sequences_of(w) && kv::shape_of(w, s).count > 0);
+        seq += found != 0 ? 1 + __builtin_ctzll(found) : 64;
+        if (seq >= kv::sequences_of(w) - 1 && found == 0) {
+            return false;
+        }
+        if (found != 0) {
+            shape = kv::shape_of(w, seq);
+        }
+    }
+    return true;
+}
+
 // exp2(m - top), 0 for a part that saw nothing (m = -inf, also where every part did).
 __device__ inline float part_weight(float m, float top) {
     return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);

@@ -497,7 +497,9 @@ __global__ __launch_bounds__(kThreads, (per_unit(TYPE, D, 16 * RT))) void attent
     for (int64_t at = begin; at < end;) {
         while (at >= base + shape.count) { // the next sequence that has units
             base += shape.count;
-            shape = mfr::kv::shape_of(p.work, ++seq);
+            if (!dev::advance(p.work, seq, shape)) {
+                return; // (lengths that changed meanwhile)
+            }
         }
         const Item item = mfr::kv::item_of(shape, base, at);
         const int64_t item_end = item.begin + shape.units;
@@ -515,6 +517,23 @@ __global__ __launch_bounds__(kThreads, (per_unit(TYPE, D, 16 * RT))) void attent
         const int32_t all_see = mfr::kv::seen_by(shape, row0 / p.work.group, p.causal != 0);
         const int32_t some_see = mfr::kv::seen_by(
             shape, (min(row0 + 16 * RT, rows) - 1) / p.work.group, p.causal != 0);
+        const Segment<TYPE, D, FULL> segment(p, lanes, item.head);
+        // This wavefront's tokens: a step of every unit.
+        constexpr int kUnit = kWaves * F::kKeys;
+        int32_t first = item.first * kUnit + wave * F::kKeys;
+        const int32_t last = min(some_see, (item.first + units) * kUnit);
+        const Pages pages(p, last, seq, item.head);
+        // Page numbers are read a step before they are used.
+        int32_t numbers[F::kTiles];
+        const auto numbers_of = [&](int32_t token) {
+#pragma unroll
+            for (int t = 0; t < F::kTiles; ++t) {
+                numbers[t] = pages.page(p, token + 16 * t);
+            }
+        };
+        if (first < last) {
+            numbers_of(first);
+        }
         // (What is in LDS of the item before was read before the barriers at its end.)
         constexpr bool kLds = kQueriesInLds<TYPE, D, RT>;
         std::conditional_t<kLds, int, Queries<TYPE, D, RT>> own;
@@ -537,31 +556,16 @@ __global__ __launch_bounds__(kThreads, (per_unit(TYPE, D, 16 * RT))) void attent
                 acc[rt][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
             }
         }
-        const Segment<TYPE, D, FULL> segment(p, lanes, item.head);
-        // This wavefront's tokens: a step of every unit.
-        constexpr int kUnit = kWaves * F::kKeys;
-        int32_t first = item.first * kUnit + wave * F::kKeys;
-        const int32_t last = min(some_see, (item.first + units) * kUnit);
-        const Pages pages(p, last, seq, item.head);
         if (first < last) {
             Tiles<TYPE, D> tiles;
             Keys<TYPE, D> keys;
             Values<TYPE, D> values;
-            // Page numbers are read a step before they are used.
-            int32_t numbers[F::kTiles];
-            const auto numbers_of = [&](int32_t token) {
-#pragma unroll
-                for (int t = 0; t < F::kTiles; ++t) {
-                    numbers[t] = pages.page(p, token + 16 * t);
-                }
-            };
             const auto tiles_of = [&](int32_t token) {
 #pragma unroll
                 for (int t = 0; t < F::kTiles; ++t) {
                     tiles[t] = pages.at(p, token + 16 * t, numbers[t]);
                 }
             };
-            numbers_of(first);
             tiles_of(first);
             numbers_of(first + kUnit);
             segment.load_keys(keys, tiles);

@@ -576,7 +576,9 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
     for (int64_t at = begin; at < end;) {
         while (at >= base + shape.count) { // the next sequence that has units
             base += shape.count;
-            shape = mfr::kv::shape_of(p.work, ++seq);
+            if (!dev::advance(p.work, seq, shape)) {
+                return; // (lengths that changed meanwhile)
+            }
         }
         const Item item = mfr::kv::item_of(shape, base, at);
         const int64_t item_end = item.begin + shape.units;

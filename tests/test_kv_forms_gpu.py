@@ -136,6 +136,46 @@ def test_many_sequences(stream, held):
 
 
 @pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("rows", [1, 150])
+def test_slots_without_rows(stream, held, rows):
+    """Thousands of slots, of which few have rows."""
+    rng = np.random.default_rng(24)
+    counts = [(0, 0)] * 5000
+    for s in (0, 1, 70, 2500, 2565, 4999):
+        counts[s] = (rows, rows + 20)
+    p, q = case(rng, stream, counts, 1, 2, 32, held, front=1, behind=1)
+    check(p, q, run(p, q))
+    k, v = (rng.standard_normal((p.rows, 1, 32)).astype(np.float32) for _ in range(2))
+    cache, batch = p.cache(), p.batch()
+    mf.kv_append(cache, batch, dev(k, stream), dev(v, stream))
+    got = cache.v.numpy()
+    values, _ = ref.rows_to_held(v, held)
+    for s in (0, 1, 70, 2500, 2565, 4999):
+        for i in (0, rows - 1):
+            place = 20 + i
+            assert np.array_equal(got[p.table[s, place // 16], :, place % 16], values[p.starts[s] + i])
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("pages", [0, 3])
+def test_no_room(stream, held, pages):
+    """No pages, or tables without entries: nothing is written, nothing is seen, queries are turned."""
+    rng = np.random.default_rng(25)
+    cache = mf.KvCache.empty(pages, 16, 2, 32, stream, ref.HELD[held])
+    batch = mf.KvBatch(dev(np.array([3, 9], np.int32), stream),
+                       mf.DeviceArray.empty((2, 0 if pages else 1), stream, np.int32),
+                       starts=dev(np.array([0, 3, 200], np.int32), stream))
+    k, v = (rng.standard_normal((200, 2, 32)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((200, 4, 32)).astype(np.float32)
+    rot = mf.rotary(32)
+    turned = mf.kv_append(cache, batch, dev(k, stream), dev(v, stream), rotary=rot, q=dev(q, stream))
+    places = np.concatenate((np.arange(3), 9 - 197 + np.arange(197)))
+    want, off = ref.turn(q, places, ref.steps(32), mf.ROTARY_HALVES)
+    assert np.all(np.abs(turned.numpy() - want) <= off)
+    assert not mf.attention_paged(turned, cache, batch).numpy().any()
+
+
+@pytest.mark.parametrize("held", HELD)
 def test_a_page_of_several_sequences(stream, held):
     """Tables may name a page more than once, in one sequence and in several."""
     rng = np.random.default_rng(14)
