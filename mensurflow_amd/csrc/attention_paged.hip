@@ -42,7 +42,7 @@ Launch launch_of(Params p, int32_t type, int shared, int cus) {
     // (-, 275, 264).
     const bool many = type != MFR_KV_F32 && rows > 96 * sequences;
     w.tile_rows = many ? mfr::paged::kManyRows : rows <= 16 * sequences ? 16 : 32;
-    w.unit = many || type == MFR_KV_F32 ? 64 : 128;
+    w.unit = many || type == MFR_KV_F32 ? 64 : 128; // a workgroup's step
     const int64_t tokens =
         shared != 0 ? w.batch.prefix : static_cast<int64_t>(mfr::kv::capacity_of(w.batch));
     const int64_t units = std::max<int64_t>(1, (tokens + w.unit - 1) / w.unit);

@@ -161,27 +161,16 @@ inline void check_heads(const float* p, int64_t ts, int64_t hs, int64_t rows, in
     }
 }
 
-#if defined(__HIP_DEVICE_COMPILE__) || defined(__HIPCC__)
+#if defined(__HIPCC__)
 namespace dev {
 
-// sequence_of for a row that a whole wavefront has, 64 starts at a time: one step for up to 64 sequences.
-__device__ inline int32_t sequence_of_wave(const Batch& b, int32_t row) {
-    if (b.starts == nullptr) {
-        return row / b.each;
-    }
-    const int32_t lane = threadIdx.x % 64;
-    int32_t low = 0, count = b.sequences;
-    while (count > 1) {
-        const int32_t step = (count - 1) / 64 + 1;
-        const int32_t at = lane * step; // 64 * 2^18 at most
+// standing_of for a row that a whole wavefront has, 64 starts at a time: one step for up to 64 sequences.
+__device__ inline Standing standing_of_wave(const Batch& b, int32_t row) {
+    return standing_of(b, row, [&](int32_t low, int32_t step, int32_t count) -> int32_t {
+        const int32_t at = static_cast<int32_t>(threadIdx.x % 64) * step; // 64 * 2^18 at most
         const uint64_t after = ~__ballot(at < count && b.starts[low + at] <= row);
-        const int32_t before = after != 0 ? __builtin_ctzll(after) : 64;
-        const int32_t skip = before > 1 ? (before - 1) * step : 0;
-        low += skip;
-        count = min(step, count - skip);
-    }
-    const Span span = span_of(b, low);
-    return row >= span.first && row - span.first < span.count ? low : -1;
+        return after != 0 ? __builtin_ctzll(after) : 64;
+    });
 }
 
 } // namespace dev

@@ -46,33 +46,45 @@ MFR_KV_BOTH Span span_of(const Batch& b, int32_t s) {
     return {first, within(b.starts[s + 1], first, b.rows) - first};
 }
 
-// The tokens of sequence s that its table has room for.
-MFR_KV_BOTH int32_t length_of(const Batch& b, int32_t s) {
-    return within(b.lengths[s], 0, capacity_of(b));
+// The tokens of a sequence that its table has room for.
+MFR_KV_BOTH int32_t tokens_of(const Batch& b, int32_t length) {
+    return within(length, 0, capacity_of(b));
 }
 
 // The place of a sequence's first row of `count`: below 0, or past the table, it has none.
-MFR_KV_BOTH int64_t first_place(const Batch& b, int32_t s, int32_t count) {
-    return static_cast<int64_t>(b.lengths[s]) - count;
+MFR_KV_BOTH int64_t first_place(int32_t length, int32_t count) {
+    return static_cast<int64_t>(length) - count;
 }
 
-// The sequence of a row, -1 if it has none.
-MFR_KV_BOTH int32_t sequence_of(const Batch& b, int32_t row) {
+// Where a row stands: its sequence (-1: none), that one's rows, and its length as it is in memory.
+struct Standing {
+    int32_t seq;
+    Span span;
+    int32_t length;
+};
+
+// `leading(low, step, count)`: of the starts low, low + step, low + 2 step, ... in front of low + count, 64 at
+// most, how many are at or before the row until the first that is not (a wavefront's ballot).
+template <typename Leading>
+MFR_KV_BOTH Standing standing_of(const Batch& b, int32_t row, Leading leading) {
+    int32_t low = 0;
     if (b.starts == nullptr) {
-        return row / b.each;
-    }
-    // The last sequence that starts at or before the row (empty ones of the same start come first).
-    int32_t low = 0, high = b.sequences;
-    while (high - low > 1) {
-        const int32_t mid = low + (high - low) / 2;
-        if (b.starts[mid] <= row) {
-            low = mid;
-        } else {
-            high = mid;
+        low = row / b.each;
+    } else {
+        // The last sequence that starts at or before the row (empty ones of the same start come first).
+        int32_t count = b.sequences;
+        while (count > 1) {
+            const int32_t step = (count - 1) / 64 + 1;
+            const int32_t before = leading(low, step, count);
+            const int32_t skip = before > 1 ? (before - 1) * step : 0;
+            low += skip;
+            count = step < count - skip ? step : count - skip;
         }
     }
+    const int32_t length = b.lengths[low]; // under way with the starts
     const Span span = span_of(b, low);
-    return row >= span.first && row - span.first < span.count ? low : -1;
+    const bool here = row >= span.first && row - span.first < span.count;
+    return {here ? low : -1, span, length};
 }
 
 // A page number that the cache has, or -1.

@@ -44,8 +44,8 @@ MFR_KV_BOTH Shape shape_of(const Work& w, int32_t s) {
     } else {
         const int32_t length = w.batch.lengths[s]; // under way with the starts
         p.span = span_of(w.batch, s);
-        p.tokens = within(length, 0, capacity_of(w.batch));
-        p.first_place = static_cast<int64_t>(length) - p.span.count;
+        p.tokens = tokens_of(w.batch, length);
+        p.first_place = first_place(length, p.span.count);
     }
     p.tiles = (p.span.count * w.group + w.tile_rows - 1) / w.tile_rows;
     p.units = p.tokens > 0 ? (p.tokens - 1) / w.unit + 1 : 1;

@@ -252,14 +252,13 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendParams p) {
             }
             if (!found) {
                 found = true;
-                const int32_t seq = mfr::kv::dev::sequence_of_wave(p.batch, row);
-                if (seq < 0) {
+                const mfr::kv::Standing at_row = mfr::kv::dev::standing_of_wave(p.batch, row);
+                if (at_row.seq < 0) {
                     break;
                 }
-                const mfr::kv::Span span = mfr::kv::span_of(p.batch, seq);
-                const int64_t place =
-                    mfr::kv::first_place(p.batch, seq, span.count) + (row - span.first);
-                page = mfr::kv::page_of(p.batch, seq, place);
+                const int64_t place = mfr::kv::first_place(at_row.length, at_row.span.count) +
+                                      (row - at_row.span.first);
+                page = mfr::kv::page_of(p.batch, at_row.seq, place);
                 slot = place & ((1 << p.cache.page_log2) - 1);
                 if (p.rotary.rot > 0) {
                     const int64_t position = p.positions != nullptr ? p.positions[row]
