@@ -668,10 +668,10 @@ int mfr_kv_append(mfr_stream_t stream, const mfr_kv_append_desc* desc);
  * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, may leave outputs of
  * that row NaN or infinite, of no other row (a score of -infinity is a weight of 0).
  *
- * The work is cut over the chip by the lengths, as the kernels find them; the same call gives the same
- * bits. Partial results go through a workspace of mfr_attention_paged_workspace() bytes: `workspace`
- * (16-byte aligned; calls that overlap in time need one each), or the stream's where it is NULL. A
- * captured call needs one of its own: MFR_E_INVALID otherwise. */
+ * out shares no memory with the other arrays. The work is cut over the chip by the lengths, as the kernels
+ * find them; the same call gives the same bits. Partial results go through a workspace of
+ * mfr_attention_paged_workspace() bytes: `workspace` (16-byte aligned; calls that overlap in time need one
+ * each), or the stream's where it is NULL. A captured call needs one of its own: MFR_E_INVALID otherwise. */
 typedef struct mfr_attention_paged_desc {
     mfr_kv_cache cache;
     mfr_kv_batch batch;

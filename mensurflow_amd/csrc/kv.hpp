@@ -29,6 +29,11 @@ constexpr int64_t kMostPages = (int64_t{1} << 31) - 1;
 constexpr int64_t kMostTokenStride = int64_t{1} << 24; // bytes: a page's 32768 rows have 2^39
 constexpr int64_t kMostStride = int64_t{1} << 40;
 
+// Whether `count` steps of a stride stay inside 2^56 elements, and so inside 64 bits.
+inline bool reaches(int64_t stride, int64_t count) {
+    return stride == 0 || count - 1 <= (int64_t{1} << 56) / stride;
+}
+
 inline int64_t type_bytes(int32_t type) {
     return type == MFR_KV_F32 ? 4 : type == MFR_KV_BF16 ? 2 : 1;
 }
@@ -56,6 +61,8 @@ inline Cache checked(const mfr_kv_cache& d, bool written, const char* what) {
     supported(d.token_stride <= kMostTokenStride / bytes && d.page_stride <= kMostStride / bytes &&
                   d.head_stride <= kMostStride / bytes,
               at + "has strides that are too long");
+    supported(reaches(d.page_stride, d.pages) && reaches(d.head_stride, d.heads),
+              at + "reaches further than memory");
     require(d.pages == 0 || (d.k != nullptr && d.v != nullptr), at + "has a null pointer");
     supported(aligned16(d.k) && aligned16(d.v) && d.page_stride * bytes % 16 == 0 &&
                   d.token_stride * bytes % 16 == 0 && d.head_stride * bytes % 16 == 0,
@@ -152,6 +159,7 @@ inline void check_heads(const float* p, int64_t ts, int64_t hs, int64_t rows, in
     require(p != nullptr, at + " is null");
     require(ts >= 0 && hs >= 0, at + " has negative strides");
     supported(ts <= kMostStride && hs <= kMostStride, at + " has strides that are too long");
+    supported(reaches(ts, rows) && reaches(hs, heads), at + " reaches further than memory");
     if (written) {
         const auto apart = [&](int64_t inner, int64_t count, int64_t outer, int64_t others) {
             return (count == 1 || inner >= d) &&

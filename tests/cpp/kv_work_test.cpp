@@ -141,7 +141,8 @@ void cuts() {
                    width,             4,         100,   nullptr,       static_cast<int32_t>(gen() % 200)};
         w.heads = 1 + gen() % 3;
         w.group = 1 + gen() % 5;
-        w.tile_rows = gen() % 2 != 0 ? 16 : 32;
+        const int32_t rows_of_forms[] = {16, 32, 128};
+        w.tile_rows = rows_of_forms[gen() % 3];
         w.unit = gen() % 2 != 0 ? 64 : 16;
         w.shared = gen() % 4 == 0;
         walk(w, 1 + gen() % 40);

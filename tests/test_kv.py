@@ -118,6 +118,8 @@ ROPE = [
     (dict(out=1 << 20, out_ts=1000), abi.MFR_E_INVALID, "in place"),
     (dict(x_ts=(1 << 40) + 1), abi.MFR_E_UNSUPPORTED, "too long"),
     (dict(d=1 << 21), abi.MFR_E_UNSUPPORTED, "too large"),
+    (dict(rows=1 << 30, x_ts=1 << 40), abi.MFR_E_UNSUPPORTED, "further than memory"),
+    (dict(rows=1 << 30, out_ts=1 << 40), abi.MFR_E_UNSUPPORTED, "further than memory"),
     (dict(positions=None, first=(1 << 31) - 3), abi.MFR_E_INVALID, "2^31"),
     (dict(positions=None, first=-(1 << 31) - 1), abi.MFR_E_INVALID, "2^31"),
 ]
@@ -161,6 +163,8 @@ CACHE = [
     (dict(page_stride=-1), abi.MFR_E_INVALID, "negative"),
     (dict(token_stride=(1 << 24) + 16), abi.MFR_E_UNSUPPORTED, "too long"),
     (dict(head_stride=(1 << 40) + 16), abi.MFR_E_UNSUPPORTED, "too long"),
+    (dict(pages=1 << 30, page_stride=1 << 38), abi.MFR_E_UNSUPPORTED, "further than memory"),
+    (dict(heads=1 << 20, head_stride=1 << 38), abi.MFR_E_UNSUPPORTED, "further than memory"),
     (dict(k=None), abi.MFR_E_INVALID, "null"), (dict(v=None), abi.MFR_E_INVALID, "null"),
     (dict(k=(1 << 24) + 8), abi.MFR_E_UNSUPPORTED, "16-byte aligned rows"),
     (dict(token_stride=72), abi.MFR_E_UNSUPPORTED, "16-byte aligned rows"),
