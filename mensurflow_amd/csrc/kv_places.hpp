@@ -100,9 +100,4 @@ MFR_KV_BOTH int32_t page_of(const Batch& b, int32_t s, int64_t place) {
     return page_checked(b, b.table[s * b.table_rs + (place >> b.page_log2)]);
 }
 
-// The page of token `place` of the prefix, 0 <= place < prefix.
-MFR_KV_BOTH int32_t prefix_page_of(const Batch& b, int32_t place) {
-    return page_checked(b, b.prefix_pages[place >> b.page_log2]);
-}
-
 } // namespace mfr::kv

@@ -148,7 +148,7 @@ void any_values() {
                     "a row of its sequence");
         }
         for (int t = 0; t < prefix; ++t) {
-            const int32_t page = prefix_page_of(h.b, t);
+            const int32_t page = page_checked(h.b, h.prefix[t >> log2]);
             require(page >= -1 && page < pages, "a prefix page that the cache has");
         }
     }
