@@ -7,8 +7,7 @@
 #pragma once
 
 #include "common.hpp"
-
-#include <cmath>
+#include "rotary_angle.hpp"
 
 namespace mfr::rotary {
 
@@ -20,7 +19,7 @@ struct Rotary {
     int32_t pairs; // neighbours turn together
     float amplitude;
     int32_t quads; // a piece is whole quads of columns, at multiples of 4
-    double turns[kMostPairs]; // a position, in whole turns
+    double quarters[kMostPairs]; // of a turn, a position
 };
 
 // Checks a rotation of heads of d and takes it over.
@@ -39,7 +38,7 @@ inline Rotary checked(const mfr_rotary& r, int64_t d, const char* what) {
     out.quads = d % 4 == 0 && (out.pairs != 0 || r.rot % 8 == 0);
     for (int i = 0; i < r.rot / 2; ++i) {
         require(std::abs(r.steps[i]) <= 1e6, at + "has steps past 10^6 or not finite");
-        out.turns[i] = r.steps[i] / 6.283185307179586476925;
+        out.quarters[i] = quarters_of(r.steps[i]);
     }
     return out;
 }
@@ -53,34 +52,14 @@ inline int32_t pieces_of(const Rotary& r, int32_t columns) {
 
 namespace mfr::rotary::dev {
 
-// (cosine, sine) of position * turns whole turns: the distance to the nearest quarter of a turn is
-// taken in double and is at most pi / 4, where the Taylor series to x^10 and x^9 are 1e-9 off; the
-// quarter then chooses sign and place.
-__device__ inline float2 angle_of(double position, double turns) {
-    const double quarters = 4.0 * (position * turns);
-    const double whole = rint(quarters);
-    const float x = static_cast<float>(quarters - whole) * 1.57079632679489662f;
-    const int quarter = static_cast<int>(whole - 4.0 * floor(0.25 * whole));
-    const float z = x * x;
-    float s = fmaf(z, 2.75573192e-6f, -1.98412698e-4f);
-    s = fmaf(z, s, 8.33333333e-3f);
-    s = fmaf(z, s, -1.66666667e-1f);
-    s = fmaf(x * z, s, x);
-    float c = fmaf(z, -2.75573192e-7f, 2.48015873e-5f);
-    c = fmaf(z, c, -1.38888889e-3f);
-    c = fmaf(z, c, 4.16666667e-2f);
-    c = fmaf(z * z, c, fmaf(z, -0.5f, 1.0f));
-    const float a = (quarter & 1) != 0 ? s : c;
-    const float b = (quarter & 1) != 0 ? c : s;
-    return make_float2(quarter == 1 || quarter == 2 ? -a : a, quarter >= 2 ? -b : b);
-}
-
-// The angles of a token into the wavefront's `table` [rot / 2].
+// The angles of a token into the wavefront's `table` [rot / 2], times the amplitude, rounded once.
 __device__ inline void fill_angles(const Rotary& r, int64_t position, bool backward, float2* table) {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     for (int i = threadIdx.x % 64; i < r.rot / 2; i += 64) {
-        const float2 t = angle_of(static_cast<double>(position), r.turns[i]);
-        table[i] = make_float2(r.amplitude * t.x, r.amplitude * (backward ? -t.y : t.y));
+        const Angle t = angle_of(static_cast<double>(position), r.quarters[i]);
+        const double amplitude = r.amplitude;
+        table[i] = make_float2(static_cast<float>(amplitude * t.cosine),
+                               static_cast<float>(amplitude * (backward ? -t.sine : t.sine)));
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
 }
