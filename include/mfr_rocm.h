@@ -549,7 +549,8 @@ enum { MFR_ROTARY_HALVES = 0, MFR_ROTARY_PAIRS = 1 };
  *   (amplitude (a cos w - b sin w), amplitude (b cos w + a sin w)).
  *
  * Cosine and sine are taken in double, within 5e-12 + 1.8e-16 w, so that far positions keep their angle,
- * and rounded to fp32 with the amplitude. The columns from rot on stay as they are.
+ * and rounded to fp32 with the amplitude; each product with them and each sum is rounded to fp32 then.
+ * The columns from rot on stay as they are.
  * A plain struct in host memory, copied by the calls that take it. */
 typedef struct mfr_rotary {
     int32_t rot;

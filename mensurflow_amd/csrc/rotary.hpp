@@ -107,13 +107,13 @@ __device__ inline Numbers load_piece(const float* x, const Piece& p) {
     return {load_columns<QUADS>(x + p.a, p.na), load_columns<QUADS>(x + p.b, p.nb)};
 }
 
-// A pair turned, or as it is.
+// A pair turned, or as it is: each product and their sum rounded to fp32 as the formula stands, so that a key
+// next to a border between two numbers of a cache falls as it does for any other program in fp32.
 struct Pair {
     float own, other;
 };
 __device__ inline Pair turned(float own, float other, float2 t, bool turns) {
-    return {turns ? fmaf(own, t.x, -(other * t.y)) : own,
-            turns ? fmaf(other, t.x, own * t.y) : other};
+    return {turns ? own * t.x - other * t.y : own, turns ? other * t.x + own * t.y : other};
 }
 
 // Columns past the piece's stay zeros.
