@@ -714,6 +714,11 @@ def _arrays_of(what: str, *operands) -> tuple:
     return arrays
 
 
+def _same_stream(a: Stream, b: Stream) -> bool:
+    """Whether work on a and on b runs in order: one Stream, or two that wrap one HIP stream."""
+    return a is b or (a.device == b.device and a.hip_stream() == b.hip_stream())
+
+
 def _same_device(what: str, stream: Stream, desc) -> None:
     if desc.held and desc.held[0].stream.device != stream.device:
         raise ValueError(f"{what}: a stream of another device than the operands'")
@@ -1084,11 +1089,15 @@ def kv_append(cache: KvCache, batch: KvBatch, k: DeviceArray, v: DeviceArray, *,
               q: DeviceArray | None = None, q_out: DeviceArray | None = None) -> DeviceArray | None:
     """The step's keys and values into the cache, the keys turned by `rotary`; the queries turned with
     them, in a new array or `q_out` (which may be q), where they are given. Rows of no sequence of a new
-    array are undefined."""
+    array are undefined. Runs on the stream of k, which has to be that of v, q and q_out; the cache and
+    the batch may be arrays of another one that this one has waited for."""
+    for name, t in (("v", v), ("q", q), ("q_out", q_out)):
+        if t is not None and not _same_stream(t.stream, k.stream):
+            raise ValueError(f"kv_append: {name} is on another stream than k")
     if q is not None and q_out is None:
-        q_out = DeviceArray.empty(q.shape, q.stream)
-    kv_append_run(cache.stream, kv_append_desc(cache, batch, k, v, rotary=rotary,
-                                               positions=positions, q=q, q_out=q_out))
+        q_out = DeviceArray.empty(q.shape, k.stream)
+    kv_append_run(k.stream, kv_append_desc(cache, batch, k, v, rotary=rotary, positions=positions, q=q,
+                                           q_out=q_out))
     return q_out
 
 
@@ -1141,7 +1150,7 @@ def attention_paged(q: DeviceArray, cache: KvCache, batch: KvBatch, *, scale: fl
                     workspace: DeviceArray | None = None) -> DeviceArray:
     """softmax(scale q k^T) v of each row's queries q [rows, q_heads, d] against the batch's shared
     prefix and its sequence's tokens up to the row's own (all of them where causal is False). Rows of
-    no sequence of a new array are undefined."""
+    no sequence of a new array are undefined. Runs on the stream of q."""
     if out is None:
         out = DeviceArray.empty(q.shape, q.stream)
     attention_paged_run(q.stream, attention_paged_desc(q, cache, batch, scale=scale, causal=causal,
