@@ -52,6 +52,11 @@ template <int D> struct Shared {
     float scales[4][kKeys];             // keys', values', log2 of the values', nothing
     uint32_t odd[kWaves];               // at edges: tokens of 16 with values that are no numbers
 };
+// Sums of 128 products of a query of up to 2^15 with numbers of up to 448 stay below 2^31: keys' scales are
+// taken times 2^-31, so that no finite one leads a score out of fp32's range before the query's power (and
+// this one) is taken back. (Below 2^-95 they lose bits: 2^-102 of the scale times a query's largest.)
+constexpr int kKeyPower = 31;
+constexpr float kKeyUnit = 0x1p-31f;
 constexpr int kAllThere = 15; // a bit for each 16 tokens whose page is one of the cache's
 
 // The numbers of the matrix cores: bf16 as it is, e4m3 as fp16.
@@ -107,6 +112,7 @@ template <int TYPE, int D> struct Loader {
     // From a tile's first token to the lane's piece of its keys (of 16 tokens' pieces) and values (of its
     // 16 tokens), and to the scales: 16 lanes of the keys', 16 of the values', and the same again.
     GlobalBytes keys, values, scales;
+    float unit; // of the scales that this lane loads
 
     __device__ __forceinline__ Loader(const Params& params, const Shape& of, const Pages& at, int w,
                                       int l)
@@ -118,6 +124,7 @@ template <int TYPE, int D> struct Loader {
         values = lane_address(p.cache.v + at.head * p.cache.head_stride,
                               8 * (lane / 32) * p.cache.token_stride +
                                   min(T::kValueBytes * (lane % (D / 4)), row_bytes - T::kValueBytes));
+        unit = (lane & 16) != 0 ? 1.0f : kKeyUnit;
         scales = lane_address((lane & 16) != 0 ? p.cache.v_scales : p.cache.k_scales, 4 * (lane % 16));
     }
 
@@ -216,7 +223,7 @@ template <int TYPE, int D> struct Loader {
                                                  Shared<D>& to) const {
         if constexpr (TYPE == MFR_KV_F8) {
             const int which = lane >> 4 & 1;
-            to.scales[which][16 * wave + lane % 16] = from.scale;
+            to.scales[which][16 * wave + lane % 16] = from.scale * unit;
             // No further down, so that a weight over its value's scale stays inside fp32: values under a
             // scale of 2^-96 lose bits.
             to.scales[3 - which][16 * wave + lane % 16] =
@@ -327,8 +334,9 @@ __device__ __forceinline__ float load_queries(Queries<TYPE, D>& to, const Params
         const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
         const int shift = max(-112, min(14 - exponent, 126));
         by = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-        // Above 0, so that scores of tokens that are not seen stay -infinity.
-        rest = fmaxf(fabsf(p.scale) / by, 0x1p-126f);
+        // Above 0, so that scores of tokens that are not seen stay -infinity. Queries past 2^112 meet the
+        // largest there is.
+        rest = fminf(fmaxf(ldexpf(fabsf(p.scale), kKeyPower - shift), 0x1p-126f), 0x1.fffffep127f);
         by = copysignf(by, p.scale);
     }
 #pragma unroll
