@@ -17,7 +17,7 @@
 //   - O^T += V^T P^T: those are the B operand, and the A operand is 8 neighbouring tokens of one column,
 //     which is how the values lie.
 // bf16 caches: three bf16 parts of queries and weights. e4m3 numbers are exact in fp16 too, whose parts
-// hold 11 bits, so two do: queries are brought to 2^15 by a power of two for each row, weights (with
+// hold 11 bits and a sign, so two hold 23: queries are brought to 2^15 by a power of two for each row, weights (with
 // the values' scales) by the softmax's reference, which is 2^15 below the largest of them.
 //
 // 4 x 512 queries of 8 x 4 heads of 128 on up to 8192 tokens in bf16: 500 us, 980 TFLOP/s of products (the
@@ -60,6 +60,7 @@ constexpr float kKeyUnit = 0x1p-31f;
 constexpr int kAllThere = 15; // a bit for each 16 tokens whose page is one of the cache's
 
 // The numbers of the matrix cores: bf16 as it is, e4m3 as fp16.
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
 template <int TYPE> constexpr int kParts = TYPE == MFR_KV_BF16 ? 3 : 2;
@@ -80,13 +81,17 @@ template <bool HIGH> __device__ __forceinline__ uint32_t widen_half(uint32_t w) 
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
 }
 
-// Two floats (up to 2^16) cut into two fp16 parts each, towards zero, so that none overflows.
+// Two floats (up to 2^15) cut into two fp16 parts each, both rounded to nearest (v_cvt_pk_f16_f32): what the
+// first leaves is up to 2^12 of fp32's last places, of either sign, and the second holds it to within one,
+// ties to even. (Cut towards zero, they were up to three last places off, and always below.)
+__device__ __forceinline__ halfx2 halves(float x, float y) {
+    return __builtin_convertvector((floatx2{x, y}), halfx2);
+}
 __device__ __forceinline__ void cut_halves(float x, float y, uint32_t& p0, uint32_t& p1) {
-    const halfx2 h = __builtin_bit_cast(halfx2, __builtin_amdgcn_cvt_pkrtz(x, y));
+    const halfx2 h = halves(x, y);
     p0 = __builtin_bit_cast(uint32_t, h);
-    p1 = __builtin_bit_cast(uint32_t,
-                            __builtin_amdgcn_cvt_pkrtz(fmaf(static_cast<float>(h[0]), -1.0f, x),
-                                                       fmaf(static_cast<float>(h[1]), -1.0f, y)));
+    p1 = __builtin_bit_cast(uint32_t, halves(fmaf(static_cast<float>(h[0]), -1.0f, x),
+                                             fmaf(static_cast<float>(h[1]), -1.0f, y)));
 }
 
 // A thread's share of a tile on its way from memory to LDS.
@@ -332,7 +337,7 @@ __device__ __forceinline__ float load_queries(Queries<TYPE, D>& to, const Params
         // A power of two, so that the largest gets the exponent 14; of 0, infinities and subnormal
         // numbers as near as there is one.
         const int exponent = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-        const int shift = max(-112, min(14 - exponent, 126));
+        const int shift = min(14 - exponent, 126);
         by = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
         // Above 0, so that scores of tokens that are not seen stay -infinity. Queries past 2^112 meet the
         // largest there is.

@@ -3,6 +3,8 @@ for few rows and for many."""
 import numpy as np
 import pytest
 
+import f8_reference as f8
+from kv_reference import Paged
 from test_attention_paged_gpu import case, check, run
 
 pytestmark = pytest.mark.gpu
@@ -28,3 +30,42 @@ def test_small_keys_under_large_queries(stream, counts, power):
     p.ks *= np.float32(2.0 ** -power)
     q *= np.float32(2.0 ** power)
     check(p, q, run(p, q), norm=False)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_queries_keep_their_bits(stream, d):
+    """Two tokens, each of one column: the weights say what the queries of many rows in 8 bits were taken as."""
+    rng = np.random.default_rng(d)
+    p = Paged(rng, stream, [(220, 2)] * 3, 2, d, "e4m3")
+    one = f8.VALUES.tolist().index(1.0)
+    for s in range(3):
+        for token in range(2):
+            at = p.table[s, 0], slice(None), token
+            p.k[at], p.v[at] = 0, 0
+            p.k[at][:, token], p.v[at][:, token] = one, one
+            p.ks[at], p.vs[at] = 1, 1
+    size = 2000.0                       # of the scores
+    q = np.zeros((p.rows, 4, d), np.float32)
+    q[..., 0] = size * (1 + rng.random(q.shape[:2]))
+    q[..., 1] = np.float32(q[..., 0].astype(np.float16))    # as it is in one part
+    got = run(p, q, scale=1.0, causal=False)
+    want, _ = p.attend(q, scale=1.0, causal=False)
+    # A last place of the number (2^-23 of up to 2 size), the difference's rounding, and those behind it.
+    off = 0.25 * (2.0 ** -23 + 2.0 ** -24) * 2 * size + 2.0 ** -21
+    error = got[..., 0].astype(np.float64) - want[..., 0]
+    assert np.abs(error).max() <= off
+    # Of either sign.
+    assert abs(error.mean()) <= off / 8
+
+
+def test_weights_keep_their_bits(stream):
+    """Rows that see one token give its value: off by the weight's parts, a product and a division."""
+    rng = np.random.default_rng(3)
+    p = Paged(rng, stream, [(110, 1)] * 40, 2, 64, "e4m3")
+    q = rng.standard_normal((p.rows, 4, 64)).astype(np.float32)
+    got = run(p, q, causal=False)
+    want, _ = p.attend(q, causal=False)
+    assert np.all(np.abs(got - want) <= (2.0 ** -23 + 4 * 2.0 ** -24) * np.abs(want))
+    # Each of 17600 weights off by up to a last place, of either sign; parts cut towards zero are 2e-8 below.
+    there = want != 0
+    assert abs(np.mean(got[there] / want[there] - 1)) <= 2.0 ** -24 / 6
