@@ -567,6 +567,78 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
     return reference;
 }
 
+// In 8 bits a weight's exponent is taken from a score before its last rounding, and the reference has one: past
+// 2^20 they no longer agree to the last places of a weight, past 2^24 not at all. The rows of far scores are
+// done again, a wavefront a row, in fp32 throughout: tokens `first` .. `last` - 1, a lane a token for scores, a
+// lane two columns for values: 300 us for 64 tokens of 128 rows, but no model is meant to have such scores.
+constexpr float kFar = 0x1p20f;
+
+template <int D>
+__device__ __forceinline__ void far_row(const Params& p, const Pages& pages, const float* q, int32_t first,
+                                        int32_t last, int lane, float* out) {
+    const uint8_t* const keys = p.cache.k + pages.head * p.cache.head_stride;
+    const uint8_t* const values = p.cache.v + pages.head * p.cache.head_stride;
+    float top = -INFINITY, sum = 0.0f, acc[2] = {0.0f, 0.0f};
+#pragma unroll 1
+    for (; first < last; first += 64) {
+        const int32_t token = min(first + lane, last - 1);
+        const int32_t page = mfr::kv::page_checked(p.work.batch, pages.table[token >> p.cache.page_log2]);
+        const int64_t number = max(page, 0);
+        const int32_t slot = token & ((1 << p.cache.page_log2) - 1);
+        const int64_t at = number * p.cache.page_stride + static_cast<int64_t>(slot) * p.cache.token_stride;
+        const int64_t scale_at = ((number * p.cache.heads + pages.head) << p.cache.page_log2) + slot;
+        float s = 0.0f;
+#pragma unroll 1
+        for (int c = 0; c < p.cache.d; c += 4) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(keys + at + c);
+            s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 0), q[c], s);
+            s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 1), q[c + 1], s);
+            s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 2), q[c + 2], s);
+            s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 3), q[c + 3], s);
+        }
+        s *= p.cache.k_scales[scale_at] * p.scale;
+        s = page >= 0 && first + lane < last ? s : -INFINITY;
+        float most = s;
+#pragma unroll
+        for (int step = 32; step > 0; step /= 2) {
+            most = fmaxf(most, __shfl_xor(most, step, 64));
+        }
+        most = fmaxf(most, top);
+        const float shrink = part_weight(top, most);
+        top = most;
+        const float weight = s == -INFINITY ? 0.0f : exp2_native(s - top);
+        sum = fmaf(sum, shrink, weight);
+        acc[0] *= shrink;
+        acc[1] *= shrink;
+        const float by = weight * p.cache.v_scales[scale_at];
+#pragma unroll 1
+        for (int j = 0; j < 64; ++j) {
+            const uint8_t* const row = values + __shfl(static_cast<long long>(at), j, 64);
+            const float w = __shfl(by, j, 64);
+            if (__shfl(weight, j, 64) == 0.0f) { // tokens that there are not, too
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const int c = lane + 64 * i;
+                const float v = c < p.cache.d ? __builtin_amdgcn_cvt_f32_fp8(row[c], 0) : 0.0f;
+                acc[i] = fmaf(w, v, acc[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int step = 32; step > 0; step /= 2) {
+        sum += __shfl_xor(sum, step, 64);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        out[lane + 64 * i] = acc[i];
+    }
+    if (lane == 0) {
+        *reinterpret_cast<float2*>(out + D) = make_float2(top, sum);
+    }
+}
+
 template <int TYPE, int D>
 __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Params p) {
     extern __shared__ uint4 lds[];
@@ -756,6 +828,27 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
         const bool whole = item.first == 0 && units == shape.units;
         const int64_t part0 = mfr::kv::part_of(index, place.chunk, item.begin) * kManyRows;
         const int32_t here = min(kManyRows, rows - row0);
+        if constexpr (TYPE == MFR_KV_F8) {
+            const auto far_at = [&](int32_t r) {
+                const float top = out[min(r, here - 1) * kPitch + D];
+                return fabsf(top) > kFar && top != -INFINITY;
+            };
+            if (__builtin_expect(__any(far_at(32 * wave + lane % 32)), 0)) {
+#pragma unroll 1
+                for (int32_t r = 32 * wave; r < min(32 * (wave + 1), here); ++r) {
+                    if (far_at(r)) { // the wavefront's own rows alone are read and written
+                        const int32_t i = (row0 + r) / p.work.group;
+                        const float* q = p.q.p + (shape.span.first + static_cast<int64_t>(i)) * p.q.ts +
+                                         (item.head * p.work.group + (row0 + r - i * p.work.group)) *
+                                             p.q.hs;
+                        const int32_t from = item.first * kKeys;
+                        const int32_t to = min(seen_at(row0 + r), (item.first + units) * kKeys);
+                        far_row<D>(p, Pages(p, to, seq, item.head), q, from, to, lane, out + r * kPitch);
+                    }
+                }
+            }
+            __syncthreads();
+        }
         constexpr int kLanes = D / 4;
 #pragma unroll 1
         for (int32_t r = threadIdx.x / kLanes; r < here; r += kThreads / kLanes) {

@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import f8_reference as f8
+import kv_reference as ref
 from kv_reference import Paged
 from test_attention_paged_gpu import case, check, run
 
@@ -69,3 +70,35 @@ def test_weights_keep_their_bits(stream):
     # Each of 17600 weights off by up to a last place, of either sign; parts cut towards zero are 2e-8 below.
     there = want != 0
     assert abs(np.mean(got[there] / want[there] - 1)) <= 2.0 ** -24 / 6
+
+
+@pytest.mark.parametrize("held", ["f32", "bf16", "e4m3"])
+@pytest.mark.parametrize("counts", [MANY, FEW])
+@pytest.mark.parametrize("power", [16, 20, 24, 26, 28, 30, 32, 36, 60, 100])
+@pytest.mark.parametrize("small", [1.0, 2.0 ** -90])
+def test_far_scores(stream, held, counts, power, small):
+    """Scores far from 0: rows whose largest one is apart from the next give its value."""
+    if small != 1.0 and held != "e4m3":
+        pytest.skip("no scales")
+    rng = np.random.default_rng(power)
+    p, q = case(rng, stream, counts, 2, 2, 64, held, prefix=40)
+    q *= np.float32(2.0 ** power)
+    if held == "e4m3":
+        p.vs *= np.float32(small) ** rng.integers(0, 2, p.vs.shape).astype(np.float32)
+    got = run(p, q)
+    looked = wrong = 0
+    for s, (n, tokens) in enumerate(p.counts):
+        k, v = p.tokens_of(s)
+        for i in range(n):
+            row, seen = p.starts[s] + i, p.prefix + max(0, min(tokens, tokens - n + i + 1))
+            for h in range(q.shape[1]):
+                kk, x = k[:seen, h // 2], q[row, h].astype(np.float64)
+                score = kk @ x / 8
+                # What fp32 may be off by (kv_reference.Paged.attend), for each of two scores.
+                off = 4 * ref.EPS32 * (72 * (np.abs(kk) @ np.abs(x)).max() / 8 + 4)
+                second, first = np.sort(score)[-2:]
+                if first - second > off + 90:       # and 2^-126 of another one's values
+                    want = v[score.argmax(), h // 2]
+                    wrong += not np.all(np.abs(got[row, h] - want) <= 2.0 ** -21 * np.abs(want) + 1e-37)
+                    looked += 1
+    assert looked > 0.5 * p.rows * q.shape[1] and wrong == 0, (looked, wrong)
