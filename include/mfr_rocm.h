@@ -665,8 +665,10 @@ int mfr_kv_append(mfr_stream_t stream, const mfr_kv_append_desc* desc);
  * through the fp32 ones. With more than 96 rows a sequence on average (query heads of one head of the cache
  * counted; over the prefix the rows of all sequences), e4m3 caches go through the fp16 ones in two parts: a
  * number of a query is held to 2^-23 of itself or 2^-39 of the query's largest then, a weight times its
- * value's scale to 2^-23 or 2^-32 of the row's largest, less under scales below 2^-96. What lies in the
- * cache behind a sequence's tokens, or is not seen by a row,
+ * value's scale to 2^-23 or 2^-32 of the row's largest, less under scales below 2^-96. Weighted values are
+ * summed before they are divided by the weights' sum, weights no more than 1 each (in those two parts, times
+ * the scale, relative to the row's largest). What lies in the cache behind a sequence's tokens, or is not
+ * seen by a row,
  * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, may leave outputs of
  * that row NaN or infinite, of no other row (a score of -infinity is a weight of 0).
  *

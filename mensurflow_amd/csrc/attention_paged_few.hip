@@ -317,11 +317,12 @@ __device__ __forceinline__ void softmax_step(Scores<TYPE, D, RT>& s,
                 most = fmaxf(most, s[rt][t][r]);
             }
         }
-        // Weights are taken against a reference that follows the maximum in steps: it moves, and the output
-        // so far with it, where the maximum has grown by more than 2^8, so that few steps do.
+        // Weights are taken against a reference that follows the maximum in steps, 2^7 above it where it
+        // moves, and the output so far with it: few steps do, and no weight is above 1. (Far scores, whose
+        // last place is 16, are then taken as their own reference.)
         most = row_max(most);
-        if (__any(most > run[rt].top + 8.0f)) {
-            const float top = fmaxf(run[rt].top, most);
+        if (__any(most > run[rt].top)) {
+            const float top = most > run[rt].top ? most + 7.0f : run[rt].top;
             float shrink = run[rt].top == -INFINITY ? 0.0f : exp2_native(run[rt].top - top);
             asm volatile("" : "+v"(shrink)); // no products with it ahead of the branch
             run[rt].top = top;

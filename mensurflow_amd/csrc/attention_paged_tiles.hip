@@ -544,9 +544,9 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
         run.sum = (sees & odd) != 0 ? NAN : run.sum;
     }
     // Weights are taken against a reference that follows the maximum in steps: it moves, and the output so
-    // far with it, where the maximum has grown by more than 2^8, so that few steps do. In 8 bits it is
-    // 2^7 below the maximum then: fp16 holds weights up to 2^15.
-    constexpr float kBelow = TYPE == MFR_KV_F8 ? 7.0f : 0.0f;
+    // far with it, where the maximum has grown by more than 2^8, so that few steps do. In bf16 it is 2^8
+    // above the maximum then, and no weight is above 1; in 8 bits 2^7 below: fp16 holds weights up to 2^15.
+    constexpr float kBelow = TYPE == MFR_KV_F8 ? 7.0f : -8.0f;
     most = max_halves(most) - kBelow;
     if (__builtin_expect(__any(most > run.top + 8.0f), 0)) {
         const float top = fmaxf(run.top, most);

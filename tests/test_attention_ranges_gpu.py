@@ -102,3 +102,46 @@ def test_far_scores(stream, held, counts, power, small):
                     wrong += not np.all(np.abs(got[row, h] - want) <= 2.0 ** -21 * np.abs(want) + 1e-37)
                     looked += 1
     assert looked > 0.5 * p.rows * q.shape[1] and wrong == 0, (looked, wrong)
+
+
+@pytest.mark.parametrize("held", ["f32", "bf16", "e4m3"])
+@pytest.mark.parametrize("counts", [[(110, 300)], [(1, 300)], [(20, 300)]])
+@pytest.mark.parametrize("rise", [0.0, 3.0, 7.5, 20.0])
+def test_large_values_under_rising_scores(stream, held, counts, rise):
+    """Values near 2^119 of 300 tokens, the later two thirds with 2^rise times the weight of the first."""
+    p = Paged(np.random.default_rng(5), stream, counts, 1, 64, held)
+    rng = np.random.default_rng(6)
+    k = np.zeros((300, 1, 64))
+    k[100:, 0, 0] = rise
+    v = 2.0 ** 119 * rng.uniform(0.5, 1.0, (300, 1, 64))
+    for numbers, scales, x in ((p.k, p.ks, k), (p.v, p.vs, v)):
+        p.fill(numbers, scales, x, p.table[0], 300)
+    q = np.zeros((p.rows, 2, 64), np.float32)
+    q[..., 0] = 8 * np.log(2)           # scale 1 / 8
+    got = run(p, q, causal=False)
+    want, bound = p.attend(q, causal=False)
+    assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("held", ["f32", "bf16", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 30])
+def test_large_values_under_rising_scores_in_several_steps(stream, held, rows):
+    """The same with so many tokens that each workgroup of a card of 256 compute units takes several steps."""
+    sequences, tokens, heads = 64, 3200, 4
+    p = Paged(np.random.default_rng(7), stream, [(rows, 1)] * sequences, heads, 64, held, page=64)
+    pages = tokens // 64
+    rng = np.random.default_rng(8)
+    k = np.zeros((pages, heads, 64, 64))
+    k[..., 0] = np.arange(tokens).reshape(pages, 1, 64) % 256 / 256 * 7.5
+    v = 2.0 ** 118 * rng.uniform(0.5, 1.0, (pages, heads, 64, 64))
+    (p.k, p.ks), (p.v, p.vs) = (ref.rows_to_held(x, held) for x in (k, v))
+    p.pages, p.width = pages, pages
+    p.table = np.tile(np.arange(pages, dtype=np.int32), (sequences, 1))
+    p.lengths[:] = tokens
+    q = np.zeros((p.rows, heads, 64), np.float32)
+    q[..., 0] = 8 * np.log(2)
+    got = run(p, q, causal=False)
+    p.counts = [(rows, tokens)]             # every sequence and row is the same
+    want, bound = p.attend(q[:rows], causal=False)
+    got = got.reshape(sequences, rows, heads, 64)
+    assert np.all(np.abs(got - want) <= bound)
