@@ -550,10 +550,15 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
     most = max_halves(most) - kBelow;
     if (__builtin_expect(__any(most > run.top + 8.0f), 0)) {
         const float top = fmaxf(run.top, most);
-        float shrink = run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(run.top - top);
+        // In 8 bits half of the step at a time: weights over small scales may be as large as steps to those of
+        // large scales are deep.
+        const float steps = TYPE == MFR_KV_F8 ? 0.5f : 1.0f;
+        float shrink = run.top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(steps * (run.top - top));
         asm volatile("" : "+v"(shrink)); // no products with it ahead of the branch
         run.top = top;
+        run.sum *= TYPE == MFR_KV_F8 ? shrink : 1.0f;
         run.sum *= shrink;
+        shrink *= TYPE == MFR_KV_F8 ? shrink : 1.0f;
 #pragma unroll
         for (int b = 0; b < D / 32; ++b) {
 #pragma unroll
@@ -568,9 +573,10 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
 }
 
 // In 8 bits a weight's exponent is taken from a score before its last rounding, and the reference has one: past
-// 2^20 they no longer agree to the last places of a weight, past 2^24 not at all. The rows of far scores are
-// done again, a wavefront a row, in fp32 throughout: tokens `first` .. `last` - 1, a lane a token for scores, a
-// lane two columns for values: 300 us for 64 tokens of 128 rows, but no model is meant to have such scores.
+// 2^20 they no longer agree to the last places of a weight, past 2^24 not at all. The rows of far scores (and
+// of more weights over the least scales than fp32 can sum, 2^17 tokens at least) are done again, a wavefront
+// a row, in fp32 throughout: tokens `first` .. `last` - 1, a lane a token for scores, a lane two columns for
+// values: 300 us for 64 tokens of 128 rows, but no model is meant to have such scores.
 constexpr float kFar = 0x1p20f;
 
 template <int D>
@@ -636,6 +642,22 @@ __device__ __forceinline__ void far_row(const Params& p, const Pages& pages, con
     }
     if (lane == 0) {
         *reinterpret_cast<float2*>(out + D) = make_float2(top, sum);
+    }
+}
+
+// Sums of weights over very small or large scales are brought near 1, with the reference: what joins parts
+// weighs them by their references alone. (Both by what the rounded reference moves.)
+constexpr int kWide = 40;
+
+template <int D> __device__ __forceinline__ void wide_row(float2 stats, int lane, float* out) {
+    const float top = stats.x + static_cast<float>(__builtin_amdgcn_frexp_expf(stats.y));
+    const float by = __builtin_amdgcn_exp2f(0.5f * (stats.x - top));
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) {
+        out[lane + 64 * i] = out[lane + 64 * i] * by * by;
+    }
+    if (lane == 0) {
+        *reinterpret_cast<float2*>(out + D) = make_float2(top, stats.y * by * by);
     }
 }
 
@@ -829,14 +851,21 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
         const int64_t part0 = mfr::kv::part_of(index, place.chunk, item.begin) * kManyRows;
         const int32_t here = min(kManyRows, rows - row0);
         if constexpr (TYPE == MFR_KV_F8) {
-            const auto far_at = [&](int32_t r) {
-                const float top = out[min(r, here - 1) * kPitch + D];
-                return fabsf(top) > kFar && top != -INFINITY;
+            const auto stats_of = [&](int32_t r) {
+                return *reinterpret_cast<const float2*>(out + min(r, here - 1) * kPitch + D);
             };
-            if (__builtin_expect(__any(far_at(32 * wave + lane % 32)), 0)) {
+            const auto is_far = [&](float2 stats) {
+                return (fabsf(stats.x) > kFar && stats.x != -INFINITY) || stats.y == INFINITY;
+            };
+            const auto is_wide = [&](float2 stats) {
+                return abs(__builtin_amdgcn_frexp_expf(stats.y)) > kWide;
+            };
+            const float2 mine_of = stats_of(32 * wave + lane % 32);
+            if (__builtin_expect(__any(is_far(mine_of) || is_wide(mine_of)), 0)) {
 #pragma unroll 1
-                for (int32_t r = 32 * wave; r < min(32 * (wave + 1), here); ++r) {
-                    if (far_at(r)) { // the wavefront's own rows alone are read and written
+                for (int32_t r = 32 * wave; r < min(32 * (wave + 1), here); ++r) { // its own rows alone
+                    const float2 stats = stats_of(r);
+                    if (is_far(stats)) {
                         const int32_t i = (row0 + r) / p.work.group;
                         const float* q = p.q.p + (shape.span.first + static_cast<int64_t>(i)) * p.q.ts +
                                          (item.head * p.work.group + (row0 + r - i * p.work.group)) *
@@ -844,6 +873,8 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
                         const int32_t from = item.first * kKeys;
                         const int32_t to = min(seen_at(row0 + r), (item.first + units) * kKeys);
                         far_row<D>(p, Pages(p, to, seq, item.head), q, from, to, lane, out + r * kPitch);
+                    } else if (is_wide(stats)) {
+                        wide_row<D>(stats, lane, out + r * kPitch);
                     }
                 }
             }

@@ -145,3 +145,27 @@ def test_large_values_under_rising_scores_in_several_steps(stream, held, rows):
     want, bound = p.attend(q[:rows], causal=False)
     got = got.reshape(sequences, rows, heads, 64)
     assert np.all(np.abs(got - want) <= bound)
+
+
+@pytest.mark.parametrize("counts", [[(150, 200), (40, 64), (110, 600)], FEW])
+@pytest.mark.parametrize("large", [2.0 ** 10, 2.0 ** 40, 2.0 ** 100])
+@pytest.mark.parametrize("zeros", ["front", "behind", "prefix", "own", "all", "mixed"])
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -126])
+def test_zeros_beside_large_values(stream, counts, large, zeros, scale):
+    """Tokens whose values are zeros under the least scale take their weight from others of large values."""
+    rng = np.random.default_rng(11)
+    p, q = case(rng, stream, counts, 2, 2, 64, "e4m3", prefix=140)
+
+    def empty(pages, tokens):
+        for t in tokens:
+            at = pages[t // 16], slice(None), t % 16
+            p.v[at], p.vs[at] = 0, scale
+
+    p.vs[np.isfinite(p.vs)] = large
+    for s, (_, tokens) in enumerate(counts):
+        if zeros != "prefix":
+            empty(p.table[s], {"front": range(tokens // 2), "behind": range(tokens // 2, tokens),
+                               "mixed": range(0, tokens, 3)}.get(zeros, range(tokens)))
+    if zeros in ("prefix", "all", "mixed"):
+        empty(p.prefix_pages, range(0, 140, 2 if zeros == "mixed" else 1))
+    check(p, q, run(p, q), norm=False)
