@@ -661,16 +661,17 @@ int mfr_kv_append(mfr_stream_t stream, const mfr_kv_append_desc* desc);
  * over the prefix's tokens and, of the row's own sequence, those at or before the row's place (causal 0:
  * all of its lengths[s]). A row that sees no token gives zeros. scale 0 means fl(1 / sqrt(d)). Scores, the
  * softmax and its sums are fp32. Caches in bf16 and e4m3 go through the bf16 matrix cores, exact
- * products of three bf16 parts of each query and weight (parts below 2^-126 are lost); fp32 caches
+ * products of three bf16 parts of each query and weight (parts below 2^-126 are lost: in 8 bits, where a
+ * weight is multiplied by its value's scale, values under scales below 2^-102 lose bits); fp32 caches
  * through the fp32 ones. With more than 96 rows a sequence on average (query heads of one head of the cache
  * counted; over the prefix the rows of all sequences), e4m3 caches go through the fp16 ones in two parts: a
  * number of a query is held to 2^-23 of itself or 2^-39 of the query's largest then, a weight times its
- * value's scale to 2^-23 or 2^-32 of the row's largest, less under scales below 2^-96. Weighted values are
- * summed before they are divided by the weights' sum, weights no more than 1 each (in those two parts, times
- * the scale, relative to the row's largest). What lies in the cache behind a sequence's tokens, or is not
- * seen by a row,
- * may be anything, NaN included. A NaN or an infinity that a row does see, in q, k or v, may leave outputs of
- * that row NaN or infinite, of no other row (a score of -infinity is a weight of 0).
+ * value's scale to 2^-23 or 2^-32 of the row's largest. Weighted values are summed before they are divided
+ * by the weights' sum, with weights of up to 1.
+ *
+ * What lies in the cache behind a sequence's tokens, or is not seen by a row, may be anything, NaN included.
+ * A NaN or an infinity that a row does see, in q, k or v, may leave outputs of that row NaN or infinite, of
+ * no other row (a score of -infinity is a weight of 0).
  *
  * out shares no memory with the other arrays. The work is cut over the chip by the lengths, as the kernels
  * find them; the same call gives the same bits. Partial results go through a workspace of

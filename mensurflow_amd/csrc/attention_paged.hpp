@@ -18,8 +18,8 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 template <int TYPE> constexpr int kBytes = TYPE == MFR_KV_F32 ? 4 : TYPE == MFR_KV_BF16 ? 2 : 1;
 
-// Unnormalised results of rows: weighted values [row][depth], and the running maximum (of base-2
-// scores) and sum [row][2].
+// Unnormalised results of rows: weighted values [row][depth], and the reference (of base-2 scores: a
+// weight is 2 to a score less it) and sum of the weights [row][2].
 struct Parts {
     float* values;
     float* stats;
@@ -67,7 +67,6 @@ void launch_join(const Params& p, hipStream_t stream);
 
 namespace mfr::paged::dev {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float floatx16 __attribute__((ext_vector_type(16)));
@@ -136,10 +135,11 @@ __device__ __forceinline__ void lds_barrier() {
 
 // The running softmax of a lane's row.
 struct Running {
-    float top = -INFINITY;
+    float top = -INFINITY; // the weights' reference: near the maximum so far
     float sum = 0.0f; // this lane's share
     int32_t seen;     // tokens that the row sees
 };
+
 // The weights of a tile of rows as B operands of bf16 products.
 struct Cut {
     bf16x8 part[3];

@@ -229,8 +229,7 @@ template <int TYPE, int D> struct Loader {
         if constexpr (TYPE == MFR_KV_F8) {
             const int which = lane >> 4 & 1;
             to.scales[which][16 * wave + lane % 16] = from.scale * unit;
-            // No further down, so that a weight over its value's scale stays inside fp32: values under a
-            // scale of 2^-96 lose bits.
+            // No further down, so that a weight over its value's scale stays inside fp32 (far_row).
             to.scales[3 - which][16 * wave + lane % 16] =
                 fmaxf(__builtin_amdgcn_logf(fabsf(from.scale)), -96.0f);
         }
@@ -573,11 +572,46 @@ __device__ __forceinline__ float settle_scores(floatx16& s, float most, Sums<D>&
 }
 
 // In 8 bits a weight's exponent is taken from a score before its last rounding, and the reference has one: past
-// 2^20 they no longer agree to the last places of a weight, past 2^24 not at all. The rows of far scores (and
-// of more weights over the least scales than fp32 can sum, 2^17 tokens at least) are done again, a wavefront
+// 2^20 they no longer agree to the last places of a weight, past 2^24 not at all. And scales below 2^-96 are
+// weighed as that, so that fp32 can sum the weights over them: they lose bits. The rows of far scores, and those
+// whose weights' sum says that such scales lead (not where all values are zeros), are done again, a wavefront
 // a row, in fp32 throughout: tokens `first` .. `last` - 1, a lane a token for scores, a lane two columns for
-// values: 300 us for 64 tokens of 128 rows, but no model is meant to have such scores.
+// values: 300 us for 64 tokens of 128 rows, but no model is meant to have such numbers.
 constexpr float kFar = 0x1p20f;
+
+// Where a token is (in bytes from a head's first row, in scales from the first).
+struct FarToken {
+    int64_t at, scale_at;
+    bool there;
+
+    __device__ __forceinline__ FarToken(const Params& p, const Pages& pages, int32_t token) {
+        const int32_t page = mfr::kv::page_checked(p.work.batch, pages.table[token >> p.cache.page_log2]);
+        const int64_t number = max(page, 0);
+        const int32_t slot = token & ((1 << p.cache.page_log2) - 1);
+        at = number * p.cache.page_stride + static_cast<int64_t>(slot) * p.cache.token_stride;
+        scale_at = ((number * p.cache.heads + pages.head) << p.cache.page_log2) + slot;
+        there = page >= 0;
+    }
+};
+
+// Whether the tokens first .. last - 1 have any value that is not 0.
+__device__ __forceinline__ bool any_value(const Params& p, const Pages& pages, int32_t first, int32_t last,
+                                          int lane) {
+    const uint8_t* const values = p.cache.v + pages.head * p.cache.head_stride;
+    bool found = false;
+#pragma unroll 1
+    for (; first < last && !__any(found); first += 64) {
+        const FarToken of(p, pages, min(first + lane, last - 1));
+        uint32_t bits = 0;
+#pragma unroll 1
+        for (int c = 0; c < p.cache.d; c += 16) {
+            const uint4 w = *reinterpret_cast<const uint4*>(values + of.at + c);
+            bits |= (w.x | w.y | w.z | w.w) & 0x7f7f7f7fu;
+        }
+        found = of.there && bits != 0 && p.cache.v_scales[of.scale_at] != 0.0f;
+    }
+    return __any(found);
+}
 
 template <int D>
 __device__ __forceinline__ void far_row(const Params& p, const Pages& pages, const float* q, int32_t first,
@@ -588,22 +622,18 @@ __device__ __forceinline__ void far_row(const Params& p, const Pages& pages, con
 #pragma unroll 1
     for (; first < last; first += 64) {
         const int32_t token = min(first + lane, last - 1);
-        const int32_t page = mfr::kv::page_checked(p.work.batch, pages.table[token >> p.cache.page_log2]);
-        const int64_t number = max(page, 0);
-        const int32_t slot = token & ((1 << p.cache.page_log2) - 1);
-        const int64_t at = number * p.cache.page_stride + static_cast<int64_t>(slot) * p.cache.token_stride;
-        const int64_t scale_at = ((number * p.cache.heads + pages.head) << p.cache.page_log2) + slot;
+        const FarToken of(p, pages, token);
         float s = 0.0f;
 #pragma unroll 1
         for (int c = 0; c < p.cache.d; c += 4) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(keys + at + c);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(keys + of.at + c);
             s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 0), q[c], s);
             s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 1), q[c + 1], s);
             s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 2), q[c + 2], s);
             s = fmaf(__builtin_amdgcn_cvt_f32_fp8(w, 3), q[c + 3], s);
         }
-        s *= p.cache.k_scales[scale_at] * p.scale;
-        s = page >= 0 && first + lane < last ? s : -INFINITY;
+        s *= p.cache.k_scales[of.scale_at] * p.scale;
+        s = of.there && first + lane < last ? s : -INFINITY;
         float most = s;
 #pragma unroll
         for (int step = 32; step > 0; step /= 2) {
@@ -616,19 +646,19 @@ __device__ __forceinline__ void far_row(const Params& p, const Pages& pages, con
         sum = fmaf(sum, shrink, weight);
         acc[0] *= shrink;
         acc[1] *= shrink;
-        const float by = weight * p.cache.v_scales[scale_at];
+        const float by = p.cache.v_scales[of.scale_at];
 #pragma unroll 1
         for (int j = 0; j < 64; ++j) {
-            const uint8_t* const row = values + __shfl(static_cast<long long>(at), j, 64);
-            const float w = __shfl(by, j, 64);
-            if (__shfl(weight, j, 64) == 0.0f) { // tokens that there are not, too
+            const uint8_t* const row = values + __shfl(static_cast<long long>(of.at), j, 64);
+            const float w = __shfl(weight, j, 64), unit = __shfl(by, j, 64);
+            if (w == 0.0f) { // tokens that there are not, too
                 continue;
             }
 #pragma unroll
             for (int i = 0; i < D / 64; ++i) {
                 const int c = lane + 64 * i;
                 const float v = c < p.cache.d ? __builtin_amdgcn_cvt_f32_fp8(row[c], 0) : 0.0f;
-                acc[i] = fmaf(w, v, acc[i]);
+                acc[i] = fmaf(w, v * unit, acc[i]);
             }
         }
     }
@@ -855,23 +885,26 @@ __global__ __launch_bounds__(kThreads, 1) void attention_paged_tiles_kernel(Para
                 return *reinterpret_cast<const float2*>(out + min(r, here - 1) * kPitch + D);
             };
             const auto is_far = [&](float2 stats) {
-                return (fabsf(stats.x) > kFar && stats.x != -INFINITY) || stats.y == INFINITY;
+                return fabsf(stats.x) > kFar && stats.x != -INFINITY;
             };
             const auto is_wide = [&](float2 stats) {
                 return abs(__builtin_amdgcn_frexp_expf(stats.y)) > kWide;
             };
+            const auto is_small = [&](float2 stats) { return stats.y >= 0x1p102f; }; // infinities, too
             const float2 mine_of = stats_of(32 * wave + lane % 32);
-            if (__builtin_expect(__any(is_far(mine_of) || is_wide(mine_of)), 0)) {
+            if (__builtin_expect(__any(is_far(mine_of) || is_wide(mine_of) || is_small(mine_of)), 0)) {
+                const int32_t from = item.first * kKeys;
+                const bool small = __any(is_small(mine_of)) &&
+                                   any_value(p, Pages(p, last, seq, item.head), from, last, lane);
 #pragma unroll 1
                 for (int32_t r = 32 * wave; r < min(32 * (wave + 1), here); ++r) { // its own rows alone
                     const float2 stats = stats_of(r);
-                    if (is_far(stats)) {
+                    if (is_far(stats) || (small && is_small(stats)) || stats.y == INFINITY) {
                         const int32_t i = (row0 + r) / p.work.group;
                         const float* q = p.q.p + (shape.span.first + static_cast<int64_t>(i)) * p.q.ts +
                                          (item.head * p.work.group + (row0 + r - i * p.work.group)) *
                                              p.q.hs;
-                        const int32_t from = item.first * kKeys;
-                        const int32_t to = min(seen_at(row0 + r), (item.first + units) * kKeys);
+                        const int32_t to = min(seen_at(row0 + r), last);
                         far_row<D>(p, Pages(p, to, seq, item.head), q, from, to, lane, out + r * kPitch);
                     } else if (is_wide(stats)) {
                         wide_row<D>(stats, lane, out + r * kPitch);

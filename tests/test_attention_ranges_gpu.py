@@ -169,3 +169,43 @@ def test_zeros_beside_large_values(stream, counts, large, zeros, scale):
     if zeros in ("prefix", "all", "mixed"):
         empty(p.prefix_pages, range(0, 140, 2 if zeros == "mixed" else 1))
     check(p, q, run(p, q), norm=False)
+
+
+@pytest.mark.parametrize("power", [-126, -118, -110, -100, -97, -95])
+@pytest.mark.parametrize("counts", [MANY, [(64, 900), (64, 700)]])
+def test_small_values_of_many_rows(stream, counts, power):
+    """Values under scales as small as there are, and zeros among them, keep their bits."""
+    rng = np.random.default_rng(-power)
+    p, q = case(rng, stream, counts, 2, 2, 64, "e4m3", prefix=40)
+    seen = np.isfinite(p.vs)
+    p.vs[seen] = np.float32(2.0 ** power) * rng.choice(np.float32([1, 1.25, 1.9]), p.vs[seen].shape)
+    p.v[np.logical_and(seen, rng.random(seen.shape) < 0.2)] = 0
+    got = run(p, q)
+    want, bound = p.attend(q)
+    there = ~np.isnan(want)
+    # In place of what `bound` allows for numbers next to fp32's least: sums of up to 940 of those.
+    off = bound - 1e-37 + 1000 * 448 * 2.0 ** -149
+    assert np.all(np.abs(got - want)[there] <= off[there])
+    assert np.count_nonzero(got[there]) > 0.9 * np.count_nonzero(want[there])
+
+
+@pytest.mark.parametrize("power", [-112, -108, -104, -100])
+def test_small_values_of_few_rows(stream, power):
+    """Of a weight times its value's scale, what lies below 2^-126 is lost, and no more."""
+    rng = np.random.default_rng(-power)
+    p, q = case(rng, stream, FEW, 2, 2, 64, "e4m3")
+    p.vs[np.isfinite(p.vs)] = np.float32(2.0 ** power)
+    got = run(p, q)
+    want, bound = p.attend(q)
+    for s, (n, tokens) in enumerate(p.counts):
+        k, v = p.tokens_of(s)
+        for i in range(n):
+            row, seen = p.starts[s] + i, tokens - n + i + 1
+            for h in range(q.shape[1]):
+                score = k[:seen, h // 2] @ q[row, h].astype(np.float64) / 8
+                weight = np.exp(score - score.max())
+                # Weights against the largest's 2^-7 at least.
+                lost = np.minimum(weight / weight.sum() * 2.0 ** power, 2.0 ** -126 / (weight.sum() * 2.0 ** -7))
+                off = bound[row, h] + lost @ np.abs(v[:seen, h // 2]) / 2.0 ** power
+                assert np.all(np.abs(got[row, h] - want[row, h]) <= off)
+                assert got[row, h].any()
