@@ -39,9 +39,11 @@ Launch launch_of(Params p, int32_t type, int shared, int cus) {
     // By the rows of a sequence, on average. 32 sequences of up to 4096 tokens, 8 heads of 128, us in tiles
     // of 16, 32 and 128 rows, bf16 (8 bits): 16 rows 83, 88, 202 (60, 74, 202); 24 rows 120, 94, 202 (94, 80,
     // 202); 64 rows 248, 167, 221 (183, 148, 228); 96 rows -, 225, 241 (-, 189, 244); 128 rows -, 317, 263
-    // (-, 275, 264). The large tiles save reading the keys again. Few sequences, whose keys stay in a cache,
-    // and short ones would do as well or better in tiles of 32: 4 of 512 rows on 600 tokens 36 and 49 us, on
-    // 4800 131 and 146; 1024 rows on a prefix of 4096 96 and 105, in 8 bits of 16384 313 and 296.
+    // (-, 275, 264). The large tiles save reading the keys again. It is not the better one everywhere: few
+    // sequences, whose keys stay in a cache, and short ones do as well or better in tiles of 32 (4 of 512 rows
+    // on 600 tokens 36 and 49 us, on 4800 131 and 146; 1024 rows on a prefix of 4096 96 and 105, in 8 bits of
+    // 16384 313 and 296), and where rows differ much most items get the other ones' height (7 single queries
+    // and a piece of 512 rows on 4096 tokens each 162 us, 35 and 120 by themselves).
     const bool many = type != MFR_KV_F32 && rows > 96 * sequences;
     w.tile_rows = many ? mfr::paged::kManyRows : rows <= 16 * sequences ? 16 : 32;
     w.unit = many || type == MFR_KV_F32 ? 64 : 128; // a workgroup's step

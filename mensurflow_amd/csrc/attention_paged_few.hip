@@ -14,10 +14,10 @@
 // bf16 and e4m3 numbers are exact in bf16. Queries, and weights (times the scales of the values), are
 // cut into three bf16 parts, so that products and sums are fp32's; fp32 caches use the fp32 products.
 //
-// One query of each of 64 sequences on up to 8191 tokens in 8 bits (8 heads of 128, 4 query heads each): 119
-// us, 4.7 TB/s; the same loads without any arithmetic take 110 to 116, more wavefronts a compute unit no less:
+// One query of each of 64 sequences on up to 8191 tokens in 8 bits (8 heads of 128, 4 query heads each): 119 to
+// 122 us, 4.7 TB/s; the same loads without any arithmetic take 110 to 116, more wavefronts a compute unit no less:
 // pages lie at random, and an eighth goes to the scales, in arrays of their own. 256 sequences of up to 1023
-// tokens: 102 us, 2.8 TB/s, four items a workgroup, at whose ends nothing is under way. One query against 4096
+// tokens: 98 us, 2.9 TB/s, four items a workgroup, at whose ends nothing is under way. One query against 4096
 // tokens in bf16: 7.5 us, one step a wavefront.
 #include "attention_paged.hpp"
 

@@ -17,14 +17,14 @@
 //   - O^T += V^T P^T: those are the B operand, and the A operand is 8 neighbouring tokens of one column,
 //     which is how the values lie.
 // bf16 caches: three bf16 parts of queries and weights. e4m3 numbers are exact in fp16 too, whose parts
-// hold 11 bits and a sign, so two hold 23: queries are brought to 2^15 by a power of two for each row, weights (with
-// the values' scales) by the softmax's reference, which is 2^15 below the largest of them.
+// hold 11 bits and a sign, so two hold 23: queries are brought to 2^15 by a power of two for each row, weights
+// (with the values' scales) by the softmax's reference, 2^7 to 2^15 below the largest of them.
 //
-// 4 x 512 queries of 8 x 4 heads of 128 on up to 8192 tokens in bf16: 500 us, 980 TFLOP/s of products (the
-// matrix cores' power: 2.2 GHz); they are 42 % busy, the vector units 41 %. 1024 rows a head on 16383 tokens
-// in 8 bits: 179 us, 770 TFLOP/s, bound by the vector instructions of a wavefront (670 a tile of 64 tokens
-// beside 64 products: widening, scales and cuts), which fill 43 % of the time and cannot be issued beside
-// others of the same SIMD.
+// 4 x 512 queries of 8 x 4 heads of 128 on up to 8192 tokens in bf16: 500 us (517-529 with the join), 980
+// TFLOP/s of products (the matrix cores' power: 2.2 GHz); they are 41 % busy, the vector units 42 %; in 8 bits
+// 475 with the join. 1024 rows a head on 16383 tokens in 8 bits: 179 us, 770 TFLOP/s, bound by the vector
+// instructions of a wavefront (670 a tile of 64 tokens beside 64 products: widening, scales and cuts), which
+// fill 43 % of the time and cannot be issued beside others of the same SIMD.
 #include "attention_paged.hpp"
 
 namespace {

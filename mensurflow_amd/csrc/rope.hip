@@ -74,8 +74,8 @@ struct RopeParams {
 
 // A wavefront takes a token's heads, or some of them where tokens are few: their pieces in a row, 64 at a
 // time, all of them under way while the angles are made. Bound by memory: 16384 tokens of 40 heads of 128
-// take 120 us (5.6 TB/s) in groups of two steps (8 heads), which keep the wavefronts of a moment near to
-// one another in memory, 125 in groups of four and 133 with a wavefront a token. 64 tokens take 5.5.
+// take 117 us (5.75 TB/s) in groups of two steps (8 heads), which keep the wavefronts of a moment near to
+// one another in memory, 125 in groups of four and 133 with a wavefront a token. 64 tokens take 5.7.
 constexpr int kAhead = 2;
 template <bool QUADS> __global__ __launch_bounds__(kThreads) void rope_kernel(RopeParams p) {
     __shared__ float2 tables[kWaves][kMostPairs];
@@ -209,7 +209,7 @@ __device__ inline void store_columns(uint8_t* row, int32_t c, float4 v, int32_t 
 // where rows are few; LANES lanes a head, a piece each (16 hold the pieces of 128 columns, but where a half
 // is no whole number of quads 17 may be needed). The first ones are under way while the row's place is
 // looked up and the angles are made. Bound by memory for prompts (8 of 2048 tokens, 8 heads of 128 into
-// bf16: 44 us, 4.5 TB/s; 52 with the row's items in two wavefronts, which both look it up), by that chain
+// bf16: 45 us, 4.5 TB/s; 52 with the row's items in two wavefronts, which both look it up), by that chain
 // of loads for a step (64 rows into 8 bits with 32 heads of queries: 6.6 us).
 template <int TYPE, bool QUADS>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendParams p) {
