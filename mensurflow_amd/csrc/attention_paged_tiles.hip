@@ -676,8 +676,9 @@ __device__ __forceinline__ void far_row(const Params& p, const Pages& pages, con
 }
 
 // Sums of weights over very small or large scales are brought near 1, with the reference: what joins parts
-// weighs them by their references alone. (Both by what the rounded reference moves.)
-constexpr int kWide = 40;
+// weighs them by their references alone, and two of 2^48 and 2^-48 leave fp32 room for 2^-30 between their
+// shares. (Both by what the rounded reference moves.)
+constexpr int kWide = 48;
 
 template <int D> __device__ __forceinline__ void wide_row(float2 stats, int lane, float* out) {
     const float top = stats.x + static_cast<float>(__builtin_amdgcn_frexp_expf(stats.y));
