@@ -719,6 +719,13 @@ def _same_stream(a: Stream, b: Stream) -> bool:
     return a is b or (a.device == b.device and a.hip_stream() == b.hip_stream())
 
 
+def _one_stream(what: str, first: str, t: DeviceArray, **others) -> None:
+    """Refuses arrays that work on the stream of t (`first`) would not be ordered with."""
+    for name, other in others.items():
+        if other is not None and not _same_stream(other.stream, t.stream):
+            raise ValueError(f"{what}: {name} is on another stream than {first}")
+
+
 def _same_device(what: str, stream: Stream, desc) -> None:
     if desc.held and desc.held[0].stream.device != stream.device:
         raise ValueError(f"{what}: a stream of another device than the operands'")
@@ -933,7 +940,9 @@ def rope_run(stream: Stream, desc: RopeDesc) -> None:
 
 def rope(x: DeviceArray, rotary: Rotary, *, positions: DeviceArray | None = None, first: int = 0,
          backward: bool = False, out: DeviceArray | None = None) -> DeviceArray:
-    """x [rows, heads, d] turned by its rows' positions, in a new array or `out` (which may be x)."""
+    """x [rows, heads, d] turned by its rows' positions, in a new array or `out` (which may be x). Runs on
+    the stream of x, which has to be that of out."""
+    _one_stream("rope", "x", x, out=out)
     if out is None:
         out = DeviceArray.empty(x.shape, x.stream)
     rope_run(x.stream, rope_desc(x, rotary, positions=positions, first=first, backward=backward,
@@ -1091,9 +1100,7 @@ def kv_append(cache: KvCache, batch: KvBatch, k: DeviceArray, v: DeviceArray, *,
     them, in a new array or `q_out` (which may be q), where they are given. Rows of no sequence of a new
     array are undefined. Runs on the stream of k, which has to be that of v, q and q_out; the cache and
     the batch may be arrays of another one that this one has waited for."""
-    for name, t in (("v", v), ("q", q), ("q_out", q_out)):
-        if t is not None and not _same_stream(t.stream, k.stream):
-            raise ValueError(f"kv_append: {name} is on another stream than k")
+    _one_stream("kv_append", "k", k, v=v, q=q, q_out=q_out)
     if q is not None and q_out is None:
         q_out = DeviceArray.empty(q.shape, k.stream)
     kv_append_run(k.stream, kv_append_desc(cache, batch, k, v, rotary=rotary, positions=positions, q=q,
@@ -1150,7 +1157,8 @@ def attention_paged(q: DeviceArray, cache: KvCache, batch: KvBatch, *, scale: fl
                     workspace: DeviceArray | None = None) -> DeviceArray:
     """softmax(scale q k^T) v of each row's queries q [rows, q_heads, d] against the batch's shared
     prefix and its sequence's tokens up to the row's own (all of them where causal is False). Rows of
-    no sequence of a new array are undefined. Runs on the stream of q."""
+    no sequence of a new array are undefined. Runs on the stream of q, which has to be that of out."""
+    _one_stream("attention_paged", "q", q, out=out)
     if out is None:
         out = DeviceArray.empty(q.shape, q.stream)
     attention_paged_run(q.stream, attention_paged_desc(q, cache, batch, scale=scale, causal=causal,

@@ -56,6 +56,26 @@ def test_operands_of_another_stream_are_refused(monkeypatch, name):
     assert ran == [own]
 
 
+@pytest.mark.parametrize("call", ["rope", "attention_paged"])
+def test_a_result_on_another_stream_is_refused(monkeypatch, call):
+    ran = []
+    monkeypatch.setattr(mf, call + "_run", lambda stream, desc: ran.append(stream))
+    own = fake(2)
+
+    def run(out_stream):
+        cache, batch, a = arrays(q=own, q_out=out_stream)
+        if call == "rope":
+            mf.rope(a["q"], mf.rotary(64), out=a["q_out"])
+        else:
+            mf.attention_paged(a["q"], cache, batch, out=a["q_out"])
+
+    with pytest.raises(ValueError, match="out is on another stream"):
+        run(fake(3))
+    assert not ran
+    run(own)
+    assert ran == [own]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("held", ["f32", "bf16", "e4m3"])
 def test_a_cache_of_another_stream(held):
